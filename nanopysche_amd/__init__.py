@@ -23,7 +23,10 @@ from .flow_moe import (
     quantize_to_fp8,
     scaling_aware_transpose,
 )
+from .decode import DecodeOutput, expert_decode, moe_decode
 from .graph import GraphedStep
+from .int8 import (Int8Experts, Int8MoECompute, Int8Tensor, int8_grouped_gemm, int8_linear, int8_matmul,
+                   quantize_to_int8)
 from .moe_layer import FP8FlowMoELayer
 from .norm import NormOutput, RMSNorm, rmsnorm, rmsnorm_backward, rmsnorm_quantize
 from .routing import (ExpertLoadTracker, RoutingPlan, expert_counts, load_balancing_loss, route, route_tokens,
@@ -58,6 +61,16 @@ __all__ = [
     "ExpertLoadTracker",
     "FP8FlowMoELayer",
     "GraphedStep",
+    "moe_decode",
+    "quantize_to_int8",
+    "int8_matmul",
+    "int8_linear",
+    "int8_grouped_gemm",
+    "Int8Tensor",
+    "Int8Experts",
+    "Int8MoECompute",
+    "expert_decode",
+    "DecodeOutput",
     "RMSNorm",
     "rmsnorm",
     "rmsnorm_quantize",

@@ -7,6 +7,7 @@ device is present when a kernel is requested, the call raises.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import functools
 import threading
@@ -38,6 +39,8 @@ GEMM_W_PAIRED = 0x800     # with GEMM_W_KMAJOR: the [K][N] weights paired too
 
 GATING_SOFTMAX = 0
 GATING_SIGMOID = 1
+DECODE_BF16 = 0
+DECODE_INT8 = 1
 GATING_L2_NORMALIZE = 1   # fm_topk_gating / fm_gating_grad flag
 
 
@@ -66,6 +69,11 @@ class FmWeightJob(C.Structure):
         ("qt", C.c_void_p), ("ld_qt", C.c_int64), ("gs_qt", C.c_int64), ("qt_col_off", C.c_int64),
         ("st", C.c_void_p), ("ld_st", C.c_int64), ("gs_st", C.c_int64),
     ]
+
+
+class FmDecodeWeights(C.Structure):
+    _fields_ = [("kind", C.c_int), ("H", C.c_int64), ("w1", C.c_void_p), ("w2", C.c_void_p), ("w3", C.c_void_p),
+                ("s1", C.c_void_p), ("s2", C.c_void_p), ("s3", C.c_void_p)]
 
 
 _vp, _i64, _i32 = C.c_void_p, C.c_int64, C.c_int
@@ -155,6 +163,19 @@ SIGNATURES = {
     "fm_grouped_gemm_ragged_k_split_workspace_bytes": (_i64, [_i32, _i64, _i64, _i32]),
     "fm_grouped_gemm_ragged_k_split": (_i32, [_i32, _OPND, _OPND, _vp, _i32, _i64, _i64, _vp, _i32, _vp,
                                               _i64, _vp, _i64, _i64, _i32, _i64, _i32, _vp, _i64, _vp]),
+    "fm_int8_quantize": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i32, _vp, _vp, _vp, _vp]),
+    "fm_int8_pack": (_i32, [_vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp]),
+    "fm_int8_unpack": (_i32, [_vp, _vp, _i64, _i64, _vp, _i32, _i64, _vp]),
+    "fm_int8_matmul": (_i32, [_vp, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _i32, _i64, _vp]),
+    "fm_int8_grouped_gemm": (_i32, [_vp, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i32, _i64,
+                                    _vp]),
+    "fm_int8_combine": (_i32, [_vp, _i64, _vp, _vp, _i64, _i32, _vp, _i32, _vp]),
+    "fm_decode_router": (_i32, [_vp, _i64, _i64, _i64, _vp, _i32, _i64, _vp, _i32, _vp, _vp, _i32, C.c_float, _i32,
+                                _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "fm_decode_workspace_bytes": (_i64, [_i64, _i64, _i32, _i32, _i64, _i64, _i32]),
+    "fm_decode_experts": (_i32, [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _i32, _i32, _i64, _i32,
+                                 C.POINTER(FmDecodeWeights), C.POINTER(FmDecodeWeights), _vp, _i32, _i64, _vp, _i64,
+                                 _vp]),
 }
 
 _lib = None
@@ -226,6 +247,15 @@ def stream_of(t: torch.Tensor) -> int:
     if index < 0:   # the raw call would take -1 as the current device
         raise ValueError(f"expected a tensor on a ROCm device, got one on {t.device} (there is no CPU fallback)")
     return torch._C._cuda_getCurrentRawStream(index)
+
+
+def on_device_of(t: torch.Tensor):
+    """A context in which t's device is the current one, where launches go."""
+    index = t.get_device()
+    return _HERE if index < 0 or torch._C._cuda_getDevice() == index else torch.cuda.device(index)
+
+
+_HERE = contextlib.nullcontext()
 
 
 def ptr(t) -> C.c_void_p:

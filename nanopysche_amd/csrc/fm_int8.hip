@@ -1,0 +1,744 @@
+// Products in 8-bit integers with a scale for each token and each channel:
+//
+//   s_r = max(max_k |x_rk|, 1e-12) / 127,  q_rk = rint(x_rk / s_r)        (rows of an operand)
+//   out[t, n] = (sum_k qx[t, k] qw[n, k]) sx[t] sw[n] (+ bias[n])
+//
+// and their forms over a routing plan's groups, with SwiGLU behind the gate|up product.
+// The sums are int32, exact for K < 2^17, so a product does not depend on how it is cut.
+// A row that holds a NaN or an infinity gets that scale and zero payload: its outputs are NaN.
+//
+// Layout.  An operand [R, K] lies in tiles of 16 rows x 64 columns, 1 KiB each, in the
+// order of the matrix cores' fragments: element (r, k) of tile (r / 16, k / 64) at byte
+// (k % 64 / 16 * 16 + r % 16) * 16 + k % 16, tiles of a row of tiles one after the other,
+// R padded to 16 and K to 128 with zeros.  Every load of a wave, from memory to LDS and
+// from LDS or memory to registers, then takes 1 KiB in order: whole lines, no bank
+// conflicts, no swizzle, and odd sizes need no bounds in the loops.
+#include <type_traits>
+
+#include "fm_common.h"
+#include "fm_dma.h"
+#include "../../include/fm_hip.h"
+
+namespace fm {
+
+namespace {
+
+constexpr int kMaxK = 131072;   // K below this: 127 * 127 K (and 128 * 128 K - 1 step) fits int32
+
+typedef int v16i __attribute__((ext_vector_type(16)));
+// 16 bytes at any address of the element's alignment
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(1)));
+
+// ---------------------------------------------------------------- quantise ----
+struct QuantArgs {
+  const void* x;
+  int64_t ld, R, C;
+  const int32_t* assign;   // row r of the output is row assign[r] / top_k of x (negative: zeros); null: row r
+  int top_k;
+  const int32_t* limit;    // rows from *limit on are left alone; null: none
+  uint8_t* q;
+  float* s;
+  int kt;
+};
+
+// 16 elements of a row from column c on, as bits, zeros from column C on.
+template <bool F32>
+struct Raw {
+  fm_u32x4 v[F32 ? 4 : 2];
+  __device__ __forceinline__ void load(const void* row, int64_t c, int64_t C) {
+    constexpr int kEach = F32 ? 4 : 8;
+    if (c + 16 <= C) {
+#pragma unroll
+      for (int i = 0; i < 16 / kEach; ++i)
+        v[i] = *FM_GLOBAL(const u32x4_any, static_cast<const uint8_t*>(row) + (c + i * kEach) * (F32 ? 4 : 2));
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 16 / kEach; ++i) v[i] = fm_u32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (c + i >= C) break;
+      if constexpr (F32) v[i / 4][i % 4] = f2u(*FM_GLOBAL(const float, static_cast<const float*>(row) + c + i));
+      else v[i / 8][i / 2 % 4] |= uint32_t(*FM_GLOBAL(const uint16_t, static_cast<const uint16_t*>(row) + c + i)) << (i % 2 * 16);
+    }
+  }
+  __device__ __forceinline__ float at(int i) const {
+    if constexpr (F32) return u2f(v[i / 4][i % 4]);
+    else return u2f(i % 2 ? v[i / 8][i / 2 % 4] & 0xffff0000u : v[i / 8][i / 2 % 4] << 16);
+  }
+  // the largest magnitude as bits: a NaN is above infinity, infinity above every number
+  __device__ __forceinline__ uint32_t top(uint32_t m) const {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t b = f2u(at(i)) & 0x7fffffffu;
+      m = b > m ? b : m;
+    }
+    return m;
+  }
+};
+
+// A workgroup takes 16 rows, a lane 16 columns of one row: a tile's payload leaves in one
+// 1 KiB store of a wave.  The NT tiles of a wave stay in registers between the maximum and
+// the rounding (NT = 0: read twice).  Bound: reading x and writing q once.
+constexpr int kQuantWaves = 8;
+template <bool F32, int NT>
+__global__ __launch_bounds__(64 * kQuantWaves) void int8_quant_kernel(QuantArgs a) {
+  __shared__ uint32_t tops[kQuantWaves][16];
+  const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4, wave = threadIdx.x >> 6;
+  const int64_t r0 = int64_t(blockIdx.x) * 16;
+  if (a.limit && r0 >= *a.limit) return;
+  int64_t src = r0 + r;
+  bool valid = src < a.R;
+  if (a.assign) {
+    const int as = valid ? a.assign[src] : -1;
+    valid = as >= 0;
+    src = valid ? as / a.top_k : 0;
+  }
+  if (!valid) src = 0;
+  const void* row = static_cast<const uint8_t*>(a.x) + src * a.ld * (F32 ? 4 : 2);
+  const int64_t C = valid ? a.C : 0;
+  Raw<F32> held[NT ? NT : 1];
+  uint32_t top = 0;
+  if constexpr (NT > 0) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) held[i].load(row, int64_t(wave + i * kQuantWaves) * 64 + c * 16, C);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) top = held[i].top(top);
+  } else {
+#pragma unroll 4
+    for (int t = wave; t < a.kt; t += kQuantWaves) {
+      Raw<F32> v;
+      v.load(row, int64_t(t) * 64 + c * 16, C);
+      top = v.top(top);
+    }
+  }
+#pragma unroll
+  for (int off = 16; off < 64; off <<= 1) {
+    const uint32_t o = __shfl_xor(top, off);
+    top = o > top ? o : top;
+  }
+  if (c == 0) tops[wave][r] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kQuantWaves; ++w) top = tops[w][r] > top ? tops[w][r] : top;
+  const bool finite = top <= 0x7f7fffffu;
+  const float s = finite ? fmaxf(u2f(top), kAmaxFloor) / 127.0f : u2f(top);
+  if (wave == 0 && c == 0) st_global(a.s + r0 + r, s);
+  const Recip d = recip_of(s);
+  auto put = [&](const Raw<F32>& v, int t) {
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t b[4];
+      // adding 1.5 * 2^23 rounds to the nearest whole number (ties to even) in the low byte
+#pragma unroll
+      for (int j = 0; j < 4; ++j) b[j] = f2u(div_rn(v.at(4 * i + j), d) + 12582912.0f);
+      const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);
+      o[i] = finite ? lo | hi : 0u;
+    }
+    st_global(a.q + ((int64_t(blockIdx.x) * a.kt + t) * 64 + lane) * 16, make_uint4(o[0], o[1], o[2], o[3]));
+  };
+  if constexpr (NT > 0) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+      if (wave + i * kQuantWaves < a.kt) put(held[i], wave + i * kQuantWaves);
+  } else {
+#pragma unroll 2
+    for (int t = wave; t < a.kt; t += kQuantWaves) {
+      Raw<F32> v;
+      v.load(row, int64_t(t) * 64 + c * 16, C);
+      put(v, t);
+    }
+  }
+}
+
+// Row-major int8 (any strides, in bytes) into tiles, groups one after the other.
+__global__ __launch_bounds__(256) void int8_pack_kernel(const uint8_t* x, int64_t gs, int64_t rs, int64_t cs, int64_t R, int64_t C,
+                                                        int kt, int64_t tiles, uint8_t* q) {
+  const int lane = threadIdx.x & 63;
+  const int64_t t = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (t >= tiles) return;
+  const int64_t rt = (R + 15) / 16, g = t / (rt * kt), tr = t / kt % rt, tk = t % kt;
+  const int64_t r = tr * 16 + (lane & 15), c = tk * 64 + (lane >> 4) * 16;
+  uint32_t o[4] = {0, 0, 0, 0};
+  if (r < R) {
+    const uint8_t* p = x + g * gs + r * rs;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (c + i < C) o[i / 4] |= uint32_t(*FM_GLOBAL(const uint8_t, p + (c + i) * cs)) << (i % 4 * 8);
+  }
+  st_global(q + (t * 64 + lane) * 16, make_uint4(o[0], o[1], o[2], o[3]));
+}
+
+// Tiles back to rows: q s as bf16 or fp32, or q itself.
+enum Unpacked : int { UP_BF16 = FM_INT8_TO_BF16, UP_F32 = FM_INT8_TO_F32, UP_I8 = FM_INT8_TO_I8 };
+template <int OUT>
+__global__ __launch_bounds__(256) void int8_unpack_kernel(const uint8_t* q, const float* s, int64_t R, int64_t C, int kt,
+                                                          int64_t tiles, uint8_t* out, int64_t ld) {
+  constexpr int kSize = OUT == UP_BF16 ? 2 : OUT == UP_F32 ? 4 : 1;
+  const int lane = threadIdx.x & 63;
+  const int64_t t = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (t >= tiles) return;
+  const int64_t r = t / kt * 16 + (lane & 15), c = t % kt * 64 + (lane >> 4) * 16;
+  const fm_u32x4 v = *FM_GLOBAL(const fm_u32x4, q + (t * 64 + lane) * 16);
+  if (r >= R || c >= C) return;
+  fm_u32x4 o[kSize];
+  if constexpr (OUT == UP_I8) {
+    o[0] = v;
+  } else {
+    const float sc = s[r];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float f[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[j] = float(int8_t(v[i] >> (8 * j))) * sc;
+      if constexpr (OUT == UP_F32) {
+        o[i] = fm_u32x4{f2u(f[0]), f2u(f[1]), f2u(f[2]), f2u(f[3])};
+      } else {
+        o[i / 2][i % 2 * 2] = hw_bf16x2(f[0], f[1]);
+        o[i / 2][i % 2 * 2 + 1] = hw_bf16x2(f[2], f[3]);
+      }
+    }
+  }
+  uint8_t* p = out + (r * ld + c) * kSize;
+  if (c + 16 <= C) {
+#pragma unroll
+    for (int i = 0; i < kSize; ++i) *FM_GLOBAL(u32x4_any, p + 16 * i) = o[i];
+    return;
+  }
+  const int left = int(C - c);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    if (i >= left) continue;
+    const int at = i * kSize;
+    const uint32_t w = o[at / 16][at / 4 % 4];
+    if constexpr (OUT == UP_F32) *FM_GLOBAL(uint32_t, p + at) = w;
+    else if constexpr (OUT == UP_BF16) *FM_GLOBAL(uint16_t, p + at) = uint16_t(w >> (at % 4 * 8));
+    else *FM_GLOBAL(uint8_t, p + at) = uint8_t(w >> (at % 4 * 8));
+  }
+}
+
+// ------------------------------------------------------------ few tokens ----
+// out[t, n] for at most 64 tokens: bound by reading the weights once.  A workgroup owns
+// 16 channels; its 4 waves take a quarter of K each, tiles straight from memory into
+// 16x16x64 MFMA fragments, U of them in flight beside the ones in use, and the four int32
+// sums meet in LDS.
+struct ProductArgs {
+  const uint8_t *a, *w, *w2;   // tiles of tokens and channels; w2: SwiGLU's up rows (else null)
+  const float *sa, *sw, *sw2;
+  int64_t w_gs, sw_gs;         // of an expert: bytes, scales
+  int kt;
+  int64_t M, N;                // rows of tokens (padded groups: of the buffer), channels (SwiGLU: hidden units)
+  const int32_t* offsets;      // [E + 1] group starts, or null: one group of M rows
+  int E;
+  const float* bias;
+  void* out;
+  int64_t ld_out;
+  int out_f32;
+};
+
+template <int TF>
+__global__ __launch_bounds__(256) void int8_few_kernel(ProductArgs p) {
+  __shared__ v4i red[3][TF][64];
+  const int lane = threadIdx.x & 63, m = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
+  const int k0 = p.kt * wave / 4, k1 = p.kt * (wave + 1) / 4;
+  constexpr int U = TF == 1 ? 8 : 4;
+  const uint8_t* w = p.w + (int64_t(blockIdx.x) * p.kt * 64 + lane) * 16;
+  const uint8_t* a = p.a + lane * 16;
+  v4i acc[TF];
+#pragma unroll
+  for (int f = 0; f < TF; ++f) acc[f] = v4i{0, 0, 0, 0};
+  v4i wv[2][U], av[2][U][TF];
+  auto load = [&](int b, int k) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t t = k + u < k1 ? k + u : k1 - 1;   // past the end: read again, not used
+      wv[b][u] = *FM_GLOBAL(const v4i, w + t * 1024);
+#pragma unroll
+      for (int f = 0; f < TF; ++f) av[b][u][f] = *FM_GLOBAL(const v4i, a + (int64_t(f) * p.kt + t) * 1024);
+    }
+  };
+  auto use = [&](int b, int k) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (k + u >= k1) break;
+#pragma unroll
+      for (int f = 0; f < TF; ++f) acc[f] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[b][u], av[b][u][f], acc[f], 0, 0, 0);
+    }
+  };
+  if (k0 < k1) {
+    load(0, k0);
+    for (int k = k0; k < k1; k += 2 * U) {
+      load(1, k + U);
+      use(0, k);
+      load(0, k + 2 * U);
+      use(1, k + U);
+    }
+  }
+  if (wave)
+#pragma unroll
+    for (int f = 0; f < TF; ++f) red[wave - 1][f][lane] = acc[f];
+  __syncthreads();
+  if (wave) return;
+  const int64_t n = int64_t(blockIdx.x) * 16 + 4 * q;
+  float sw[4], bias[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    sw[i] = n + i < p.N ? p.sw[n + i] : 0.f;
+    bias[i] = p.bias && n + i < p.N ? p.bias[n + i] : 0.f;
+  }
+#pragma unroll
+  for (int f = 0; f < TF; ++f) {
+    const int64_t t = 16 * f + m;
+    if (t >= p.M) break;
+    const v4i s = acc[f] + red[0][f][lane] + red[1][f][lane] + red[2][f][lane];
+    const float sa = p.sa[t];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (n + i >= p.N) break;
+      const float v = float(s[i]) * sa * sw[i] + bias[i];
+      if (p.out_f32) st_global(static_cast<float*>(p.out) + t * p.ld_out + n + i, v);
+      else st_global(static_cast<uint16_t*>(p.out) + t * p.ld_out + n + i, uint16_t(hw_bf16x2(v, v)));
+    }
+  }
+}
+
+// ------------------------------------------------------------- many tokens ----
+// out tile of TI channels x TJ tokens, WI x WJ waves of FA x FB 32x32 MFMA blocks; K runs in
+// halves of 64 through a ring of four LDS slots: while one half is multiplied from
+// registers the next is read from LDS and the two after it are on their way from memory.
+// Persistent: the ring runs on into the workgroup's next output tile, so its stores and
+// the next tile's first loads overlap.  SWIGLU: half of a wave's rows are gate rows, the
+// others the same hidden units' up rows, and h = silu(g) u leaves in fp32.
+template <int WI_, int WJ_, int FA_, int FB_>
+struct Shape {
+  static constexpr int WI = WI_, WJ = WJ_, FA = FA_, FB = FB_, W = WI * WJ;
+  static constexpr int TI = 32 * FA * WI, TJ = 32 * FB * WJ;
+  static constexpr int PI = TI / 16 / W, PJ = TJ / 16 / W;   // tiles a wave moves per half
+  static constexpr int kSlot = (TI + TJ) * 64;
+  static constexpr int kStage = W * 2048;
+  static_assert(TI % (16 * W) == 0 && TJ % (16 * W) == 0, "whole pieces");
+};
+constexpr int kProductExperts = 1024;
+
+struct OutTile {
+  int e, i, j0, j1;   // expert, channel tile, rows [j0, j1)
+};
+
+template <typename S, bool SWIGLU>
+__global__ __launch_bounds__(64 * S::W) void int8_product_kernel(ProductArgs p) {
+  constexpr int FA = S::FA, FB = S::FB;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * S::kSlot + S::kStage];
+  __shared__ int first[kProductExperts + 1];   // token tiles before each expert
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wi = wave / S::WJ, wj = wave % S::WJ, row32 = lane & 31, half = lane >> 5;
+
+  // token tiles of every expert, added up
+  const int rows_i = SWIGLU ? S::TI / 2 : S::TI;
+  const int NI = int((p.N + rows_i - 1) / rows_i);
+  if (p.offsets) {
+    for (int e = tid; e < p.E; e += 64 * S::W) first[e + 1] = (p.offsets[e + 1] - p.offsets[e] + S::TJ - 1) / S::TJ;
+    __syncthreads();
+    if (wave == 0) {
+      int sum = 0;
+      for (int e0 = 0; e0 < p.E; e0 += 64) {
+        int v = e0 + lane < p.E ? first[e0 + lane + 1] : 0;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+          const int o = __shfl_up(v, off);
+          if (lane >= off) v += o;
+        }
+        if (e0 + lane < p.E) first[e0 + lane + 1] = sum + v;
+        sum += __shfl(v, 63);
+      }
+      if (lane == 0) first[0] = 0;
+    }
+  } else if (tid == 0) {
+    first[0] = 0;
+    first[1] = int((p.M + S::TJ - 1) / S::TJ);
+  }
+  __syncthreads();
+  const int64_t n_tiles = int64_t(__builtin_amdgcn_readfirstlane(first[p.E])) * NI;
+  // an XCD takes a run of tiles, its workgroups in turn, so those running together share operands in its L2
+  const int xcd = blockIdx.x & 7, nbx = gridDim.x / 8;
+  const int64_t lo = n_tiles * xcd / 8, hi = n_tiles * (xcd + 1) / 8;
+  auto tile_at = [&](int64_t c, OutTile& t) -> bool {
+    const int64_t at = lo + blockIdx.x / 8 + c * nbx;
+    if (at >= hi) return false;
+    int e = 0, n = p.E;   // the last expert whose tiles start at or before
+    while (n > 1) {
+      const int h = n / 2;
+      if (int64_t(__builtin_amdgcn_readfirstlane(first[e + h])) * NI <= at) e += h, n -= h;
+      else n = h;
+    }
+    const int f0 = __builtin_amdgcn_readfirstlane(first[e]), nj = __builtin_amdgcn_readfirstlane(first[e + 1]) - f0;
+    const int64_t l = at - int64_t(f0) * NI;
+    const int g = int(l / (8 * NI)), gj = nj - 8 * g < 8 ? nj - 8 * g : 8, r = int(l - int64_t(g) * 8 * NI);
+    t.e = e;
+    t.i = r / gj;
+    const int j = 8 * g + r % gj;
+    const int b = p.offsets ? __builtin_amdgcn_readfirstlane(p.offsets[e]) : 0;
+    const int end = p.offsets ? __builtin_amdgcn_readfirstlane(p.offsets[e + 1]) : int(p.M);
+    t.j0 = b + j * S::TJ;
+    t.j1 = t.j0 + S::TJ < end ? t.j0 + S::TJ : end;
+    return true;
+  };
+
+  // what the wave moves: its tiles of the operands, row tiles past the end read from the last one
+  v4i src[S::PI + S::PJ];
+  const int64_t row_bytes = int64_t(p.kt) * 1024;
+  auto aim = [&](const OutTile& t) {
+#pragma unroll
+    for (int u = 0; u < S::PI; ++u) {
+      int64_t rt = wave * S::PI + u;
+      const uint8_t* base = p.w;
+      if constexpr (SWIGLU) {
+        // of a wave's 2 FA row tiles the first FA are gate rows, the others the same units' up rows
+        if (rt / FA % 2) base = p.w2;
+        rt = int64_t(t.i) * (S::TI / 32) + rt / (2 * FA) * FA + rt % FA;
+      } else {
+        rt += int64_t(t.i) * (S::TI / 16);
+      }
+      const int64_t last = (p.N + 15) / 16 - 1;
+      src[u] = make_rsrc(base + t.e * p.w_gs + (rt < last ? rt : last) * row_bytes);
+    }
+#pragma unroll
+    for (int u = 0; u < S::PJ; ++u) {
+      const int64_t rt = t.j0 / 16 + wave * S::PJ + u, last = (t.j1 - 1) / 16;
+      src[S::PI + u] = make_rsrc(p.a + (rt < last ? rt : last) * row_bytes);
+    }
+  };
+  const uint32_t ring = lds_addr(smem);
+  auto issue = [&](int slot, int k) {
+#pragma unroll
+    for (int u = 0; u < S::PI; ++u)
+      bdma16(src[u], lane * 16, uint32_t(k) * 1024, ring + slot * S::kSlot + (wave * S::PI + u) * 1024);
+#pragma unroll
+    for (int u = 0; u < S::PJ; ++u)
+      bdma16(src[S::PI + u], lane * 16, uint32_t(k) * 1024, ring + slot * S::kSlot + S::TI * 64 + (wave * S::PJ + u) * 1024);
+  };
+
+  struct Frags {
+    v4i a[2][FA], b[2][FB];
+  };
+  auto read = [&](int slot, Frags& f) {
+    // 32 rows x 32 deep: lane (row32, half) takes chunk 2 s + half of its row
+    const uint8_t* st = smem + slot * S::kSlot + (row32 >> 4) * 1024 + half * 256 + (row32 & 15) * 16;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int x = 0; x < FA; ++x) f.a[s][x] = *reinterpret_cast<const v4i*>(st + (wi * FA + x) * 2048 + s * 512);
+#pragma unroll
+      for (int x = 0; x < FB; ++x) f.b[s][x] = *reinterpret_cast<const v4i*>(st + S::TI * 64 + (wj * FB + x) * 2048 + s * 512);
+    }
+  };
+  v16i acc[FA][FB];
+  auto multiply = [&](const Frags& f) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int x = 0; x < FA; ++x)
+#pragma unroll
+        for (int y = 0; y < FB; ++y)
+          acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.a[s][x], f.b[s][y], acc[x][y], 0, 0, 0);
+  };
+
+  // the tile that is issued runs up to four halves ahead of the one that is multiplied
+  OutTile cur, ahead;
+  if (!tile_at(0, cur)) return;
+  int64_t ca = 0;
+  int ka = 0;
+  ahead = cur;
+  aim(ahead);
+  bool more = true;
+  auto issue_next = [&](int slot) {
+    if (ka == p.kt) {   // on to the next tile; behind the last one its last half again, which nothing reads
+      OutTile t;
+      more = more && tile_at(ca + 1, t);
+      if (more) {
+        ++ca;
+        ka = 0;
+        aim(t);
+      } else {
+        ka = p.kt - 1;
+      }
+    }
+    issue(slot, ka);
+    ++ka;
+  };
+#pragma unroll 1
+  for (int s = 0; s < 4; ++s) issue_next(s);
+  constexpr int kPer = S::PI + S::PJ;
+  FM_WAIT_VMCNT(3 * kPer);
+  block_barrier();
+  Frags f0, f1;
+  read(0, f0);
+  int g = 0;   // slot of the half in f0 (0 or 2)
+  uint8_t* stage = smem + 4 * S::kSlot + wave * 2048;
+  for (int64_t c = 0;; ++c) {
+#pragma unroll
+    for (int x = 0; x < FA; ++x)
+#pragma unroll
+      for (int y = 0; y < FB; ++y)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[x][y][i] = 0;
+#pragma unroll 1
+    for (int k = 0; k < p.kt; k += 2) {   // kt is even
+      // the next half has landed (the two after it in flight; stores of the tile before, if
+      // any, only make this wait longer) and every wave has read this one: its slot is free
+      FM_WAIT_VMCNT(2 * kPer);
+      block_barrier();
+      issue_next(g);
+      read(g + 1, f1);
+      multiply(f0);
+      __builtin_amdgcn_sched_barrier(0);
+      FM_WAIT_VMCNT(2 * kPer);
+      block_barrier();
+      issue_next(g + 1);
+      g ^= 2;
+      read(g, f0);
+      multiply(f1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // block (x, y): lane holds token row32 of y, channels 8 r + 4 half + 0..3 of x
+    const int64_t iw = int64_t(cur.i) * rows_i + wi * (SWIGLU ? 16 * FA : 32 * FA);
+#pragma unroll
+    for (int y = 0; y < FB; ++y) {
+      const int64_t t0 = cur.j0 + (wj * FB + y) * 32, t = t0 + row32;
+      const bool tv = t < cur.j1;
+      const float sa = tv ? p.sa[t] : 0.f;
+      if constexpr (SWIGLU) {
+#pragma unroll
+        for (int x = 0; x < FA / 2; ++x)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int64_t n = iw + x * 32 + 8 * r + 4 * half;   // H is a multiple of 128: inside
+            const v4f s1 = *FM_GLOBAL(const v4f, p.sw + cur.e * p.sw_gs + n), s3 = *FM_GLOBAL(const v4f, p.sw2 + cur.e * p.sw_gs + n);
+            float h[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float gate = float(acc[x][y][4 * r + i]) * sa * s1[i], up = float(acc[x + FA / 2][y][4 * r + i]) * sa * s3[i];
+              h[i] = gate / (1.f + expf(-gate)) * up;
+            }
+            if (tv) st_global(static_cast<float*>(p.out) + t * p.ld_out + n, make_float4(h[0], h[1], h[2], h[3]));
+          }
+      } else {
+#pragma unroll
+        for (int x = 0; x < FA; ++x) {
+          const int64_t n0 = iw + x * 32;
+          float v[16];
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int64_t n = n0 + 8 * r + 4 * half + i;
+              const bool nv = n < p.N;
+              v[4 * r + i] = float(acc[x][y][4 * r + i]) * sa * (nv ? p.sw[cur.e * p.sw_gs + n] : 0.f);
+              if (p.bias) v[4 * r + i] += nv ? p.bias[n] : 0.f;
+            }
+          if (p.out_f32) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int64_t n = n0 + 8 * r + 4 * half;
+              float* o = static_cast<float*>(p.out) + t * p.ld_out + n;
+              if (!tv) continue;
+              if (n + 4 <= p.N) {
+                *FM_GLOBAL(u32x4_any, o) = fm_u32x4{f2u(v[4 * r]), f2u(v[4 * r + 1]), f2u(v[4 * r + 2]), f2u(v[4 * r + 3])};
+              } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  if (n + i < p.N) st_global(o + i, v[4 * r + i]);
+              }
+            }
+          } else {
+            // through LDS: 32 tokens x 64 bytes, 16-byte unit u of row t at u ^ (t / 2 % 4)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              *reinterpret_cast<fm_u32x2*>(stage + row32 * 64 + ((r ^ (row32 >> 1)) & 3) * 16 + half * 8) =
+                  fm_u32x2{hw_bf16x2(v[4 * r], v[4 * r + 1]), hw_bf16x2(v[4 * r + 2], v[4 * r + 3])};
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              const int tr = b * 16 + (lane >> 2), u = lane & 3;
+              const fm_u32x4 o = *reinterpret_cast<const fm_u32x4*>(stage + tr * 64 + ((u ^ (tr >> 1)) & 3) * 16);
+              const int64_t n = n0 + 8 * u;
+              uint16_t* d = static_cast<uint16_t*>(p.out) + (t0 + tr) * p.ld_out + n;
+              if (t0 + tr >= cur.j1) continue;
+              if (n + 8 <= p.N) {
+                *FM_GLOBAL(u32x4_any, d) = o;
+              } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                  if (n + i < p.N) st_global(d + i, uint16_t(o[i / 2] >> (i % 2 * 16)));
+              }
+            }
+          }
+        }
+      }
+    }
+    if (!tile_at(c + 1, cur)) break;
+  }
+  FM_WAIT_VMCNT(0);
+}
+
+// out[t] = sum_k w[t, k] y[row of (t, k)], y fp32
+__global__ __launch_bounds__(256) void int8_combine_kernel(const float* y, int64_t D, const int32_t* row_of, const float* w, int K,
+                                                           void* out, int out_f32) {
+  const int64_t t = blockIdx.y, c = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 4;
+  if (c >= D) return;
+  fm_f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int k = 0; k < K; ++k) {
+    const int r = row_of[t * K + k];
+    if (r >= 0) sum += *FM_GLOBAL(const fm_f32x4, y + r * D + c) * w[t * K + k];
+  }
+  if (out_f32) st_global(static_cast<float*>(out) + t * D + c, make_float4(sum[0], sum[1], sum[2], sum[3]));
+  else st_global(static_cast<uint16_t*>(out) + t * D + c, make_uint2(hw_bf16x2(sum[0], sum[1]), hw_bf16x2(sum[2], sum[3])));
+}
+
+template <bool F32>
+void launch_quant(const QuantArgs& a, int64_t row_tiles, hipStream_t s) {
+  const dim3 grid{unsigned(row_tiles)}, block(64 * kQuantWaves);
+  if (a.kt <= 2 * kQuantWaves) hipLaunchKernelGGL((int8_quant_kernel<F32, 2>), grid, block, 0, s, a);
+  else if (a.kt <= 4 * kQuantWaves) hipLaunchKernelGGL((int8_quant_kernel<F32, 4>), grid, block, 0, s, a);
+  else if (a.kt <= 8 * kQuantWaves) hipLaunchKernelGGL((int8_quant_kernel<F32, 8>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((int8_quant_kernel<F32, 0>), grid, block, 0, s, a);
+}
+
+using Large = Shape<2, 4, 4, 2>;
+using Small = Shape<2, 2, 2, 1>;
+
+template <typename S, bool SWIGLU>
+void launch_product(const ProductArgs& p, int64_t token_tiles, hipStream_t s) {
+  const int rows_i = SWIGLU ? S::TI / 2 : S::TI;
+  const int64_t tiles = token_tiles * ((p.N + rows_i - 1) / rows_i);
+  static const int64_t fit = resident_workgroups(int8_product_kernel<S, SWIGLU>, 64 * S::W);
+  int64_t grid = tiles < fit ? tiles : fit;
+  grid = (grid + 7) / 8 * 8;   // a multiple of the XCDs
+  hipLaunchKernelGGL((int8_product_kernel<S, SWIGLU>), dim3{unsigned(grid)}, dim3(64 * S::W), 0, s, p);
+}
+
+bool product_sizes_ok(int64_t M, int64_t N, int64_t K) {
+  return M >= 0 && M < (int64_t(1) << 31) - 256 && N >= 1 && N < (int64_t(1) << 31) - 256 && K >= 1 && K < kMaxK;
+}
+
+}  // namespace
+
+}  // namespace fm
+
+using namespace fm;
+
+extern "C" {
+
+int fm_int8_quantize(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t ld_x, const int32_t* assign_of_row,
+                     int top_k, const int32_t* limit, void* q, float* s, void* stream) {
+  FM_REQUIRE(x && q && s, "fm_int8_quantize: null pointer");
+  FM_REQUIRE(x_dtype == FM_DTYPE_BF16 || x_dtype == FM_DTYPE_F32, "fm_int8_quantize: x must be bf16 or fp32");
+  FM_REQUIRE(product_sizes_ok(rows, 1, cols) && ld_x >= cols, "fm_int8_quantize: needs 1 <= columns < 131072 and a pitch that covers them");
+  FM_REQUIRE(!assign_of_row || top_k >= 1, "fm_int8_quantize: top_k must be positive");
+  FM_REQUIRE(aligned16(q) && reinterpret_cast<uintptr_t>(x) % (x_dtype == FM_DTYPE_F32 ? 4 : 2) == 0, "fm_int8_quantize: misaligned buffer");
+  if (rows == 0) return 0;
+  const QuantArgs a{x, ld_x, rows, cols, assign_of_row, top_k, limit, static_cast<uint8_t*>(q), s, int((cols + 127) / 128 * 2)};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (x_dtype == FM_DTYPE_F32) launch_quant<true>(a, (rows + 15) / 16, st);
+  else launch_quant<false>(a, (rows + 15) / 16, st);
+  return check_launch("fm_int8_quantize");
+}
+
+int fm_int8_pack(const void* x, int64_t groups, int64_t rows, int64_t cols, int64_t group_stride, int64_t row_stride,
+                 int64_t col_stride, void* q, void* stream) {
+  FM_REQUIRE(x && q && aligned16(q), "fm_int8_pack: null or misaligned pointer");
+  FM_REQUIRE(groups >= 1 && rows >= 1 && product_sizes_ok(rows, 1, cols) && (groups == 1 || rows % 16 == 0),
+             "fm_int8_pack: needs 1 <= columns < 131072, and groups of a multiple of 16 rows");
+  const int64_t kt = (cols + 127) / 128 * 2, tiles = groups * ((rows + 15) / 16) * kt;
+  FM_REQUIRE(tiles < (int64_t(1) << 32), "fm_int8_pack: too large");
+  hipLaunchKernelGGL(int8_pack_kernel, dim3{unsigned((tiles + 3) / 4)}, dim3(256), 0, static_cast<hipStream_t>(stream),
+                     static_cast<const uint8_t*>(x), group_stride, row_stride, col_stride, rows, cols, int(kt), tiles,
+                     static_cast<uint8_t*>(q));
+  return check_launch("fm_int8_pack");
+}
+
+int fm_int8_unpack(const void* q, const float* s, int64_t rows, int64_t cols, void* out, int out_kind, int64_t ld_out, void* stream) {
+  FM_REQUIRE(q && out && aligned16(q) && (s || out_kind == UP_I8), "fm_int8_unpack: null or misaligned pointer");
+  FM_REQUIRE(product_sizes_ok(rows, 1, cols) && ld_out >= cols && out_kind >= UP_BF16 && out_kind <= UP_I8, "fm_int8_unpack: bad sizes or kind");
+  if (rows == 0) return 0;
+  const int kt = int((cols + 127) / 128 * 2);
+  const int64_t tiles = (rows + 15) / 16 * kt;
+  FM_REQUIRE(tiles < (int64_t(1) << 32), "fm_int8_unpack: too large");
+  const dim3 grid{unsigned((tiles + 3) / 4)}, block(256);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const uint8_t* p = static_cast<const uint8_t*>(q);
+  uint8_t* o = static_cast<uint8_t*>(out);
+  if (out_kind == UP_BF16) hipLaunchKernelGGL(int8_unpack_kernel<UP_BF16>, grid, block, 0, st, p, s, rows, cols, kt, tiles, o, ld_out);
+  else if (out_kind == UP_F32) hipLaunchKernelGGL(int8_unpack_kernel<UP_F32>, grid, block, 0, st, p, s, rows, cols, kt, tiles, o, ld_out);
+  else hipLaunchKernelGGL(int8_unpack_kernel<UP_I8>, grid, block, 0, st, p, s, rows, cols, kt, tiles, o, ld_out);
+  return check_launch("fm_int8_unpack");
+}
+
+int fm_int8_matmul(const void* a, const float* sa, int64_t M, const void* w, const float* sw, int64_t N, int64_t K, const float* bias,
+                   void* out, int out_dtype, int64_t ld_out, void* stream) {
+  FM_REQUIRE(a && sa && w && sw && out && aligned16(a) && aligned16(w), "fm_int8_matmul: null or misaligned pointer");
+  FM_REQUIRE(product_sizes_ok(M, N, K), "fm_int8_matmul: needs sizes of at least 1 and K < 131072");
+  FM_REQUIRE((out_dtype == FM_DTYPE_BF16 || out_dtype == FM_DTYPE_F32) && ld_out >= N, "fm_int8_matmul: bad output type or pitch");
+  if (M == 0) return 0;
+  const ProductArgs p{static_cast<const uint8_t*>(a), static_cast<const uint8_t*>(w), nullptr, sa, sw, nullptr, 0, 0,
+                      int((K + 127) / 128 * 2), M, N, nullptr, 1, bias, out, ld_out, int(out_dtype == FM_DTYPE_F32)};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (M <= 64) {
+    const dim3 grid{unsigned((N + 15) / 16)}, block(256);
+    if (M <= 16) hipLaunchKernelGGL(int8_few_kernel<1>, grid, block, 0, st, p);
+    else if (M <= 32) hipLaunchKernelGGL(int8_few_kernel<2>, grid, block, 0, st, p);
+    else if (M <= 48) hipLaunchKernelGGL(int8_few_kernel<3>, grid, block, 0, st, p);
+    else hipLaunchKernelGGL(int8_few_kernel<4>, grid, block, 0, st, p);
+  } else {
+    const int64_t large = (M + 255) / 256 * ((N + 255) / 256);
+    if (large >= device_cus() / 2) launch_product<Large, false>(p, (M + 255) / 256, st);
+    else launch_product<Small, false>(p, (M + 63) / 64, st);
+  }
+  return check_launch("fm_int8_matmul");
+}
+
+int fm_int8_grouped_gemm(const void* a, const float* sa, int64_t rows, const int32_t* offsets, int E, const void* w, const float* sw,
+                         const void* w_up, const float* sw_up, int64_t N, int64_t K, int64_t tokens, void* out, int out_dtype,
+                         int64_t ld_out, void* stream) {
+  FM_REQUIRE(a && sa && offsets && w && sw && out && aligned16(a) && aligned16(w) && aligned16(w_up), "fm_int8_grouped_gemm: null or misaligned pointer");
+  FM_REQUIRE(E >= 1 && E <= kProductExperts && rows >= 0 && rows % 128 == 0 && product_sizes_ok(rows, N, K) && K % 128 == 0 && N % 16 == 0,
+             "fm_int8_grouped_gemm: needs rows and K multiples of 128, N of 16, and at most 1024 experts");
+  FM_REQUIRE((w_up == nullptr) == (sw_up == nullptr) && (!w_up || (N % 128 == 0 && out_dtype == FM_DTYPE_F32 && ld_out % 4 == 0 && aligned16(out) && aligned16(sw) && aligned16(sw_up))),
+             "fm_int8_grouped_gemm: SwiGLU needs N a multiple of 128 and an aligned fp32 output");
+  FM_REQUIRE((out_dtype == FM_DTYPE_BF16 || out_dtype == FM_DTYPE_F32) && ld_out >= N, "fm_int8_grouped_gemm: bad output type or pitch");
+  if (rows == 0) return 0;
+  const ProductArgs p{static_cast<const uint8_t*>(a), static_cast<const uint8_t*>(w), static_cast<const uint8_t*>(w_up), sa, sw, sw_up, N * K, N,
+                      int(K / 64), rows, N, offsets, E, nullptr, out, ld_out, int(out_dtype == FM_DTYPE_F32)};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  // about how many token tiles the groups give: their rows, and a partly filled tile each
+  const int64_t all = rows / 128 + E, groups = tokens < E ? tokens : E;
+  const int64_t rows_i = w_up ? 128 : 256, large = (tokens / 256 + groups) * ((N + rows_i - 1) / rows_i);
+  const bool big = large >= device_cus() / 2 && tokens >= 128 * int64_t(E);
+  if (w_up) {
+    if (big) launch_product<Large, true>(p, all, st);
+    else launch_product<Small, true>(p, 2 * all, st);
+  } else {
+    if (big) launch_product<Large, false>(p, all, st);
+    else launch_product<Small, false>(p, 2 * all, st);
+  }
+  return check_launch("fm_int8_grouped_gemm");
+}
+
+int fm_int8_combine(const float* y, int64_t D, const int32_t* row_of, const float* weights, int64_t T, int K, void* out, int out_dtype,
+                    void* stream) {
+  FM_REQUIRE(y && row_of && weights && out && aligned16(y) && aligned16(out), "fm_int8_combine: null or misaligned pointer");
+  FM_REQUIRE(T >= 0 && T < 65536LL * 1024 && K >= 1 && D >= 4 && D % 4 == 0 && (out_dtype == FM_DTYPE_BF16 || out_dtype == FM_DTYPE_F32),
+             "fm_int8_combine: bad sizes");
+  if (T == 0) return 0;
+  for (int64_t t0 = 0; t0 < T; t0 += 65535) {
+    const int64_t n = T - t0 < 65535 ? T - t0 : 65535;
+    hipLaunchKernelGGL(int8_combine_kernel, dim3(unsigned((D / 4 + 255) / 256), unsigned(n)), dim3(256), 0, static_cast<hipStream_t>(stream), y, D,
+                       row_of + t0 * K, weights + t0 * K, K, static_cast<uint8_t*>(out) + t0 * D * (out_dtype == FM_DTYPE_F32 ? 4 : 2),
+                       int(out_dtype == FM_DTYPE_F32));
+  }
+  return check_launch("fm_int8_combine");
+}
+
+}  // extern "C"
