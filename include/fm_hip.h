@@ -609,16 +609,17 @@ int fm_grouped_gemm_ragged_k_split(int kind, const FmGemmOperand* a_t, const FmG
  * int8 weights.  D and hidden sizes are multiples of 128, D at most 14336, at most
  * 1024 experts, K at most 16.
  *
- * fm_decode_router: x [T, D] bf16; with `norm` [D], RMSNorm first (model/norm.py:32-49,
- * not rounded: its two bf16 pieces go to x_hi, x_lo [T, D]); logits =
- * xn gate^T + bias + score_bias in fp32; weights [T, K] and indices [T, K] as
- * fm_topk_gating without replay.  bias, score_bias and norm may be NULL; logits
- * [T, E] is scratch, needed where E * D > 65536.
- *
  * fm_decode_experts: out[t] = sum_k weights[t, k] expert(indices[t, k] - expert_offset)(x[t])
  * (+ shared(x[t])), slots of experts outside [0, E) adding nothing.  x_lo (NULL:
  * zero) is added to x.  The workspace (16-byte aligned, fm_decode_workspace_bytes
- * bytes) holds every slice's share of the outputs in fp32. */
+ * bytes) holds h and the shares of the outputs in fp32.
+ *
+ * fm_moe_decode: the whole layer.  x [T, D] bf16; with `norm` [D], RMSNorm first
+ * (model/norm.py:32-49, not rounded: kept as two bf16 pieces); logits =
+ * xn gate^T + bias + score_bias in fp32; weights [T, K] and indices [T, K] (both
+ * written) as fm_topk_gating without replay; then fm_decode_experts of them.  bias,
+ * score_bias, norm and shared may be NULL.  Its workspace is
+ * fm_moe_decode_workspace_bytes bytes. */
 #define FM_DECODE_BF16 0   /* w1, w2, w3 [E * H, D] bf16, contiguous                          */
 #define FM_DECODE_INT8 1   /* int8 tiles: w1, w3 [E][H x D], w2 [E][D x H] (transposed)       */
 typedef struct FmDecodeWeights {
@@ -627,11 +628,13 @@ typedef struct FmDecodeWeights {
   const void *w1, *w2, *w3;
   const float *s1, *s2, *s3;   /* int8: scales [E * H], [E, D], [E * H] */
 } FmDecodeWeights;
-int fm_decode_router(const void* x, int64_t ld_x, int64_t T, int64_t D, const void* gate, int gate_dtype, int64_t ld_g,
-                     const void* bias, int bias_dtype, const float* score_bias, const void* norm, int norm_dtype,
-                     float eps, int E, int K, int gating, int flags, float* logits, void* x_hi, void* x_lo,
-                     float* weights, int64_t* indices, void* stream);
-int64_t fm_decode_workspace_bytes(int64_t T, int64_t D, int K, int E, int64_t H, int64_t H_shared, int kind);
+int fm_moe_decode(const void* x, int64_t ld_x, int64_t T, int64_t D, const void* gate, int gate_dtype, int64_t ld_g,
+                  const void* bias, int bias_dtype, const float* score_bias, const void* norm, int norm_dtype, float eps,
+                  int E, int K, int gating, int flags, const FmDecodeWeights* experts, const FmDecodeWeights* shared,
+                  float* weights, int64_t* indices, void* out, int out_dtype, int64_t ld_out, void* workspace,
+                  int64_t workspace_bytes, void* stream);
+int64_t fm_moe_decode_workspace_bytes(int64_t T, int64_t D, int K, int E, int64_t H, int64_t H_shared);
+int64_t fm_decode_workspace_bytes(int64_t T, int64_t D, int K, int E, int64_t H, int64_t H_shared);
 int fm_decode_experts(const void* x, const void* x_lo, int64_t ld_x, int64_t T, int64_t D, const float* weights,
                       const void* indices, int indices_i64, int K, int64_t expert_offset, int E,
                       const FmDecodeWeights* experts, const FmDecodeWeights* shared, void* out, int out_dtype,
@@ -653,21 +656,24 @@ int fm_decode_experts(const void* x, const void* x_lo, int64_t ld_x, int64_t T, 
  *   infinity gets scale NaN or infinity and zero payload.  With assign_of_row, output
  *   row r is row assign_of_row[r] / top_k of x (zeros where negative: a routing plan's
  *   padding); rows from *limit (a multiple of 16, device memory, or NULL) on are left
- *   as they are.
+ *   as they are.  top (or NULL): the rows' largest magnitudes as fp32 bits, if they are
+ *   known; clear (or NULL): words set to 0, one a row and 16 ceil(rows / 16) in all.
  * fm_int8_pack: int8 values with byte strides into tiles.  fm_int8_unpack: tiles into
  *   rows: q * s as bf16 (0) or fp32 (1), or q (2).
  * fm_int8_matmul: out [M, N] bf16 or fp32.
  * fm_int8_grouped_gemm: rows [offsets[e], offsets[e + 1]) (multiples of 128) of the
  *   tokens times expert e's channels; `tokens` is the host's estimate of the rows that
  *   hold one (it only picks a kernel).  With w_up, out is silu(gate) * up in fp32 (N = H
- *   a multiple of 128).  K a multiple of 128, N of 16.
+ *   a multiple of 128) and top[r] is raised to the largest magnitude of row r, as fp32
+ *   bits.  K a multiple of 128, N of 16.
  * fm_int8_combine: out[t] = sum_k weights[t, k] y[row_of[t * K + k]], y [rows, D] fp32,
  *   negative rows adding nothing. */
 #define FM_INT8_TO_BF16 0
 #define FM_INT8_TO_F32 1
 #define FM_INT8_TO_I8 2
 int fm_int8_quantize(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t ld_x, const int32_t* assign_of_row,
-                     int top_k, const int32_t* limit, void* q, float* s, void* stream);
+                     int top_k, const int32_t* limit, const uint32_t* top, uint32_t* clear, void* q, float* s,
+                     void* stream);
 int fm_int8_pack(const void* x, int64_t groups, int64_t rows, int64_t cols, int64_t group_stride, int64_t row_stride,
                  int64_t col_stride, void* q, void* stream);
 int fm_int8_unpack(const void* q, const float* s, int64_t rows, int64_t cols, void* out, int out_kind, int64_t ld_out,
@@ -675,8 +681,8 @@ int fm_int8_unpack(const void* q, const float* s, int64_t rows, int64_t cols, vo
 int fm_int8_matmul(const void* a, const float* sa, int64_t M, const void* w, const float* sw, int64_t N, int64_t K,
                    const float* bias, void* out, int out_dtype, int64_t ld_out, void* stream);
 int fm_int8_grouped_gemm(const void* a, const float* sa, int64_t rows, const int32_t* offsets, int E, const void* w,
-                         const float* sw, const void* w_up, const float* sw_up, int64_t N, int64_t K, int64_t tokens,
-                         void* out, int out_dtype, int64_t ld_out, void* stream);
+                         const float* sw, const void* w_up, const float* sw_up, uint32_t* top, int64_t N, int64_t K,
+                         int64_t tokens, void* out, int out_dtype, int64_t ld_out, void* stream);
 int fm_int8_combine(const float* y, int64_t D, const int32_t* row_of, const float* weights, int64_t T, int K, void* out,
                     int out_dtype, void* stream);
 

@@ -163,16 +163,18 @@ SIGNATURES = {
     "fm_grouped_gemm_ragged_k_split_workspace_bytes": (_i64, [_i32, _i64, _i64, _i32]),
     "fm_grouped_gemm_ragged_k_split": (_i32, [_i32, _OPND, _OPND, _vp, _i32, _i64, _i64, _vp, _i32, _vp,
                                               _i64, _vp, _i64, _i64, _i32, _i64, _i32, _vp, _i64, _vp]),
-    "fm_int8_quantize": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i32, _vp, _vp, _vp, _vp]),
+    "fm_int8_quantize": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp]),
     "fm_int8_pack": (_i32, [_vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp]),
     "fm_int8_unpack": (_i32, [_vp, _vp, _i64, _i64, _vp, _i32, _i64, _vp]),
     "fm_int8_matmul": (_i32, [_vp, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _i32, _i64, _vp]),
-    "fm_int8_grouped_gemm": (_i32, [_vp, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i32, _i64,
-                                    _vp]),
+    "fm_int8_grouped_gemm": (_i32, [_vp, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i32,
+                                    _i64, _vp]),
     "fm_int8_combine": (_i32, [_vp, _i64, _vp, _vp, _i64, _i32, _vp, _i32, _vp]),
-    "fm_decode_router": (_i32, [_vp, _i64, _i64, _i64, _vp, _i32, _i64, _vp, _i32, _vp, _vp, _i32, C.c_float, _i32,
-                                _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp]),
-    "fm_decode_workspace_bytes": (_i64, [_i64, _i64, _i32, _i32, _i64, _i64, _i32]),
+    "fm_moe_decode": (_i32, [_vp, _i64, _i64, _i64, _vp, _i32, _i64, _vp, _i32, _vp, _vp, _i32, C.c_float, _i32, _i32,
+                             _i32, _i32, C.POINTER(FmDecodeWeights), C.POINTER(FmDecodeWeights), _vp, _vp, _vp, _i32,
+                             _i64, _vp, _i64, _vp]),
+    "fm_moe_decode_workspace_bytes": (_i64, [_i64, _i64, _i32, _i32, _i64, _i64]),
+    "fm_decode_workspace_bytes": (_i64, [_i64, _i64, _i32, _i32, _i64, _i64]),
     "fm_decode_experts": (_i32, [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _i32, _i32, _i64, _i32,
                                  C.POINTER(FmDecodeWeights), C.POINTER(FmDecodeWeights), _vp, _i32, _i64, _vp, _i64,
                                  _vp]),

@@ -62,4 +62,15 @@ __device__ __forceinline__ void block_barrier() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
+// The lane id read from the hardware (v_mbcnt) at each use.  Volatile, so the
+// compiler neither hoists nor shares it: values derived from the lane between
+// tiles are rebuilt from it instead of being kept live across the K loops,
+// where the register budget is spent (a spilled value's reload waits for
+// every load in flight, the operand prefetch included).
+__device__ __forceinline__ int fresh_lane() {
+  int l;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
+  return l;
+}
+
 }  // namespace fm

@@ -950,16 +950,6 @@ __global__ __launch_bounds__(512) void gemm256_mk_kernel(GemmParams pm, GemmPara
 // Per-lane values (expert x = lane: tile count, inclusive scan, offsets) live
 // in the wave's own 1 KiB of LDS between tiles, so they cost no registers
 // across the K loop.
-// The lane id read from the hardware (v_mbcnt) at each use.  Volatile, so the
-// compiler neither hoists nor shares it: values derived from the lane between
-// tiles are rebuilt from it instead of being kept live across the K loops,
-// where the register budget is spent (a spilled value's reload waits for
-// every load in flight, the operand prefetch included).
-__device__ __forceinline__ int fresh_lane() {
-  int l;
-  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
-  return l;
-}
 
 struct TileQueue {
   int* lds;                    // [4][64] ints of this wave

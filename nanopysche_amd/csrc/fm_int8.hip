@@ -25,7 +25,6 @@ namespace {
 
 constexpr int kMaxK = 131072;   // K below this: 127 * 127 K (and 128 * 128 K - 1 step) fits int32
 
-typedef int v16i __attribute__((ext_vector_type(16)));
 // 16 bytes at any address of the element's alignment
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(1)));
 
@@ -36,6 +35,8 @@ struct QuantArgs {
   const int32_t* assign;   // row r of the output is row assign[r] / top_k of x (negative: zeros); null: row r
   int top_k;
   const int32_t* limit;    // rows from *limit on are left alone; null: none
+  const uint32_t* top;     // the rows' largest magnitudes as bits where they are known, or null
+  uint32_t* clear;         // [rows, padded to 16] set to 0, or null
   uint8_t* q;
   float* s;
   int kt;
@@ -55,6 +56,7 @@ struct Raw {
     }
 #pragma unroll
     for (int i = 0; i < 16 / kEach; ++i) v[i] = fm_u32x4{0, 0, 0, 0};
+    if (c >= C) return;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       if (c + i >= C) break;
@@ -77,16 +79,37 @@ struct Raw {
   }
 };
 
+__device__ __forceinline__ float int8_scale(uint32_t top) {
+  return top <= 0x7f7fffffu ? fmaxf(u2f(top), kAmaxFloor) / 127.0f : u2f(top);
+}
+// 16 quotients rounded to whole numbers as bytes; `finite`: else zeros
+template <bool F32>
+__device__ __forceinline__ fm_u32x4 int8_round(const Raw<F32>& v, Recip d, bool finite) {
+  fm_u32x4 o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t b[4];
+    // adding 1.5 * 2^23 rounds to the nearest whole number (ties to even) in the low byte
+#pragma unroll
+    for (int j = 0; j < 4; ++j) b[j] = f2u(div_rn(v.at(4 * i + j), d) + 12582912.0f);
+    const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);
+    o[i] = finite ? lo | hi : 0u;
+  }
+  return o;
+}
+
 // A workgroup takes 16 rows, a lane 16 columns of one row: a tile's payload leaves in one
 // 1 KiB store of a wave.  The NT tiles of a wave stay in registers between the maximum and
-// the rounding (NT = 0: read twice).  Bound: reading x and writing q once.
+// the rounding (NT = 0: read twice).  GIVEN: the maxima are known, and gridDim.y workgroups
+// share the columns.  Bound: reading x and writing q once.
 constexpr int kQuantWaves = 8;
-template <bool F32, int NT>
+template <bool F32, int NT, bool GIVEN>
 __global__ __launch_bounds__(64 * kQuantWaves) void int8_quant_kernel(QuantArgs a) {
   __shared__ uint32_t tops[kQuantWaves][16];
   const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4, wave = threadIdx.x >> 6;
   const int64_t r0 = int64_t(blockIdx.x) * 16;
   if (a.limit && r0 >= *a.limit) return;
+  if (a.clear && threadIdx.x < 16) st_global(a.clear + r0 + threadIdx.x, 0u);
   int64_t src = r0 + r;
   bool valid = src < a.R;
   if (a.assign) {
@@ -97,57 +120,63 @@ __global__ __launch_bounds__(64 * kQuantWaves) void int8_quant_kernel(QuantArgs 
   if (!valid) src = 0;
   const void* row = static_cast<const uint8_t*>(a.x) + src * a.ld * (F32 ? 4 : 2);
   const int64_t C = valid ? a.C : 0;
-  Raw<F32> held[NT ? NT : 1];
-  uint32_t top = 0;
-  if constexpr (NT > 0) {
-#pragma unroll
-    for (int i = 0; i < NT; ++i) held[i].load(row, int64_t(wave + i * kQuantWaves) * 64 + c * 16, C);
-#pragma unroll
-    for (int i = 0; i < NT; ++i) top = held[i].top(top);
-  } else {
-#pragma unroll 4
-    for (int t = wave; t < a.kt; t += kQuantWaves) {
-      Raw<F32> v;
-      v.load(row, int64_t(t) * 64 + c * 16, C);
-      top = v.top(top);
-    }
-  }
-#pragma unroll
-  for (int off = 16; off < 64; off <<= 1) {
-    const uint32_t o = __shfl_xor(top, off);
-    top = o > top ? o : top;
-  }
-  if (c == 0) tops[wave][r] = top;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kQuantWaves; ++w) top = tops[w][r] > top ? tops[w][r] : top;
-  const bool finite = top <= 0x7f7fffffu;
-  const float s = finite ? fmaxf(u2f(top), kAmaxFloor) / 127.0f : u2f(top);
-  if (wave == 0 && c == 0) st_global(a.s + r0 + r, s);
-  const Recip d = recip_of(s);
-  auto put = [&](const Raw<F32>& v, int t) {
-    uint32_t o[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t b[4];
-      // adding 1.5 * 2^23 rounds to the nearest whole number (ties to even) in the low byte
-#pragma unroll
-      for (int j = 0; j < 4; ++j) b[j] = f2u(div_rn(v.at(4 * i + j), d) + 12582912.0f);
-      const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);
-      o[i] = finite ? lo | hi : 0u;
-    }
-    st_global(a.q + ((int64_t(blockIdx.x) * a.kt + t) * 64 + lane) * 16, make_uint4(o[0], o[1], o[2], o[3]));
+  uint8_t* const q = a.q + (int64_t(blockIdx.x) * a.kt * 64 + lane) * 16;
+  auto put = [&](const Raw<F32>& v, Recip d, bool finite, int t) {
+    const fm_u32x4 o = int8_round(v, d, finite);
+    st_global(q + int64_t(t) * 1024, make_uint4(o[0], o[1], o[2], o[3]));
   };
-  if constexpr (NT > 0) {
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-      if (wave + i * kQuantWaves < a.kt) put(held[i], wave + i * kQuantWaves);
-  } else {
-#pragma unroll 2
-    for (int t = wave; t < a.kt; t += kQuantWaves) {
+  if constexpr (GIVEN) {
+    const uint32_t top = valid ? a.top[r0 + r] : 0u;
+    const float s = int8_scale(top);
+    if (blockIdx.y == 0 && wave == 0 && c == 0) st_global(a.s + r0 + r, s);
+    const Recip d = recip_of(s);
+    const int step = kQuantWaves * gridDim.y;
+#pragma unroll 4
+    for (int t = wave + kQuantWaves * blockIdx.y; t < a.kt; t += step) {
       Raw<F32> v;
       v.load(row, int64_t(t) * 64 + c * 16, C);
-      put(v, t);
+      put(v, d, top <= 0x7f7fffffu, t);
+    }
+  } else {
+    Raw<F32> held[NT ? NT : 1];
+    uint32_t top = 0;
+    if constexpr (NT > 0) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) held[i].load(row, int64_t(wave + i * kQuantWaves) * 64 + c * 16, C);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) top = held[i].top(top);
+    } else {
+#pragma unroll 4
+      for (int t = wave; t < a.kt; t += kQuantWaves) {
+        Raw<F32> v;
+        v.load(row, int64_t(t) * 64 + c * 16, C);
+        top = v.top(top);
+      }
+    }
+#pragma unroll
+    for (int off = 16; off < 64; off <<= 1) {
+      const uint32_t o = __shfl_xor(top, off);
+      top = o > top ? o : top;
+    }
+    if (c == 0) tops[wave][r] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kQuantWaves; ++w) top = tops[w][r] > top ? tops[w][r] : top;
+    const float s = int8_scale(top);
+    const bool finite = top <= 0x7f7fffffu;
+    if (wave == 0 && c == 0) st_global(a.s + r0 + r, s);
+    const Recip d = recip_of(s);
+    if constexpr (NT > 0) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+        if (wave + i * kQuantWaves < a.kt) put(held[i], d, finite, wave + i * kQuantWaves);
+    } else {
+#pragma unroll 2
+      for (int t = wave; t < a.kt; t += kQuantWaves) {
+        Raw<F32> v;
+        v.load(row, int64_t(t) * 64 + c * 16, C);
+        put(v, d, finite, t);
+      }
     }
   }
 }
@@ -235,6 +264,7 @@ struct ProductArgs {
   void* out;
   int64_t ld_out;
   int out_f32;
+  uint32_t* top;               // SwiGLU: the rows' largest |h| as bits, raised by every wave
 };
 
 template <int TF>
@@ -305,7 +335,7 @@ __global__ __launch_bounds__(256) void int8_few_kernel(ProductArgs p) {
 }
 
 // ------------------------------------------------------------- many tokens ----
-// out tile of TI channels x TJ tokens, WI x WJ waves of FA x FB 32x32 MFMA blocks; K runs in
+// out tile of TI channels x TJ tokens, WI x WJ waves of FA x FB 16x16x64 MFMA blocks; K runs in
 // halves of 64 through a ring of four LDS slots: while one half is multiplied from
 // registers the next is read from LDS and the two after it are on their way from memory.
 // Persistent: the ring runs on into the workgroup's next output tile, so its stores and
@@ -314,7 +344,7 @@ __global__ __launch_bounds__(256) void int8_few_kernel(ProductArgs p) {
 template <int WI_, int WJ_, int FA_, int FB_>
 struct Shape {
   static constexpr int WI = WI_, WJ = WJ_, FA = FA_, FB = FB_, W = WI * WJ;
-  static constexpr int TI = 32 * FA * WI, TJ = 32 * FB * WJ;
+  static constexpr int TI = 16 * FA * WI, TJ = 16 * FB * WJ;
   static constexpr int PI = TI / 16 / W, PJ = TJ / 16 / W;   // tiles a wave moves per half
   static constexpr int kSlot = (TI + TJ) * 64;
   static constexpr int kStage = W * 2048;
@@ -326,6 +356,126 @@ struct OutTile {
   int e, i, j0, j1;   // expert, channel tile, rows [j0, j1)
 };
 
+// 4 scales or biases of channels from n on (n a multiple of 4), zeros from N on.
+__device__ __forceinline__ v4f four_of(const float* p, int64_t n, int64_t N) {
+  typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
+  if (n + 4 <= N) return *FM_GLOBAL(const v4f_any, p + n);
+  v4f v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+    if (n + i < N) v[i] = *FM_GLOBAL(const float, p + n + i);
+  return v;
+}
+
+// A wave's blocks of an output tile: block (x, y) holds token lane % 16 of y, channels
+// 4 (lane / 16) + 0..3 of x.  bf16 rows go through the wave's 2 KiB of LDS, so that a
+// store covers 64 bytes of 16 rows.  The lane is asked for again, so that nothing derived
+// from it stays in registers through the loop over K, which leaves none to spare.
+template <typename S, bool SWIGLU>
+__device__ __forceinline__ void store_tile(const ProductArgs& p, const OutTile& cur, const v4i (&acc)[S::FA][S::FB], uint8_t* stage,
+                                           int wi, int wj) {
+  constexpr int FA = S::FA, FB = S::FB;
+  const int lane = fresh_lane(), m = lane & 15, q = lane >> 4;
+  const float *sw = p.sw + cur.e * p.sw_gs, *sw2 = p.sw2 + cur.e * p.sw_gs;
+  const int64_t iw = int64_t(cur.i) * (SWIGLU ? S::TI / 2 : S::TI) + wi * (SWIGLU ? 8 * FA : 16 * FA);
+  const int64_t tw = cur.j0 + wj * FB * 16;
+  float sa[FB];
+#pragma unroll
+  for (int y = 0; y < FB; ++y) sa[y] = tw + 16 * y + m < cur.j1 ? *FM_GLOBAL(const float, p.sa + tw + 16 * y + m) : 0.f;
+  if constexpr (SWIGLU) {
+    uint32_t top[FB];
+#pragma unroll
+    for (int y = 0; y < FB; ++y) top[y] = 0;
+#pragma unroll
+    for (int x = 0; x < FA / 2; ++x) {
+      const int64_t n = iw + x * 16 + 4 * q;   // H is a multiple of 128: inside
+      const v4f s1 = *FM_GLOBAL(const v4f, sw + n), s3 = *FM_GLOBAL(const v4f, sw2 + n);
+#pragma unroll
+      for (int y = 0; y < FB; ++y) {
+        const int64_t t = tw + 16 * y + m;
+        float h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float gate = float(acc[x][y][i]) * sa[y] * s1[i], up = float(acc[x + FA / 2][y][i]) * sa[y] * s3[i];
+          h[i] = gate / (1.f + expf(-gate)) * up;
+          const uint32_t b = f2u(h[i]) & 0x7fffffffu;   // a NaN is above infinity, infinity above every number
+          top[y] = b > top[y] ? b : top[y];
+        }
+        if (t < cur.j1) st_global(static_cast<float*>(p.out) + t * p.ld_out + n, make_float4(h[0], h[1], h[2], h[3]));
+      }
+    }
+    // a maximum does not depend on the order in which the waves raise it
+#pragma unroll
+    for (int y = 0; y < FB; ++y) {
+#pragma unroll
+      for (int off = 16; off < 64; off <<= 1) {
+        const uint32_t o = __shfl_xor(top[y], off);
+        top[y] = o > top[y] ? o : top[y];
+      }
+      if (q == 0 && tw + 16 * y + m < cur.j1) atomicMax(p.top + tw + 16 * y + m, top[y]);
+    }
+  } else {
+    static_assert(FA % 2 == 0 && FB % 2 == 0, "blocks in squares of four");
+#pragma unroll
+    for (int x = 0; x < FA; x += 2) {
+      const int64_t n0 = iw + x * 16;
+      if (n0 >= p.N) break;
+      v4f s[2], bias[2];
+#pragma unroll
+      for (int xx = 0; xx < 2; ++xx) {
+        s[xx] = four_of(sw, n0 + 16 * xx + 4 * q, p.N);
+        bias[xx] = p.bias ? four_of(p.bias, n0 + 16 * xx + 4 * q, p.N) : v4f{0.f, 0.f, 0.f, 0.f};
+      }
+#pragma unroll
+      for (int y = 0; y < FB; y += 2) {
+#pragma unroll
+        for (int yy = 0; yy < 2; ++yy)
+#pragma unroll
+          for (int xx = 0; xx < 2; ++xx) {
+            v4f v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = float(acc[x + xx][y + yy][i]) * sa[y + yy] * s[xx][i] + bias[xx][i];
+            if (p.out_f32) {
+              const int64_t t = tw + 16 * (y + yy) + m, n = n0 + 16 * xx + 4 * q;
+              float* o = static_cast<float*>(p.out) + t * p.ld_out + n;
+              if (t < cur.j1) {
+                if (n + 4 <= p.N) {
+                  *FM_GLOBAL(u32x4_any, o) = __builtin_bit_cast(fm_u32x4, v);
+                } else {
+#pragma unroll
+                  for (int i = 0; i < 3; ++i)
+                    if (n + i < p.N) st_global(o + i, v[i]);
+                }
+              }
+            } else {
+              // 32 tokens x 64 bytes, 16-byte unit u of row t at u ^ (t / 2 % 4)
+              const int tr = 16 * yy + m, u = 2 * xx + (q >> 1);
+              *reinterpret_cast<fm_u32x2*>(stage + tr * 64 + ((u ^ (tr >> 1)) & 3) * 16 + (q & 1) * 8) =
+                  fm_u32x2{hw_bf16x2(v[0], v[1]), hw_bf16x2(v[2], v[3])};
+            }
+          }
+        if (!p.out_f32) {
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const int tr = b * 16 + (lane >> 2), u = lane & 3;
+            const fm_u32x4 o = *reinterpret_cast<const fm_u32x4*>(stage + tr * 64 + ((u ^ (tr >> 1)) & 3) * 16);
+            const int64_t t = tw + 16 * y + tr, n = n0 + 8 * u;
+            uint16_t* d = static_cast<uint16_t*>(p.out) + t * p.ld_out + n;
+            if (t >= cur.j1) continue;
+            if (n + 8 <= p.N) {
+              *FM_GLOBAL(u32x4_any, d) = o;
+            } else {
+#pragma unroll
+              for (int i = 0; i < 7; ++i)
+                if (n + i < p.N) st_global(d + i, uint16_t(o[i / 2] >> (i % 2 * 16)));
+            }
+          }
+        }
+      }
+    }
+  }
+}
+
 template <typename S, bool SWIGLU>
 __global__ __launch_bounds__(64 * S::W) void int8_product_kernel(ProductArgs p) {
   constexpr int FA = S::FA, FB = S::FB;
@@ -333,7 +483,7 @@ __global__ __launch_bounds__(64 * S::W) void int8_product_kernel(ProductArgs p) 
   __shared__ int first[kProductExperts + 1];   // token tiles before each expert
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wi = wave / S::WJ, wj = wave % S::WJ, row32 = lane & 31, half = lane >> 5;
+  const int wi = wave % S::WI, wj = wave / S::WI;   // a SIMD's two waves hold different tokens
 
   // token tiles of every expert, added up
   const int rows_i = SWIGLU ? S::TI / 2 : S::TI;
@@ -360,22 +510,22 @@ __global__ __launch_bounds__(64 * S::W) void int8_product_kernel(ProductArgs p) 
     first[1] = int((p.M + S::TJ - 1) / S::TJ);
   }
   __syncthreads();
-  const int64_t n_tiles = int64_t(__builtin_amdgcn_readfirstlane(first[p.E])) * NI;
+  const int n_tiles = __builtin_amdgcn_readfirstlane(first[p.E]) * NI;   // below 2^31 (launcher)
   // an XCD takes a run of tiles, its workgroups in turn, so those running together share operands in its L2
   const int xcd = blockIdx.x & 7, nbx = gridDim.x / 8;
-  const int64_t lo = n_tiles * xcd / 8, hi = n_tiles * (xcd + 1) / 8;
-  auto tile_at = [&](int64_t c, OutTile& t) -> bool {
-    const int64_t at = lo + blockIdx.x / 8 + c * nbx;
+  const int each = n_tiles / 8, more_x = n_tiles % 8;
+  const int lo = each * xcd + (xcd < more_x ? xcd : more_x), hi = lo + each + (xcd < more_x);
+  auto tile_at = [&](int c, OutTile& t) -> bool {
+    const int at = lo + int(blockIdx.x / 8) + c * nbx;
     if (at >= hi) return false;
     int e = 0, n = p.E;   // the last expert whose tiles start at or before
     while (n > 1) {
       const int h = n / 2;
-      if (int64_t(__builtin_amdgcn_readfirstlane(first[e + h])) * NI <= at) e += h, n -= h;
+      if (__builtin_amdgcn_readfirstlane(first[e + h]) * NI <= at) e += h, n -= h;
       else n = h;
     }
     const int f0 = __builtin_amdgcn_readfirstlane(first[e]), nj = __builtin_amdgcn_readfirstlane(first[e + 1]) - f0;
-    const int64_t l = at - int64_t(f0) * NI;
-    const int g = int(l / (8 * NI)), gj = nj - 8 * g < 8 ? nj - 8 * g : 8, r = int(l - int64_t(g) * 8 * NI);
+    const int l = at - f0 * NI, g = l / (8 * NI), gj = nj - 8 * g < 8 ? nj - 8 * g : 8, r = l - g * 8 * NI;
     t.e = e;
     t.i = r / gj;
     const int j = 8 * g + r % gj;
@@ -392,21 +542,21 @@ __global__ __launch_bounds__(64 * S::W) void int8_product_kernel(ProductArgs p) 
   auto aim = [&](const OutTile& t) {
 #pragma unroll
     for (int u = 0; u < S::PI; ++u) {
-      int64_t rt = wave * S::PI + u;
+      int rt = wave * S::PI + u;
       const uint8_t* base = p.w;
       if constexpr (SWIGLU) {
-        // of a wave's 2 FA row tiles the first FA are gate rows, the others the same units' up rows
-        if (rt / FA % 2) base = p.w2;
-        rt = int64_t(t.i) * (S::TI / 32) + rt / (2 * FA) * FA + rt % FA;
+        // of a wave's FA row tiles the first half are gate rows, the others the same units' up rows
+        if (rt / (FA / 2) % 2) base = p.w2;
+        rt = t.i * (S::TI / 32) + rt / FA * (FA / 2) + rt % (FA / 2);
       } else {
-        rt += int64_t(t.i) * (S::TI / 16);
+        rt += t.i * (S::TI / 16);
       }
-      const int64_t last = (p.N + 15) / 16 - 1;
+      const int last = int((p.N + 15) / 16) - 1;
       src[u] = make_rsrc(base + t.e * p.w_gs + (rt < last ? rt : last) * row_bytes);
     }
 #pragma unroll
     for (int u = 0; u < S::PJ; ++u) {
-      const int64_t rt = t.j0 / 16 + wave * S::PJ + u, last = (t.j1 - 1) / 16;
+      const int rt = t.j0 / 16 + wave * S::PJ + u, last = (t.j1 - 1) / 16;
       src[S::PI + u] = make_rsrc(p.a + (rt < last ? rt : last) * row_bytes);
     }
   };
@@ -421,39 +571,33 @@ __global__ __launch_bounds__(64 * S::W) void int8_product_kernel(ProductArgs p) 
   };
 
   struct Frags {
-    v4i a[2][FA], b[2][FB];
+    v4i a[FA], b[FB];
   };
   auto read = [&](int slot, Frags& f) {
-    // 32 rows x 32 deep: lane (row32, half) takes chunk 2 s + half of its row
-    const uint8_t* st = smem + slot * S::kSlot + (row32 >> 4) * 1024 + half * 256 + (row32 & 15) * 16;
+    const uint8_t* st = smem + slot * S::kSlot + lane * 16;   // a tile lies as its fragment is read
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
+    for (int y = 0; y < FB; ++y) f.b[y] = *reinterpret_cast<const v4i*>(st + S::TI * 64 + (wj * FB + y) * 1024);
 #pragma unroll
-      for (int x = 0; x < FA; ++x) f.a[s][x] = *reinterpret_cast<const v4i*>(st + (wi * FA + x) * 2048 + s * 512);
-#pragma unroll
-      for (int x = 0; x < FB; ++x) f.b[s][x] = *reinterpret_cast<const v4i*>(st + S::TI * 64 + (wj * FB + x) * 2048 + s * 512);
-    }
+    for (int x = 0; x < FA; ++x) f.a[x] = *reinterpret_cast<const v4i*>(st + (wi * FA + x) * 1024);
   };
-  v16i acc[FA][FB];
+  v4i acc[FA][FB];
   auto multiply = [&](const Frags& f) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int x = 0; x < FA; ++x)
 #pragma unroll
-      for (int x = 0; x < FA; ++x)
-#pragma unroll
-        for (int y = 0; y < FB; ++y)
-          acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.a[s][x], f.b[s][y], acc[x][y], 0, 0, 0);
+      for (int y = 0; y < FB; ++y) acc[x][y] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f.a[x], f.b[y], acc[x][y], 0, 0, 0);
   };
 
   // the tile that is issued runs up to four halves ahead of the one that is multiplied
-  OutTile cur, ahead;
+  OutTile cur;
   if (!tile_at(0, cur)) return;
-  int64_t ca = 0;
+  int ca = 0;
   int ka = 0;
-  ahead = cur;
-  aim(ahead);
+  aim(cur);
+  // a wave whose tokens lie behind the group's end only moves data: such a tile takes about half as long
+  bool active = cur.j0 + wj * FB * 16 < cur.j1;
   bool more = true;
-  auto issue_next = [&](int slot) {
+  auto advance = [&]() {
     if (ka == p.kt) {   // on to the next tile; behind the last one its last half again, which nothing reads
       OutTile t;
       more = more && tile_at(ca + 1, t);
@@ -465,119 +609,56 @@ __global__ __launch_bounds__(64 * S::W) void int8_product_kernel(ProductArgs p) 
         ka = p.kt - 1;
       }
     }
-    issue(slot, ka);
-    ++ka;
+  };
+  constexpr int kPer = S::PI + S::PJ;
+  // one half: the next one has landed (the two after it in flight; stores of the tile before,
+  // if any, only make this wait longer) and every wave has read the one in `now`, whose slot
+  // takes the half after those.  The reads of the next half go out under the first MFMAs: left
+  // to itself the compiler reads after them, and every half waits for LDS.
+  auto half_step = [&](int slot, const Frags& now, Frags& next) {
+    advance();
+    FM_WAIT_VMCNT(2 * kPer);
+    block_barrier();
+    issue(slot, ka++);
+    if (!active) return;
+    read((slot + 1) & 3, next);
+    multiply(now);
+#pragma unroll
+    for (int i = 0; i < FA + FB; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);   // one read of LDS
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // one MFMA
+    }
+    __builtin_amdgcn_sched_barrier(0);
   };
 #pragma unroll 1
-  for (int s = 0; s < 4; ++s) issue_next(s);
-  constexpr int kPer = S::PI + S::PJ;
+  for (int s = 0; s < 4; ++s) {
+    advance();
+    issue(s, ka);
+    ++ka;
+  }
   FM_WAIT_VMCNT(3 * kPer);
   block_barrier();
   Frags f0, f1;
   read(0, f0);
   int g = 0;   // slot of the half in f0 (0 or 2)
   uint8_t* stage = smem + 4 * S::kSlot + wave * 2048;
-  for (int64_t c = 0;; ++c) {
+  for (int c = 0;; ++c) {
 #pragma unroll
     for (int x = 0; x < FA; ++x)
 #pragma unroll
-      for (int y = 0; y < FB; ++y)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[x][y][i] = 0;
+      for (int y = 0; y < FB; ++y) acc[x][y] = v4i{0, 0, 0, 0};
 #pragma unroll 1
     for (int k = 0; k < p.kt; k += 2) {   // kt is even
-      // the next half has landed (the two after it in flight; stores of the tile before, if
-      // any, only make this wait longer) and every wave has read this one: its slot is free
-      FM_WAIT_VMCNT(2 * kPer);
-      block_barrier();
-      issue_next(g);
-      read(g + 1, f1);
-      multiply(f0);
-      __builtin_amdgcn_sched_barrier(0);
-      FM_WAIT_VMCNT(2 * kPer);
-      block_barrier();
-      issue_next(g + 1);
+      half_step(g, f0, f1);
+      half_step(g + 1, f1, f0);
       g ^= 2;
-      read(g, f0);
-      multiply(f1);
-      __builtin_amdgcn_sched_barrier(0);
     }
-    // block (x, y): lane holds token row32 of y, channels 8 r + 4 half + 0..3 of x
-    const int64_t iw = int64_t(cur.i) * rows_i + wi * (SWIGLU ? 16 * FA : 32 * FA);
-#pragma unroll
-    for (int y = 0; y < FB; ++y) {
-      const int64_t t0 = cur.j0 + (wj * FB + y) * 32, t = t0 + row32;
-      const bool tv = t < cur.j1;
-      const float sa = tv ? p.sa[t] : 0.f;
-      if constexpr (SWIGLU) {
-#pragma unroll
-        for (int x = 0; x < FA / 2; ++x)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int64_t n = iw + x * 32 + 8 * r + 4 * half;   // H is a multiple of 128: inside
-            const v4f s1 = *FM_GLOBAL(const v4f, p.sw + cur.e * p.sw_gs + n), s3 = *FM_GLOBAL(const v4f, p.sw2 + cur.e * p.sw_gs + n);
-            float h[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float gate = float(acc[x][y][4 * r + i]) * sa * s1[i], up = float(acc[x + FA / 2][y][4 * r + i]) * sa * s3[i];
-              h[i] = gate / (1.f + expf(-gate)) * up;
-            }
-            if (tv) st_global(static_cast<float*>(p.out) + t * p.ld_out + n, make_float4(h[0], h[1], h[2], h[3]));
-          }
-      } else {
-#pragma unroll
-        for (int x = 0; x < FA; ++x) {
-          const int64_t n0 = iw + x * 32;
-          float v[16];
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int64_t n = n0 + 8 * r + 4 * half + i;
-              const bool nv = n < p.N;
-              v[4 * r + i] = float(acc[x][y][4 * r + i]) * sa * (nv ? p.sw[cur.e * p.sw_gs + n] : 0.f);
-              if (p.bias) v[4 * r + i] += nv ? p.bias[n] : 0.f;
-            }
-          if (p.out_f32) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int64_t n = n0 + 8 * r + 4 * half;
-              float* o = static_cast<float*>(p.out) + t * p.ld_out + n;
-              if (!tv) continue;
-              if (n + 4 <= p.N) {
-                *FM_GLOBAL(u32x4_any, o) = fm_u32x4{f2u(v[4 * r]), f2u(v[4 * r + 1]), f2u(v[4 * r + 2]), f2u(v[4 * r + 3])};
-              } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  if (n + i < p.N) st_global(o + i, v[4 * r + i]);
-              }
-            }
-          } else {
-            // through LDS: 32 tokens x 64 bytes, 16-byte unit u of row t at u ^ (t / 2 % 4)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              *reinterpret_cast<fm_u32x2*>(stage + row32 * 64 + ((r ^ (row32 >> 1)) & 3) * 16 + half * 8) =
-                  fm_u32x2{hw_bf16x2(v[4 * r], v[4 * r + 1]), hw_bf16x2(v[4 * r + 2], v[4 * r + 3])};
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-              const int tr = b * 16 + (lane >> 2), u = lane & 3;
-              const fm_u32x4 o = *reinterpret_cast<const fm_u32x4*>(stage + tr * 64 + ((u ^ (tr >> 1)) & 3) * 16);
-              const int64_t n = n0 + 8 * u;
-              uint16_t* d = static_cast<uint16_t*>(p.out) + (t0 + tr) * p.ld_out + n;
-              if (t0 + tr >= cur.j1) continue;
-              if (n + 8 <= p.N) {
-                *FM_GLOBAL(u32x4_any, d) = o;
-              } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                  if (n + i < p.N) st_global(d + i, uint16_t(o[i / 2] >> (i % 2 * 16)));
-              }
-            }
-          }
-        }
-      }
-    }
+    if (active) store_tile<S, SWIGLU>(p, cur, acc, stage, wi, wj);
     if (!tile_at(c + 1, cur)) break;
+    active = cur.j0 + wj * FB * 16 < cur.j1;
+    // the next tile's first half, read again rather than kept in registers while the tile was
+    // stored; its slot is refilled after the next barrier
+    read(g, f0);
   }
   FM_WAIT_VMCNT(0);
 }
@@ -599,15 +680,27 @@ __global__ __launch_bounds__(256) void int8_combine_kernel(const float* y, int64
 
 template <bool F32>
 void launch_quant(const QuantArgs& a, int64_t row_tiles, hipStream_t s) {
-  const dim3 grid{unsigned(row_tiles)}, block(64 * kQuantWaves);
-  if (a.kt <= 2 * kQuantWaves) hipLaunchKernelGGL((int8_quant_kernel<F32, 2>), grid, block, 0, s, a);
-  else if (a.kt <= 4 * kQuantWaves) hipLaunchKernelGGL((int8_quant_kernel<F32, 4>), grid, block, 0, s, a);
-  else if (a.kt <= 8 * kQuantWaves) hipLaunchKernelGGL((int8_quant_kernel<F32, 8>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((int8_quant_kernel<F32, 0>), grid, block, 0, s, a);
+  const dim3 block(64 * kQuantWaves);
+  dim3 grid{unsigned(row_tiles)};
+  if (a.top) {
+    // columns shared until the workgroups fill the chip twice, eight tiles a wave at least
+    int64_t y = (4 * device_cus() + row_tiles - 1) / row_tiles;
+    const int64_t most = (a.kt + 8 * kQuantWaves - 1) / (8 * kQuantWaves);
+    grid.y = unsigned(y < most ? y : most);
+    hipLaunchKernelGGL((int8_quant_kernel<F32, 0, true>), grid, block, 0, s, a);
+  } else if (a.kt <= 2 * kQuantWaves) {
+    hipLaunchKernelGGL((int8_quant_kernel<F32, 2, false>), grid, block, 0, s, a);
+  } else if (a.kt <= 4 * kQuantWaves) {
+    hipLaunchKernelGGL((int8_quant_kernel<F32, 4, false>), grid, block, 0, s, a);
+  } else if (a.kt <= 8 * kQuantWaves) {
+    hipLaunchKernelGGL((int8_quant_kernel<F32, 8, false>), grid, block, 0, s, a);
+  } else {
+    hipLaunchKernelGGL((int8_quant_kernel<F32, 0, false>), grid, block, 0, s, a);
+  }
 }
 
-using Large = Shape<2, 4, 4, 2>;
-using Small = Shape<2, 2, 2, 1>;
+using Large = Shape<2, 4, 8, 4>;
+using Small = Shape<2, 2, 4, 2>;
 
 template <typename S, bool SWIGLU>
 void launch_product(const ProductArgs& p, int64_t token_tiles, hipStream_t s) {
@@ -632,14 +725,14 @@ using namespace fm;
 extern "C" {
 
 int fm_int8_quantize(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t ld_x, const int32_t* assign_of_row,
-                     int top_k, const int32_t* limit, void* q, float* s, void* stream) {
+                     int top_k, const int32_t* limit, const uint32_t* top, uint32_t* clear, void* q, float* s, void* stream) {
   FM_REQUIRE(x && q && s, "fm_int8_quantize: null pointer");
   FM_REQUIRE(x_dtype == FM_DTYPE_BF16 || x_dtype == FM_DTYPE_F32, "fm_int8_quantize: x must be bf16 or fp32");
   FM_REQUIRE(product_sizes_ok(rows, 1, cols) && ld_x >= cols, "fm_int8_quantize: needs 1 <= columns < 131072 and a pitch that covers them");
   FM_REQUIRE(!assign_of_row || top_k >= 1, "fm_int8_quantize: top_k must be positive");
   FM_REQUIRE(aligned16(q) && reinterpret_cast<uintptr_t>(x) % (x_dtype == FM_DTYPE_F32 ? 4 : 2) == 0, "fm_int8_quantize: misaligned buffer");
   if (rows == 0) return 0;
-  const QuantArgs a{x, ld_x, rows, cols, assign_of_row, top_k, limit, static_cast<uint8_t*>(q), s, int((cols + 127) / 128 * 2)};
+  const QuantArgs a{x, ld_x, rows, cols, assign_of_row, top_k, limit, top, clear, static_cast<uint8_t*>(q), s, int((cols + 127) / 128 * 2)};
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (x_dtype == FM_DTYPE_F32) launch_quant<true>(a, (rows + 15) / 16, st);
   else launch_quant<false>(a, (rows + 15) / 16, st);
@@ -683,7 +776,7 @@ int fm_int8_matmul(const void* a, const float* sa, int64_t M, const void* w, con
   FM_REQUIRE((out_dtype == FM_DTYPE_BF16 || out_dtype == FM_DTYPE_F32) && ld_out >= N, "fm_int8_matmul: bad output type or pitch");
   if (M == 0) return 0;
   const ProductArgs p{static_cast<const uint8_t*>(a), static_cast<const uint8_t*>(w), nullptr, sa, sw, nullptr, 0, 0,
-                      int((K + 127) / 128 * 2), M, N, nullptr, 1, bias, out, ld_out, int(out_dtype == FM_DTYPE_F32)};
+                      int((K + 127) / 128 * 2), M, N, nullptr, 1, bias, out, ld_out, int(out_dtype == FM_DTYPE_F32), nullptr};
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (M <= 64) {
     const dim3 grid{unsigned((N + 15) / 16)}, block(256);
@@ -700,17 +793,17 @@ int fm_int8_matmul(const void* a, const float* sa, int64_t M, const void* w, con
 }
 
 int fm_int8_grouped_gemm(const void* a, const float* sa, int64_t rows, const int32_t* offsets, int E, const void* w, const float* sw,
-                         const void* w_up, const float* sw_up, int64_t N, int64_t K, int64_t tokens, void* out, int out_dtype,
+                         const void* w_up, const float* sw_up, uint32_t* top, int64_t N, int64_t K, int64_t tokens, void* out, int out_dtype,
                          int64_t ld_out, void* stream) {
   FM_REQUIRE(a && sa && offsets && w && sw && out && aligned16(a) && aligned16(w) && aligned16(w_up), "fm_int8_grouped_gemm: null or misaligned pointer");
   FM_REQUIRE(E >= 1 && E <= kProductExperts && rows >= 0 && rows % 128 == 0 && product_sizes_ok(rows, N, K) && K % 128 == 0 && N % 16 == 0,
              "fm_int8_grouped_gemm: needs rows and K multiples of 128, N of 16, and at most 1024 experts");
-  FM_REQUIRE((w_up == nullptr) == (sw_up == nullptr) && (!w_up || (N % 128 == 0 && out_dtype == FM_DTYPE_F32 && ld_out % 4 == 0 && aligned16(out) && aligned16(sw) && aligned16(sw_up))),
-             "fm_int8_grouped_gemm: SwiGLU needs N a multiple of 128 and an aligned fp32 output");
+  FM_REQUIRE((w_up == nullptr) == (sw_up == nullptr) && (w_up == nullptr) == (top == nullptr) && (!w_up || (N % 128 == 0 && out_dtype == FM_DTYPE_F32 && ld_out % 4 == 0 && aligned16(out) && aligned16(sw) && aligned16(sw_up))),
+             "fm_int8_grouped_gemm: SwiGLU needs the row maxima, N a multiple of 128 and an aligned fp32 output");
   FM_REQUIRE((out_dtype == FM_DTYPE_BF16 || out_dtype == FM_DTYPE_F32) && ld_out >= N, "fm_int8_grouped_gemm: bad output type or pitch");
   if (rows == 0) return 0;
   const ProductArgs p{static_cast<const uint8_t*>(a), static_cast<const uint8_t*>(w), static_cast<const uint8_t*>(w_up), sa, sw, sw_up, N * K, N,
-                      int(K / 64), rows, N, offsets, E, nullptr, out, ld_out, int(out_dtype == FM_DTYPE_F32)};
+                      int(K / 64), rows, N, offsets, E, nullptr, out, ld_out, int(out_dtype == FM_DTYPE_F32), top};
   hipStream_t st = static_cast<hipStream_t>(stream);
   // about how many token tiles the groups give: their rows, and a partly filled tile each
   const int64_t all = rows / 128 + E, groups = tokens < E ? tokens : E;

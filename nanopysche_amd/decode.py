@@ -46,8 +46,9 @@ def _no_gradients(*tensors) -> None:
 
 
 def _same_device(x: torch.Tensor, **tensors) -> None:
+    index = x.get_device()
     for name, t in tensors.items():
-        if t is not None and t.device != x.device:
+        if t is not None and t.get_device() != index:
             raise ValueError(f"{name} is on {t.device}, x on {x.device}")
 
 
@@ -75,62 +76,59 @@ def _pitch(x: torch.Tensor) -> int:
     return x.stride(0) if x.shape[0] > 1 else x.shape[1]   # a single row's stride says nothing
 
 
-def _weights_struct(experts, num_experts: int, x: torch.Tensor, what: str):
-    """(FmDecodeWeights, the tensors it points to) of (w1, w2, w3) or Int8Experts."""
+def _weights_struct(experts, num_experts: int, x: torch.Tensor, what: str) -> _lib.FmDecodeWeights:
+    """The kernels' view of (w1, w2, w3) or Int8Experts (the caller keeps the tensors)."""
     from .int8 import Int8Experts
 
     D = x.shape[1]
-    w = _lib.FmDecodeWeights()
     if isinstance(experts, Int8Experts):
         if experts.num_experts != num_experts or experts.d_model != D:
             raise ValueError(f"{what}: int8 weights of {experts.num_experts} experts of width {experts.d_model}, "
                              f"expected {num_experts} of width {D}")
         _same_device(x, **{what: experts.w1.data})
-        w.kind, w.H = _lib.DECODE_INT8, experts.hidden_size
-        keep = (experts.w1.data, experts.w2.data, experts.w3.data, experts.w1.scale, experts.w2.scale, experts.w3.scale)
-        w.w1, w.w2, w.w3, w.s1, w.s2, w.s3 = (t.data_ptr() for t in keep)
-        return w, keep
+        w1, w2, w3 = experts.w1, experts.w2, experts.w3
+        return _lib.FmDecodeWeights(_lib.DECODE_INT8, experts.hidden_size, w1.data.data_ptr(), w2.data.data_ptr(),
+                                    w3.data.data_ptr(), w1.scale.data_ptr(), w2.scale.data_ptr(), w3.scale.data_ptr())
     try:
         w1, w2, w3 = experts
     except (TypeError, ValueError):
         raise TypeError(f"{what} must be (w1, w2, w3) or Int8Experts") from None
     _no_gradients(w1, w2, w3)
-    keep = []
-    for t in (w1, w2, w3):
-        if t.dim() != 2 or t.shape != w1.shape or t.shape[1] != D or t.shape[0] % num_experts:
-            raise ValueError(f"{what}: w1, w2, w3 must be [E * H, D] with E = {num_experts} and D = {D}, got {tuple(t.shape)}")
+    shape = w1.shape
+    if len(shape) != 2 or shape[1] != D or w2.shape != shape or w3.shape != shape or shape[0] % num_experts:
+        raise ValueError(f"{what}: w1, w2, w3 must be [E * H, D] with E = {num_experts} and D = {D}, got {tuple(shape)}, "
+                         f"{tuple(w2.shape)}, {tuple(w3.shape)}")
+    H = shape[0] // num_experts
+    if H % 128 or not H:
+        raise ValueError(f"{what}: hidden size must be a multiple of 128, got {H}")
+    for t in experts:
         if t.dtype != torch.bfloat16:
             raise TypeError(f"{what}: weights must be bfloat16 (or Int8Experts), got {t.dtype}")
-        _same_device(x, **{what: t})
         if not t.is_contiguous() or t.data_ptr() % 16:
             raise ValueError(f"{what}: weights must be contiguous, on 16-byte boundaries")
-        keep.append(t)
-    w.kind, w.H = _lib.DECODE_BF16, w1.shape[0] // num_experts
-    if w.H % 128 or not w.H:
-        raise ValueError(f"{what}: hidden size must be a multiple of 128, got {w.H}")
-    w.w1, w.w2, w.w3 = (t.data_ptr() for t in keep)
-    return w, keep
+    _same_device(x, w1=w1, w2=w2, w3=w3)
+    return _lib.FmDecodeWeights(_lib.DECODE_BF16, H, w1.data_ptr(), w2.data_ptr(), w3.data_ptr())
 
 
-def _run_experts(x, x_lo, weights, indices, experts, num_experts, offset, shared, out_dtype):
-    T, D = x.shape
-    K = indices.shape[1]
-    w, keep = _weights_struct(experts, num_experts, x, "experts")
-    ws, keep_s = (None, ()) if shared is None else _weights_struct(shared, 1, x, "shared")
+def _both(experts, num_experts, shared, x):
+    w = _weights_struct(experts, num_experts, x, "experts")
+    ws = None if shared is None else _weights_struct(shared, 1, x, "shared")
     if ws is not None and ws.kind != w.kind:
         raise ValueError("experts and shared must both be bf16 or both Int8Experts")
-    Hs = 0 if ws is None else ws.H
-    nbytes = _lib.size_of("fm_decode_workspace_bytes", T, D, K, num_experts, w.H, Hs, w.kind)
+    return w, ws
+
+
+def _workspace(size: str, x, K, num_experts, w, ws):
+    T, D = x.shape
+    nbytes = _lib.size_of(size, T, D, K, num_experts, w.H, 0 if ws is None else ws.H)
     if nbytes < 0:
-        raise ValueError(f"sizes outside the few-token kernels' range: {T} tokens, D {D}, hidden {w.H} / {Hs}, "
+        raise ValueError(f"sizes outside the few-token kernels' range: {T} tokens, D {D}, hidden {w.H}, "
                          f"{num_experts} experts, top {K}")
-    out = torch.empty(T, D, dtype=out_dtype, device=x.device)
-    work = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    _lib.call("fm_decode_experts", x.data_ptr(), _lib.addr(x_lo), _pitch(x), T, D, weights.data_ptr(), indices.data_ptr(),
-              int(indices.dtype == torch.int64), K, int(offset), num_experts, w, ws, out.data_ptr(),
-              _lib.DTYPE_F32 if out_dtype == torch.float32 else _lib.DTYPE_BF16, D, work.data_ptr(), nbytes,
-              _lib.stream_of(x))
-    return out
+    return torch.empty(nbytes, dtype=torch.uint8, device=x.device), nbytes
+
+
+def _dtype_code(dtype: torch.dtype) -> int:
+    return _lib.DTYPE_F32 if dtype == torch.float32 else _lib.DTYPE_BF16
 
 
 def _check_routing(T: int, num_experts: int, top_k: int) -> None:
@@ -166,8 +164,13 @@ def expert_decode(x: torch.Tensor, weights: torch.Tensor, indices: torch.Tensor,
     if T == 0:
         return torch.empty_like(x)
     with _lib.on_device_of(x2):
-        out = _run_experts(x2, None, w, idx, experts, int(num_experts), expert_offset, shared, x.dtype)
-    return out.reshape(x.shape)
+        ww, ws = _both(experts, num_experts, shared, x2)
+        work, nbytes = _workspace("fm_decode_workspace_bytes", x2, K, num_experts, ww, ws)
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        _lib.call("fm_decode_experts", x2.data_ptr(), None, _pitch(x2), T, x2.shape[1], w.data_ptr(), idx.data_ptr(),
+                  int(idx.dtype == torch.int64), K, int(expert_offset), num_experts, ww, ws, out.data_ptr(),
+                  _dtype_code(x.dtype), x2.shape[1], work.data_ptr(), nbytes, _lib.stream_of(x2))
+    return out
 
 
 def _gate_rows(gate: torch.Tensor) -> torch.Tensor:
@@ -224,19 +227,15 @@ def moe_decode(x: torch.Tensor, gate_weight: torch.Tensor, experts, top_k: int, 
     dev = x2.device
     weights = torch.empty(T, K, dtype=torch.float32, device=dev)
     indices = torch.empty(T, K, dtype=torch.int64, device=dev)
+    out = torch.empty(x.shape, dtype=x.dtype, device=dev)
     if T == 0:
-        return DecodeOutput(torch.empty_like(x), weights, indices)
+        return DecodeOutput(out, weights, indices)
     with _lib.on_device_of(x2):
-        logits = torch.empty(T, E, dtype=torch.float32, device=dev)
-        hi = lo = None
-        if norm is not None:
-            hi, lo = torch.empty(2, T, D, dtype=torch.bfloat16, device=dev).unbind(0)
+        w, ws = _both(experts, E, shared, x2)
+        work, nbytes = _workspace("fm_moe_decode_workspace_bytes", x2, K, E, w, ws)
         addr = _lib.addr
-        _lib.call("fm_decode_router", x2.data_ptr(), _pitch(x2), T, D, gate.data_ptr(), _code(gate), gate.stride(0),
-                  addr(bias), _code(bias), addr(score), addr(norm), _code(norm), float(norm_eps), E, K, gating_code,
-                  flags, logits.data_ptr(), addr(hi), addr(lo), weights.data_ptr(), indices.data_ptr(),
-                  _lib.stream_of(x2))
-        if hi is None:
-            hi = x2
-        out = _run_experts(hi, lo, weights, indices, experts, E, 0, shared, x.dtype)
-    return DecodeOutput(out.reshape(x.shape), weights, indices)
+        _lib.call("fm_moe_decode", x2.data_ptr(), _pitch(x2), T, D, gate.data_ptr(), _dtype_code(gate.dtype),
+                  gate.stride(0), addr(bias), _code(bias), addr(score), addr(norm), _code(norm), float(norm_eps), E, K,
+                  gating_code, flags, w, ws, weights.data_ptr(), indices.data_ptr(), out.data_ptr(),
+                  _dtype_code(x.dtype), D, work.data_ptr(), nbytes, _lib.stream_of(x2))
+    return DecodeOutput(out, weights, indices)

@@ -106,13 +106,14 @@ def _unpack(t: Int8Tensor, dtype: torch.dtype) -> torch.Tensor:
     return out
 
 
-def _quantize(x: torch.Tensor, rows: int, assign=None, top_k: int = 1, limit=None) -> Int8Tensor:
-    """Rows of x [R, K] (of the assignments' tokens, with ``assign``) up to ``limit``."""
+def _quantize(x: torch.Tensor, rows: int, assign=None, top_k: int = 1, limit=None, top=None, clear=None) -> Int8Tensor:
+    """Rows of x [R, K] (of the assignments' tokens, with ``assign``) up to ``limit``, by
+    their maxima ``top`` where they are known; sets ``clear`` to 0."""
     t = _empty(rows, x.shape[1], x.device)
     ld = x.stride(0) if x.shape[0] > 1 else x.shape[1]
     addr = _lib.addr
     _lib.call("fm_int8_quantize", x.data_ptr(), _lib.DTYPE_BF16 if x.dtype == torch.bfloat16 else _lib.DTYPE_F32, rows,
-              x.shape[1], ld, addr(assign), top_k, addr(limit), t.data.data_ptr(), t.scale.data_ptr(), _lib.stream_of(x))
+              x.shape[1], ld, addr(assign), top_k, addr(limit), addr(top), addr(clear), t.data.data_ptr(), t.scale.data_ptr(), _lib.stream_of(x))
     return t
 
 
@@ -188,14 +189,14 @@ def int8_grouped_gemm(tokens: Int8Tensor, weights: Int8Tensor, plan: RoutingPlan
         raise TypeError("out_dtype must be bfloat16 or float32")
     _same_device(tokens.data, weights=weights.data, plan=plan.offsets)
     with _lib.on_device_of(tokens.data):
-        return _grouped(tokens, weights, None, plan, weights.rows // E, out_dtype)
+        return _grouped(tokens, weights, None, None, plan, weights.rows // E, out_dtype)
 
 
-def _grouped(tokens, w, up, plan, N, out_dtype):
+def _grouped(tokens, w, up, top, plan, N, out_dtype):
     out = torch.empty(tokens.rows, N, dtype=out_dtype, device=tokens.device)
     _lib.call("fm_int8_grouped_gemm", tokens.data.data_ptr(), tokens.scale.data_ptr(), tokens.rows,
               plan.offsets.data_ptr(), plan.num_experts, w.data.data_ptr(), w.scale.data_ptr(),
-              None if up is None else up.data.data_ptr(), None if up is None else up.scale.data_ptr(), N, tokens.cols,
+              None if up is None else up.data.data_ptr(), None if up is None else up.scale.data_ptr(), _lib.addr(top), N, tokens.cols,
               plan.num_tokens * plan.top_k, out.data_ptr(),
               _lib.DTYPE_F32 if out_dtype == torch.float32 else _lib.DTYPE_BF16, N, _lib.stream_of(out))
     return out
@@ -287,9 +288,11 @@ class Int8MoECompute:
                 indices = indices - int(expert_offset)
             plan = route_tokens(indices.reshape(T, K), E)
             end = plan.offsets[E:]
-            q = _quantize(x2, plan.rows_max, plan.assign_of_row, K, end)
-            h = _grouped(q, w.w1, w.w3, plan, w.hidden_size, torch.float32)
-            y = _grouped(_quantize(h, plan.rows_max, limit=end), w.w2, None, plan, D, torch.float32)
+            top = torch.empty(plan.rows_max, dtype=torch.int32, device=x.device)   # largest |h| of every row, as bits
+            q = _quantize(x2, plan.rows_max, plan.assign_of_row, K, end, clear=top)
+            h = _grouped(q, w.w1, w.w3, top, plan, w.hidden_size, torch.float32)
+            q = _quantize(h, plan.rows_max, limit=end, top=top)
+            y = _grouped(q, w.w2, None, None, plan, D, torch.float32)
             rw = weights.reshape(T, K).to(torch.float32).contiguous()
             out = torch.empty(T, D, dtype=x.dtype, device=x.device)
             _lib.call("fm_int8_combine", y.data_ptr(), D, plan.row_of.data_ptr(), rw.data_ptr(), T, K, out.data_ptr(),
