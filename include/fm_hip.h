@@ -660,7 +660,9 @@ int fm_decode_experts(const void* x, const void* x_lo, int64_t ld_x, int64_t T, 
  *   known; clear (or NULL): words set to 0, one a row and 16 ceil(rows / 16) in all.
  * fm_int8_pack: int8 values with byte strides into tiles.  fm_int8_unpack: tiles into
  *   rows: q * s as bf16 (0) or fp32 (1), or q (2).
- * fm_int8_matmul: out [M, N] bf16 or fp32.
+ * fm_int8_matmul: out [M, N] bf16 or fp32.  fm_int8_linear: the same of x [M, K] (bf16 or
+ *   fp32), quantised as fm_int8_quantize does, through a workspace of
+ *   fm_int8_linear_workspace_bytes bytes (0 for a few rows).
  * fm_int8_grouped_gemm: rows [offsets[e], offsets[e + 1]) (multiples of 128) of the
  *   tokens times expert e's channels; `tokens` is the host's estimate of the rows that
  *   hold one (it only picks a kernel).  With w_up, out is silu(gate) * up in fp32 (N = H
@@ -680,6 +682,10 @@ int fm_int8_unpack(const void* q, const float* s, int64_t rows, int64_t cols, vo
                    void* stream);
 int fm_int8_matmul(const void* a, const float* sa, int64_t M, const void* w, const float* sw, int64_t N, int64_t K,
                    const float* bias, void* out, int out_dtype, int64_t ld_out, void* stream);
+int64_t fm_int8_linear_workspace_bytes(int64_t M, int64_t K);
+int fm_int8_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ld_x, const void* w, const float* sw, int64_t N,
+                   const float* bias, void* out, int out_dtype, int64_t ld_out, void* workspace, int64_t workspace_bytes,
+                   void* stream);
 int fm_int8_grouped_gemm(const void* a, const float* sa, int64_t rows, const int32_t* offsets, int E, const void* w,
                          const float* sw, const void* w_up, const float* sw_up, uint32_t* top, int64_t N, int64_t K,
                          int64_t tokens, void* out, int out_dtype, int64_t ld_out, void* stream);

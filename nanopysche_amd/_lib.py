@@ -167,6 +167,8 @@ SIGNATURES = {
     "fm_int8_pack": (_i32, [_vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp]),
     "fm_int8_unpack": (_i32, [_vp, _vp, _i64, _i64, _vp, _i32, _i64, _vp]),
     "fm_int8_matmul": (_i32, [_vp, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _i32, _i64, _vp]),
+    "fm_int8_linear_workspace_bytes": (_i64, [_i64, _i64]),
+    "fm_int8_linear": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _i32, _i64, _vp, _i64, _vp]),
     "fm_int8_grouped_gemm": (_i32, [_vp, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i32,
                                     _i64, _vp]),
     "fm_int8_combine": (_i32, [_vp, _i64, _vp, _vp, _i64, _i32, _vp, _i32, _vp]),

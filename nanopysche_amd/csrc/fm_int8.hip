@@ -27,6 +27,7 @@ constexpr int kMaxK = 131072;   // K below this: 127 * 127 K (and 128 * 128 K - 
 
 // 16 bytes at any address of the element's alignment
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
 
 // ---------------------------------------------------------------- quantise ----
 struct QuantArgs {
@@ -247,6 +248,17 @@ __global__ __launch_bounds__(256) void int8_unpack_kernel(const uint8_t* q, cons
   }
 }
 
+// 4 scales or biases of channels from n on (n a multiple of 4), zeros from N on.
+__device__ __forceinline__ v4f four_of(const float* p, int64_t n, int64_t N) {
+  typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
+  if (n + 4 <= N) return *FM_GLOBAL(const v4f_any, p + n);
+  v4f v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 3; ++i)
+    if (n + i < N) v[i] = *FM_GLOBAL(const float, p + n + i);
+  return v;
+}
+
 // ------------------------------------------------------------ few tokens ----
 // out[t, n] for at most 64 tokens: bound by reading the weights once.  A workgroup owns
 // 16 channels; its 4 waves take a quarter of K each, tiles straight from memory into
@@ -267,15 +279,64 @@ struct ProductArgs {
   uint32_t* top;               // SwiGLU: the rows' largest |h| as bits, raised by every wave
 };
 
-template <int TF>
-__global__ __launch_bounds__(256) void int8_few_kernel(ProductArgs p) {
+// QUANT 1 (bf16) or 2 (fp32): the tokens (at most kFusedRows) come as floats and every
+// workgroup quantises them into LDS while its first weights are on their way: a launch and
+// a round trip through memory fewer, for 2 or 4 M K bytes more from the caches a workgroup.
+constexpr int kFusedRows = 4, kFusedBytes = 32 * 1024;
+struct FusedRows {
+  const void* x;
+  int64_t ld, K;
+};
+
+template <bool F32>
+__device__ __forceinline__ void quantise_rows(const FusedRows& x, int M, int kt, uint8_t* q, float* scale, uint32_t (*tops)[kFusedRows]) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, chunks = kt * 4;
+  for (int r = 0; r < M; ++r) {
+    const void* row = static_cast<const uint8_t*>(x.x) + r * x.ld * (F32 ? 4 : 2);
+    uint32_t top = 0;
+    for (int c = tid; c < chunks; c += 256) {
+      Raw<F32> v;
+      v.load(row, int64_t(c) * 16, x.K);
+      top = v.top(top);
+    }
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const uint32_t o = __shfl_xor(top, off);
+      top = o > top ? o : top;
+    }
+    if (lane == 0) tops[wave][r] = top;
+  }
+  __syncthreads();
+  for (int r = 0; r < M; ++r) {
+    const void* row = static_cast<const uint8_t*>(x.x) + r * x.ld * (F32 ? 4 : 2);
+    uint32_t top = tops[0][r];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) top = tops[w][r] > top ? tops[w][r] : top;
+    const float s = int8_scale(top);
+    if (tid == 0) scale[r] = s;
+    const Recip d = recip_of(s);
+    for (int c = tid; c < chunks; c += 256) {
+      Raw<F32> v;
+      v.load(row, int64_t(c) * 16, x.K);
+      *reinterpret_cast<fm_u32x4*>(q + (r * chunks + c) * 16) = int8_round(v, d, top <= 0x7f7fffffu);
+    }
+  }
+  __syncthreads();
+}
+
+template <int TF, int QUANT>
+__global__ __launch_bounds__(256) void int8_few_kernel(ProductArgs p, FusedRows x) {
   __shared__ v4i red[3][TF][64];
+  __shared__ __attribute__((aligned(16))) uint8_t held[QUANT ? kFusedBytes : 16];
+  __shared__ float held_scale[kFusedRows];
+  __shared__ uint32_t tops[4][kFusedRows];
   const int lane = threadIdx.x & 63, m = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
   const int k0 = p.kt * wave / 4, k1 = p.kt * (wave + 1) / 4;
   constexpr int U = TF == 1 ? 8 : 4;
   const uint8_t* w = p.w + (int64_t(blockIdx.x) * p.kt * 64 + lane) * 16;
   const uint8_t* a = p.a + lane * 16;
+  const uint8_t* mine = held + ((m < p.M ? m : 0) * p.kt * 4 + q) * 16;
   v4i acc[TF];
 #pragma unroll
   for (int f = 0; f < TF; ++f) acc[f] = v4i{0, 0, 0, 0};
@@ -285,8 +346,9 @@ __global__ __launch_bounds__(256) void int8_few_kernel(ProductArgs p) {
     for (int u = 0; u < U; ++u) {
       const int64_t t = k + u < k1 ? k + u : k1 - 1;   // past the end: read again, not used
       wv[b][u] = *FM_GLOBAL(const v4i, w + t * 1024);
+      if constexpr (QUANT == 0)
 #pragma unroll
-      for (int f = 0; f < TF; ++f) av[b][u][f] = *FM_GLOBAL(const v4i, a + (int64_t(f) * p.kt + t) * 1024);
+        for (int f = 0; f < TF; ++f) av[b][u][f] = *FM_GLOBAL(const v4i, a + (int64_t(f) * p.kt + t) * 1024);
     }
   };
   auto use = [&](int b, int k) {
@@ -294,17 +356,21 @@ __global__ __launch_bounds__(256) void int8_few_kernel(ProductArgs p) {
     for (int u = 0; u < U; ++u) {
       if (k + u >= k1) break;
 #pragma unroll
-      for (int f = 0; f < TF; ++f) acc[f] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[b][u], av[b][u][f], acc[f], 0, 0, 0);
+      for (int f = 0; f < TF; ++f) {
+        v4i tok;
+        if constexpr (QUANT) tok = *reinterpret_cast<const v4i*>(mine + (k + u) * 64);
+        else tok = av[b][u][f];
+        acc[f] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[b][u], tok, acc[f], 0, 0, 0);
+      }
     }
   };
-  if (k0 < k1) {
-    load(0, k0);
-    for (int k = k0; k < k1; k += 2 * U) {
-      load(1, k + U);
-      use(0, k);
-      load(0, k + 2 * U);
-      use(1, k + U);
-    }
+  if (k0 < k1) load(0, k0), load(1, k0 + U);
+  if constexpr (QUANT) quantise_rows<QUANT == 2>(x, int(p.M), p.kt, held, held_scale, tops);
+  for (int k = k0; k < k1; k += 2 * U) {
+    use(0, k);
+    if (k + 2 * U < k1) load(0, k + 2 * U);
+    use(1, k + U);
+    if (k + 3 * U < k1) load(1, k + 3 * U);
   }
   if (wave)
 #pragma unroll
@@ -312,60 +378,52 @@ __global__ __launch_bounds__(256) void int8_few_kernel(ProductArgs p) {
   __syncthreads();
   if (wave) return;
   const int64_t n = int64_t(blockIdx.x) * 16 + 4 * q;
-  float sw[4], bias[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    sw[i] = n + i < p.N ? p.sw[n + i] : 0.f;
-    bias[i] = p.bias && n + i < p.N ? p.bias[n + i] : 0.f;
-  }
+  if (n >= p.N) return;
+  const v4f sw = four_of(p.sw, n, p.N), bias = p.bias ? four_of(p.bias, n, p.N) : v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int f = 0; f < TF; ++f) {
     const int64_t t = 16 * f + m;
     if (t >= p.M) break;
     const v4i s = acc[f] + red[0][f][lane] + red[1][f][lane] + red[2][f][lane];
-    const float sa = p.sa[t];
+    const float sa = QUANT ? held_scale[m] : p.sa[t];
+    v4f v;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 4; ++i) v[i] = float(s[i]) * sa * sw[i] + bias[i];
+    if (n + 4 <= p.N) {
+      if (p.out_f32) *FM_GLOBAL(u32x4_any, static_cast<float*>(p.out) + t * p.ld_out + n) = __builtin_bit_cast(fm_u32x4, v);
+      else *FM_GLOBAL(u32x2_any, static_cast<uint16_t*>(p.out) + t * p.ld_out + n) = fm_u32x2{hw_bf16x2(v[0], v[1]), hw_bf16x2(v[2], v[3])};
+      continue;
+    }
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
       if (n + i >= p.N) break;
-      const float v = float(s[i]) * sa * sw[i] + bias[i];
-      if (p.out_f32) st_global(static_cast<float*>(p.out) + t * p.ld_out + n + i, v);
-      else st_global(static_cast<uint16_t*>(p.out) + t * p.ld_out + n + i, uint16_t(hw_bf16x2(v, v)));
+      if (p.out_f32) st_global(static_cast<float*>(p.out) + t * p.ld_out + n + i, v[i]);
+      else st_global(static_cast<uint16_t*>(p.out) + t * p.ld_out + n + i, uint16_t(hw_bf16x2(v[i], v[i])));
     }
   }
 }
 
 // ------------------------------------------------------------- many tokens ----
 // out tile of TI channels x TJ tokens, WI x WJ waves of FA x FB 16x16x64 MFMA blocks; K runs in
-// halves of 64 through a ring of four LDS slots: while one half is multiplied from
-// registers the next is read from LDS and the two after it are on their way from memory.
+// halves of 64 through a ring of NS LDS slots: while one half is multiplied from
+// registers the next is read from LDS and the NS - 2 after it are on their way from memory.
 // Persistent: the ring runs on into the workgroup's next output tile, so its stores and
 // the next tile's first loads overlap.  SWIGLU: half of a wave's rows are gate rows, the
 // others the same hidden units' up rows, and h = silu(g) u leaves in fp32.
-template <int WI_, int WJ_, int FA_, int FB_>
+template <int WI_, int WJ_, int FA_, int FB_, int NS_>
 struct Shape {
-  static constexpr int WI = WI_, WJ = WJ_, FA = FA_, FB = FB_, W = WI * WJ;
+  static constexpr int WI = WI_, WJ = WJ_, FA = FA_, FB = FB_, W = WI * WJ, NS = NS_;   // NS: LDS slots
   static constexpr int TI = 16 * FA * WI, TJ = 16 * FB * WJ;
   static constexpr int PI = TI / 16 / W, PJ = TJ / 16 / W;   // tiles a wave moves per half
   static constexpr int kSlot = (TI + TJ) * 64;
   static constexpr int kStage = W * 2048;
-  static_assert(TI % (16 * W) == 0 && TJ % (16 * W) == 0, "whole pieces");
+  static_assert(TI % (16 * W) == 0 && TJ % (16 * W) == 0 && NS % 2 == 0, "whole pieces, pairs of halves");
 };
 constexpr int kProductExperts = 1024;
 
 struct OutTile {
   int e, i, j0, j1;   // expert, channel tile, rows [j0, j1)
 };
-
-// 4 scales or biases of channels from n on (n a multiple of 4), zeros from N on.
-__device__ __forceinline__ v4f four_of(const float* p, int64_t n, int64_t N) {
-  typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
-  if (n + 4 <= N) return *FM_GLOBAL(const v4f_any, p + n);
-  v4f v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < 3; ++i)
-    if (n + i < N) v[i] = *FM_GLOBAL(const float, p + n + i);
-  return v;
-}
 
 // A wave's blocks of an output tile: block (x, y) holds token lane % 16 of y, channels
 // 4 (lane / 16) + 0..3 of x.  bf16 rows go through the wave's 2 KiB of LDS, so that a
@@ -479,7 +537,7 @@ __device__ __forceinline__ void store_tile(const ProductArgs& p, const OutTile& 
 template <typename S, bool SWIGLU>
 __global__ __launch_bounds__(64 * S::W) void int8_product_kernel(ProductArgs p) {
   constexpr int FA = S::FA, FB = S::FB;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * S::kSlot + S::kStage];
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[S::NS * S::kSlot + S::kStage];
   __shared__ int first[kProductExperts + 1];   // token tiles before each expert
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -588,7 +646,7 @@ __global__ __launch_bounds__(64 * S::W) void int8_product_kernel(ProductArgs p) 
       for (int y = 0; y < FB; ++y) acc[x][y] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f.a[x], f.b[y], acc[x][y], 0, 0, 0);
   };
 
-  // the tile that is issued runs up to four halves ahead of the one that is multiplied
+  // the tile that is issued runs up to NS halves ahead of the one that is multiplied
   OutTile cur;
   if (!tile_at(0, cur)) return;
   int ca = 0;
@@ -611,17 +669,17 @@ __global__ __launch_bounds__(64 * S::W) void int8_product_kernel(ProductArgs p) 
     }
   };
   constexpr int kPer = S::PI + S::PJ;
-  // one half: the next one has landed (the two after it in flight; stores of the tile before,
+  // one half: the next one has landed (the others in flight; stores of the tile before,
   // if any, only make this wait longer) and every wave has read the one in `now`, whose slot
   // takes the half after those.  The reads of the next half go out under the first MFMAs: left
   // to itself the compiler reads after them, and every half waits for LDS.
   auto half_step = [&](int slot, const Frags& now, Frags& next) {
     advance();
-    FM_WAIT_VMCNT(2 * kPer);
+    FM_WAIT_VMCNT((S::NS - 2) * kPer);
     block_barrier();
     issue(slot, ka++);
     if (!active) return;
-    read((slot + 1) & 3, next);
+    read(slot + 1 == S::NS ? 0 : slot + 1, next);
     multiply(now);
 #pragma unroll
     for (int i = 0; i < FA + FB; ++i) {
@@ -631,17 +689,17 @@ __global__ __launch_bounds__(64 * S::W) void int8_product_kernel(ProductArgs p) 
     __builtin_amdgcn_sched_barrier(0);
   };
 #pragma unroll 1
-  for (int s = 0; s < 4; ++s) {
+  for (int s = 0; s < S::NS; ++s) {
     advance();
     issue(s, ka);
     ++ka;
   }
-  FM_WAIT_VMCNT(3 * kPer);
+  FM_WAIT_VMCNT((S::NS - 1) * kPer);
   block_barrier();
   Frags f0, f1;
   read(0, f0);
-  int g = 0;   // slot of the half in f0 (0 or 2)
-  uint8_t* stage = smem + 4 * S::kSlot + wave * 2048;
+  int g = 0;   // slot of the half in f0
+  uint8_t* stage = smem + S::NS * S::kSlot + wave * 2048;
   for (int c = 0;; ++c) {
 #pragma unroll
     for (int x = 0; x < FA; ++x)
@@ -651,7 +709,7 @@ __global__ __launch_bounds__(64 * S::W) void int8_product_kernel(ProductArgs p) 
     for (int k = 0; k < p.kt; k += 2) {   // kt is even
       half_step(g, f0, f1);
       half_step(g + 1, f1, f0);
-      g ^= 2;
+      g = g + 2 == S::NS ? 0 : g + 2;
     }
     if (active) store_tile<S, SWIGLU>(p, cur, acc, stage, wi, wj);
     if (!tile_at(c + 1, cur)) break;
@@ -699,8 +757,9 @@ void launch_quant(const QuantArgs& a, int64_t row_tiles, hipStream_t s) {
   }
 }
 
-using Large = Shape<2, 4, 8, 4>;
-using Small = Shape<2, 2, 4, 2>;
+using Large = Shape<2, 4, 8, 4, 4>;
+using Medium = Shape<2, 4, 8, 2, 4>;
+using Small = Shape<2, 2, 4, 2, 6>;
 
 template <typename S, bool SWIGLU>
 void launch_product(const ProductArgs& p, int64_t token_tiles, hipStream_t s) {
@@ -711,6 +770,35 @@ void launch_product(const ProductArgs& p, int64_t token_tiles, hipStream_t s) {
   grid = (grid + 7) / 8 * 8;   // a multiple of the XCDs
   hipLaunchKernelGGL((int8_product_kernel<S, SWIGLU>), dim3{unsigned(grid)}, dim3(64 * S::W), 0, s, p);
 }
+
+// The shape that is fastest by what a half costs on it and the rounds of output tiles that a
+// launch needs: 0.95 us for the 256 x 256 tile, 0.59 for 256 x 128, one workgroup a CU; 0.32
+// for 128 x 64 while it has a CU to itself, 0.5 when two share one.  Measured (us, the three
+// shapes, dense M x N x K): 77 x 2831 x 1409 17.6 / 15.3 / 9.2; 512 x 4096 x 14336 136 / 95 /
+// 52; 1024 x 4096 x 4096 47 / 31 / 31; 2048 x 4096 x 4096 50 / 36 / 56; 2048 x 5632 x 2048
+// 32 / 36 / 49; 8192 x 14336 x 4096 427 / 534 / 842.
+// tokens over `groups` groups (dense: one); rows: of the padded buffer, or 0.
+template <bool SWIGLU>
+void launch_shape(const ProductArgs& p, int64_t tokens, int64_t groups, int64_t rows, hipStream_t s) {
+  const int64_t cus = device_cus(), up = SWIGLU ? 2 : 1;
+  // output tiles, about: the tokens' and, over a plan, a partly filled one for every other group
+  auto tiles = [&](int64_t ti, int64_t tj) {
+    const int64_t j = rows ? tokens / tj + (groups + 1) / 2 : (tokens + tj - 1) / tj;
+    return j * ((p.N * up + ti - 1) / ti);
+  };
+  auto rounds = [](int64_t n, int64_t at_once) { return (n + at_once - 1) / at_once; };
+  const int64_t small = tiles(Small::TI, Small::TJ);
+  const int64_t large_us = 95 * rounds(tiles(Large::TI, Large::TJ), cus), medium_us = 59 * rounds(tiles(Medium::TI, Medium::TJ), cus);
+  const int64_t small_us = small <= cus ? 32 : 50 * rounds(small, 2 * cus);
+  // a bound of the token tiles: every group is a multiple of 128 rows
+  auto most = [&](int64_t tj) { return rows ? rows / 128 * (tj < 128 ? 128 / tj : 1) : (tokens + tj - 1) / tj; };
+  if (small_us <= medium_us && small_us <= large_us) launch_product<Small, SWIGLU>(p, most(Small::TJ), s);
+  else if (large_us <= medium_us * 108 / 100) launch_product<Large, SWIGLU>(p, most(Large::TJ), s);
+  else launch_product<Medium, SWIGLU>(p, most(Medium::TJ), s);
+}
+
+// Whether fm_int8_linear quantises in its product's kernel: rows that fit its LDS.
+bool fused_rows(int64_t M, int64_t K) { return M <= kFusedRows && M * ((K + 127) / 128 * 128) <= kFusedBytes; }
 
 bool product_sizes_ok(int64_t M, int64_t N, int64_t K) {
   return M >= 0 && M < (int64_t(1) << 31) - 256 && N >= 1 && N < (int64_t(1) << 31) - 256 && K >= 1 && K < kMaxK;
@@ -780,16 +868,46 @@ int fm_int8_matmul(const void* a, const float* sa, int64_t M, const void* w, con
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (M <= 64) {
     const dim3 grid{unsigned((N + 15) / 16)}, block(256);
-    if (M <= 16) hipLaunchKernelGGL(int8_few_kernel<1>, grid, block, 0, st, p);
-    else if (M <= 32) hipLaunchKernelGGL(int8_few_kernel<2>, grid, block, 0, st, p);
-    else if (M <= 48) hipLaunchKernelGGL(int8_few_kernel<3>, grid, block, 0, st, p);
-    else hipLaunchKernelGGL(int8_few_kernel<4>, grid, block, 0, st, p);
+    const FusedRows none{nullptr, 0, 0};
+    if (M <= 16) hipLaunchKernelGGL((int8_few_kernel<1, 0>), grid, block, 0, st, p, none);
+    else if (M <= 32) hipLaunchKernelGGL((int8_few_kernel<2, 0>), grid, block, 0, st, p, none);
+    else if (M <= 48) hipLaunchKernelGGL((int8_few_kernel<3, 0>), grid, block, 0, st, p, none);
+    else hipLaunchKernelGGL((int8_few_kernel<4, 0>), grid, block, 0, st, p, none);
   } else {
-    const int64_t large = (M + 255) / 256 * ((N + 255) / 256);
-    if (large >= device_cus() / 2) launch_product<Large, false>(p, (M + 255) / 256, st);
-    else launch_product<Small, false>(p, (M + 63) / 64, st);
+    launch_shape<false>(p, M, 1, 0, st);
   }
   return check_launch("fm_int8_matmul");
+}
+
+int64_t fm_int8_linear_workspace_bytes(int64_t M, int64_t K) {
+  if (!product_sizes_ok(M, 1, K)) return -1;
+  const int64_t tiles = (M + 15) / 16;
+  return fused_rows(M, K) ? 0 : tiles * ((K + 127) / 128) * 2048 + tiles * 64;
+}
+
+int fm_int8_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ld_x, const void* w, const float* sw, int64_t N,
+                   const float* bias, void* out, int out_dtype, int64_t ld_out, void* workspace, int64_t workspace_bytes, void* stream) {
+  FM_REQUIRE(x && w && sw && out && aligned16(w), "fm_int8_linear: null or misaligned pointer");
+  FM_REQUIRE(product_sizes_ok(M, N, K) && ld_x >= K, "fm_int8_linear: needs sizes of at least 1, K < 131072 and a pitch that covers a row");
+  FM_REQUIRE((x_dtype == FM_DTYPE_BF16 || x_dtype == FM_DTYPE_F32) && reinterpret_cast<uintptr_t>(x) % (x_dtype == FM_DTYPE_F32 ? 4 : 2) == 0,
+             "fm_int8_linear: x must be bf16 or fp32, aligned to its elements");
+  FM_REQUIRE((out_dtype == FM_DTYPE_BF16 || out_dtype == FM_DTYPE_F32) && ld_out >= N, "fm_int8_linear: bad output type or pitch");
+  if (M == 0) return 0;
+  if (fused_rows(M, K)) {
+    const ProductArgs p{nullptr, static_cast<const uint8_t*>(w), nullptr, nullptr, sw, nullptr, 0, 0, int((K + 127) / 128 * 2), M, N, nullptr, 1,
+                        bias, out, ld_out, int(out_dtype == FM_DTYPE_F32), nullptr};
+    const FusedRows r{x, ld_x, K};
+    const dim3 grid{unsigned((N + 15) / 16)}, block(256);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (x_dtype == FM_DTYPE_F32) hipLaunchKernelGGL((int8_few_kernel<1, 2>), grid, block, 0, st, p, r);
+    else hipLaunchKernelGGL((int8_few_kernel<1, 1>), grid, block, 0, st, p, r);
+    return check_launch("fm_int8_linear");
+  }
+  FM_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= fm_int8_linear_workspace_bytes(M, K),
+             "fm_int8_linear: the workspace must be fm_int8_linear_workspace_bytes bytes, 16-byte aligned");
+  float* s = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (M + 15) / 16 * ((K + 127) / 128) * 2048);
+  if (int rc = fm_int8_quantize(x, x_dtype, M, K, ld_x, nullptr, 1, nullptr, nullptr, nullptr, workspace, s, stream)) return rc;
+  return fm_int8_matmul(workspace, s, M, w, sw, N, K, bias, out, out_dtype, ld_out, stream);
 }
 
 int fm_int8_grouped_gemm(const void* a, const float* sa, int64_t rows, const int32_t* offsets, int E, const void* w, const float* sw,
@@ -805,17 +923,8 @@ int fm_int8_grouped_gemm(const void* a, const float* sa, int64_t rows, const int
   const ProductArgs p{static_cast<const uint8_t*>(a), static_cast<const uint8_t*>(w), static_cast<const uint8_t*>(w_up), sa, sw, sw_up, N * K, N,
                       int(K / 64), rows, N, offsets, E, nullptr, out, ld_out, int(out_dtype == FM_DTYPE_F32), top};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  // about how many token tiles the groups give: their rows, and a partly filled tile each
-  const int64_t all = rows / 128 + E, groups = tokens < E ? tokens : E;
-  const int64_t rows_i = w_up ? 128 : 256, large = (tokens / 256 + groups) * ((N + rows_i - 1) / rows_i);
-  const bool big = large >= device_cus() / 2 && tokens >= 128 * int64_t(E);
-  if (w_up) {
-    if (big) launch_product<Large, true>(p, all, st);
-    else launch_product<Small, true>(p, 2 * all, st);
-  } else {
-    if (big) launch_product<Large, false>(p, all, st);
-    else launch_product<Small, false>(p, 2 * all, st);
-  }
+  if (w_up) launch_shape<true>(p, tokens, tokens < E ? tokens : E, rows, st);
+  else launch_shape<false>(p, tokens, tokens < E ? tokens : E, rows, st);
   return check_launch("fm_int8_grouped_gemm");
 }
 

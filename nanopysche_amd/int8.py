@@ -140,6 +140,22 @@ def quantize_to_int8(x: torch.Tensor) -> Int8Tensor:
         return _quantize(x2, x2.shape[0])
 
 
+def _out_code(dtype: torch.dtype) -> int:
+    if dtype == torch.bfloat16:
+        return _lib.DTYPE_BF16
+    if dtype == torch.float32:
+        return _lib.DTYPE_F32
+    raise TypeError("out_dtype must be bfloat16 or float32")
+
+
+def _bias(bias: Optional[torch.Tensor], N: int) -> Optional[torch.Tensor]:
+    if bias is None:
+        return None
+    if tuple(bias.shape) != (N,):
+        raise ValueError(f"bias must be [{N}], got {tuple(bias.shape)}")
+    return bias.to(torch.float32).contiguous()
+
+
 def int8_matmul(a: Int8Tensor, b: Int8Tensor, bias: Optional[torch.Tensor] = None,
                 out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """a b^T with both operands' scales: tokens a [M, K] and channels b [N, K] ->
@@ -147,32 +163,43 @@ def int8_matmul(a: Int8Tensor, b: Int8Tensor, bias: Optional[torch.Tensor] = Non
     _lib.require_device(a.data, "a")
     if a.cols != b.cols:
         raise ValueError(f"a has {a.cols} columns, b {b.cols}")
-    if out_dtype not in (torch.bfloat16, torch.float32):
-        raise TypeError("out_dtype must be bfloat16 or float32")
+    code = _out_code(out_dtype)
+    _no_gradients(bias)
     _same_device(a.data, b=b.data, bias=bias)
     M, N = a.rows, b.rows
-    if bias is not None:
-        if tuple(bias.shape) != (N,):
-            raise ValueError(f"bias must be [{N}], got {tuple(bias.shape)}")
-        _no_gradients(bias)
-        bias = bias.to(torch.float32).contiguous()
+    bias = _bias(bias, N)
     out = torch.empty(M, N, dtype=out_dtype, device=a.device)
     if M and N:
         with _lib.on_device_of(out):
             _lib.call("fm_int8_matmul", a.data.data_ptr(), a.scale.data_ptr(), M, b.data.data_ptr(), b.scale.data_ptr(),
-                      N, a.cols, _lib.addr(bias), out.data_ptr(),
-                      _lib.DTYPE_F32 if out_dtype == torch.float32 else _lib.DTYPE_BF16, N, _lib.stream_of(out))
+                      N, a.cols, _lib.addr(bias), out.data_ptr(), code, N, _lib.stream_of(out))
     return out
 
 
 def int8_linear(x: torch.Tensor, weight: Int8Tensor, bias: Optional[torch.Tensor] = None,
                 out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """x [..., K] (bf16 or fp32), quantised by token, times int8 weights [N, K] ->
-    [..., N] in ``out_dtype`` (default x's)."""
+    [..., N] in ``out_dtype`` (default x's), plus bias [N]: ``int8_matmul`` of
+    ``quantize_to_int8(x)``, the same bits."""
     if x.dim() < 1 or x.shape[-1] != weight.cols:
         raise ValueError(f"x {tuple(x.shape)} does not end in the weight's {weight.cols} columns")
-    out = int8_matmul(quantize_to_int8(x), weight, bias, x.dtype if out_dtype is None else out_dtype)
-    return out.reshape(*x.shape[:-1], weight.rows)
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    code = _out_code(out_dtype)
+    x2 = _float_rows(x)
+    _no_gradients(x, bias)
+    _same_device(x, weight=weight.data, bias=bias)
+    M, K = x2.shape
+    N = weight.rows
+    bias = _bias(bias, N)
+    out = torch.empty(*x.shape[:-1], N, dtype=out_dtype, device=x.device)
+    if M and N:
+        with _lib.on_device_of(x2):
+            nbytes = _lib.size_of("fm_int8_linear_workspace_bytes", M, K)
+            work = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+            _lib.call("fm_int8_linear", x2.data_ptr(), _lib.DTYPE_BF16 if x2.dtype == torch.bfloat16 else _lib.DTYPE_F32, M,
+                      K, x2.stride(0) if M > 1 else K, weight.data.data_ptr(), weight.scale.data_ptr(), N, _lib.addr(bias),
+                      out.data_ptr(), code, N, _lib.addr(work), nbytes, _lib.stream_of(x2))
+    return out
 
 
 def int8_grouped_gemm(tokens: Int8Tensor, weights: Int8Tensor, plan: RoutingPlan,
@@ -185,8 +212,7 @@ def int8_grouped_gemm(tokens: Int8Tensor, weights: Int8Tensor, plan: RoutingPlan
     if tokens.rows != plan.rows_max or tokens.cols != weights.cols or weights.rows % E:
         raise ValueError(f"tokens [{tokens.rows}, {tokens.cols}] and weights [{weights.rows}, {weights.cols}] do not fit "
                          f"a plan of {plan.rows_max} rows and {E} experts")
-    if out_dtype not in (torch.bfloat16, torch.float32):
-        raise TypeError("out_dtype must be bfloat16 or float32")
+    _out_code(out_dtype)
     _same_device(tokens.data, weights=weights.data, plan=plan.offsets)
     with _lib.on_device_of(tokens.data):
         return _grouped(tokens, weights, None, None, plan, weights.rows // E, out_dtype)

@@ -102,6 +102,21 @@ def test_matmul_matches_exact_sums(dev, M, N, K):
     check_product(fm.int8_matmul(a, w, bias), qa, sa, qw, sw, bias)
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 40, 129), (1, 17, 20000), (2, 33, 4096), (4, 64, 8192), (4, 20, 8193), (5, 20, 300), (90, 70, 300)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_linear_is_quantise_and_matmul(dev, M, N, K, dtype):
+    """A few rows are quantised inside the product: the same bits."""
+    x = torch.randn(M + 1, K + 3, generator=torch.Generator().manual_seed(1)).to(dtype).to(dev)[1:, 1:K + 1]
+    if M > 1:
+        x[1] = 0
+    w = fm.quantize_to_int8(torch.randn(N, K, generator=torch.Generator().manual_seed(2)).to(dev))
+    bias = torch.randn(N, generator=torch.Generator().manual_seed(3)).to(dev)
+    for b in (None, bias):
+        for out in (torch.float32, torch.bfloat16):
+            got = fm.int8_linear(x, w, b, out_dtype=out)
+            assert torch.equal(got, fm.int8_matmul(fm.quantize_to_int8(x), w, b, out_dtype=out))
+
+
 @pytest.mark.parametrize("M", [5, 200])
 def test_longest_sum_does_not_overflow(dev, M):
     q = torch.full((M, MAX_INT8_K), -128, dtype=torch.int8, device=dev)
