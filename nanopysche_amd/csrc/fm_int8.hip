@@ -405,19 +405,20 @@ __global__ __launch_bounds__(256) void int8_few_kernel(ProductArgs p, FusedRows 
 
 // ------------------------------------------------------------- many tokens ----
 // out tile of TI channels x TJ tokens, WI x WJ waves of FA x FB 16x16x64 MFMA blocks; K runs in
-// halves of 64 through a ring of NS LDS slots: while one half is multiplied from
+// steps of 64 KS through a ring of NS LDS slots: while one step is multiplied from
 // registers the next is read from LDS and the NS - 2 after it are on their way from memory.
 // Persistent: the ring runs on into the workgroup's next output tile, so its stores and
 // the next tile's first loads overlap.  SWIGLU: half of a wave's rows are gate rows, the
 // others the same hidden units' up rows, and h = silu(g) u leaves in fp32.
-template <int WI_, int WJ_, int FA_, int FB_, int NS_>
+template <int WI_, int WJ_, int FA_, int FB_, int KS_, int NS_>
 struct Shape {
-  static constexpr int WI = WI_, WJ = WJ_, FA = FA_, FB = FB_, W = WI * WJ, NS = NS_;   // NS: LDS slots
+  static constexpr int WI = WI_, WJ = WJ_, FA = FA_, FB = FB_, W = WI * WJ;
+  static constexpr int KS = KS_, NS = NS_;   // 64s of K in a step; slots of the ring
   static constexpr int TI = 16 * FA * WI, TJ = 16 * FB * WJ;
-  static constexpr int PI = TI / 16 / W, PJ = TJ / 16 / W;   // tiles a wave moves per half
-  static constexpr int kSlot = (TI + TJ) * 64;
+  static constexpr int PI = TI / 16 / W, PJ = TJ / 16 / W;   // row tiles that a wave moves
+  static constexpr int kSlot = (TI + TJ) * 64 * KS;
   static constexpr int kStage = W * 2048;
-  static_assert(TI % (16 * W) == 0 && TJ % (16 * W) == 0 && NS % 2 == 0, "whole pieces, pairs of halves");
+  static_assert(TI % (16 * W) == 0 && TJ % (16 * W) == 0 && (KS == 1 || KS == 2), "whole pieces; K is a multiple of 128");
 };
 constexpr int kProductExperts = 1024;
 
@@ -619,44 +620,51 @@ __global__ __launch_bounds__(64 * S::W) void int8_product_kernel(ProductArgs p) 
     }
   };
   const uint32_t ring = lds_addr(smem);
-  auto issue = [&](int slot, int k) {
+  auto issue = [&](int slot, int k) {   // step k: tiles KS k .. of each row tile
 #pragma unroll
-    for (int u = 0; u < S::PI; ++u)
-      bdma16(src[u], lane * 16, uint32_t(k) * 1024, ring + slot * S::kSlot + (wave * S::PI + u) * 1024);
+    for (int u = 0; u < S::PI + S::PJ; ++u) {
+      const int row = u < S::PI ? wave * S::PI + u : S::TI / 16 + wave * S::PJ + u - S::PI;
 #pragma unroll
-    for (int u = 0; u < S::PJ; ++u)
-      bdma16(src[S::PI + u], lane * 16, uint32_t(k) * 1024, ring + slot * S::kSlot + S::TI * 64 + (wave * S::PJ + u) * 1024);
+      for (int i = 0; i < S::KS; ++i)
+        bdma16(src[u], lane * 16, uint32_t(k * S::KS + i) * 1024, ring + slot * S::kSlot + (row * S::KS + i) * 1024);
+    }
   };
 
   struct Frags {
-    v4i a[FA], b[FB];
+    v4i a[S::KS][FA], b[S::KS][FB];
   };
   auto read = [&](int slot, Frags& f) {
     const uint8_t* st = smem + slot * S::kSlot + lane * 16;   // a tile lies as its fragment is read
 #pragma unroll
-    for (int y = 0; y < FB; ++y) f.b[y] = *reinterpret_cast<const v4i*>(st + S::TI * 64 + (wj * FB + y) * 1024);
+    for (int k = 0; k < S::KS; ++k) {
 #pragma unroll
-    for (int x = 0; x < FA; ++x) f.a[x] = *reinterpret_cast<const v4i*>(st + (wi * FA + x) * 1024);
+      for (int y = 0; y < FB; ++y) f.b[k][y] = *reinterpret_cast<const v4i*>(st + (S::TI / 16 + wj * FB + y) * S::KS * 1024 + k * 1024);
+#pragma unroll
+      for (int x = 0; x < FA; ++x) f.a[k][x] = *reinterpret_cast<const v4i*>(st + (wi * FA + x) * S::KS * 1024 + k * 1024);
+    }
   };
   v4i acc[FA][FB];
   auto multiply = [&](const Frags& f) {
 #pragma unroll
-    for (int x = 0; x < FA; ++x)
+    for (int k = 0; k < S::KS; ++k)
 #pragma unroll
-      for (int y = 0; y < FB; ++y) acc[x][y] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f.a[x], f.b[y], acc[x][y], 0, 0, 0);
+      for (int x = 0; x < FA; ++x)
+#pragma unroll
+        for (int y = 0; y < FB; ++y) acc[x][y] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f.a[k][x], f.b[k][y], acc[x][y], 0, 0, 0);
   };
 
-  // the tile that is issued runs up to NS halves ahead of the one that is multiplied
+  // the tile that is issued runs up to NS steps ahead of the one that is multiplied
   OutTile cur;
   if (!tile_at(0, cur)) return;
   int ca = 0;
   int ka = 0;
+  const int steps = p.kt / S::KS;
   aim(cur);
   // a wave whose tokens lie behind the group's end only moves data: such a tile takes about half as long
   bool active = cur.j0 + wj * FB * 16 < cur.j1;
   bool more = true;
   auto advance = [&]() {
-    if (ka == p.kt) {   // on to the next tile; behind the last one its last half again, which nothing reads
+    if (ka == steps) {   // on to the next tile; behind the last one its last step again, which nothing reads
       OutTile t;
       more = more && tile_at(ca + 1, t);
       if (more) {
@@ -664,16 +672,16 @@ __global__ __launch_bounds__(64 * S::W) void int8_product_kernel(ProductArgs p) 
         ka = 0;
         aim(t);
       } else {
-        ka = p.kt - 1;
+        ka = steps - 1;
       }
     }
   };
-  constexpr int kPer = S::PI + S::PJ;
-  // one half: the next one has landed (the others in flight; stores of the tile before,
+  constexpr int kPer = (S::PI + S::PJ) * S::KS;
+  // one step: the next one has landed (the others in flight; stores of the tile before,
   // if any, only make this wait longer) and every wave has read the one in `now`, whose slot
-  // takes the half after those.  The reads of the next half go out under the first MFMAs: left
-  // to itself the compiler reads after them, and every half waits for LDS.
-  auto half_step = [&](int slot, const Frags& now, Frags& next) {
+  // takes the step after those.  The reads of the next step go out under the first MFMAs: left
+  // to itself the compiler reads after them, and every step waits for LDS.
+  auto one_step = [&](int slot, const Frags& now, Frags& next) {
     advance();
     FM_WAIT_VMCNT((S::NS - 2) * kPer);
     block_barrier();
@@ -682,7 +690,7 @@ __global__ __launch_bounds__(64 * S::W) void int8_product_kernel(ProductArgs p) 
     read(slot + 1 == S::NS ? 0 : slot + 1, next);
     multiply(now);
 #pragma unroll
-    for (int i = 0; i < FA + FB; ++i) {
+    for (int i = 0; i < (FA + FB) * S::KS; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);   // one read of LDS
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // one MFMA
     }
@@ -698,23 +706,27 @@ __global__ __launch_bounds__(64 * S::W) void int8_product_kernel(ProductArgs p) 
   block_barrier();
   Frags f0, f1;
   read(0, f0);
-  int g = 0;   // slot of the half in f0
+  int g = 0;   // slot of the step in f0
   uint8_t* stage = smem + S::NS * S::kSlot + wave * 2048;
   for (int c = 0;; ++c) {
 #pragma unroll
     for (int x = 0; x < FA; ++x)
 #pragma unroll
       for (int y = 0; y < FB; ++y) acc[x][y] = v4i{0, 0, 0, 0};
+    auto after = [](int slot) { return slot + 1 == S::NS ? 0 : slot + 1; };
 #pragma unroll 1
-    for (int k = 0; k < p.kt; k += 2) {   // kt is even
-      half_step(g, f0, f1);
-      half_step(g + 1, f1, f0);
-      g = g + 2 == S::NS ? 0 : g + 2;
+    for (int k = 0;;) {
+      one_step(g, f0, f1);
+      g = after(g);
+      if (++k == steps) break;
+      one_step(g, f1, f0);
+      g = after(g);
+      if (++k == steps) break;
     }
     if (active) store_tile<S, SWIGLU>(p, cur, acc, stage, wi, wj);
     if (!tile_at(c + 1, cur)) break;
     active = cur.j0 + wj * FB * 16 < cur.j1;
-    // the next tile's first half, read again rather than kept in registers while the tile was
+    // the next tile's first step, read now rather than kept in registers while the tile was
     // stored; its slot is refilled after the next barrier
     read(g, f0);
   }
@@ -757,9 +769,9 @@ void launch_quant(const QuantArgs& a, int64_t row_tiles, hipStream_t s) {
   }
 }
 
-using Large = Shape<2, 4, 8, 4, 4>;
-using Medium = Shape<2, 4, 8, 2, 4>;
-using Small = Shape<2, 2, 4, 2, 6>;
+using Large = Shape<2, 4, 8, 4, 1, 4>;
+using Medium = Shape<2, 4, 8, 2, 1, 4>;
+using Small = Shape<2, 2, 4, 2, 1, 5>;   // two workgroups to a CU
 
 template <typename S, bool SWIGLU>
 void launch_product(const ProductArgs& p, int64_t token_tiles, hipStream_t s) {
@@ -773,10 +785,10 @@ void launch_product(const ProductArgs& p, int64_t token_tiles, hipStream_t s) {
 
 // The shape that is fastest by what a half costs on it and the rounds of output tiles that a
 // launch needs: 0.95 us for the 256 x 256 tile, 0.59 for 256 x 128, one workgroup a CU; 0.32
-// for 128 x 64 while it has a CU to itself, 0.5 when two share one.  Measured (us, the three
-// shapes, dense M x N x K): 77 x 2831 x 1409 17.6 / 15.3 / 9.2; 512 x 4096 x 14336 136 / 95 /
-// 52; 1024 x 4096 x 4096 47 / 31 / 31; 2048 x 4096 x 4096 50 / 36 / 56; 2048 x 5632 x 2048
-// 32 / 36 / 49; 8192 x 14336 x 4096 427 / 534 / 842.
+// for 128 x 64 while it has a CU to itself, 0.42 when two share one.  Measured (us, the three
+// shapes, dense M x N x K): 77 x 2831 x 1409 17.6 / 15.3 / 9.7; 512 x 5632 x 2048 28 / 19 / 15;
+// 512 x 4096 x 14336 136 / 95 / 57; 1024 x 4096 x 4096 47 / 31 / 25; 2048 x 4096 x 4096 50 /
+// 36 / 56; 2048 x 5632 x 2048 32 / 36 / 49; 8192 x 14336 x 4096 427 / 534 / 842.
 // tokens over `groups` groups (dense: one); rows: of the padded buffer, or 0.
 template <bool SWIGLU>
 void launch_shape(const ProductArgs& p, int64_t tokens, int64_t groups, int64_t rows, hipStream_t s) {
@@ -789,7 +801,7 @@ void launch_shape(const ProductArgs& p, int64_t tokens, int64_t groups, int64_t 
   auto rounds = [](int64_t n, int64_t at_once) { return (n + at_once - 1) / at_once; };
   const int64_t small = tiles(Small::TI, Small::TJ);
   const int64_t large_us = 95 * rounds(tiles(Large::TI, Large::TJ), cus), medium_us = 59 * rounds(tiles(Medium::TI, Medium::TJ), cus);
-  const int64_t small_us = small <= cus ? 32 : 50 * rounds(small, 2 * cus);
+  const int64_t small_us = small <= cus ? 32 : 42 * rounds(small, 2 * cus);
   // a bound of the token tiles: every group is a multiple of 128 rows
   auto most = [&](int64_t tj) { return rows ? rows / 128 * (tj < 128 ? 128 / tj : 1) : (tokens + tj - 1) / tj; };
   if (small_us <= medium_us && small_us <= large_us) launch_product<Small, SWIGLU>(p, most(Small::TJ), s);
