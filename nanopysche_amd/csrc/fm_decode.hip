@@ -46,7 +46,7 @@ constexpr int kDecodeExperts = 1024; // most experts
 constexpr int kDecodeDim = 14336;    // widest token 
 
 // ------------------------------------------------------------------ router ----
-constexpr int64_t kRouterOne = 256 * 1024;   // elements of a gate that one workgroup reads for a token
+constexpr int64_t kRouterOne = 64 * 1024;   // elements of a gate that one workgroup reads for a token
 
 struct RouterArgs {
   const uint16_t* x;
@@ -177,7 +177,8 @@ __device__ __forceinline__ void gate_token(const RouterArgs& a, Gate& s, int t) 
 // workgroup write the normed row's two pieces.
 template <int EP, bool NORM, bool GF32>
 __global__ __launch_bounds__(kRouterThreads) void decode_router_kernel(RouterArgs a, int per, int gate) {
-  constexpr int NW = kRouterThreads / 64, U = GF32 ? 2 : 4;   // steps of 512 columns whose loads leave together
+  // U: steps of 512 columns whose loads leave together
+  constexpr int NW = kRouterThreads / 64, U = (EP == 8 || (EP == 4 && NORM) ? 4 : 8) / (GF32 ? 2 : 1);
   __shared__ Gate s;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
@@ -959,14 +960,16 @@ int fm_moe_decode(const void* x, int64_t ld_x, int64_t T, int64_t D, const void*
   // one workgroup a token where a gate is small enough for one CU to read; else 32 experts a workgroup and a second launch
   const bool one = int64_t(E) * D <= kRouterOne;
   if (!one) {
-    launch_router<4>(a, 32, false, s);
+    launch_router<1>(a, kRouterThreads / 64, false, s);
     hipLaunchKernelGGL(decode_gate_kernel, dim3{unsigned(T)}, dim3(kRouterThreads), 0, s, a);
   } else if (E <= 8) {
     launch_router<1>(a, E, true, s);
   } else if (E <= 16) {
     launch_router<2>(a, E, true, s);
-  } else {
+  } else if (E <= 32) {
     launch_router<4>(a, E, true, s);
+  } else {
+    launch_router<8>(a, E, true, s);
   }
   if (int rc = check_launch("fm_moe_decode")) return rc;
   return fm_decode_experts(norm ? x_hi : x, norm ? x_lo : nullptr, norm ? D : ld_x, T, D, weights, indices, 1, K, 0, E, experts, shared,
