@@ -863,8 +863,15 @@ __global__ __launch_bounds__(256) void decode_combine_kernel(ExpertArgs a, const
   else st_global(static_cast<uint16_t*>(out) + t * ld_o + col, make_uint2(hw_bf16x2(sum[0], sum[1]), hw_bf16x2(sum[2], sum[3])));
 }
 
-// The launch: hidden units of a gate|up workgroup (64, or fewer where the reached experts
-// give too few workgroups to fill the chip) and of a share of the down product.
+// The launch: hidden units of a gate|up workgroup and of a share of the down product.
+// Gate|up: 64 share the tokens' chunks among four waves and win from about three tokens an
+// expert on; with fewer, 32 (or 16, below 128 workgroups) give more workgroups with less to
+// wait for.  us a layer at 64 / 32 / 16 hidden units (MI355X): 64 tokens, 4 experts of 4096 x
+// 4096 105 / 128 / 126; 64 tokens, 32 int8 experts of 7168 x 2048 291 / 340 / 352; 5 tokens,
+// 64 experts of 2048 x 1408 105 / 98 / 98; 1 token, 8 of 128 experts of 2048 x 768 41 / 34 / 37;
+// 1 token, 2 of 8 experts of 2048 x 1408 32.3 / 28.3 / 27.9.
+// Down: as few shares as give every CU a workgroup, since each writes and the last kernel
+// reads 4 D bytes a token (512 instead of 256 workgroups: 1 to 3% slower at 5 and 17 tokens).
 struct DecodePlan {
   int hs, R, Rs;               // hidden units: of a gate|up workgroup; of a share, the shared expert's
   int P, Ps;                   // shares
@@ -872,13 +879,13 @@ struct DecodePlan {
   int64_t h, hs_at, part, part_s, bytes;   // offsets of h (two pieces), the shared expert's h, the shares, its shares
 };
 inline DecodePlan decode_plan(int64_t T, int64_t D, int64_t K, int64_t E, int64_t H, int64_t Hs) {
-  constexpr int64_t kFill = 512;   // workgroups: two a CU
+  constexpr int64_t kFill = 256;   // workgroups
   DecodePlan p;
   p.reach = E < T * K ? E : T * K;
   const int64_t units = p.reach * H + Hs;
-  p.hs = units / 64 >= kFill ? 64 : units / 32 >= kFill / 2 ? 32 : 16;
+  p.hs = T * K >= 3 * p.reach ? 64 : units / 32 >= kFill / 2 ? 32 : 16;
   const int64_t cols = (D + 511) / 512;
-  // shares of at least 64 hidden units, so many that the workgroups fill the chip
+  // shares of at least 64 hidden units
   auto shares = [&](int64_t h, int& R, int& P) {
     int64_t want = (kFill * h + units * cols - 1) / (units * cols);
     const int64_t most = h / 64;

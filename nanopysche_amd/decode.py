@@ -40,9 +40,11 @@ class DecodeOutput(NamedTuple):
 
 
 def _no_gradients(*tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("the few-token kernels are forward only: call them under torch.no_grad(), or use "
-                           "FP8FlowMoELayer / FP8FlowMoECompute to train")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("the few-token and int8 kernels are forward only: call them under torch.no_grad(), "
+                                   "or use FP8FlowMoELayer / FP8FlowMoECompute to train")
 
 
 def _same_device(x: torch.Tensor, **tensors) -> None:

@@ -19,6 +19,7 @@ from typing import Optional
 import torch
 
 from . import _lib
+from .decode import DecodeOutput, moe_decode
 from .flow_moe import FP8FlowMoECompute, FP8FlowMoEConfig, FP8SharedExpertCompute
 from .norm import DEFAULT_EPS, rmsnorm
 from .routing import (ExpertLoadTracker, capacity_select, gather_rows, route, route_tokens, router_backward,
@@ -262,6 +263,26 @@ class FP8FlowMoELayer:
         if self.shared is not None:
             out = out + self.shared(x)
         return out, aux
+
+    def decode(self, x: torch.Tensor, experts=None, shared=None) -> DecodeOutput:
+        """The layer for a decoding step of 1 to 64 tokens, forward only
+        (``moe_decode``): DecodeOutput(out, weights, indices) with the layer's
+        router, norm, experts and shared expert, whose weights must be bf16, or
+        with int8 ``experts`` (and ``shared``) made from them
+        (``Int8Experts.quantize``).  The recipe, jitter and capacity dropping, which
+        serve training, do not take part, and there is no auxiliary loss."""
+        if self.gate_weight is None:
+            raise RuntimeError("set_weights() must be called before the layer runs")
+        if self.shared is None and shared is not None:
+            raise ValueError("the layer has no shared expert")
+        if shared is None and self.shared is not None:
+            if experts is not None:
+                raise ValueError("int8 experts need the shared expert's int8 weights too")
+            shared = self.shared.block._w
+        return moe_decode(x, self.gate_weight, self.block._w if experts is None else experts, self.top_k,
+                          gate_bias=self.gate_bias, score_bias=self.score_bias, gating=self.gating,
+                          normalize_expert_weights=self.normalize_expert_weights, norm_weight=self.norm_weight,
+                          norm_eps=self.norm_eps, shared=shared)
 
     def _forward_with_capacity(self, x, noise, replay_indices, load_tracker):
         """MoEBase.forward with ``capacity_factor`` (reference ``model/moe.py:1338-1393``):

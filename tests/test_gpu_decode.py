@@ -75,15 +75,22 @@ def test_experts_match_float64(dev, T, E, K, H, D, dtype):
     check(got, *layer64(x.double(), torch.zeros_like(x, dtype=torch.float64), weights, indices, w, E))
 
 
-@pytest.mark.parametrize("H,E,K,T", [(4096, 16, 8, 20), (2048, 32, 4, 40), (2048, 8, 2, 5), (1408, 8, 2, 1)])
-def test_every_slice_size(dev, H, E, K, T):
-    """Hidden sizes and reached experts that take 128, 128, 64 or 32, and 16 hidden units a workgroup."""
+@pytest.mark.parametrize("H,E,K,T", [(4096, 16, 8, 20), (2048, 8, 2, 12), (2048, 64, 4, 2), (4096, 32, 6, 2), (1408, 8, 2, 1)])
+@pytest.mark.parametrize("norm", [False, True])
+def test_every_slice_size(dev, H, E, K, T, norm):
+    """Tokens and experts that take 64, 64, 32, 32 and 16 hidden units a workgroup, x in one piece and in two."""
     D = 256
     x = randn_bf16((T, D), seed=T).to(dev)
-    weights, indices = (t.to(dev) for t in routing(T, E, K, T))
+    gate = randn_bf16((E, D), seed=1, std=0.2).to(dev)
+    nw = (1 + 0.1 * torch.randn(D, generator=torch.Generator().manual_seed(4))).to(dev) if norm else None
     w = [t.to(dev) for t in expert_weights(E, H, D, 5)]
-    got = fm.expert_decode(x.float(), weights, indices, w, E)
-    check(got, *layer64(x.double(), torch.zeros_like(x, dtype=torch.float64), weights, indices, w, E))
+    r = fm.moe_decode(x.float(), gate, w, K, norm_weight=nw)
+    x64 = x.double()
+    ex = torch.zeros_like(x64)
+    if norm:
+        x64 = x64 * torch.rsqrt(x64.square().mean(1, keepdim=True) + 1e-6) * nw.double()
+        ex = 2.0 ** -16 * x64.abs()
+    check(r.out, *layer64(x64, ex, r.weights, r.indices, w, E))
 
 
 def router64(x, gate, bias, score, K, gating, l2):
