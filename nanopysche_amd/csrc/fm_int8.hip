@@ -418,6 +418,7 @@ struct Shape {
   static constexpr int PI = TI / 16 / W, PJ = TJ / 16 / W;   // row tiles that a wave moves
   static constexpr int kSlot = (TI + TJ) * 64 * KS;
   static constexpr int kStage = W * 2048;
+  static constexpr bool kHalves = W == 8 && WJ % 2 == 0;   // waves 0..3 hold the first half of the tokens, 4..7 the second
   static_assert(TI % (16 * W) == 0 && TJ % (16 * W) == 0 && (KS == 1 || KS == 2), "whole pieces; K is a multiple of 128");
 };
 constexpr int kProductExperts = 1024;
@@ -574,9 +575,15 @@ __global__ __launch_bounds__(64 * S::W) void int8_product_kernel(ProductArgs p) 
   const int xcd = blockIdx.x & 7, nbx = gridDim.x / 8;
   const int each = n_tiles / 8, more_x = n_tiles % 8;
   const int lo = each * xcd + (xcd < more_x ? xcd : more_x), hi = lo + each + (xcd < more_x);
+  // where the last round leaves half or more of an XCD's workgroups idle, two share a tile's
+  // tokens: half of them take half of the time where each SIMD holds a wave of either half
+  const int mine = blockIdx.x / 8, whole = (hi - lo) / nbx, rem = (hi - lo) % nbx;
+  const bool halves = S::kHalves && 2 * rem <= nbx;
   auto tile_at = [&](int c, OutTile& t) -> bool {
-    const int at = lo + int(blockIdx.x / 8) + c * nbx;
-    if (at >= hi) return false;
+    int at = lo + c * nbx + mine;
+    const bool halve = halves && c == whole && mine >= rem;   // the second half of the tile of `mine - rem`
+    if (halve) at -= rem;
+    if (c > whole || at >= hi) return false;
     int e = 0, n = p.E;   // the last expert whose tiles start at or before
     while (n > 1) {
       const int h = n / 2;
@@ -592,7 +599,12 @@ __global__ __launch_bounds__(64 * S::W) void int8_product_kernel(ProductArgs p) 
     const int end = p.offsets ? __builtin_amdgcn_readfirstlane(p.offsets[e + 1]) : int(p.M);
     t.j0 = b + j * S::TJ;
     t.j1 = t.j0 + S::TJ < end ? t.j0 + S::TJ : end;
-    return true;
+    if (halves && c == whole) {
+      const int mid = t.j0 + S::TJ / 2;
+      if (halve) t.j0 = mid;
+      else if (mid < t.j1) t.j1 = mid;
+    }
+    return t.j0 < t.j1;
   };
 
   // what the wave moves: its tiles of the operands, row tiles past the end read from the last one
@@ -778,17 +790,20 @@ void launch_product(const ProductArgs& p, int64_t token_tiles, hipStream_t s) {
   const int rows_i = SWIGLU ? S::TI / 2 : S::TI;
   const int64_t tiles = token_tiles * ((p.N + rows_i - 1) / rows_i);
   static const int64_t fit = resident_workgroups(int8_product_kernel<S, SWIGLU>, 64 * S::W);
-  int64_t grid = tiles < fit ? tiles : fit;
+  int64_t grid = tiles * (S::kHalves ? 2 : 1) < fit ? tiles * (S::kHalves ? 2 : 1) : fit;
   grid = (grid + 7) / 8 * 8;   // a multiple of the XCDs
   hipLaunchKernelGGL((int8_product_kernel<S, SWIGLU>), dim3{unsigned(grid)}, dim3(64 * S::W), 0, s, p);
 }
 
-// The shape that is fastest by what a half costs on it and the rounds of output tiles that a
-// launch needs: 0.95 us for the 256 x 256 tile, 0.59 for 256 x 128, one workgroup a CU; 0.32
-// for 128 x 64 while it has a CU to itself, 0.42 when two share one.  Measured (us, the three
-// shapes, dense M x N x K): 77 x 2831 x 1409 17.6 / 15.3 / 9.7; 512 x 5632 x 2048 28 / 19 / 15;
-// 512 x 4096 x 14336 136 / 95 / 57; 1024 x 4096 x 4096 47 / 31 / 25; 2048 x 4096 x 4096 50 /
-// 36 / 56; 2048 x 5632 x 2048 32 / 36 / 49; 8192 x 14336 x 4096 427 / 534 / 842.
+// The shape that is fastest by what 64 of K cost on it and the rounds of output tiles that a
+// launch needs: 0.95 us for the 256 x 256 tile, 0.59 for 256 x 128, one workgroup a CU, 0.68
+// and 0.43 for a round of halved tiles; 0.32 for 128 x 64 while it has a CU to itself, 0.42 when
+// two share one.  Measured (us, small, medium, large, dense M x N x K): 77 x 2831 x 1409 9.6 /
+// 15.5 / 18.1; 512 x 5632 x 2048 15.5 / 16.2 / 28.8; 512 x 4096 x 14336 53 / 85 / 102;
+// 1024 x 4096 x 4096 25.9 / 25.1 / 33.8; 1500 x 3500 x 3000 27.7 / 25.9 / 39.2; 2048 x 4096 x
+// 4096 46 / 36 / 39; 4096 x 2816 x 2048 37.3 / 35.7 / 34.1; 4096 x 4096 x 14336 308 / 224 / 194;
+// 8192 x 14336 x 4096 652 / 538 / 424.  Halved last rounds: the large shape 47 -> 33.8 at
+// 1024 x 4096 x 4096 and 348 -> 304 for 4096 slots on 8 experts x 4096 x 14336.
 // tokens over `groups` groups (dense: one); rows: of the padded buffer, or 0.
 template <bool SWIGLU>
 void launch_shape(const ProductArgs& p, int64_t tokens, int64_t groups, int64_t rows, hipStream_t s) {
@@ -799,8 +814,10 @@ void launch_shape(const ProductArgs& p, int64_t tokens, int64_t groups, int64_t 
     return j * ((p.N * up + ti - 1) / ti);
   };
   auto rounds = [](int64_t n, int64_t at_once) { return (n + at_once - 1) / at_once; };
+  // a last round of half the workgroups or fewer is one of halved tiles
+  auto cost = [&](int64_t n, int64_t one, int64_t half) { return one * (n / cus) + (n % cus == 0 ? 0 : n % cus * 2 <= cus ? half : one); };
   const int64_t small = tiles(Small::TI, Small::TJ);
-  const int64_t large_us = 95 * rounds(tiles(Large::TI, Large::TJ), cus), medium_us = 59 * rounds(tiles(Medium::TI, Medium::TJ), cus);
+  const int64_t large_us = cost(tiles(Large::TI, Large::TJ), 95, 68), medium_us = cost(tiles(Medium::TI, Medium::TJ), 59, 43);
   const int64_t small_us = small <= cus ? 32 : 42 * rounds(small, 2 * cus);
   // a bound of the token tiles: every group is a multiple of 128 rows
   auto most = [&](int64_t tj) { return rows ? rows / 128 * (tj < 128 ? 128 / tj : 1) : (tokens + tj - 1) / tj; };

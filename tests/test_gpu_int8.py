@@ -87,7 +87,7 @@ def check_product(out, qa, sa, qw, sw, bias):
 
 SHAPES = [(1, 1, 1), (1, 17, 64), (3, 100, 130), (16, 48, 128), (17, 33, 1000), (33, 65, 200), (48, 15, 640), (49, 300, 2049),
           (64, 64, 4096), (65, 1, 100), (65, 127, 257), (100, 129, 64), (128, 128, 128), (129, 257, 300), (300, 500, 700),
-          (1000, 640, 1409), (4097, 2049, 130), (4300, 2300, 200)]
+          (1000, 640, 1409), (4097, 2049, 130), (4300, 2300, 200), (4090, 4300, 200), (1500, 3500, 130)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
@@ -126,8 +126,8 @@ def test_longest_sum_does_not_overflow(dev, M):
     assert torch.all(out == float(128 * 128 * MAX_INT8_K))
 
 
-@pytest.mark.parametrize("counts", [(5,), (0, 200, 0, 1), (300, 128, 129, 0, 700), (1,) * 70 + (0, 513)])
-@pytest.mark.parametrize("N,K", [(16, 128), (272, 384), (640, 256)])
+@pytest.mark.parametrize("counts", [(5,), (0, 200, 0, 1), (300, 128, 129, 0, 700), (1,) * 70 + (0, 513), (128,) * 8, (2000, 2200)])
+@pytest.mark.parametrize("N,K", [(16, 128), (272, 384), (640, 256), (4096, 128)])
 def test_grouped_matches_exact_sums(dev, counts, N, K):
     E = len(counts)
     idx = torch.cat([torch.full((c,), e, dtype=torch.int64) for e, c in enumerate(counts)])
