@@ -71,9 +71,18 @@ struct Raw {
   }
   // the largest magnitude as bits: a NaN is above infinity, infinity above every number
   __device__ __forceinline__ uint32_t top(uint32_t m) const {
+    if constexpr (F32) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const uint32_t b = f2u(at(i)) & 0x7fffffffu;
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t b = v[i / 4][i % 4] & 0x7fffffffu;
+        m = b > m ? b : m;
+      }
+    } else {
+      typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+      u16x2 t = {0, 0};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t = __builtin_elementwise_max(t, __builtin_bit_cast(u16x2, v[i / 4][i % 4] & 0x7fff7fffu));
+      const uint32_t b = uint32_t(t[0] > t[1] ? t[0] : t[1]) << 16;
       m = b > m ? b : m;
     }
     return m;
@@ -776,6 +785,8 @@ void launch_quant(const QuantArgs& a, int64_t row_tiles, hipStream_t s) {
     hipLaunchKernelGGL((int8_quant_kernel<F32, 4, false>), grid, block, 0, s, a);
   } else if (a.kt <= 8 * kQuantWaves) {
     hipLaunchKernelGGL((int8_quant_kernel<F32, 8, false>), grid, block, 0, s, a);
+  } else if (!F32 && a.kt <= 16 * kQuantWaves) {
+    hipLaunchKernelGGL((int8_quant_kernel<F32, F32 ? 8 : 16, false>), grid, block, 0, s, a);
   } else {
     hipLaunchKernelGGL((int8_quant_kernel<F32, 0, false>), grid, block, 0, s, a);
   }
