@@ -606,8 +606,8 @@ int fm_grouped_gemm_ragged_k_split(int kind, const FmGemmOperand* a_t, const FmG
 /* ------------------------------------------------- a MoE layer for few tokens ----
  * A decoding step of 1..64 tokens through router, experts and shared expert
  * (reference model/moe.py:133-184 and :1338-1393 at those sizes), in bf16 or with
- * int8 weights.  D and hidden sizes are multiples of 128, D at most 14336, at most
- * 1024 experts, K at most 16.
+ * int8 weights.  D and hidden sizes H are multiples of 128, D at most 14336, H at most
+ * 2^20 and H D below 2^30, at most 1024 experts, K at most 16.
  *
  * fm_decode_experts: out[t] = sum_k weights[t, k] expert(indices[t, k] - expert_offset)(x[t])
  * (+ shared(x[t])), slots of experts outside [0, E) adding nothing.  x_lo (NULL:

@@ -9,10 +9,10 @@
 //
 // What bounds it is reading the reached experts' weights once: 3 H D elements of
 // 2 bytes (bf16, as the layer stores them) or 1 (int8 with a scale per channel).
-// Three kernels share the chip: the router (a workgroup a token), gate|up (a
-// workgroup takes 16 to 64 hidden units of one expert over all of its tokens and
-// leaves h), and down (512 output columns of one expert over a share of the hidden
-// units); the last one adds the shares per token in a fixed order.  Weights go from
+// Four launches: the router (a workgroup a token; a large gate over many workgroups and a
+// launch of its own for the picks), gate|up (a workgroup takes 16 to 64 hidden units of
+// one expert over all of its tokens and leaves h), down (512 output columns of one expert
+// over a share of the hidden units), and the sum of the shares per token, in a fixed order.  Weights go from
 // memory straight into MFMA fragments: with at most 16 tokens each feeds one MFMA, and
 // LDS would only add latency.  The tokens' operand goes through LDS, a chunk at a time.
 //
@@ -43,7 +43,7 @@ namespace {
 constexpr int kDecodeTokens = 64;    // most tokens of a call
 constexpr int kDecodeTopK = 16;      // most experts of a token
 constexpr int kDecodeExperts = 1024; // most experts
-constexpr int kDecodeDim = 14336;    // widest token 
+constexpr int kDecodeDim = 14336;    // widest token
 
 // ------------------------------------------------------------------ router ----
 constexpr int64_t kRouterOne = 64 * 1024;   // elements of a gate that one workgroup reads for a token
@@ -928,7 +928,7 @@ int64_t decode_router_bytes(int64_t T, int64_t D, int64_t E) { return T * D * 4 
 bool decode_sizes_ok(int64_t T, int64_t D, int64_t K, int64_t E, int64_t H, int64_t Hs) {
   return T >= 1 && T <= kDecodeTokens && D >= 128 && D <= kDecodeDim && D % 128 == 0 && K >= 1 && K <= kDecodeTopK &&
          E >= 1 && E <= kDecodeExperts && H >= 128 && H % 128 == 0 && H <= (1 << 20) && Hs >= 0 && Hs % 128 == 0 &&
-         Hs <= (1 << 20) && (H > Hs ? H : Hs) * D < (int64_t(1) << 31);
+         Hs <= (1 << 20) && (H > Hs ? H : Hs) * D < (int64_t(1) << 30);   // a matrix's bytes are below 2^31
 }
 
 }  // namespace

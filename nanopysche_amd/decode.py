@@ -4,9 +4,9 @@ optional RMSNorm and shared expert around it) at 1 to 64 tokens, forward only.
 
 The layer built for prompts permutes tokens into padded groups and runs about
 ten launches; at these sizes the time is reading the reached experts' weights
-once.  Here the router is one launch (two for a large gate), a second kernel
-takes every reached expert's slices of hidden units through gate, up, SwiGLU
-and down, and a third adds the slices' shares per token.
+once.  Here the router is one launch (two for a large gate), the next takes slices
+of every reached expert's hidden units through gate, up and SwiGLU, the next
+shares of them through the down product, and the last adds the shares per token.
 
 The experts' weights are bf16 as the layer holds them, or int8 with a scale per
 output channel (``Int8Experts``), which halves the bytes; activations are not
@@ -214,7 +214,7 @@ def moe_decode(x: torch.Tensor, gate_weight: torch.Tensor, experts, top_k: int, 
     x's shape and dtype."""
     x2 = _rows(x)
     T, D = x2.shape
-    _no_gradients(x, gate_weight, gate_bias, norm_weight)
+    _no_gradients(x, gate_weight, gate_bias, score_bias, norm_weight)
     if gate_weight.dim() != 2 or gate_weight.shape[1] != D:
         raise ValueError(f"gate_weight must be [E, {D}], got {tuple(gate_weight.shape)}")
     E, K = gate_weight.shape[0], int(top_k)

@@ -309,6 +309,8 @@ class Int8MoECompute:
             raise ValueError(f"weights {tuple(weights.shape)} and indices {tuple(indices.shape)} must be [T, K] for {T} tokens")
         if T <= MAX_DECODE_TOKENS and D <= MAX_DECODE_DIM and K <= MAX_DECODE_TOP_K:
             return expert_decode(x, weights, indices, w, E, expert_offset)
+        if T == 0:
+            return torch.empty_like(x)
         with _lib.on_device_of(x2):
             if expert_offset:
                 indices = indices - int(expert_offset)

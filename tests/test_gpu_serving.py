@@ -191,3 +191,20 @@ def test_rows_behind_the_groups_are_left(dev):
                   w.data.data_ptr(), w.scale.data_ptr(), None, None, None, 64, 128, 3, out.data_ptr(), _lib.DTYPE_F32, 64,
                   _lib.stream_of(out))
         assert torch.all(out[end:] == 7.0) and torch.all(out[:end] == 128.0)
+
+
+@pytest.mark.parametrize("T,D", [(0, 128), (0, 14464), (65, 14464), (66000, 128)])
+def test_block_of_no_tokens_wide_ones_and_many(dev, T, D):
+    """Beyond the few-token kernels' width, and more tokens than a grid's second dimension holds."""
+    E, H = 3, 128
+    g = torch.Generator().manual_seed(1)
+    q = [torch.randint(-127, 128, (E * H, D), generator=g, dtype=torch.int8).to(dev) for _ in range(3)]
+    block = fm.Int8MoECompute(fm.Int8Experts.from_int8(q[0], torch.full((E * H,), 1e-3, device=dev), q[1], torch.full((E, D), 1e-3, device=dev),
+                                                       q[2], torch.full((E * H,), 1e-3, device=dev), E))
+    x, w = torch.randn(T, D, generator=g).to(dev), torch.rand(T, 1, generator=g).to(dev)
+    idx = torch.randint(0, E, (T, 1), generator=g).to(dev)
+    out = block(x, w, idx)
+    assert out.shape == x.shape and torch.isfinite(out).all()
+    if T > 128:   # a token's output does not depend on the others
+        assert torch.equal(block(x[-100:], w[-100:], idx[-100:]), out[-100:])
+        assert torch.equal(block(x[:100], w[:100], idx[:100]), out[:100])

@@ -172,7 +172,7 @@ def test_library_refuses_decode_sizes():
     assert n > 0
     for T, D, K, E, H, Hs in [(0, 256, 2, 4, 128, 0), (65, 256, 2, 4, 128, 0), (3, 200, 2, 4, 128, 0), (3, 14464, 2, 4, 128, 0),
                               (3, 256, 0, 4, 128, 0), (3, 256, 17, 40, 128, 0), (3, 256, 2, 1025, 128, 0), (3, 256, 2, 4, 100, 0),
-                              (3, 256, 2, 4, 128, 100), (3, 14336, 2, 4, 1 << 20, 0)]:
+                              (3, 256, 2, 4, 128, 100), (3, 14336, 2, 4, 1 << 20, 0), (3, 8192, 2, 4, 128, 131072)]:
         assert size(T, D, K, E, H, Hs) == -1
 
     def run(match, x=P, ld=256, T=3, D=256, K=2, E=4, w=w, ws=None, out_dtype=0, ld_out=256, work=P, nbytes=n, idx=P):
