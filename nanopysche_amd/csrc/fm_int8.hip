@@ -191,20 +191,39 @@ __global__ __launch_bounds__(64 * kQuantWaves) void int8_quant_kernel(QuantArgs 
   }
 }
 
-// Row-major int8 (any strides, in bytes) into tiles, groups one after the other.
+// Int8 values (any strides, in bytes) into tiles, groups one after the other, a tile a wave.
+// Rows of contiguous columns: a lane's 16 bytes in one load.  Columns of contiguous rows (w2 as
+// the expert block stores it): a lane loads the tile's 16 rows of one column, and the wave
+// turns them in LDS.  A byte at a time otherwise and at the edges.  us for 8 x 14336 x 4096
+// (470 MB): rows 160, columns 246; by bytes 560 and 840, and 670 to 880 with a gap between.
 __global__ __launch_bounds__(256) void int8_pack_kernel(const uint8_t* x, int64_t gs, int64_t rs, int64_t cs, int64_t R, int64_t C,
                                                         int kt, int64_t tiles, uint8_t* q) {
-  const int lane = threadIdx.x & 63;
-  const int64_t t = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  __shared__ __attribute__((aligned(16))) uint8_t turn[4][64 * 20];   // 20 bytes a column: 64 columns' dwords on distinct banks
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
+  const int64_t t = int64_t(blockIdx.x) * 4 + wave;
   if (t >= tiles) return;
-  const int64_t rt = (R + 15) / 16, g = t / (rt * kt), tr = t / kt % rt, tk = t % kt;
-  const int64_t r = tr * 16 + (lane & 15), c = tk * 64 + (lane >> 4) * 16;
+  const int64_t rt = (R + 15) / 16, g = t / (rt * kt), r0 = t / kt % rt * 16, c0 = t % kt * 64;
+  const int64_t r = r0 + (lane & 15), c = c0 + (lane >> 4) * 16;
   uint32_t o[4] = {0, 0, 0, 0};
-  if (r < R) {
-    const uint8_t* p = x + g * gs + r * rs;
+  if (cs != 1 && rs == 1 && r0 + 16 <= R && c0 + 64 <= C) {
+    const fm_u32x4 v = *FM_GLOBAL(const u32x4_any, x + g * gs + r0 + (c0 + lane) * cs);
+    uint8_t* mine = turn[wave];
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (c + i < C) o[i / 4] |= uint32_t(*FM_GLOBAL(const uint8_t, p + (c + i) * cs)) << (i % 4 * 8);
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<uint32_t*>(mine + lane * 20 + 4 * i) = v[i];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // LDS keeps a wave's order
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i / 4] |= uint32_t(mine[((lane >> 4) * 16 + i) * 20 + (lane & 15)]) << (i % 4 * 8);
+  } else if (r < R) {
+    const uint8_t* p = x + g * gs + r * rs;
+    if (cs == 1 && c + 16 <= C) {
+      const fm_u32x4 v = *FM_GLOBAL(const u32x4_any, p + c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = v[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (c + i < C) o[i / 4] |= uint32_t(*FM_GLOBAL(const uint8_t, p + (c + i) * cs)) << (i % 4 * 8);
+    }
   }
   st_global(q + (t * 64 + lane) * 16, make_uint4(o[0], o[1], o[2], o[3]));
 }

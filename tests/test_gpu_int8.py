@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import nanopysche_amd as fm
-from nanopysche_amd.int8 import MAX_INT8_K, _quantize
+from nanopysche_amd.int8 import MAX_INT8_K, _pack, _quantize
 from tests.helpers import randn_bf16, zipf_routing
 from tests.test_gpu_decode import check, expert_weights, layer64
 
@@ -155,6 +155,20 @@ def test_quantise_of_a_plan_gathers_and_stops(dev):
     got, a = t.values()[:end].float(), plan.assign_of_row[:end].long()
     assert torch.equal(got[a >= 0], q[a[a >= 0] // K]) and torch.equal(t.scale[:end][a >= 0], s[a[a >= 0] // K])
     assert torch.all(got[a < 0] == 0)
+
+
+@pytest.mark.parametrize("R,C", [(1, 1), (16, 64), (17, 65), (48, 128), (160, 300), (33, 1)])
+def test_pack_of_any_strides(dev, R, C):
+    """Rows, columns, every second element and repeated rows, from odd addresses; groups too."""
+    g = torch.Generator().manual_seed(R * C)
+    base = torch.randint(-128, 128, (2 * R * C * 6 + 7,), generator=g, dtype=torch.int8).to(dev)
+    one = torch.ones(R, device=dev)
+    for q in (base[3:3 + R * C].view(R, C), base[1:1 + R * C].view(C, R).t(), base[:4 * R * C].view(2 * R, 2 * C)[::2, ::2],
+              base[5:5 + 2 * R * C].view(C, 2 * R)[:, 1:R + 1].t(), base[2:2 + C].expand(R, C)):
+        assert torch.equal(fm.Int8Tensor.from_int8(q, one).values(), q)
+    if R % 16 == 0:
+        w = base[:2 * R * C].view(2, C, R).transpose(1, 2)
+        assert torch.equal(_pack(w, torch.ones(2 * R, device=dev)).values(), w.reshape(2 * R, C))
 
 
 def block64(x, weights, indices, w, E):
