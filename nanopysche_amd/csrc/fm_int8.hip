@@ -195,7 +195,7 @@ __global__ __launch_bounds__(64 * kQuantWaves) void int8_quant_kernel(QuantArgs 
 // Rows of contiguous columns: a lane's 16 bytes in one load.  Columns of contiguous rows (w2 as
 // the expert block stores it): a lane loads the tile's 16 rows of one column, and the wave
 // turns them in LDS.  A byte at a time otherwise and at the edges.  us for 8 x 14336 x 4096
-// (470 MB): rows 160, columns 246; by bytes 560 and 840, and 670 to 880 with a gap between.
+// (470 MB): rows 160, columns 246; by bytes 840 and 560, and 670 to 880 with a gap between.
 __global__ __launch_bounds__(256) void int8_pack_kernel(const uint8_t* x, int64_t gs, int64_t rs, int64_t cs, int64_t R, int64_t C,
                                                         int kt, int64_t tiles, uint8_t* q) {
   __shared__ __attribute__((aligned(16))) uint8_t turn[4][64 * 20];   // 20 bytes a column: 64 columns' dwords on distinct banks
