@@ -108,18 +108,25 @@ __device__ __forceinline__ fm_u32x4 int8_round(const Raw<F32>& v, Recip d, bool 
   return o;
 }
 
-// A workgroup takes 16 rows, a lane 16 columns of one row: a tile's payload leaves in one
-// 1 KiB store of a wave.  The NT tiles of a wave stay in registers between the maximum and
-// the rounding (NT = 0: read twice).  GIVEN: the maxima are known, and gridDim.y workgroups
-// share the columns.  Bound: reading x and writing q once.
+// A workgroup takes RW rows, a lane 16 columns of one row, a wave 64 / RW such chunks side by
+// side: of 16 rows a tile's payload leaves in one 1 KiB store, of 4 in pieces of 64 bytes.  The NT
+// chunks of a lane stay in registers between the maximum and the rounding (NT = 0: read
+// twice).  GIVEN: the maxima are known, and gridDim.y workgroups share the columns.  Bound:
+// reading x and writing q once (8192 x 4096 bf16 in 20.4 us, 4.9 TB/s), by few rows what a CU
+// can have in flight.  So a workgroup takes 2 or 4 rows while no more workgroups than CUs come
+// of it, else 8.  us with 16 / 8 / 4 / 2 rows: 16 x 4096 bf16 7.4 / 4.9 / 3.6 / 3.0; 64 x 14336
+// 28.7 / 11.9 / 7.1 / 4.3; 512 x 14336 29.7 / 13.4 / 8.6 / 7.6; 1024 x 8192 14.8 / 9.3 / 7.5 / 7.9;
+// 1409 x 2817 fp32 9.6 / 6.7 / 6.8 / 7.1; 2048 x 14336 36.9 / 19.8 / 21.9 / 25.0; 8192 x 4096 20.4 /
+// 20.4 / 21.9 / 27.8; 16384 x 2048 20.9 / 18.8 / 20.9 / 28.6.
 constexpr int kQuantWaves = 8;
-template <bool F32, int NT, bool GIVEN>
+template <bool F32, int NT, bool GIVEN, int RW>
 __global__ __launch_bounds__(64 * kQuantWaves) void int8_quant_kernel(QuantArgs a) {
-  __shared__ uint32_t tops[kQuantWaves][16];
-  const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4, wave = threadIdx.x >> 6;
-  const int64_t r0 = int64_t(blockIdx.x) * 16;
+  constexpr int kSide = 64 / RW;
+  __shared__ uint32_t tops[kQuantWaves][RW];
+  const int lane = threadIdx.x & 63, r = lane % RW, wave = threadIdx.x >> 6;
+  const int64_t r0 = int64_t(blockIdx.x) * RW;
   if (a.limit && r0 >= *a.limit) return;
-  if (a.clear && threadIdx.x < 16) st_global(a.clear + r0 + threadIdx.x, 0u);
+  if (a.clear && threadIdx.x < RW) st_global(a.clear + r0 + threadIdx.x, 0u);
   int64_t src = r0 + r;
   bool valid = src < a.R;
   if (a.assign) {
@@ -130,62 +137,62 @@ __global__ __launch_bounds__(64 * kQuantWaves) void int8_quant_kernel(QuantArgs 
   if (!valid) src = 0;
   const void* row = static_cast<const uint8_t*>(a.x) + src * a.ld * (F32 ? 4 : 2);
   const int64_t C = valid ? a.C : 0;
-  uint8_t* const q = a.q + (int64_t(blockIdx.x) * a.kt * 64 + lane) * 16;
-  auto put = [&](const Raw<F32>& v, Recip d, bool finite, int t) {
+  const int n = a.kt * 4, c0 = wave * kSide + lane / RW, step = kQuantWaves * kSide;   // chunks of a row; the lane's are c0 + step i
+  uint8_t* const q = a.q + (r0 / 16 * a.kt * 64 + r0 % 16 + r) * 16;
+  auto put = [&](const Raw<F32>& v, Recip d, bool finite, int c) {
     const fm_u32x4 o = int8_round(v, d, finite);
-    st_global(q + int64_t(t) * 1024, make_uint4(o[0], o[1], o[2], o[3]));
+    st_global(q + int64_t(c) * 256, make_uint4(o[0], o[1], o[2], o[3]));
   };
   if constexpr (GIVEN) {
     const uint32_t top = valid ? a.top[r0 + r] : 0u;
     const float s = int8_scale(top);
-    if (blockIdx.y == 0 && wave == 0 && c == 0) st_global(a.s + r0 + r, s);
+    if (blockIdx.y == 0 && threadIdx.x < RW) st_global(a.s + r0 + r, s);
     const Recip d = recip_of(s);
-    const int step = kQuantWaves * gridDim.y;
 #pragma unroll 4
-    for (int t = wave + kQuantWaves * blockIdx.y; t < a.kt; t += step) {
+    for (int c = c0 + step * blockIdx.y; c < n; c += step * gridDim.y) {
       Raw<F32> v;
-      v.load(row, int64_t(t) * 64 + c * 16, C);
-      put(v, d, top <= 0x7f7fffffu, t);
+      v.load(row, int64_t(c) * 16, C);
+      put(v, d, top <= 0x7f7fffffu, c);
     }
   } else {
     Raw<F32> held[NT ? NT : 1];
     uint32_t top = 0;
     if constexpr (NT > 0) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i) held[i].load(row, int64_t(wave + i * kQuantWaves) * 64 + c * 16, C);
+      for (int i = 0; i < NT; ++i) held[i].load(row, int64_t(c0 + step * i) * 16, C);
 #pragma unroll
       for (int i = 0; i < NT; ++i) top = held[i].top(top);
     } else {
 #pragma unroll 4
-      for (int t = wave; t < a.kt; t += kQuantWaves) {
+      for (int c = c0; c < n; c += step) {
         Raw<F32> v;
-        v.load(row, int64_t(t) * 64 + c * 16, C);
+        v.load(row, int64_t(c) * 16, C);
         top = v.top(top);
       }
     }
 #pragma unroll
-    for (int off = 16; off < 64; off <<= 1) {
+    for (int off = RW; off < 64; off <<= 1) {
       const uint32_t o = __shfl_xor(top, off);
       top = o > top ? o : top;
     }
-    if (c == 0) tops[wave][r] = top;
+    if (lane < RW) tops[wave][r] = top;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kQuantWaves; ++w) top = tops[w][r] > top ? tops[w][r] : top;
     const float s = int8_scale(top);
     const bool finite = top <= 0x7f7fffffu;
-    if (wave == 0 && c == 0) st_global(a.s + r0 + r, s);
+    if (threadIdx.x < RW) st_global(a.s + r0 + r, s);
     const Recip d = recip_of(s);
     if constexpr (NT > 0) {
 #pragma unroll
       for (int i = 0; i < NT; ++i)
-        if (wave + i * kQuantWaves < a.kt) put(held[i], d, finite, wave + i * kQuantWaves);
+        if (c0 + step * i < n) put(held[i], d, finite, c0 + step * i);
     } else {
 #pragma unroll 2
-      for (int t = wave; t < a.kt; t += kQuantWaves) {
+      for (int c = c0; c < n; c += step) {
         Raw<F32> v;
-        v.load(row, int64_t(t) * 64 + c * 16, C);
-        put(v, d, finite, t);
+        v.load(row, int64_t(c) * 16, C);
+        put(v, d, finite, c);
       }
     }
   }
@@ -788,26 +795,32 @@ __global__ __launch_bounds__(256) void int8_combine_kernel(const float* y, int64
   else st_global(static_cast<uint16_t*>(out) + t * D + c, make_uint2(hw_bf16x2(sum[0], sum[1]), hw_bf16x2(sum[2], sum[3])));
 }
 
+template <bool F32, int RW>
+void launch_rows(const QuantArgs& a, int64_t row_tiles, hipStream_t s) {
+  const dim3 grid{unsigned(row_tiles * (16 / RW))}, block(64 * kQuantWaves);
+  constexpr int kStep = kQuantWaves * 64 / RW;
+  const int each = (a.kt * 4 + kStep - 1) / kStep;   // chunks of a lane
+  if (each <= 2) hipLaunchKernelGGL((int8_quant_kernel<F32, 2, false, RW>), grid, block, 0, s, a);
+  else if (each <= 4) hipLaunchKernelGGL((int8_quant_kernel<F32, 4, false, RW>), grid, block, 0, s, a);
+  else if (each <= 8) hipLaunchKernelGGL((int8_quant_kernel<F32, 8, false, RW>), grid, block, 0, s, a);
+  else if (!F32 && each <= 16) hipLaunchKernelGGL((int8_quant_kernel<F32, F32 ? 8 : 16, false, RW>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((int8_quant_kernel<F32, 0, false, RW>), grid, block, 0, s, a);
+}
+
 template <bool F32>
 void launch_quant(const QuantArgs& a, int64_t row_tiles, hipStream_t s) {
-  const dim3 block(64 * kQuantWaves);
-  dim3 grid{unsigned(row_tiles)};
   if (a.top) {
-    // columns shared until the workgroups fill the chip twice, eight tiles a wave at least
-    int64_t y = (4 * device_cus() + row_tiles - 1) / row_tiles;
-    const int64_t most = (a.kt + 8 * kQuantWaves - 1) / (8 * kQuantWaves);
-    grid.y = unsigned(y < most ? y : most);
-    hipLaunchKernelGGL((int8_quant_kernel<F32, 0, true>), grid, block, 0, s, a);
-  } else if (a.kt <= 2 * kQuantWaves) {
-    hipLaunchKernelGGL((int8_quant_kernel<F32, 2, false>), grid, block, 0, s, a);
-  } else if (a.kt <= 4 * kQuantWaves) {
-    hipLaunchKernelGGL((int8_quant_kernel<F32, 4, false>), grid, block, 0, s, a);
-  } else if (a.kt <= 8 * kQuantWaves) {
-    hipLaunchKernelGGL((int8_quant_kernel<F32, 8, false>), grid, block, 0, s, a);
-  } else if (!F32 && a.kt <= 16 * kQuantWaves) {
-    hipLaunchKernelGGL((int8_quant_kernel<F32, F32 ? 8 : 16, false>), grid, block, 0, s, a);
+    constexpr int RW = 8;
+    // columns shared until the workgroups fill the chip twice, eight chunks a lane at least
+    const int64_t rows = row_tiles * (16 / RW), y = (4 * device_cus() + rows - 1) / rows;
+    const int64_t each = 8 * kQuantWaves * (64 / RW), most = (a.kt * 4 + each - 1) / each;
+    hipLaunchKernelGGL((int8_quant_kernel<F32, 0, true, RW>), dim3(unsigned(rows), unsigned(y < most ? y : most)), dim3(64 * kQuantWaves), 0, s, a);
+  } else if (row_tiles * 8 <= device_cus()) {
+    launch_rows<F32, 2>(a, row_tiles, s);
+  } else if (row_tiles * 4 <= device_cus()) {
+    launch_rows<F32, 4>(a, row_tiles, s);
   } else {
-    hipLaunchKernelGGL((int8_quant_kernel<F32, 0, false>), grid, block, 0, s, a);
+    launch_rows<F32, 8>(a, row_tiles, s);
   }
 }
 

@@ -24,7 +24,7 @@ def plain_rows(x):
     return torch.round(x / s[:, None]), s
 
 
-@pytest.mark.parametrize("rows", [1, 15, 16, 17, 130])
+@pytest.mark.parametrize("rows", [1, 15, 16, 17, 130, 600, 1100])
 @pytest.mark.parametrize("cols", [1, 15, 16, 63, 64, 65, 127, 129, 1000, 1025, 2048, 2049, 4097, 8192, 8200, 20001])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_quantise_is_exact(dev, rows, cols, dtype):
