@@ -295,10 +295,11 @@ __device__ __forceinline__ v4f four_of(const float* p, int64_t n, int64_t N) {
 }
 
 // ------------------------------------------------------------ few tokens ----
-// out[t, n] for at most 64 tokens: bound by reading the weights once.  A workgroup owns
-// 16 channels; its 4 waves take a quarter of K each, tiles straight from memory into
-// 16x16x64 MFMA fragments, U of them in flight beside the ones in use, and the four int32
-// sums meet in LDS.
+// out[t, n], bound by reading the weights once for up to 32 tokens and by the latency of a
+// chain over K for more.  A workgroup owns 16 channels and TF tiles of 16 tokens; its 4 waves
+// take a quarter of K each, tiles straight from memory into 16x16x64 MFMA fragments, U of them
+// in flight beside the ones in use, and the four int32 sums meet in LDS.  More tokens are
+// further passes over the weights.
 struct ProductArgs {
   const uint8_t *a, *w, *w2;   // tiles of tokens and channels; w2: SwiGLU's up rows (else null)
   const float *sa, *sw, *sw2;
@@ -360,17 +361,23 @@ __device__ __forceinline__ void quantise_rows(const FusedRows& x, int M, int kt,
 }
 
 template <int TF, int QUANT>
-__global__ __launch_bounds__(256) void int8_few_kernel(ProductArgs p, FusedRows x) {
+__global__ __launch_bounds__(256) void int8_few_kernel(ProductArgs p, FusedRows x, int passes) {
   __shared__ v4i red[3][TF][64];
   __shared__ __attribute__((aligned(16))) uint8_t held[QUANT ? kFusedBytes : 16];
   __shared__ float held_scale[kFusedRows];
   __shared__ uint32_t tops[4][kFusedRows];
   const int lane = threadIdx.x & 63, m = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
+  // the passes over a channel tile go to one XCD, whose L2 then holds its weights
+  const int64_t nt = int64_t(blockIdx.x / (8 * passes)) * 8 + blockIdx.x % 8;
+  if (nt * 16 >= p.N) return;
+  const int t0 = int(blockIdx.x / 8 % passes) * TF, last = int((p.M - 1) / 16);   // token tiles
   const int k0 = p.kt * wave / 4, k1 = p.kt * (wave + 1) / 4;
   constexpr int U = TF == 1 ? 8 : 4;
-  const uint8_t* w = p.w + (int64_t(blockIdx.x) * p.kt * 64 + lane) * 16;
-  const uint8_t* a = p.a + lane * 16;
+  const uint8_t* w = p.w + (nt * p.kt * 64 + lane) * 16;
+  const uint8_t* a[TF];
+#pragma unroll
+  for (int f = 0; f < TF; ++f) a[f] = p.a + (int64_t(t0 + f < last ? t0 + f : last) * p.kt * 64 + lane) * 16;
   const uint8_t* mine = held + ((m < p.M ? m : 0) * p.kt * 4 + q) * 16;
   v4i acc[TF];
 #pragma unroll
@@ -383,7 +390,7 @@ __global__ __launch_bounds__(256) void int8_few_kernel(ProductArgs p, FusedRows 
       wv[b][u] = *FM_GLOBAL(const v4i, w + t * 1024);
       if constexpr (QUANT == 0)
 #pragma unroll
-        for (int f = 0; f < TF; ++f) av[b][u][f] = *FM_GLOBAL(const v4i, a + (int64_t(f) * p.kt + t) * 1024);
+        for (int f = 0; f < TF; ++f) av[b][u][f] = *FM_GLOBAL(const v4i, a[f] + t * 1024);
     }
   };
   auto use = [&](int b, int k) {
@@ -412,12 +419,12 @@ __global__ __launch_bounds__(256) void int8_few_kernel(ProductArgs p, FusedRows 
     for (int f = 0; f < TF; ++f) red[wave - 1][f][lane] = acc[f];
   __syncthreads();
   if (wave) return;
-  const int64_t n = int64_t(blockIdx.x) * 16 + 4 * q;
+  const int64_t n = nt * 16 + 4 * q;
   if (n >= p.N) return;
   const v4f sw = four_of(p.sw, n, p.N), bias = p.bias ? four_of(p.bias, n, p.N) : v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int f = 0; f < TF; ++f) {
-    const int64_t t = 16 * f + m;
+    const int64_t t = 16 * (t0 + f) + m;
     if (t >= p.M) break;
     const v4i s = acc[f] + red[0][f][lane] + red[1][f][lane] + red[2][f][lane];
     const float sa = QUANT ? held_scale[m] : p.sa[t];
@@ -869,6 +876,14 @@ void launch_shape(const ProductArgs& p, int64_t tokens, int64_t groups, int64_t 
   else launch_product<Medium, SWIGLU>(p, most(Medium::TJ), s);
 }
 
+// Whether int8_few_kernel takes a product of 16-row tiles of tokens and of channels: up to 6
+// workgroups a CU, or one pass over the weights.  us, it / the 128 x 64 tile (N x K at M): 512 x 4096
+// at 16 3.2 / 14.8, at 512 6.8 / 15.8; 2831 x 1409 at 96 5.8 / 9.1, at 256 8.9 / 9.5, at 384 11.5 / 9.7;
+// 4096 x 4096 at 128 10.4 / 15.9, at 192 14.0 / 16.2, at 256 17.3 / 16.2; 4096 x 14336 at 96 32.3 / 45.8,
+// at 192 52.5 / 50.0; 14336 x 4096 at 32 19.5 / 22.2, at 64 25.2 / 24.1; 28672 x 4096 at 16 24.0 /
+// 26.3, at 32 31.9 / 27.1.
+bool few_rounds(int64_t tiles, int64_t channels) { return tiles == 1 || (tiles + 1) / 2 * channels <= 6 * int64_t(device_cus()); }
+
 // Whether fm_int8_linear quantises in its product's kernel: rows that fit its LDS.
 bool fused_rows(int64_t M, int64_t K) { return M <= kFusedRows && M * ((K + 127) / 128 * 128) <= kFusedBytes; }
 
@@ -938,13 +953,14 @@ int fm_int8_matmul(const void* a, const float* sa, int64_t M, const void* w, con
   const ProductArgs p{static_cast<const uint8_t*>(a), static_cast<const uint8_t*>(w), nullptr, sa, sw, nullptr, 0, 0,
                       int((K + 127) / 128 * 2), M, N, nullptr, 1, bias, out, ld_out, int(out_dtype == FM_DTYPE_F32), nullptr};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (M <= 64) {
-    const dim3 grid{unsigned((N + 15) / 16)}, block(256);
+  const int64_t tiles = (M + 15) / 16, channels = (N + 15) / 16;
+  if (few_rounds(tiles, channels)) {
     const FusedRows none{nullptr, 0, 0};
-    if (M <= 16) hipLaunchKernelGGL((int8_few_kernel<1, 0>), grid, block, 0, st, p, none);
-    else if (M <= 32) hipLaunchKernelGGL((int8_few_kernel<2, 0>), grid, block, 0, st, p, none);
-    else if (M <= 48) hipLaunchKernelGGL((int8_few_kernel<3, 0>), grid, block, 0, st, p, none);
-    else hipLaunchKernelGGL((int8_few_kernel<4, 0>), grid, block, 0, st, p, none);
+    const bool one = tiles * channels <= device_cus() || tiles == 1;
+    const int64_t passes = one ? tiles : (tiles + 1) / 2;
+    const dim3 grid{unsigned((channels + 7) / 8 * 8 * passes)}, block(256);
+    if (one) hipLaunchKernelGGL((int8_few_kernel<1, 0>), grid, block, 0, st, p, none, int(passes));
+    else hipLaunchKernelGGL((int8_few_kernel<2, 0>), grid, block, 0, st, p, none, int(passes));
   } else {
     launch_shape<false>(p, M, 1, 0, st);
   }
@@ -969,10 +985,10 @@ int fm_int8_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ld_
     const ProductArgs p{nullptr, static_cast<const uint8_t*>(w), nullptr, nullptr, sw, nullptr, 0, 0, int((K + 127) / 128 * 2), M, N, nullptr, 1,
                         bias, out, ld_out, int(out_dtype == FM_DTYPE_F32), nullptr};
     const FusedRows r{x, ld_x, K};
-    const dim3 grid{unsigned((N + 15) / 16)}, block(256);
+    const dim3 grid{unsigned(((N + 15) / 16 + 7) / 8 * 8)}, block(256);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (x_dtype == FM_DTYPE_F32) hipLaunchKernelGGL((int8_few_kernel<1, 2>), grid, block, 0, st, p, r);
-    else hipLaunchKernelGGL((int8_few_kernel<1, 1>), grid, block, 0, st, p, r);
+    if (x_dtype == FM_DTYPE_F32) hipLaunchKernelGGL((int8_few_kernel<1, 2>), grid, block, 0, st, p, r, 1);
+    else hipLaunchKernelGGL((int8_few_kernel<1, 1>), grid, block, 0, st, p, r, 1);
     return check_launch("fm_int8_linear");
   }
   FM_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= fm_int8_linear_workspace_bytes(M, K),

@@ -87,7 +87,8 @@ def check_product(out, qa, sa, qw, sw, bias):
 
 SHAPES = [(1, 1, 1), (1, 17, 64), (3, 100, 130), (16, 48, 128), (17, 33, 1000), (33, 65, 200), (48, 15, 640), (49, 300, 2049),
           (64, 64, 4096), (65, 1, 100), (65, 127, 257), (100, 129, 64), (128, 128, 128), (129, 257, 300), (300, 500, 700),
-          (1000, 640, 1409), (4097, 2049, 130), (4300, 2300, 200), (4090, 4300, 200), (1500, 3500, 130)]
+          (1000, 640, 1409), (4097, 2049, 130), (4300, 2300, 200), (4090, 4300, 200), (1500, 3500, 130), (65, 9001, 300), (129, 6001, 257),
+          (300, 3001, 700), (33, 20001, 64), (512, 700, 130), (3000, 5, 300)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
