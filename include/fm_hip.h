@@ -649,7 +649,7 @@ int fm_decode_experts(const void* x, const void* x_lo, int64_t ld_x, int64_t T, 
  * matrix cores' fragments: element (r, k) at byte
  *   ((r / 16 * kt + k / 64) * 64 + k % 64 / 16 * 16 + r % 16) * 16 + k % 16,
  * kt = 2 ceil(K / 128), zeros in the padding; ceil(R / 16) * kt * 1024 bytes on a
- * 16-byte boundary, 16 ceil(R / 16) scales.  Groups (experts) follow one another.
+ * 16-byte boundary, R scales.  Groups (experts) follow one another.
  *
  * fm_int8_quantize: rows of x (bf16 or fp32, any element-aligned base and pitch):
  *   s = max(amax, 1e-12) / 127, q = rint(x / s), ties to even; a row with a NaN or an

@@ -146,7 +146,7 @@ __global__ __launch_bounds__(64 * kQuantWaves) void int8_quant_kernel(QuantArgs 
   if constexpr (GIVEN) {
     const uint32_t top = valid ? a.top[r0 + r] : 0u;
     const float s = int8_scale(top);
-    if (blockIdx.y == 0 && threadIdx.x < RW) st_global(a.s + r0 + r, s);
+    if (blockIdx.y == 0 && threadIdx.x < RW && r0 + r < a.R) st_global(a.s + r0 + r, s);
     const Recip d = recip_of(s);
 #pragma unroll 4
     for (int c = c0 + step * blockIdx.y; c < n; c += step * gridDim.y) {
@@ -181,7 +181,7 @@ __global__ __launch_bounds__(64 * kQuantWaves) void int8_quant_kernel(QuantArgs 
     for (int w = 0; w < kQuantWaves; ++w) top = tops[w][r] > top ? tops[w][r] : top;
     const float s = int8_scale(top);
     const bool finite = top <= 0x7f7fffffu;
-    if (threadIdx.x < RW) st_global(a.s + r0 + r, s);
+    if (threadIdx.x < RW && r0 + r < a.R) st_global(a.s + r0 + r, s);
     const Recip d = recip_of(s);
     if constexpr (NT > 0) {
 #pragma unroll

@@ -59,7 +59,7 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     _lib.require_device(x, "x")
     if x.dim() < 1 or x.dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"x must be a bfloat16 or float32 [..., D], got {x.dtype} {tuple(x.shape)}")
-    x2 = x.reshape(-1, x.shape[-1])
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     if x2.dtype != torch.bfloat16:
         x2 = x2.to(torch.bfloat16)
     T, D = x2.shape
@@ -103,13 +103,15 @@ def _weights_struct(experts, num_experts: int, x: torch.Tensor, what: str) -> _l
     H = shape[0] // num_experts
     if H % 128 or not H:
         raise ValueError(f"{what}: hidden size must be a multiple of 128, got {H}")
-    for t in experts:
+    at = []
+    for t in (w1, w2, w3):
         if t.dtype != torch.bfloat16:
             raise TypeError(f"{what}: weights must be bfloat16 (or Int8Experts), got {t.dtype}")
-        if not t.is_contiguous() or t.data_ptr() % 16:
+        at.append(t.data_ptr())
+        if at[-1] % 16 or not t.is_contiguous():
             raise ValueError(f"{what}: weights must be contiguous, on 16-byte boundaries")
     _same_device(x, w1=w1, w2=w2, w3=w3)
-    return _lib.FmDecodeWeights(_lib.DECODE_BF16, H, w1.data_ptr(), w2.data_ptr(), w3.data_ptr())
+    return _lib.FmDecodeWeights(_lib.DECODE_BF16, H, *at)
 
 
 def _both(experts, num_experts, shared, x):

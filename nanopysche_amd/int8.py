@@ -76,8 +76,8 @@ class Int8Tensor:
 
 
 def _empty(rows: int, cols: int, dev) -> Int8Tensor:
-    scale = torch.empty((rows + 15) // 16 * 16, dtype=torch.float32, device=dev)   # the kernels fill whole tiles
-    return Int8Tensor(torch.empty(_payload_bytes(rows, cols), dtype=torch.uint8, device=dev), scale[:rows], rows, cols)
+    return Int8Tensor(torch.empty(_payload_bytes(rows, cols), dtype=torch.uint8, device=dev),
+                      torch.empty(rows, dtype=torch.float32, device=dev), rows, cols)
 
 
 def _pack(q: torch.Tensor, scale: torch.Tensor) -> Int8Tensor:
@@ -124,9 +124,10 @@ def _float_rows(x: torch.Tensor) -> torch.Tensor:
     if x.dim() < 1:
         raise ValueError("expected a tensor with at least 1 dimension")
     _check_cols(x.shape[-1])
-    x2 = x.reshape(-1, x.shape[-1])
-    ld = x2.stride(0) if x2.shape[0] > 1 else x2.shape[1]
-    return x2 if x2.stride(1) == 1 and ld >= x2.shape[1] else x2.contiguous()
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    rows, cols = x2.shape
+    ld, one = x2.stride()
+    return x2 if one == 1 and (ld >= cols or rows == 1) else x2.contiguous()
 
 
 def quantize_to_int8(x: torch.Tensor) -> Int8Tensor:
@@ -153,7 +154,7 @@ def _bias(bias: Optional[torch.Tensor], N: int) -> Optional[torch.Tensor]:
         return None
     if tuple(bias.shape) != (N,):
         raise ValueError(f"bias must be [{N}], got {tuple(bias.shape)}")
-    return bias.to(torch.float32).contiguous()
+    return bias if bias.dtype == torch.float32 and bias.is_contiguous() else bias.to(torch.float32).contiguous()
 
 
 def int8_matmul(a: Int8Tensor, b: Int8Tensor, bias: Optional[torch.Tensor] = None,
