@@ -368,10 +368,10 @@ __global__ __launch_bounds__(256) void int8_few_kernel(ProductArgs p, FusedRows 
   __shared__ uint32_t tops[4][kFusedRows];
   const int lane = threadIdx.x & 63, m = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
-  // the passes over a channel tile go to one XCD, whose L2 then holds its weights
-  const int64_t nt = int64_t(blockIdx.x / (8 * passes)) * 8 + blockIdx.x % 8;
+  // an XCD takes a run of channel tiles with all of their passes, so its L2 holds the weights for them
+  const int64_t id = int64_t(blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8, nt = id / passes;
   if (nt * 16 >= p.N) return;
-  const int t0 = int(blockIdx.x / 8 % passes) * TF, last = int((p.M - 1) / 16);   // token tiles
+  const int t0 = int(id % passes) * TF, last = int((p.M - 1) / 16);   // token tiles
   const int k0 = p.kt * wave / 4, k1 = p.kt * (wave + 1) / 4;
   constexpr int U = TF == 1 ? 8 : 4;
   const uint8_t* w = p.w + (nt * p.kt * 64 + lane) * 16;
@@ -958,7 +958,7 @@ int fm_int8_matmul(const void* a, const float* sa, int64_t M, const void* w, con
     const FusedRows none{nullptr, 0, 0};
     const bool one = tiles * channels <= device_cus() || tiles == 1;
     const int64_t passes = one ? tiles : (tiles + 1) / 2;
-    const dim3 grid{unsigned((channels + 7) / 8 * 8 * passes)}, block(256);
+    const dim3 grid{unsigned((channels * passes + 7) / 8 * 8)}, block(256);
     if (one) hipLaunchKernelGGL((int8_few_kernel<1, 0>), grid, block, 0, st, p, none, int(passes));
     else hipLaunchKernelGGL((int8_few_kernel<2, 0>), grid, block, 0, st, p, none, int(passes));
   } else {
