@@ -368,8 +368,9 @@ __global__ __launch_bounds__(256) void int8_few_kernel(ProductArgs p, FusedRows 
   __shared__ uint32_t tops[4][kFusedRows];
   const int lane = threadIdx.x & 63, m = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
-  // an XCD takes a run of channel tiles with all of their passes, so its L2 holds the weights for them
-  const int64_t id = int64_t(blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8, nt = id / passes;
+  // an XCD takes a run of channel tiles with all of their passes, so its L2 holds the weights for
+  // them; weights that are read once go in order (1 x 4096 -> 14336: 11.6 us, in runs 12.4)
+  const int64_t id = passes == 1 ? blockIdx.x : int64_t(blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8, nt = id / passes;
   if (nt * 16 >= p.N) return;
   const int t0 = int(id % passes) * TF, last = int((p.M - 1) / 16);   // token tiles
   const int k0 = p.kt * wave / 4, k1 = p.kt * (wave + 1) / 4;
