@@ -855,6 +855,11 @@ void launch_product(const ProductArgs& p, int64_t token_tiles, hipStream_t s) {
 // 4096 46 / 36 / 39; 4096 x 2816 x 2048 37.3 / 35.7 / 34.1; 4096 x 4096 x 14336 308 / 224 / 194;
 // 8192 x 14336 x 4096 652 / 538 / 424.  Halved last rounds: the large shape 47 -> 33.8 at
 // 1024 x 4096 x 4096 and 348 -> 304 for 4096 slots on 8 experts x 4096 x 14336.
+// Over a plan whose groups hold a token tile of the 256 x 128 shape or less, weights that are read
+// once bound every shape, and that one reads them fastest: us of gate|up and down, small / medium /
+// large, 65 tokens x 2 on 8 experts of 4096 x 14336 248 / 193 / 218 and 126 / 129 / 139; 128 x 8 on 32
+// of 7168 x 2048 248 / 207 / 213 and 133 / 119 / 128; 1024 x 6 on 64 of 2048 x 1408 102 / 98 / 104
+// and 70 / 62 / 63; 512 x 2 on 8 of 4096 x 14336 331 / 260 / 239 and 158 / 135 / 138.
 // tokens over `groups` groups (dense: one); rows: of the padded buffer, or 0.
 template <bool SWIGLU>
 void launch_shape(const ProductArgs& p, int64_t tokens, int64_t groups, int64_t rows, hipStream_t s) {
@@ -872,7 +877,9 @@ void launch_shape(const ProductArgs& p, int64_t tokens, int64_t groups, int64_t 
   const int64_t small_us = small <= cus ? 32 : 42 * rounds(small, 2 * cus);
   // a bound of the token tiles: every group is a multiple of 128 rows
   auto most = [&](int64_t tj) { return rows ? rows / 128 * (tj < 128 ? 128 / tj : 1) : (tokens + tj - 1) / tj; };
-  if (small_us <= medium_us && small_us <= large_us) launch_product<Small, SWIGLU>(p, most(Small::TJ), s);
+  const bool stream = rows && tokens <= groups * Medium::TJ && groups * ((p.N * up + Medium::TI - 1) / Medium::TI) * 2 >= cus;
+  if (stream) launch_product<Medium, SWIGLU>(p, most(Medium::TJ), s);
+  else if (small_us <= medium_us && small_us <= large_us) launch_product<Small, SWIGLU>(p, most(Small::TJ), s);
   else if (large_us <= medium_us * 108 / 100) launch_product<Large, SWIGLU>(p, most(Large::TJ), s);
   else launch_product<Medium, SWIGLU>(p, most(Medium::TJ), s);
 }
