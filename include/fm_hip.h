@@ -654,8 +654,8 @@ int fm_decode_experts(const void* x, const void* x_lo, int64_t ld_x, int64_t T, 
  * fm_int8_quantize: rows of x (bf16 or fp32, any element-aligned base and pitch):
  *   s = max(amax, 1e-12) / 127, q = rint(x / s), ties to even; a row with a NaN or an
  *   infinity gets scale NaN or infinity and zero payload.  With assign_of_row, output
- *   row r is row assign_of_row[r] / top_k of x (zeros where negative: a routing plan's
- *   padding); rows from *limit (a multiple of 16, device memory, or NULL) on are left
+ *   row r is row assign_of_row[r] / top_k of x (zeros and scale 0 where negative: a
+ *   routing plan's padding); rows from *limit (a multiple of 16, device memory, or NULL) on are left
  *   as they are.  top (or NULL): the rows' largest magnitudes as fp32 bits, if they are
  *   known; clear (or NULL): words set to 0, one a row and 16 ceil(rows / 16) in all.
  * fm_int8_pack: int8 values with byte strides into tiles.  fm_int8_unpack: tiles into
@@ -667,7 +667,7 @@ int fm_decode_experts(const void* x, const void* x_lo, int64_t ld_x, int64_t T, 
  *   tokens times expert e's channels; `tokens` is the host's estimate of the rows that
  *   hold one (it only picks a kernel).  With w_up, out is silu(gate) * up in fp32 (N = H
  *   a multiple of 128) and top[r] is raised to the largest magnitude of row r, as fp32
- *   bits.  K a multiple of 128, N of 16.
+ *   bits; tokens of scale 0 are left out of both.  K a multiple of 128, N of 16.
  * fm_int8_combine: out[t] = sum_k weights[t, k] y[row_of[t * K + k]], y [rows, D] fp32,
  *   negative rows adding nothing. */
 #define FM_INT8_TO_BF16 0

@@ -148,10 +148,11 @@ __global__ __launch_bounds__(64 * kQuantWaves) void int8_quant_kernel(QuantArgs 
     const float s = int8_scale(top);
     if (blockIdx.y == 0 && threadIdx.x < RW && r0 + r < a.R) st_global(a.s + r0 + r, s);
     const Recip d = recip_of(s);
+    const int64_t read = top ? C : 0;   // a row of zeros (a plan's padding) need not be there
 #pragma unroll 4
     for (int c = c0 + step * blockIdx.y; c < n; c += step * gridDim.y) {
       Raw<F32> v;
-      v.load(row, int64_t(c) * 16, C);
+      v.load(row, int64_t(c) * 16, read);
       put(v, d, top <= 0x7f7fffffu, c);
     }
   } else {
@@ -181,7 +182,7 @@ __global__ __launch_bounds__(64 * kQuantWaves) void int8_quant_kernel(QuantArgs 
     for (int w = 0; w < kQuantWaves; ++w) top = tops[w][r] > top ? tops[w][r] : top;
     const float s = int8_scale(top);
     const bool finite = top <= 0x7f7fffffu;
-    if (threadIdx.x < RW && r0 + r < a.R) st_global(a.s + r0 + r, s);
+    if (threadIdx.x < RW && r0 + r < a.R) st_global(a.s + r0 + r, valid ? s : 0.f);   // 0 marks a plan's padding
     const Recip d = recip_of(s);
     if constexpr (NT > 0) {
 #pragma unroll
@@ -486,6 +487,7 @@ __device__ __forceinline__ void store_tile(const ProductArgs& p, const OutTile& 
 #pragma unroll
   for (int y = 0; y < FB; ++y) sa[y] = tw + 16 * y + m < cur.j1 ? *FM_GLOBAL(const float, p.sa + tw + 16 * y + m) : 0.f;
   if constexpr (SWIGLU) {
+    // rows of scale 0 are none or a plan's padding, whose h nothing reads
     uint32_t top[FB];
 #pragma unroll
     for (int y = 0; y < FB; ++y) top[y] = 0;
@@ -504,7 +506,7 @@ __device__ __forceinline__ void store_tile(const ProductArgs& p, const OutTile& 
           const uint32_t b = f2u(h[i]) & 0x7fffffffu;   // a NaN is above infinity, infinity above every number
           top[y] = b > top[y] ? b : top[y];
         }
-        if (t < cur.j1) st_global(static_cast<float*>(p.out) + t * p.ld_out + n, make_float4(h[0], h[1], h[2], h[3]));
+        if (sa[y] != 0.f) st_global(static_cast<float*>(p.out) + t * p.ld_out + n, make_float4(h[0], h[1], h[2], h[3]));
       }
     }
     // a maximum does not depend on the order in which the waves raise it
@@ -515,7 +517,7 @@ __device__ __forceinline__ void store_tile(const ProductArgs& p, const OutTile& 
         const uint32_t o = __shfl_xor(top[y], off);
         top[y] = o > top[y] ? o : top[y];
       }
-      if (q == 0 && tw + 16 * y + m < cur.j1) atomicMax(p.top + tw + 16 * y + m, top[y]);
+      if (q == 0 && sa[y] != 0.f) atomicMax(p.top + tw + 16 * y + m, top[y]);
     }
   } else {
     static_assert(FA % 2 == 0 && FB % 2 == 0, "blocks in squares of four");

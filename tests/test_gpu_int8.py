@@ -9,6 +9,7 @@ import pytest
 import torch
 
 import nanopysche_amd as fm
+from nanopysche_amd import _lib
 from nanopysche_amd.int8 import MAX_INT8_K, _pack, _quantize
 from tests.helpers import randn_bf16, zipf_routing
 from tests.test_gpu_decode import check, expert_weights, layer64
@@ -155,7 +156,31 @@ def test_quantise_of_a_plan_gathers_and_stops(dev):
     q, s = plain_rows(x)
     got, a = t.values()[:end].float(), plan.assign_of_row[:end].long()
     assert torch.equal(got[a >= 0], q[a[a >= 0] // K]) and torch.equal(t.scale[:end][a >= 0], s[a[a >= 0] // K])
-    assert torch.all(got[a < 0] == 0)
+    assert torch.all(got[a < 0] == 0) and torch.all(t.scale[:end][a < 0] == 0)
+
+
+def test_padding_of_a_plan_is_left_out_of_swiglu(dev):
+    """Its h is not written, its maximum not raised, and a row of maximum 0 is not read."""
+    T, E, K, D, H = 100, 6, 2, 256, 384
+    _, idx = zipf_routing(T, E, K, 1.0, seed=3, zero_experts=(2,))
+    plan = fm.route_tokens(idx.to(dev), E)
+    end = int(plan.offsets[E])
+    x = randn_bf16((T, D), seed=1).to(dev)
+    x[3] = 0
+    x[4] *= 1e-30   # below the scale's floor: a row like another
+    t = _quantize(x, plan.rows_max, plan.assign_of_row, K, plan.offsets[E:])
+    w = [fm.Int8Tensor.from_int8(*random_int8(dev, E * H, D, s)) for s in (2, 3)]
+    top = torch.zeros(plan.rows_max, dtype=torch.int32, device=dev)
+    h = torch.full((plan.rows_max, H), float("nan"), device=dev)
+    _lib.call("fm_int8_grouped_gemm", t.data.data_ptr(), t.scale.data_ptr(), t.rows, plan.offsets.data_ptr(), E, w[0].data.data_ptr(),
+              w[0].scale.data_ptr(), w[1].data.data_ptr(), w[1].scale.data_ptr(), top.data_ptr(), H, D, T * K, h.data_ptr(),
+              _lib.DTYPE_F32, H, _lib.stream_of(h))
+    pad = plan.assign_of_row[:end] < 0
+    assert pad.any() and torch.isnan(h[:end][pad]).all() and torch.isfinite(h[:end][~pad]).all()
+    assert torch.equal(top[:end].view(torch.float32), torch.where(pad, 0, h[:end].abs().amax(1)))
+    q = _quantize(h, plan.rows_max, limit=plan.offsets[E:], top=top)
+    got, want = q.values()[:end].float(), plain_rows(h[:end][~pad])
+    assert torch.all(got[pad] == 0) and torch.equal(got[~pad], want[0]) and torch.equal(q.scale[:end][~pad], want[1])
 
 
 @pytest.mark.parametrize("R,C", [(1, 1), (16, 64), (17, 65), (48, 128), (160, 300), (33, 1)])
