@@ -24,6 +24,7 @@ from .decode import MAX_DECODE_DIM, MAX_DECODE_TOKENS, MAX_DECODE_TOP_K, _no_gra
 from .routing import RoutingPlan, route_tokens
 
 MAX_INT8_K = 131071   # longest product whose int32 sums cannot overflow
+MAX_INT8_ROWS = 2 ** 31 - 256   # rows of an operand are fewer
 
 
 def _payload_bytes(rows: int, cols: int) -> int:
@@ -35,18 +36,55 @@ def _check_cols(cols: int) -> None:
         raise ValueError(f"int8 rows hold 1 to {MAX_INT8_K} columns, got {cols}")
 
 
+def _check_payload(data: torch.Tensor, rows: int, cols: int) -> None:
+    if not isinstance(data, torch.Tensor) or data.dtype != torch.uint8:
+        raise TypeError(f"data must be a uint8 tensor, got {getattr(data, 'dtype', type(data))}")
+    if data.numel() < _payload_bytes(rows, cols) or not data.is_contiguous():
+        raise ValueError(f"data must be {_payload_bytes(rows, cols)} contiguous bytes for [{rows}, {cols}], "
+                         f"got {tuple(data.shape)} of strides {data.stride()}")
+
+
+def _check_scale(scale: torch.Tensor, rows: int, data: torch.Tensor) -> None:
+    if not isinstance(scale, torch.Tensor) or scale.dtype != torch.float32:
+        raise TypeError(f"scale must be a float32 tensor, got {getattr(scale, 'dtype', type(scale))}")
+    if scale.shape != (rows,) or not scale.is_contiguous() or scale.device != data.device:
+        raise ValueError(f"scale must be [{rows}], contiguous, on {data.device}, got {tuple(scale.shape)} of strides "
+                         f"{scale.stride()} on {scale.device}")
+
+
 @dataclass
 class Int8Tensor:
     """An int8 matrix [rows, cols] with an fp32 scale per row.
 
     data   uint8 buffer: 16 x 64 tiles in the matrix cores' order (``include/fm_hip.h``)
-    scale  [rows] fp32
+    scale  [rows] fp32, contiguous, on the buffer's device
+
+    The kernels read as far as rows and cols say, so the fields are checked when they are
+    set: data and scale may be replaced by tensors that fit, the sizes stay.
     """
 
     data: torch.Tensor
     scale: torch.Tensor
     rows: int
     cols: int
+
+    def __post_init__(self):
+        if not isinstance(self.rows, int) or not isinstance(self.cols, int) or not 0 <= self.rows < MAX_INT8_ROWS:
+            raise ValueError(f"rows and cols must be whole numbers, rows 0 to {MAX_INT8_ROWS - 1}, got {self.rows} and {self.cols}")
+        _check_cols(self.cols)
+        _check_payload(self.data, self.rows, self.cols)
+        _check_scale(self.scale, self.rows, self.data)
+
+    def __setattr__(self, name, value):
+        if "cols" in self.__dict__:   # the last field that __init__ sets
+            if name in ("rows", "cols"):
+                raise AttributeError(f"the sizes of an Int8Tensor do not change: {name}")
+            if name == "data":
+                _check_payload(value, self.rows, self.cols)
+                _check_scale(self.scale, self.rows, value)
+            elif name == "scale":
+                _check_scale(value, self.rows, self.data)
+        object.__setattr__(self, name, value)
 
     @property
     def shape(self):
@@ -76,8 +114,10 @@ class Int8Tensor:
 
 
 def _empty(rows: int, cols: int, dev) -> Int8Tensor:
-    return Int8Tensor(torch.empty(_payload_bytes(rows, cols), dtype=torch.uint8, device=dev),
-                      torch.empty(rows, dtype=torch.float32, device=dev), rows, cols)
+    t = Int8Tensor.__new__(Int8Tensor)   # fits by construction: 2 us of checks less a call
+    t.__dict__.update(data=torch.empty(_payload_bytes(rows, cols), dtype=torch.uint8, device=dev),
+                      scale=torch.empty(rows, dtype=torch.float32, device=dev), rows=rows, cols=cols)
+    return t
 
 
 def _pack(q: torch.Tensor, scale: torch.Tensor) -> Int8Tensor:
