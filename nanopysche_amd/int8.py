@@ -272,12 +272,38 @@ def _grouped(tokens, w, up, top, plan, N, out_dtype):
 @dataclass
 class Int8Experts:
     """SwiGLU experts in int8, laid out once: w1, w3 [E * H, D] with a scale per hidden
-    unit, w2 transposed [E * D, H] with a scale per output column."""
+    unit, w2 transposed [E * D, H] with a scale per output column; H and D multiples of 128.
+    The fields are checked when they are set: one may be replaced by one that fits the others."""
 
     w1: Int8Tensor
     w2: Int8Tensor
     w3: Int8Tensor
     num_experts: int
+
+    def __post_init__(self):
+        self._check(self.w1, self.w2, self.w3, self.num_experts)
+
+    def __setattr__(self, name, value):
+        if "num_experts" in self.__dict__:   # the last field that __init__ sets
+            self._check(*(value if f == name else getattr(self, f) for f in ("w1", "w2", "w3", "num_experts")))
+        object.__setattr__(self, name, value)
+
+    @staticmethod
+    def _check(w1, w2, w3, num_experts):
+        for name, w in (("w1", w1), ("w2", w2), ("w3", w3)):
+            if not isinstance(w, Int8Tensor):
+                raise TypeError(f"{name} must be an Int8Tensor, got {type(w)}")
+        E = num_experts
+        if not isinstance(E, int) or E < 1 or w1.rows % E:
+            raise ValueError(f"num_experts must be a positive whole number that divides w1's {w1.rows} rows, got {E}")
+        H, D = w1.rows // E, w1.cols
+        if w3.shape != (E * H, D) or w2.shape != (E * D, H):
+            raise ValueError(f"w1 {tuple(w1.shape)} of {E} experts needs w3 [{E * H}, {D}] and w2, transposed, [{E * D}, {H}], "
+                             f"got {tuple(w3.shape)} and {tuple(w2.shape)}")
+        if H % 128 or D % 128:
+            raise ValueError(f"d_model ({D}) and hidden_size ({H}) must be multiples of 128")
+        if w2.device != w1.device or w3.device != w1.device:
+            raise ValueError(f"w1, w2 and w3 must be on one device, got {w1.device}, {w2.device} and {w3.device}")
 
     @property
     def hidden_size(self) -> int:

@@ -79,3 +79,47 @@ def test_what_fits_is_accepted(launched):  # noqa: F811
         e.scale = torch.ones(32)
     fm.int8_linear(bf(3, 256), t)
     assert launched == ["fm_int8_linear"]
+
+
+WRONG_EXPERTS = [
+    (ValueError, "transposed", dict(w2=int8_tensor(4 * 128, 256))),   # as the expert block stores it
+    (ValueError, "transposed", dict(w3=int8_tensor(16, 256))),
+    (ValueError, "transposed", dict(w1=int8_tensor(4 * 256, 256))),
+    (ValueError, "transposed", dict(w1=int8_tensor(4 * 128, 384))),
+    (ValueError, "num_experts", dict(num_experts=0)),
+    (ValueError, "num_experts", dict(num_experts=3)),
+    (ValueError, "num_experts", dict(num_experts=4.0)),
+    (ValueError, "transposed", dict(num_experts=8)),
+    (TypeError, "Int8Tensor", dict(w3=torch.zeros(4 * 128, 256))),
+    (ValueError, "one device", dict(w2=Int8Tensor(torch.zeros(4 * 256 * 128, dtype=U8, device="meta"),
+                                                  torch.ones(4 * 256, device="meta"), 4 * 256, 128))),
+]
+
+
+def experts(**kw):
+    f = dict(w1=int8_tensor(4 * 128, 256), w2=int8_tensor(4 * 256, 128), w3=int8_tensor(4 * 128, 256), num_experts=4)
+    f.update(kw)
+    return f
+
+
+@pytest.mark.parametrize("error,match,wrong", WRONG_EXPERTS + [
+    (ValueError, "multiples of 128", dict(w1=int8_tensor(4 * 64, 256), w2=int8_tensor(4 * 256, 64), w3=int8_tensor(4 * 64, 256))),
+    (ValueError, "multiples of 128", dict(w1=int8_tensor(4 * 128, 192), w2=int8_tensor(4 * 192, 128), w3=int8_tensor(4 * 128, 192))),
+    (ValueError, "transposed", dict(w1=int8_tensor(0, 256), w3=int8_tensor(0, 256))),
+])
+def test_experts_that_do_not_fit_each_other_are_refused(error, match, wrong):
+    with pytest.raises(error, match=match):
+        fm.Int8Experts(**experts(**wrong))
+
+
+@pytest.mark.parametrize("error,match,wrong", WRONG_EXPERTS)
+def test_experts_are_replaced_only_by_ones_that_fit(error, match, wrong):
+    e = fm.Int8Experts(**experts())
+    before = dict(e.__dict__)
+    with pytest.raises(error, match=match):
+        for name, value in wrong.items():
+            setattr(e, name, value)
+    assert all(e.__dict__[n] is v for n, v in before.items())
+    e.label = "layer 3"   # a program's own attribute
+    e.w1 = int8_tensor(4 * 128, 256)
+    assert e.w1 is not before["w1"] and (e.hidden_size, e.d_model) == (128, 256)
