@@ -89,6 +89,7 @@ def _weights_struct(experts, num_experts: int, x: torch.Tensor, what: str) -> _l
                              f"expected {num_experts} of width {D}")
         _same_device(x, **{what: experts.w1.data})
         w1, w2, w3 = experts.w1, experts.w2, experts.w3
+        _no_gradients(w1.scale, w2.scale, w3.scale)
         return _lib.FmDecodeWeights(_lib.DECODE_INT8, experts.hidden_size, w1.data.data_ptr(), w2.data.data_ptr(),
                                     w3.data.data_ptr(), w1.scale.data_ptr(), w2.scale.data_ptr(), w3.scale.data_ptr())
     try:

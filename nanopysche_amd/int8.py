@@ -110,6 +110,7 @@ class Int8Tensor:
         """q * scale, rounded once to ``out_dtype`` (bf16 or fp32)."""
         if out_dtype not in (torch.bfloat16, torch.float32):
             raise TypeError("out_dtype must be bfloat16 or float32")
+        _no_gradients(self.scale)
         return _unpack(self, out_dtype)
 
 
@@ -124,6 +125,7 @@ def _pack(q: torch.Tensor, scale: torch.Tensor) -> Int8Tensor:
     """Groups q [G, rows, cols] one after the other."""
     G, R, K = q.shape
     _check_cols(K)
+    _no_gradients(scale)
     if tuple(scale.shape) != (G * R,) or scale.device != q.device:
         raise ValueError(f"scale must be [{G * R}] on {q.device}, got {tuple(scale.shape)} on {scale.device}")
     t = _empty(G * R, K, q.device)
@@ -205,7 +207,7 @@ def int8_matmul(a: Int8Tensor, b: Int8Tensor, bias: Optional[torch.Tensor] = Non
     if a.cols != b.cols:
         raise ValueError(f"a has {a.cols} columns, b {b.cols}")
     code = _out_code(out_dtype)
-    _no_gradients(bias)
+    _no_gradients(a.scale, b.scale, bias)
     _same_device(a.data, b=b.data, bias=bias)
     M, N = a.rows, b.rows
     bias = _bias(bias, N)
@@ -227,7 +229,7 @@ def int8_linear(x: torch.Tensor, weight: Int8Tensor, bias: Optional[torch.Tensor
     out_dtype = x.dtype if out_dtype is None else out_dtype
     code = _out_code(out_dtype)
     x2 = _float_rows(x)
-    _no_gradients(x, bias)
+    _no_gradients(x, weight.scale, bias)
     _same_device(x, weight=weight.data, bias=bias)
     M, K = x2.shape
     N = weight.rows
@@ -254,6 +256,7 @@ def int8_grouped_gemm(tokens: Int8Tensor, weights: Int8Tensor, plan: RoutingPlan
         raise ValueError(f"tokens [{tokens.rows}, {tokens.cols}] and weights [{weights.rows}, {weights.cols}] do not fit "
                          f"a plan of {plan.rows_max} rows and {E} experts")
     _out_code(out_dtype)
+    _no_gradients(tokens.scale, weights.scale)
     _same_device(tokens.data, weights=weights.data, plan=plan.offsets)
     with _lib.on_device_of(tokens.data):
         return _grouped(tokens, weights, None, None, plan, weights.rows // E, out_dtype)
@@ -369,7 +372,7 @@ class Int8MoECompute:
         T, D = x2.shape
         if D != w.d_model:
             raise ValueError(f"x has {D} columns, the experts {w.d_model}")
-        _no_gradients(x, weights)
+        _no_gradients(x, weights, w.w1.scale, w.w2.scale, w.w3.scale)
         _same_device(x, weights=weights, indices=indices, experts=w.w1.data)
         K = indices.shape[-1] if indices.dim() else 0
         if K < 1 or indices.numel() != T * K or weights.numel() != T * K or weights.shape[-1] != K:

@@ -8,7 +8,7 @@ import torch
 
 import nanopysche_amd as fm
 from nanopysche_amd.int8 import Int8Tensor, _empty
-from tests.test_host_decode_int8 import bf, int8_tensor, launched  # noqa: F401
+from tests.test_host_decode_int8 import IDX, bf, int8_experts, int8_tensor, launched  # noqa: F401
 
 U8 = torch.uint8
 FITS = 8 * 2048   # bytes of [64, 256]
@@ -123,3 +123,59 @@ def test_experts_are_replaced_only_by_ones_that_fit(error, match, wrong):
     e.label = "layer 3"   # a program's own attribute
     e.w1 = int8_tensor(4 * 128, 256)
     assert e.w1 is not before["w1"] and (e.hidden_size, e.d_model) == (128, 256)
+
+
+def plan_of(rows, E):
+    """A plan of one token, as far as the checks read it."""
+    i32 = torch.zeros(rows, dtype=torch.int32)
+    return fm.RoutingPlan(1, 1, E, rows, i32[:E], torch.zeros(E + 1, dtype=torch.int32), i32[:1], i32, i32[:1], i32[:E])
+
+
+def learned(t):
+    t.scale.requires_grad_()
+    return t
+
+
+def learned_experts(name, E=4, H=128, D=256):
+    ex = int8_experts(E, H, D)
+    learned(getattr(ex, name))
+    return ex
+
+
+Q = torch.zeros(512, 256, dtype=torch.int8)
+USES_OF_SCALES = {
+    "from_int8": lambda: Int8Tensor.from_int8(Q[:3], torch.ones(3, requires_grad=True)),
+    "experts_from_int8": lambda: fm.Int8Experts.from_int8(Q, torch.ones(512), Q, torch.ones(4, 256, requires_grad=True), Q,
+                                                          torch.ones(512), 4),
+    "dequantize": lambda: learned(int8_tensor(3, 100)).dequantize(),
+    "matmul_a": lambda: fm.int8_matmul(learned(int8_tensor(3, 100)), int8_tensor(4, 100)),
+    "matmul_b": lambda: fm.int8_matmul(int8_tensor(3, 100), learned(int8_tensor(4, 100))),
+    "linear": lambda: fm.int8_linear(bf(3, 100), learned(int8_tensor(4, 100))),
+    "grouped_tokens": lambda: fm.int8_grouped_gemm(learned(int8_tensor(256, 128)), int8_tensor(64, 128), plan_of(256, 2)),
+    "grouped_weights": lambda: fm.int8_grouped_gemm(int8_tensor(256, 128), learned(int8_tensor(64, 128)), plan_of(256, 2)),
+    **{f"block_{n}_{T}": lambda n=n, T=T: fm.Int8MoECompute(learned_experts(n))(bf(T, 256), torch.ones(T, 1),
+                                                                            torch.zeros(T, 1, dtype=torch.int64))
+       for n in ("w1", "w2", "w3") for T in (3, 70)},
+    "decode": lambda: fm.moe_decode(bf(3, 256), bf(4, 256), learned_experts("w3"), 2),
+    "decode_shared": lambda: fm.moe_decode(bf(3, 256), bf(4, 256), int8_experts(4, 128, 256), 2,
+                                           shared=learned_experts("w2", 1)),
+    "expert_decode": lambda: fm.expert_decode(bf(3, 256), torch.ones(3, 2), IDX, learned_experts("w1"), 4),
+}
+
+
+@pytest.mark.parametrize("name", USES_OF_SCALES)
+def test_a_scale_that_requires_a_gradient_is_refused(launched, name):  # noqa: F811
+    with pytest.raises(RuntimeError, match="forward only"):
+        USES_OF_SCALES[name]()
+    assert launched == []
+    if not name.startswith("block") or name.endswith("_3"):   # a plan's sizes come from the library, its arrays from the GPU
+        with torch.no_grad():
+            USES_OF_SCALES[name]()
+        assert launched
+
+
+def test_a_packed_scale_carries_no_gradient(launched):  # noqa: F811
+    with torch.no_grad():
+        t = Int8Tensor.from_int8(Q[:3], torch.ones(3, requires_grad=True))
+    assert not t.scale.requires_grad
+    assert fm.int8_linear(bf(3, 256), t).shape == (3, 3) and t.values().shape == (3, 256)
