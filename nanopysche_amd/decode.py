@@ -20,6 +20,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from . import _lib
 from .norm import DEFAULT_EPS
@@ -45,6 +46,11 @@ def _no_gradients(*tensors) -> None:
             if t is not None and t.requires_grad:
                 raise RuntimeError("the few-token and int8 kernels are forward only: call them under torch.no_grad(), "
                                    "or use FP8FlowMoELayer / FP8FlowMoECompute to train")
+    # tangents live inside a dual level, whether or not gradients are recorded
+    if fwAD._current_level >= 0 and torch._C._is_fwd_grad_enabled():
+        for t in tensors:
+            if t is not None and fwAD.unpack_dual(t).tangent is not None:
+                raise RuntimeError("the few-token and int8 kernels are forward only: they carry no forward-mode tangents")
 
 
 def _same_device(x: torch.Tensor, **tensors) -> None:

@@ -5,6 +5,7 @@ import copy
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 import nanopysche_amd as fm
 from nanopysche_amd.int8 import Int8Tensor, _empty
@@ -179,3 +180,51 @@ def test_a_packed_scale_carries_no_gradient(launched):  # noqa: F811
         t = Int8Tensor.from_int8(Q[:3], torch.ones(3, requires_grad=True))
     assert not t.scale.requires_grad
     assert fm.int8_linear(bf(3, 256), t).shape == (3, 3) and t.values().shape == (3, 256)
+
+
+def dual(*shape, dtype=torch.float32):
+    return fwAD.make_dual(torch.zeros(*shape, dtype=dtype), torch.ones(*shape, dtype=dtype))
+
+
+def with_dual_scale(t):
+    t.scale = dual(t.rows)
+    return t
+
+
+USES_OF_DUALS = {
+    "quantise": lambda: fm.quantize_to_int8(dual(3, 100)),
+    "from_int8": lambda: Int8Tensor.from_int8(Q[:3], dual(3)),
+    "dequantize": lambda: with_dual_scale(int8_tensor(3, 100)).dequantize(),
+    "matmul": lambda: fm.int8_matmul(int8_tensor(3, 100), with_dual_scale(int8_tensor(4, 100))),
+    "matmul_bias": lambda: fm.int8_matmul(int8_tensor(3, 100), int8_tensor(4, 100), dual(4)),
+    "linear": lambda: fm.int8_linear(dual(3, 100), int8_tensor(4, 100)),
+    "linear_view": lambda: fm.int8_linear(dual(6, 100)[::2], int8_tensor(4, 100)),
+    "grouped": lambda: fm.int8_grouped_gemm(with_dual_scale(int8_tensor(256, 128)), int8_tensor(64, 128), plan_of(256, 2)),
+    "block": lambda: fm.Int8MoECompute(int8_experts(4, 128, 256))(bf(70, 256), dual(70, 1), torch.zeros(70, 1, dtype=torch.int64)),
+    "expert_decode": lambda: fm.expert_decode(dual(3, 256, dtype=torch.bfloat16), torch.ones(3, 2), IDX, int8_experts(4, 128, 256), 4),
+    "decode_gate": lambda: fm.moe_decode(bf(3, 256), dual(4, 256, dtype=torch.bfloat16), int8_experts(4, 128, 256), 2),
+    "decode_norm": lambda: fm.moe_decode(bf(3, 256), bf(4, 256), int8_experts(4, 128, 256), 2, norm_weight=dual(256)),
+    "decode_weights": lambda: fm.moe_decode(bf(3, 256), bf(4, 256), [bf(512, 256), dual(512, 256, dtype=torch.bfloat16), bf(512, 256)], 2),
+}
+
+
+@pytest.mark.parametrize("name", USES_OF_DUALS)
+@pytest.mark.parametrize("grad", [True, False])
+def test_a_forward_mode_tangent_is_refused(launched, name, grad):  # noqa: F811
+    """torch.no_grad() does not stop forward-mode differentiation, so it does not silence the refusal."""
+    with fwAD.dual_level(), torch.set_grad_enabled(grad):
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            USES_OF_DUALS[name]()
+        assert launched == []
+        fm.int8_linear(torch.zeros(3, 100), int8_tensor(4, 100))   # no tangent
+        assert launched == ["fm_int8_linear"]
+
+
+def test_inference_mode_takes_a_dual(launched):  # noqa: F811
+    """It stops both modes, as for torch's own operations."""
+    with fwAD.dual_level():
+        x = dual(3, 100)
+        with torch.inference_mode():
+            assert fwAD.unpack_dual(x * 2).tangent is None
+            fm.int8_linear(x, int8_tensor(4, 100))
+    assert launched == ["fm_int8_linear"]
