@@ -30,6 +30,7 @@ MAX_DECODE_TOKENS = 64
 MAX_DECODE_DIM = 14336
 MAX_DECODE_EXPERTS = 1024
 MAX_DECODE_TOP_K = 16
+MAX_DECODE_MATRIX = 2 ** 30   # elements of an expert's matrix are fewer
 
 
 class DecodeOutput(NamedTuple):

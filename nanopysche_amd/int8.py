@@ -20,7 +20,8 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .decode import MAX_DECODE_DIM, MAX_DECODE_TOKENS, MAX_DECODE_TOP_K, _no_gradients, _same_device, expert_decode
+from .decode import (MAX_DECODE_DIM, MAX_DECODE_MATRIX, MAX_DECODE_TOKENS, MAX_DECODE_TOP_K, _no_gradients, _same_device,
+                     expert_decode)
 from .routing import RoutingPlan, route_tokens
 
 MAX_INT8_K = 131071   # longest product whose int32 sums cannot overflow
@@ -357,7 +358,8 @@ class Int8MoECompute:
     Tokens: route (stable counting sort) -> gather and quantise by token -> grouped
     product gate|up with SwiGLU behind it -> quantise h by token -> grouped product
     down -> weighted sum, in fp32 between the products and rounded once.  Up to 64
-    tokens go through ``expert_decode`` instead, whose activations are not quantised."""
+    tokens (D up to 14336, K up to 16, H D below 2^30) go through ``expert_decode`` instead,
+    which does not quantise activations but takes an fp32 x rounded to bf16."""
 
     def __init__(self, experts: Int8Experts):
         self.experts = experts
@@ -377,7 +379,7 @@ class Int8MoECompute:
         K = indices.shape[-1] if indices.dim() else 0
         if K < 1 or indices.numel() != T * K or weights.numel() != T * K or weights.shape[-1] != K:
             raise ValueError(f"weights {tuple(weights.shape)} and indices {tuple(indices.shape)} must be [T, K] for {T} tokens")
-        if T <= MAX_DECODE_TOKENS and D <= MAX_DECODE_DIM and K <= MAX_DECODE_TOP_K:
+        if T <= MAX_DECODE_TOKENS and D <= MAX_DECODE_DIM and K <= MAX_DECODE_TOP_K and w.hidden_size * D < MAX_DECODE_MATRIX:
             return expert_decode(x, weights, indices, w, E, expert_offset)
         if T == 0:
             return torch.empty_like(x)

@@ -8,6 +8,8 @@ import torch
 import torch.autograd.forward_ad as fwAD
 
 import nanopysche_amd as fm
+from nanopysche_amd import _lib
+from nanopysche_amd.decode import MAX_DECODE_DIM, MAX_DECODE_MATRIX, MAX_DECODE_TOKENS, MAX_DECODE_TOP_K
 from nanopysche_amd.int8 import Int8Tensor, _empty
 from tests.test_host_decode_int8 import IDX, bf, int8_experts, int8_tensor, launched  # noqa: F401
 
@@ -228,3 +230,31 @@ def test_inference_mode_takes_a_dual(launched):  # noqa: F811
             assert fwAD.unpack_dual(x * 2).tangent is None
             fm.int8_linear(x, int8_tensor(4, 100))
     assert launched == ["fm_int8_linear"]
+
+
+def unread(rows, cols):
+    """An operand whose payload is never touched, so that its pages stay unmapped."""
+    return Int8Tensor(torch.empty((rows + 15) // 16 * ((cols + 127) // 128) * 2048, dtype=U8), torch.ones(rows), rows, cols)
+
+
+@pytest.mark.parametrize("T,D,H,K,few", [
+    (64, 14336, 74880, 1, True), (64, 14336, 75008, 1, False), (1, 8320, 130944, 1, False), (64, 14336, 128, 1, True),
+    (1, 14464, 128, 1, False), (65, 128, 128, 1, False), (64, 128, 128, 16, True), (64, 128, 128, 17, False)])
+def test_any_number_of_tokens_of_any_expert_size(launched, T, D, H, K, few):  # noqa: F811
+    """The block's tokens take the few-token kernels wherever those take the sizes, else the products."""
+    ex = fm.Int8Experts(unread(H, D), unread(D, H), unread(H, D), 1)
+    out = fm.Int8MoECompute(ex)(torch.zeros(T, D), torch.ones(T, K), torch.zeros(T, K, dtype=torch.int64))
+    assert out.shape == (T, D)
+    products = ["fm_route_sort", "fm_int8_quantize", "fm_int8_grouped_gemm", "fm_int8_quantize", "fm_int8_grouped_gemm", "fm_int8_combine"]
+    assert launched == (["fm_decode_experts"] if few else products)
+    assert (_lib.load().fm_decode_workspace_bytes(T, D, K, 1, H, 0) >= 0) == few
+
+
+def test_the_few_token_limits_are_the_librarys():
+    size = _lib.load().fm_decode_workspace_bytes
+    for T, D, K, H in [(MAX_DECODE_TOKENS, 128, 1, 128), (1, MAX_DECODE_DIM, 1, 128), (1, 128, MAX_DECODE_TOP_K, 128),
+                       (1, 1024, 1, MAX_DECODE_MATRIX // 1024 - 128)]:
+        assert size(T, D, K, 1, H, 0) >= 0
+    for T, D, K, H in [(MAX_DECODE_TOKENS + 1, 128, 1, 128), (1, MAX_DECODE_DIM + 128, 1, 128), (1, 128, MAX_DECODE_TOP_K + 1, 128),
+                       (1, 1024, 1, MAX_DECODE_MATRIX // 1024)]:
+        assert size(T, D, K, 1, H, 0) == -1
