@@ -923,6 +923,18 @@ int expert_of_weights(const FmDecodeWeights* w, bool i8, Expert& x) {
   return 0;
 }
 
+// Weights, output and pitch of x, before anything is launched.
+int decode_operands_ok(int64_t ld_x, int64_t D, const FmDecodeWeights* experts, const FmDecodeWeights* shared, const void* out,
+                       int out_dtype, int64_t ld_out, Expert& r, Expert& s) {
+  FM_REQUIRE(experts->kind == FM_DECODE_BF16 || experts->kind == FM_DECODE_INT8, "fm_decode_experts: bad weight kind");
+  FM_REQUIRE(ld_x >= D && ld_x % 8 == 0 && ld_x <= (1 << 23), "fm_decode_experts: rows must start on 16-byte boundaries, at a pitch of at most 2^23");
+  FM_REQUIRE((out_dtype == FM_DTYPE_BF16 || out_dtype == FM_DTYPE_F32) && aligned16(out) && ld_out >= D && ld_out % 4 == 0,
+             "fm_decode_experts: output must be bf16 or fp32, 16-byte aligned, its pitch at least D and a multiple of 4");
+  const bool i8 = experts->kind == FM_DECODE_INT8;
+  if (int rc = expert_of_weights(experts, i8, r)) return rc;
+  return shared ? expert_of_weights(shared, i8, s) : 0;
+}
+
 int64_t decode_router_bytes(int64_t T, int64_t D, int64_t E) { return T * D * 4 + T * E * 4; }
 
 bool decode_sizes_ok(int64_t T, int64_t D, int64_t K, int64_t E, int64_t H, int64_t Hs) {
@@ -953,8 +965,10 @@ int fm_moe_decode(const void* x, int64_t ld_x, int64_t T, int64_t D, const void*
   FM_REQUIRE(aligned16(x) && ld_x >= D && ld_x % 8 == 0 && aligned16(gate) && ld_g >= D && ld_g % (gate_dtype == FM_DTYPE_F32 ? 4 : 8) == 0 &&
                  aligned16(norm), "fm_moe_decode: rows must start on 16-byte boundaries");
   const int64_t need = fm_decode_workspace_bytes(T, D, K, E, experts->H, shared ? shared->H : 0);
-  FM_REQUIRE(need >= 0 && aligned16(workspace) && workspace_bytes >= need + decode_router_bytes(T, D, E),
+  FM_REQUIRE(need >= 0 && (!shared || shared->H > 0) && aligned16(workspace) && workspace_bytes >= need + decode_router_bytes(T, D, E),
              "fm_moe_decode: hidden sizes must be multiples of 128 and the workspace fm_moe_decode_workspace_bytes bytes");
+  Expert routed{}, shared_expert{};
+  if (int rc = decode_operands_ok(norm ? D : ld_x, D, experts, shared, out, out_dtype, ld_out, routed, shared_expert)) return rc;
   // behind the experts' workspace: the normed rows' two pieces, the logits
   uint8_t* own = static_cast<uint8_t*>(workspace) + need;
   uint16_t *x_hi = reinterpret_cast<uint16_t*>(own), *x_lo = x_hi + T * D;
@@ -1001,17 +1015,15 @@ int fm_decode_experts(const void* x, const void* x_lo, int64_t ld_x, int64_t T, 
   const int64_t Hs = shared ? shared->H : 0;
   FM_REQUIRE(decode_sizes_ok(T, D, K, E, experts->H, Hs) && (!shared || Hs > 0),
              "fm_decode_experts: needs 1..64 tokens, D and hidden sizes multiples of 128 (D up to 14336), K <= 16 and at most 1024 experts");
-  FM_REQUIRE(experts->kind == FM_DECODE_BF16 || experts->kind == FM_DECODE_INT8, "fm_decode_experts: bad weight kind");
-  FM_REQUIRE(aligned16(x) && aligned16(x_lo) && ld_x >= D && ld_x % 8 == 0 && ld_x <= (1 << 23) && aligned16(workspace),
-             "fm_decode_experts: rows must start on 16-byte boundaries, at a pitch of at most 2^23");
-  FM_REQUIRE((out_dtype == FM_DTYPE_BF16 || out_dtype == FM_DTYPE_F32) && aligned16(out) && ld_out >= D && ld_out % 4 == 0,
-             "fm_decode_experts: output must be bf16 or fp32, 16-byte aligned, its pitch at least D and a multiple of 4");
+  FM_REQUIRE(aligned16(x) && aligned16(x_lo) && aligned16(workspace), "fm_decode_experts: rows and workspace must start on 16-byte boundaries");
+  Expert routed{}, shared_expert{};
+  if (int rc = decode_operands_ok(ld_x, D, experts, shared, out, out_dtype, ld_out, routed, shared_expert)) return rc;
   const bool i8 = experts->kind == FM_DECODE_INT8;
   const DecodePlan p = decode_plan(T, D, K, E, experts->H, Hs);
   FM_REQUIRE(workspace_bytes >= p.bytes, "fm_decode_experts: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
              (long long)p.bytes);
   ExpertArgs a{static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(x_lo), ld_x, int(T), int(D), K, E, indices,
-               indices_i64, expert_offset, {}, {}};
+               indices_i64, expert_offset, routed, shared_expert};
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   auto place = [&](Expert& e, int64_t rows, int R, int P, int64_t h, int64_t part) {
     e.S = e.H / p.hs;
@@ -1021,12 +1033,8 @@ int fm_decode_experts(const void* x, const void* x_lo, int64_t ld_x, int64_t T, 
     e.hlo = e.hhi + rows * e.H;
     e.part = reinterpret_cast<float*>(ws + part);
   };
-  if (int rc = expert_of_weights(experts, i8, a.r)) return rc;
   place(a.r, T * K, p.R, p.P, p.h, p.part);
-  if (shared) {
-    if (int rc = expert_of_weights(shared, i8, a.s)) return rc;
-    place(a.s, T, p.Rs, p.Ps, p.hs_at, p.part_s);
-  }
+  if (shared) place(a.s, T, p.Rs, p.Ps, p.hs_at, p.part_s);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int64_t up = p.reach * a.r.S + a.s.S, down = (p.reach * a.r.P + a.s.P) * ((D + 511) / 512);
   if (i8) {
