@@ -978,7 +978,7 @@ int fm_moe_decode(const void* x, int64_t ld_x, int64_t T, int64_t D, const void*
                      gating == FM_GATING_SIGMOID, (flags & FM_GATING_L2_NORMALIZE) != 0, logits,
                      x_hi, x_lo, weights, indices};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  // one workgroup a token where a gate is small enough for one CU to read; else 32 experts a workgroup and a second launch
+  // one workgroup a token where a gate is small enough for one CU to read; else eight experts a workgroup and a second launch
   const bool one = int64_t(E) * D <= kRouterOne;
   if (!one) {
     launch_router<1>(a, kRouterThreads / 64, false, s);
