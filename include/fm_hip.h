@@ -619,7 +619,7 @@ int fm_grouped_gemm_ragged_k_split(int kind, const FmGemmOperand* a_t, const FmG
  * xn gate^T + bias + score_bias in fp32; weights [T, K] and indices [T, K] (both
  * written) as fm_topk_gating without replay; then fm_decode_experts of them.  bias,
  * score_bias, norm and shared may be NULL.  Its workspace is
- * fm_moe_decode_workspace_bytes bytes. */
+ * fm_moe_decode_workspace_bytes bytes.  A refused call has launched nothing. */
 #define FM_DECODE_BF16 0   /* w1, w2, w3 [E * H, D] bf16, contiguous                          */
 #define FM_DECODE_INT8 1   /* int8 tiles: w1, w3 [E][H x D], w2 [E][D x H] (transposed)       */
 typedef struct FmDecodeWeights {
@@ -652,7 +652,8 @@ int fm_decode_experts(const void* x, const void* x_lo, int64_t ld_x, int64_t T, 
  * 16-byte boundary, R scales.  Groups (experts) follow one another.
  *
  * fm_int8_quantize: rows of x (bf16 or fp32, any element-aligned base and pitch):
- *   s = max(amax, 1e-12) / 127, q = rint(x / s), ties to even; a row with a NaN or an
+ *   s = max(amax, 1e-12) / 127, q = rint(x / s), both in fp32, ties to even (an x of half its row's
+ *   amax is 63.5 steps: the last bit of s decides between 63 and 64); a row with a NaN or an
  *   infinity gets scale NaN or infinity and zero payload.  With assign_of_row, output
  *   row r is row assign_of_row[r] / top_k of x (zeros and scale 0 where negative: a
  *   routing plan's padding); rows from *limit (a multiple of 16, device memory, or NULL) on are left

@@ -5,6 +5,8 @@
 //
 // and their forms over a routing plan's groups, with SwiGLU behind the gate|up product.
 // The sums are int32, exact for K < 2^17, so a product does not depend on how it is cut.
+// s and x / s are rounded fp32 quotients: an x of exactly half its row's maximum (one bf16 element
+// in 800) lies at 63.5 steps and becomes 63 or 64 as the last bit of s falls (64 in 95% of them).
 // A row that holds a NaN or an infinity gets that scale and zero payload: its outputs are NaN.
 //
 // Layout.  An operand [R, K] lies in tiles of 16 rows x 64 columns, 1 KiB each, in the

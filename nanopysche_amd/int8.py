@@ -329,7 +329,7 @@ class Int8Experts:
 
     @staticmethod
     def quantize(w1: torch.Tensor, w2: torch.Tensor, w3: torch.Tensor, num_experts: int) -> "Int8Experts":
-        """From bf16 or fp32 weights [E * H, D] in the expert block's storage."""
+        """From bf16 or fp32 weights [E * H, D] in the expert block's storage, detached."""
         H, D = Int8Experts._sizes(w1, w2, w3, num_experts)
         _same_device(w1, w2=w2, w3=w3)
         w2t = w2.detach().reshape(num_experts, H, D).transpose(1, 2).reshape(num_experts * D, H)

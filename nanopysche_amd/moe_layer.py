@@ -267,7 +267,8 @@ class FP8FlowMoELayer:
     def decode(self, x: torch.Tensor, experts=None, shared=None) -> DecodeOutput:
         """The layer for a decoding step of 1 to 64 tokens, forward only
         (``moe_decode``): DecodeOutput(out, weights, indices) with the layer's
-        router, norm, experts and shared expert, whose weights must be bf16, or
+        router, norm, experts and shared expert, whose weights must be bf16,
+        contiguous and on 16-byte boundaries, or
         with int8 ``experts`` (and ``shared``) made from them
         (``Int8Experts.quantize``).  The recipe, jitter and capacity dropping, which
         serve training, do not take part, and there is no auxiliary loss."""
