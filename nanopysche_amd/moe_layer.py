@@ -268,10 +268,10 @@ class FP8FlowMoELayer:
         """The layer for a decoding step of 1 to 64 tokens, forward only
         (``moe_decode``): DecodeOutput(out, weights, indices) with the layer's
         router, norm, experts and shared expert, whose weights must be bf16,
-        contiguous and on 16-byte boundaries, or
-        with int8 ``experts`` (and ``shared``) made from them
-        (``Int8Experts.quantize``).  The recipe, jitter and capacity dropping, which
-        serve training, do not take part, and there is no auxiliary loss."""
+        contiguous and on 16-byte boundaries, or with int8 ``experts`` (and
+        ``shared``) made from them (``Int8Experts.quantize``).  The recipe, jitter and
+        capacity dropping, which serve training, do not take part, and there is no
+        auxiliary loss."""
         if self.gate_weight is None:
             raise RuntimeError("set_weights() must be called before the layer runs")
         if self.shared is None and shared is not None:
