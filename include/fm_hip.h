@@ -693,6 +693,58 @@ int fm_int8_grouped_gemm(const void* a, const float* sa, int64_t rows, const int
 int fm_int8_combine(const float* y, int64_t D, const int32_t* row_of, const float* weights, int64_t T, int K, void* out,
                     int out_dtype, void* stream);
 
+/* -------------------------------------- activations in 8 bits, for the backward ----
+ * Blocks of 32 values along a row share a power of two s = 2^k, k = max(floor(log2 max|x|) - 6, -127)
+ * (OCP MX int8); q = min(max(rint(x / s), -127), 127), the code is k + 127 (e8m0), 255 for a block with a NaN
+ * or an infinity, which stands for NaNs.  q s is exact in bf16 and fp32.  No counterpart in the reference, which keeps activations in
+ * the model's type or recomputes them (distributed/fsdp.py:80-117).
+ * Payload int8 [rows, ld_q], ld_q = cols rounded up to 32, on 8 bytes, zeros behind cols; codes [rows, ld_c], ld_c = ld_q / 32.
+ * Other matrices: bf16 or fp32 with rows at any element; fewer than 2^24 columns.
+ *
+ * fm_act8_compress: rows of x into the format; with tile_valid, rows of 128-row tiles with a negative entry are left alone.
+ * fm_act8_restore: the values, row r from row index[r] (int32; zeros where it is outside [0, src_rows)) or, with a null
+ *   index, from row r.
+ * fm_act8_swiglu: h = silu(g) u in fp32, rounded once; g and u in the format.  fm_act8_swiglu_backward: dg = dh u s (1 + g (1 - s)),
+ *   du = dh silu(g) from them, s = sigmoid(g).
+ * fm_act8_rmsnorm: y = x r w, r = 1 / sqrt(mean(x^2) + eps) (rstd [T] fp32); x in the format.  fm_act8_rmsnorm_backward: from it, with
+ *   a = dy w, dx = r a - (r^3 / D) (sum a x) x and, through a workspace, dw = sum_t dy x r (w's dtype; null: not wanted).
+ *   D up to 16384. */
+int fm_act8_compress(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t ld_x, void* q, int64_t ld_q, void* codes,
+                     int64_t ld_c, const int32_t* tile_valid, void* stream);
+int fm_act8_restore(const void* q, int64_t ld_q, const void* codes, int64_t ld_c, int64_t src_rows, int64_t cols,
+                    const int32_t* index, int64_t rows, void* out, int out_dtype, int64_t ld_out, void* stream);
+int fm_act8_swiglu(const void* g, int64_t ld_g, const void* u, int64_t ld_u, int dtype, int64_t rows, int64_t H, void* h,
+                   int64_t ld_h, void* qg, void* cg, void* qu, void* cu, int64_t ld_q, int64_t ld_c, void* stream);
+int fm_act8_swiglu_backward(const void* dh, int64_t ld_dh, int dtype, int64_t rows, int64_t H, const void* qg, const void* cg,
+                            const void* qu, const void* cu, int64_t ld_q, int64_t ld_c, void* dg, int64_t ld_dg, void* du,
+                            int64_t ld_du, void* stream);
+int fm_act8_rmsnorm(const void* x, int dtype, int64_t ld_x, int64_t T, int64_t D, const void* w, int w_dtype, float eps, void* y,
+                    int64_t ld_y, void* q, int64_t ld_q, void* codes, int64_t ld_c, float* rstd, void* stream);
+int64_t fm_act8_rmsnorm_backward_workspace_bytes(int64_t T, int64_t D);
+int fm_act8_rmsnorm_backward(const void* dy, int64_t ld_dy, int dtype, int64_t T, int64_t D, const void* q, int64_t ld_q,
+                             const void* codes, int64_t ld_c, const void* w, int w_dtype, const float* rstd, void* dx,
+                             int64_t ld_dx, void* dw, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ------------------------------- balance loss of packed and padded sequences ----
+ * The load-balancing loss (reference model/moe.py:267-281) of each sequence, averaged, over the tokens that count:
+ *   f_se = slots of sequence s at expert e / n_s, P_se = mean of its p_te, loss = (E / S') sum_s sum_e f_se P_se
+ *   + z_mult mean_t logsumexp(l_t)^2; S': sequences with n_s > 0; p = softmax(l), or (sigmoid) sigma / (sum sigma + 1e-8).
+ * Sequence s is tokens [cu[s], cu[s + 1]) (ascending int32 in [0, T]; null: one sequence of all), of which those count whose mask
+ * byte is not 0 (null: all).  The logits [T, E] fp32 of others may hold anything, indices [T, K] outside [0, E) fill no slot.
+ * E up to 1024.
+ * fm_balance_forward: f [S, E] = E slots / n_s^2 and inverse [2] = {1 / S', 1 / N} for the backward, counts [S, E], loss; acc [E] and
+ *   acc_total [1] (int64 or null) are raised by the counts and the tokens that count.  Workspace on 16 bytes.
+ * fm_balance_backward: dlogits [T, E] = dloss times the gradient, zeros for tokens that do not count (add: added to what
+ *   is there). */
+int64_t fm_balance_workspace_bytes(int64_t T, int E, int64_t S);
+int fm_balance_forward(const float* logits, int64_t ld, int64_t T, int E, const void* indices, int indices_i64, int K,
+                       const int32_t* cu, int64_t S, const uint8_t* mask, int sigmoid, float z_mult, float* f, int32_t* counts,
+                       float* inverse, float* loss, int64_t* acc, int64_t* acc_total, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+int fm_balance_backward(const float* logits, int64_t ld, int64_t T, int E, const int32_t* cu, int64_t S, const uint8_t* mask,
+                        int sigmoid, float z_mult, const float* f, const float* inverse, const float* dloss, float* dlogits,
+                        int64_t ld_d, int add, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -23,6 +23,9 @@ from .flow_moe import (
     quantize_to_fp8,
     scaling_aware_transpose,
 )
+from .act8 import (Activation8, RMSNormKept, SwigluKept, compress_activation, rmsnorm_8bit, rmsnorm_backward_8bit,
+                   rmsnorm_compress, swiglu_8bit, swiglu_backward_8bit, swiglu_compress)
+from .balance import BalanceOutput, BalanceState, balance_backward, balance_forward, balance_loss
 from .decode import DecodeOutput, expert_decode, moe_decode
 from .graph import GraphedStep
 from .int8 import (Int8Experts, Int8MoECompute, Int8Tensor, int8_grouped_gemm, int8_linear, int8_matmul,
@@ -76,4 +79,19 @@ __all__ = [
     "rmsnorm_quantize",
     "rmsnorm_backward",
     "NormOutput",
+    "Activation8",
+    "compress_activation",
+    "SwigluKept",
+    "swiglu_compress",
+    "swiglu_backward_8bit",
+    "swiglu_8bit",
+    "RMSNormKept",
+    "rmsnorm_compress",
+    "rmsnorm_backward_8bit",
+    "rmsnorm_8bit",
+    "BalanceOutput",
+    "BalanceState",
+    "balance_forward",
+    "balance_backward",
+    "balance_loss",
 ]

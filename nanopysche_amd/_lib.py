@@ -180,6 +180,20 @@ SIGNATURES = {
     "fm_decode_experts": (_i32, [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _i32, _i32, _i64, _i32,
                                  C.POINTER(FmDecodeWeights), C.POINTER(FmDecodeWeights), _vp, _i32, _i64, _vp, _i64,
                                  _vp]),
+    "fm_act8_compress": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp]),
+    "fm_act8_restore": (_i32, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _i32, _i64, _vp]),
+    "fm_act8_swiglu": (_i32, [_vp, _i64, _vp, _i64, _i32, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _vp]),
+    "fm_act8_swiglu_backward": (_i32, [_vp, _i64, _i32, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _i64,
+                                       _vp]),
+    "fm_act8_rmsnorm": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i32, C.c_float, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp]),
+    "fm_act8_rmsnorm_backward_workspace_bytes": (_i64, [_i64, _i64]),
+    "fm_act8_rmsnorm_backward": (_i32, [_vp, _i64, _i32, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _vp, _vp, _i64, _vp, _vp,
+                                        _i64, _vp]),
+    "fm_balance_workspace_bytes": (_i64, [_i64, _i32, _i64]),
+    "fm_balance_forward": (_i32, [_vp, _i64, _i64, _i32, _vp, _i32, _i32, _vp, _i64, _vp, _i32, C.c_float, _vp, _vp, _vp, _vp,
+                                  _vp, _vp, _vp, _i64, _vp]),
+    "fm_balance_backward": (_i32, [_vp, _i64, _i64, _i32, _vp, _i64, _vp, _i32, C.c_float, _vp, _vp, _vp, _vp, _i64, _i32,
+                                   _vp]),
 }
 
 _lib = None

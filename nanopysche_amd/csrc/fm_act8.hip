@@ -1,0 +1,665 @@
+// Activations kept in 8 bits between forward and backward (format: fm_act8.h), and the two
+// element-wise layers that keep their inputs so:
+//   fm_act8_compress, fm_act8_restore   rows into the format and back (the rows of an index)
+//   fm_act8_swiglu, .._swiglu_backward  h = silu(g) u, g and u kept; dg, du from what was kept
+//   fm_act8_rmsnorm, .._rmsnorm_backward  y = x r w, x kept; dx, dw from what was kept
+// All of them move bytes: one pass each, every value read and written once.  A lane holds eight
+// neighbours (16 bytes of bf16), four lanes a block, so a block's scale costs two exchanges within
+// quads and no LDS.
+#include <type_traits>
+
+#include "fm_act8.h"
+#include "fm_silu.h"
+#include "../../include/fm_hip.h"
+
+namespace fm {
+namespace {
+
+// ------------------------------------------------------------ rows of eight ----
+// Eight neighbours of a row as they are stored, n of them in the row (zeros behind).  TAIL: n may lie between 0 and 8.
+template <typename T>
+struct Eight {
+  static constexpr int kWords = sizeof(T) * 2;
+  uint32_t w[kWords];
+  template <bool TAIL = true>
+  __device__ __forceinline__ void load(const T* p, int n) {
+    if (n >= 8) {
+#pragma unroll
+      for (int i = 0; i < kWords / 4; ++i) {
+        const u32x4_el v = reinterpret_cast<const u32x4_el*>(p)[i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[4 * i + j] = v[j];
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
+    if constexpr (!TAIL) return;
+#pragma unroll
+    for (int i = 0; i < 7; ++i) {
+      if constexpr (sizeof(T) == 2) w[i / 2] |= i < n ? uint32_t(p[i]) << (16 * (i & 1)) : 0u;
+      else w[i] = i < n ? f2u(p[i]) : 0u;
+    }
+  }
+  __device__ __forceinline__ void widen(float (&v)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (sizeof(T) == 2) v[i] = u2f(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+      else v[i] = u2f(w[i]);
+    }
+  }
+};
+
+// The first n of eight values, rounded to T.
+template <typename T, bool TAIL = true>
+__device__ __forceinline__ void store8(T* p, const float (&v)[8], int n) {
+  uint32_t w[Eight<T>::kWords];
+#pragma unroll
+  for (int i = 0; i < Eight<T>::kWords; ++i) {
+    if constexpr (sizeof(T) == 2) w[i] = hw_bf16x2(v[2 * i], v[2 * i + 1]);
+    else w[i] = f2u(v[i]);
+  }
+  if (n >= 8) {
+#pragma unroll
+    for (int i = 0; i < Eight<T>::kWords / 4; ++i)
+      *FM_GLOBAL(u32x4_el, reinterpret_cast<u32x4_el*>(p) + i) = u32x4_el{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+    return;
+  }
+  if constexpr (!TAIL) return;
+#pragma unroll
+  for (int i = 0; i < 7; ++i) {
+    if (i >= n) break;
+    if constexpr (sizeof(T) == 2) st_global(p + i, uint16_t(w[i / 2] >> (16 * (i & 1))));
+    else st_global(reinterpret_cast<uint32_t*>(p) + i, w[i]);
+  }
+}
+
+// Division of 0 <= n < 2^31 by a fixed d >= 1: (n + mulhi(n, m)) >> l (Granlund and Montgomery, PLDI 1994).
+struct FastDiv {
+  uint32_t m, l, d;
+  explicit FastDiv(uint32_t div) : d(div) {
+    l = 0;
+    while ((uint64_t(1) << l) < div) ++l;
+    m = uint32_t(((uint64_t(1) << 32) * ((uint64_t(1) << l) - div)) / div + 1);
+  }
+  __device__ __forceinline__ uint32_t quotient(uint32_t n) const { return (n + __umulhi(n, m)) >> l; }
+};
+
+// A matrix's eights, row by row, ld_q / 8 (a multiple of 4) to a row: eight i is columns
+// [8 (i % per), + 8) of row i / per.
+struct Items {
+  FastDiv per;
+  uint32_t n;      // fewer than 2^31
+  int64_t row0;    // first row
+  int cols;
+};
+struct Item {
+  int64_t row;
+  int col, n;      // n of the eight lie in the row (at most 0 behind it)
+  bool in;
+};
+// Eights u of U of a thread; one past the last stands for the last and is not stored.
+template <int U>
+__device__ __forceinline__ Item item_of(const Items& t, int u) {
+  const uint32_t i = blockIdx.x * (256u * U) + u * 256u + threadIdx.x;
+  const uint32_t j = i < t.n ? i : t.n - 1;
+  const uint32_t r = t.per.quotient(j);
+  const int col = int(j - r * t.per.d) * 8;
+  return Item{t.row0 + r, col, t.cols - col, i < t.n};
+}
+
+__device__ __forceinline__ void store_kept(uint8_t* q, int64_t ld_q, uint8_t* codes, int64_t ld_c, int64_t row, int col, uint2 b,
+                                           uint32_t code) {
+  st_global(q + row * ld_q + col, b);
+  if ((threadIdx.x & 3) == 0) st_global(codes + row * ld_c + (col >> 5), uint8_t(code));
+}
+
+// --------------------------------------------------------------- compress ----
+struct CompressArgs {
+  const void* x;
+  int64_t ld_x;
+  uint8_t* q;
+  int64_t ld_q;
+  uint8_t* codes;
+  int64_t ld_c;
+  const int32_t* tile_valid;   // rows of 128-row tiles with a negative entry are left alone; null: none
+};
+
+template <typename T, int U>
+__global__ __launch_bounds__(256) void compress_kernel(Items t, CompressArgs a) {
+  Item it[U];
+  Eight<T> x[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    it[u] = item_of<U>(t, u);
+    if (a.tile_valid && a.tile_valid[it[u].row >> 7] < 0) it[u].in = false;
+    x[u].load(static_cast<const T*>(a.x) + it[u].row * a.ld_x + it[u].col, it[u].in ? it[u].n : 0);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float v[8];
+    x[u].widen(v);
+    uint32_t code;
+    const uint2 b = act_encode8(v, code);
+    if (it[u].in) store_kept(a.q, a.ld_q, a.codes, a.ld_c, it[u].row, it[u].col, b, code);
+  }
+}
+
+// ---------------------------------------------------------------- restore ----
+struct RestoreArgs {
+  Act8 x;
+  const int32_t* index;   // output row r is row index[r] of x, zeros where it is outside [0, src_rows); null: row r
+  int64_t src_rows;
+  void* out;
+  int64_t ld_out;
+};
+
+template <typename T, int U, bool GATHER>
+__global__ __launch_bounds__(256) void restore_kernel(Items t, RestoreArgs a) {
+  Item it[U];
+  uint2 b[U];
+  uint32_t code[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    it[u] = item_of<U>(t, u);
+    int64_t r = it[u].row;
+    bool zero = false;
+    if constexpr (GATHER) {
+      r = a.index[r];
+      zero = r < 0 || r >= a.src_rows;
+    }
+    b[u] = zero ? make_uint2(0, 0) : a.x.bytes(r, it[u].col);
+    code[u] = zero ? 0u : a.x.code(r, it[u].col);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float v[8];
+    act_decode8(b[u], act_scale(code[u]), v);
+    if (it[u].in) store8(static_cast<T*>(a.out) + it[u].row * a.ld_out + it[u].col, v, it[u].n);
+  }
+}
+
+// ----------------------------------------------------------------- SwiGLU ----
+struct SwigluArgs {
+  const void *g, *u;
+  int64_t ld_g, ld_u;
+  void* h;
+  int64_t ld_h;
+  uint8_t *qg, *qu, *cg, *cu;
+  int64_t ld_q, ld_c;
+};
+
+template <typename T, int U>
+__global__ __launch_bounds__(256) void swiglu_kernel(Items t, SwigluArgs a) {
+  Item it[U];
+  Eight<T> g[U], up[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    it[u] = item_of<U>(t, u);
+    g[u].load(static_cast<const T*>(a.g) + it[u].row * a.ld_g + it[u].col, it[u].n);
+    up[u].load(static_cast<const T*>(a.u) + it[u].row * a.ld_u + it[u].col, it[u].n);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float gv[8], uv[8], h[8];
+    g[u].widen(gv);
+    up[u].widen(uv);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = silu_only(gv[i]) * uv[i];
+    uint32_t gc, uc;
+    const uint2 gb = act_encode8(gv, gc), ub = act_encode8(uv, uc);
+    if (!it[u].in) continue;
+    store8(static_cast<T*>(a.h) + it[u].row * a.ld_h + it[u].col, h, it[u].n);
+    store_kept(a.qg, a.ld_q, a.cg, a.ld_c, it[u].row, it[u].col, gb, gc);
+    store_kept(a.qu, a.ld_q, a.cu, a.ld_c, it[u].row, it[u].col, ub, uc);
+  }
+}
+
+struct SwigluBwdArgs {
+  const void* dh;
+  int64_t ld_dh;
+  Act8 g, u;
+  void *dg, *du;
+  int64_t ld_dg, ld_du;
+};
+
+template <typename T, int U>
+__global__ __launch_bounds__(256) void swiglu_backward_kernel(Items t, SwigluBwdArgs a) {
+  Item it[U];
+  Eight<T> dh[U];
+  uint2 g[U], up[U];
+  uint32_t gc[U], uc[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    it[u] = item_of<U>(t, u);
+    g[u] = a.g.bytes(it[u].row, it[u].col);
+    up[u] = a.u.bytes(it[u].row, it[u].col);
+    gc[u] = a.g.code(it[u].row, it[u].col);
+    uc[u] = a.u.code(it[u].row, it[u].col);
+    dh[u].load(static_cast<const T*>(a.dh) + it[u].row * a.ld_dh + it[u].col, it[u].n);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float gv[8], uv[8], dv[8];
+    act_decode8(g[u], act_scale(gc[u]), gv);
+    act_decode8(up[u], act_scale(uc[u]), uv);
+    dh[u].widen(dv);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const SigSilu s = sig_silu(gv[i]);
+      gv[i] = ((dv[i] * uv[i]) * s.s) * (1.f + gv[i] * (1.f - s.s));
+      uv[i] = dv[i] * s.silu;
+    }
+    if (!it[u].in) continue;
+    store8(static_cast<T*>(a.dg) + it[u].row * a.ld_dg + it[u].col, gv, it[u].n);
+    store8(static_cast<T*>(a.du) + it[u].row * a.ld_du + it[u].col, uv, it[u].n);
+  }
+}
+
+// ---------------------------------------------------------------- RMSNorm ----
+// A row sits in the registers of W waves, two eights a lane at most: lane l of them holds columns 8 l .. + 8 and, past the
+// waves' first 512 W, 8 l + 512 W .. + 8.  W = 1 takes up to 1024 columns, four rows to a workgroup of four waves; wider rows
+// take a workgroup of W = ceil(D / 1024) waves each, so the lanes of any width are busy and the backward keeps w,
+// dw's share and a row's operands in about a hundred registers.
+struct NormArgs {
+  const void* x;
+  int64_t ld_x, T;
+  int D;
+  const void* w;
+  float eps;
+  void* y;
+  int64_t ld_y;
+  uint8_t* q;
+  int64_t ld_q;
+  uint8_t* codes;
+  int64_t ld_c;
+  float* rstd;
+};
+
+__device__ __forceinline__ float wave_sum64(float v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
+  return v;
+}
+
+// Sum over a row's waves, in wave order; `parity` alternates between rows, so one barrier is enough.
+template <bool ONE>
+__device__ __forceinline__ float row_sum(float v, float (*sums)[16], int parity) {
+  v = wave_sum64(v);
+  if constexpr (!ONE) {
+    if ((threadIdx.x & 63) == 0) sums[parity][threadIdx.x >> 6] = v;
+    __syncthreads();
+    const int waves = int(blockDim.x >> 6);
+    v = sums[parity][0];
+    for (int i = 1; i < waves; ++i) v += sums[parity][i];
+  }
+  return v;
+}
+
+template <typename T, typename WT, int NC, bool ONE, bool TAIL>
+__global__ __launch_bounds__(ONE ? 256 : 1024) void norm_kernel(NormArgs a) {
+  __shared__ float sums[1][16];
+  const int lane = ONE ? threadIdx.x & 63 : threadIdx.x;
+  const int step = ONE ? 512 : int(blockDim.x) * 8;
+  const int64_t row = ONE ? int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6) : int64_t(blockIdx.x);
+  if (ONE && row >= a.T) return;
+  const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
+  Eight<T> xr[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) xr[c].template load<TAIL>(x + step * c + 8 * lane, a.D - (step * c + 8 * lane));
+  Eight<WT> wr[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+    wr[c].template load<TAIL>(static_cast<const WT*>(a.w) + step * c + 8 * lane, a.D - (step * c + 8 * lane));
+  float ss = 0.f;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    float v[8];
+    xr[c].widen(v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
+  }
+  ss = row_sum<ONE>(ss, sums, 0);
+  const float r = 1.0f / sqrtf(ss / float(a.D) + a.eps);
+  if (lane == 0) st_global(a.rstd + row, r);
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int col = step * c + 8 * lane;
+    if (col >= a.ld_q) break;
+    float v[8], wv[8], yv[8];
+    xr[c].widen(v);
+    wr[c].widen(wv);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) yv[j] = (v[j] * r) * wv[j];
+    uint32_t code;
+    const uint2 b = act_encode8(v, code);
+    store8<T, TAIL>(static_cast<T*>(a.y) + row * a.ld_y + col, yv, a.D - col);
+    store_kept(a.q, a.ld_q, a.codes, a.ld_c, row, col, b, code);
+  }
+}
+
+// A workgroup takes the rows [slice * rps, + rps) (W = 1: its waves every fourth of them) and writes the slice's share of dw.
+struct NormBwdArgs {
+  const void* dy;
+  int64_t ld_dy;
+  Act8 x;
+  int64_t T;
+  int D;
+  const void* w;
+  const float* rstd;
+  void* dx;
+  int64_t ld_dx;
+  float* part;      // [slices, ld_p], or null: no dw
+  int64_t ld_p, rps;
+};
+
+template <typename T, int NC, bool TAIL>
+struct NormRow {
+  uint2 q[NC];
+  uint32_t code[NC];
+  Eight<T> dy[NC];
+  float r;
+  __device__ __forceinline__ void load(const NormBwdArgs& a, int64_t row, int lane, int step) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int col = step * c + 8 * lane;
+      const int at = col < a.x.ld_q ? col : 0;   // behind the row: its first bytes, with a dy of zeros
+      q[c] = a.x.bytes(row, at);
+      code[c] = a.x.code(row, at);
+      dy[c].template load<TAIL>(static_cast<const T*>(a.dy) + row * a.ld_dy + col, a.D - col);
+    }
+    r = a.rstd[row];
+  }
+};
+
+template <typename T, typename WT, int NC, bool ONE, bool TAIL>
+__global__ __launch_bounds__(ONE ? 256 : 1024) void norm_backward_kernel(NormBwdArgs a) {
+  __shared__ float sums[2][16];
+  const int lane = ONE ? threadIdx.x & 63 : threadIdx.x, wave = threadIdx.x >> 6;
+  const int step = ONE ? 512 : int(blockDim.x) * 8;
+  const int64_t r0 = int64_t(blockIdx.x) * a.rps, r1 = r0 + a.rps < a.T ? r0 + a.rps : a.T;
+  const float inv_d = 1.0f / float(a.D);
+  float wv[NC][8], pdw[NC][8];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int col = step * c + 8 * lane;
+    Eight<WT> wr;
+    wr.template load<TAIL>(static_cast<const WT*>(a.w) + col, a.D - col);
+    wr.widen(wv[c]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) pdw[c][j] = 0.f;
+  }
+  constexpr int kStep = ONE ? 4 : 1;
+  int parity = 0;
+  for (int64_t row = r0 + (ONE ? wave : 0); row < r1; row += kStep, parity ^= 1) {
+    NormRow<T, NC, TAIL> n;
+    n.load(a, row, lane, step);
+    float dot = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      float xv[8], dv[8];
+      act_decode8(n.q[c], act_scale(n.code[c]), xv);
+      n.dy[c].widen(dv);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        pdw[c][j] = fmaf(dv[j], xv[j] * n.r, pdw[c][j]);
+        dot = fmaf(dv[j] * wv[c][j], xv[j], dot);
+      }
+    }
+    dot = row_sum<ONE>(dot, sums, parity);
+    const float k = ((n.r * n.r) * n.r) * (dot * inv_d);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int col = step * c + 8 * lane;
+      if (col >= a.D) break;
+      float xv[8], dv[8];
+      act_decode8(n.q[c], act_scale(n.code[c]), xv);
+      n.dy[c].widen(dv);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) dv[j] = n.r * (dv[j] * wv[c][j]) - k * xv[j];
+      store8<T, TAIL>(static_cast<T*>(a.dx) + row * a.ld_dx + col, dv, a.D - col);
+    }
+  }
+  if (a.part == nullptr) return;
+  if constexpr (ONE) {   // the four waves' shares, in wave order
+    __shared__ float acc[4][NC * 512];
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[wave][(c * 8 + j) * 64 + lane] = pdw[c][j];
+    __syncthreads();
+    for (int i = threadIdx.x; i < NC * 512; i += 256) {
+      const int col = (i >> 9) * 512 + (i & 63) * 8 + ((i >> 6) & 7);
+      if (col < a.D) st_global(a.part + blockIdx.x * a.ld_p + col, ((acc[0][i] + acc[1][i]) + acc[2][i]) + acc[3][i]);
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int col = step * c + 8 * lane;
+      if (col < a.D) store8<float, false>(a.part + blockIdx.x * a.ld_p + col, pdw[c], 8);   // ld_p is D rounded up to 8
+    }
+  }
+}
+
+// dw from the slices' shares: a workgroup takes 64 columns, sixteen rows of threads every sixteenth slice each, and
+// adds the sixteen sums in order.
+template <typename WT>
+__global__ __launch_bounds__(256) void norm_dw_kernel(const float* part, int64_t ld_p, int slices, int D, WT* dw) {
+  __shared__ float4 acc[16][16];
+  const int q = threadIdx.x & 15, g = threadIdx.x >> 4;
+  const int col = blockIdx.x * 64 + q * 4;
+  float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (col < ld_p) {
+    for (int s = g; s < slices; s += 16) {
+      const float4 v = *reinterpret_cast<const float4*>(part + s * ld_p + col);
+      t.x += v.x;
+      t.y += v.y;
+      t.z += v.z;
+      t.w += v.w;
+    }
+  }
+  acc[g][q] = t;
+  __syncthreads();
+  if (threadIdx.x >= 64) return;
+  const int c = blockIdx.x * 64 + threadIdx.x;
+  if (c >= D) return;
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s += reinterpret_cast<const float*>(&acc[i][0])[threadIdx.x];
+  if constexpr (sizeof(WT) == 2) st_global(dw + c, f32_to_bf16(s));
+  else st_global(dw + c, s);
+}
+
+// ----------------------------------------------------------------- launches ----
+constexpr int64_t kMaxItems = int64_t(1) << 30;   // of one launch; longer matrices go in runs of rows
+constexpr int64_t kMaxCols = (int64_t(1) << 24) - 1;   // 128 rows stay below that
+constexpr int kNormMaxD = 16384;
+
+// Calls go(items, unroll tag, workgroups) over the eights of a [rows, cols] matrix.  Four eights a thread keep 64
+// bytes a lane in flight; a matrix that then leaves CUs without two workgroups takes one a thread.
+template <int UMAX, typename F>
+int for_items(int64_t rows, int64_t cols, F go) {
+  const int64_t per = (cols + kActBlock - 1) / kActBlock * (kActBlock / 8);
+  int64_t run = kMaxItems / per;
+  run = run < 128 ? run : run / 128 * 128;   // whole 128-row tiles
+  for (int64_t r = 0; r < rows; r += run) {
+    const int64_t n = (rows - r < run ? rows - r : run) * per;
+    const Items t{FastDiv(uint32_t(per)), uint32_t(n), r, int(cols)};
+    if (n >= int64_t(512) * UMAX * device_cus()) go(t, std::integral_constant<int, UMAX>{}, unsigned((n + 256 * UMAX - 1) / (256 * UMAX)));
+    else go(t, std::integral_constant<int, 1>{}, unsigned((n + 255) / 256));
+  }
+  return 0;
+}
+
+template <typename F>
+void for_dtype(int dtype, F go) {
+  if (dtype == FM_DTYPE_BF16) go(uint16_t{});
+  else go(float{});
+}
+
+bool dtype_ok(int d) { return d == FM_DTYPE_BF16 || d == FM_DTYPE_F32; }
+bool kept_ok(const void* q, int64_t ld_q, const void* codes, int64_t ld_c, int64_t cols) {
+  return q && codes && ld_q >= cols && ld_q % kActBlock == 0 && ld_c * kActBlock >= ld_q && (reinterpret_cast<uintptr_t>(q) & 7) == 0;
+}
+
+// ---- the norm's shapes
+int norm_waves(int64_t D) { return int((D + 1023) / 1024); }
+int64_t norm_rows_per_slice(int64_t T, int64_t D) {
+  const int64_t least = norm_waves(D) == 1 ? 8 : 4, r = (T + 1023) / 1024;
+  return r < least ? least : r;
+}
+
+// go(eights a lane, one wave to a row, a width that is no multiple of 8)
+template <typename F>
+void for_norm(int64_t D, F go) {
+  using yes = std::true_type;
+  using no = std::false_type;
+  auto with_tail = [&](auto nc, auto one) {
+    if (D % 8) go(nc, one, yes{});
+    else go(nc, one, no{});
+  };
+  if (D <= 512) with_tail(std::integral_constant<int, 1>{}, yes{});
+  else if (D <= 1024) with_tail(std::integral_constant<int, 2>{}, yes{});
+  else with_tail(std::integral_constant<int, 2>{}, no{});
+}
+
+}  // namespace
+}  // namespace fm
+
+using namespace fm;
+
+extern "C" {
+
+int fm_act8_compress(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t ld_x, void* q, int64_t ld_q, void* codes,
+                     int64_t ld_c, const int32_t* tile_valid, void* stream) {
+  FM_REQUIRE(rows >= 0 && cols >= 1 && cols <= kMaxCols, "fm_act8_compress: bad sizes");
+  FM_REQUIRE(dtype_ok(x_dtype), "fm_act8_compress: x must be bf16 or fp32");
+  if (rows == 0) return 0;
+  FM_REQUIRE(x && ld_x >= 0, "fm_act8_compress: null x or negative pitch");
+  FM_REQUIRE(kept_ok(q, ld_q, codes, ld_c, cols) && ld_q == (cols + 31) / 32 * 32, "fm_act8_compress: the payload's pitch is cols rounded up to 32, "
+             "on 8 bytes, a code to 32 columns");
+  const CompressArgs a{x, ld_x, static_cast<uint8_t*>(q), ld_q, static_cast<uint8_t*>(codes), ld_c, tile_valid};
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  for_dtype(x_dtype, [&](auto t) {
+    for_items<4>(rows, cols, [&](const Items& items, auto u, unsigned wgs) {
+      hipLaunchKernelGGL((compress_kernel<decltype(t), decltype(u)::value>), dim3(wgs), dim3(256), 0, s, items, a);
+    });
+  });
+  return check_launch("fm_act8_compress");
+}
+
+int fm_act8_restore(const void* q, int64_t ld_q, const void* codes, int64_t ld_c, int64_t src_rows, int64_t cols, const int32_t* index,
+                    int64_t rows, void* out, int out_dtype, int64_t ld_out, void* stream) {
+  FM_REQUIRE(rows >= 0 && src_rows >= 0 && cols >= 1 && cols <= kMaxCols, "fm_act8_restore: bad sizes");
+  FM_REQUIRE(dtype_ok(out_dtype), "fm_act8_restore: the output must be bf16 or fp32");
+  FM_REQUIRE(index || rows <= src_rows, "fm_act8_restore: more rows than there are");
+  if (rows == 0) return 0;
+  FM_REQUIRE(out && ld_out >= cols, "fm_act8_restore: null output or a pitch below cols");
+  FM_REQUIRE(src_rows == 0 || kept_ok(q, ld_q, codes, ld_c, cols), "fm_act8_restore: bad payload, codes or pitches");
+  const RestoreArgs a{Act8{static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(codes), ld_q, ld_c}, index, src_rows, out, ld_out};
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  for_dtype(out_dtype, [&](auto t) {
+    for_items<4>(rows, cols, [&](const Items& items, auto u, unsigned wgs) {
+      if (index) hipLaunchKernelGGL((restore_kernel<decltype(t), decltype(u)::value, true>), dim3(wgs), dim3(256), 0, s, items, a);
+      else hipLaunchKernelGGL((restore_kernel<decltype(t), decltype(u)::value, false>), dim3(wgs), dim3(256), 0, s, items, a);
+    });
+  });
+  return check_launch("fm_act8_restore");
+}
+
+int fm_act8_swiglu(const void* g, int64_t ld_g, const void* u, int64_t ld_u, int dtype, int64_t rows, int64_t H, void* h, int64_t ld_h,
+                   void* qg, void* cg, void* qu, void* cu, int64_t ld_q, int64_t ld_c, void* stream) {
+  FM_REQUIRE(rows >= 0 && H >= 1 && H <= kMaxCols, "fm_act8_swiglu: bad sizes");
+  FM_REQUIRE(dtype_ok(dtype), "fm_act8_swiglu: gate and up must be bf16 or fp32");
+  if (rows == 0) return 0;
+  FM_REQUIRE(g && u && h && ld_g >= 0 && ld_u >= 0 && ld_h >= H, "fm_act8_swiglu: null pointer or bad pitch");
+  FM_REQUIRE(kept_ok(qg, ld_q, cg, ld_c, H) && kept_ok(qu, ld_q, cu, ld_c, H), "fm_act8_swiglu: bad payload, codes or pitches");
+  const SwigluArgs a{g, u, ld_g, ld_u, h, ld_h, static_cast<uint8_t*>(qg), static_cast<uint8_t*>(qu), static_cast<uint8_t*>(cg),
+                     static_cast<uint8_t*>(cu), ld_q, ld_c};
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  for_dtype(dtype, [&](auto t) {
+    for_items<2>(rows, H, [&](const Items& items, auto n, unsigned wgs) {
+      hipLaunchKernelGGL((swiglu_kernel<decltype(t), decltype(n)::value>), dim3(wgs), dim3(256), 0, s, items, a);
+    });
+  });
+  return check_launch("fm_act8_swiglu");
+}
+
+int fm_act8_swiglu_backward(const void* dh, int64_t ld_dh, int dtype, int64_t rows, int64_t H, const void* qg, const void* cg, const void* qu,
+                            const void* cu, int64_t ld_q, int64_t ld_c, void* dg, int64_t ld_dg, void* du, int64_t ld_du, void* stream) {
+  FM_REQUIRE(rows >= 0 && H >= 1 && H <= kMaxCols, "fm_act8_swiglu_backward: bad sizes");
+  FM_REQUIRE(dtype_ok(dtype), "fm_act8_swiglu_backward: dh must be bf16 or fp32");
+  if (rows == 0) return 0;
+  FM_REQUIRE(dh && dg && du && ld_dh >= 0 && ld_dg >= H && ld_du >= H, "fm_act8_swiglu_backward: null pointer or bad pitch");
+  FM_REQUIRE(kept_ok(qg, ld_q, cg, ld_c, H) && kept_ok(qu, ld_q, cu, ld_c, H), "fm_act8_swiglu_backward: bad payload, codes or pitches");
+  const SwigluBwdArgs a{dh, ld_dh, Act8{static_cast<const uint8_t*>(qg), static_cast<const uint8_t*>(cg), ld_q, ld_c},
+                        Act8{static_cast<const uint8_t*>(qu), static_cast<const uint8_t*>(cu), ld_q, ld_c}, dg, du, ld_dg, ld_du};
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  for_dtype(dtype, [&](auto t) {
+    for_items<2>(rows, H, [&](const Items& items, auto n, unsigned wgs) {
+      hipLaunchKernelGGL((swiglu_backward_kernel<decltype(t), decltype(n)::value>), dim3(wgs), dim3(256), 0, s, items, a);
+    });
+  });
+  return check_launch("fm_act8_swiglu_backward");
+}
+
+int fm_act8_rmsnorm(const void* x, int dtype, int64_t ld_x, int64_t T, int64_t D, const void* w, int w_dtype, float eps, void* y, int64_t ld_y,
+                    void* q, int64_t ld_q, void* codes, int64_t ld_c, float* rstd, void* stream) {
+  FM_REQUIRE(T >= 0 && T < (int64_t(1) << 31) && D >= 1 && D <= kNormMaxD, "fm_act8_rmsnorm: D must be 1 to %d, T below 2^31", kNormMaxD);
+  FM_REQUIRE(dtype_ok(dtype) && dtype_ok(w_dtype), "fm_act8_rmsnorm: x and the weight must be bf16 or fp32");
+  if (T == 0) return 0;
+  FM_REQUIRE(x && w && y && rstd && ld_x >= 0 && ld_y >= D, "fm_act8_rmsnorm: null pointer or bad pitch");
+  FM_REQUIRE(kept_ok(q, ld_q, codes, ld_c, D) && ld_q == (D + 31) / 32 * 32, "fm_act8_rmsnorm: bad payload, codes or pitches");
+  const NormArgs a{x, ld_x, T, int(D), w, eps, y, ld_y, static_cast<uint8_t*>(q), ld_q, static_cast<uint8_t*>(codes), ld_c, rstd};
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  for_dtype(dtype, [&](auto t) {
+    for_dtype(w_dtype, [&](auto wt) {
+      for_norm(D, [&](auto nc, auto one, auto tail) {
+        constexpr bool kOne = decltype(one)::value;
+        hipLaunchKernelGGL((norm_kernel<decltype(t), decltype(wt), decltype(nc)::value, kOne, decltype(tail)::value>),
+                           dim3(unsigned(kOne ? (T + 3) / 4 : T)), dim3(kOne ? 256 : 64 * norm_waves(D)), 0, s, a);
+      });
+    });
+  });
+  return check_launch("fm_act8_rmsnorm");
+}
+
+int64_t fm_act8_rmsnorm_backward_workspace_bytes(int64_t T, int64_t D) {
+  if (T <= 0 || D <= 0) return 0;
+  const int64_t rps = norm_rows_per_slice(T, D);
+  return (T + rps - 1) / rps * ((D + 7) / 8 * 8) * int64_t(sizeof(float));
+}
+
+int fm_act8_rmsnorm_backward(const void* dy, int64_t ld_dy, int dtype, int64_t T, int64_t D, const void* q, int64_t ld_q, const void* codes,
+                             int64_t ld_c, const void* w, int w_dtype, const float* rstd, void* dx, int64_t ld_dx, void* dw,
+                             void* workspace, int64_t workspace_bytes, void* stream) {
+  FM_REQUIRE(T >= 1 && T < (int64_t(1) << 31) && D >= 1 && D <= kNormMaxD, "fm_act8_rmsnorm_backward: D must be 1 to %d, T 1 to 2^31 - 1", kNormMaxD);
+  FM_REQUIRE(dtype_ok(dtype) && dtype_ok(w_dtype), "fm_act8_rmsnorm_backward: dy and the weight must be bf16 or fp32");
+  FM_REQUIRE(dy && w && rstd && dx && ld_dy >= 0 && ld_dx >= D, "fm_act8_rmsnorm_backward: null pointer or bad pitch");
+  FM_REQUIRE(kept_ok(q, ld_q, codes, ld_c, D), "fm_act8_rmsnorm_backward: bad payload, codes or pitches");
+  FM_REQUIRE(dw == nullptr || (workspace && aligned16(workspace) && workspace_bytes >= fm_act8_rmsnorm_backward_workspace_bytes(T, D)),
+             "fm_act8_rmsnorm_backward: dw needs a workspace of fm_act8_rmsnorm_backward_workspace_bytes(T, D) bytes on 16");
+  const int64_t rps = norm_rows_per_slice(T, D), slices = (T + rps - 1) / rps, ld_p = (D + 7) / 8 * 8;
+  float* part = static_cast<float*>(workspace);
+  const NormBwdArgs a{dy, ld_dy, Act8{static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(codes), ld_q, ld_c}, T, int(D), w, rstd,
+                      dx, ld_dx, dw ? part : nullptr, ld_p, rps};
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  for_dtype(dtype, [&](auto t) {
+    for_dtype(w_dtype, [&](auto wt) {
+      for_norm(D, [&](auto nc, auto one, auto tail) {
+        constexpr bool kOne = decltype(one)::value;
+        hipLaunchKernelGGL((norm_backward_kernel<decltype(t), decltype(wt), decltype(nc)::value, kOne, decltype(tail)::value>),
+                           dim3(unsigned(slices)), dim3(kOne ? 256 : 64 * norm_waves(D)), 0, s, a);
+      });
+    });
+  });
+  if (int rc = check_launch("fm_act8_rmsnorm_backward")) return rc;
+  if (dw == nullptr) return 0;
+  for_dtype(w_dtype, [&](auto wt) {
+    using WT = decltype(wt);
+    hipLaunchKernelGGL(norm_dw_kernel<WT>, dim3(unsigned((D + 63) / 64)), dim3(256), 0, s, part, ld_p, int(slices), int(D), static_cast<WT*>(dw));
+  });
+  return check_launch("fm_act8_rmsnorm_backward");
+}
+
+}  // extern "C"

@@ -165,16 +165,24 @@ class RMSNorm(torch.nn.Module):
     """``RMSNorm(size, eps=1e-6, full_precision=True)`` of the reference
     (``model/norm.py:18-49``) on the HIP kernels: fp32 weight initialised to
     ones, fp32 arithmetic, bf16 in and out.  ``full_precision=False`` (bf16
-    arithmetic) is not offered."""
+    arithmetic) is not offered.  ``checkpoint_8bit``: the input is kept for the
+    backward in 8 bits (``rmsnorm_8bit``; any size up to 16384, bf16 or fp32)."""
 
-    def __init__(self, size: int, *, eps: float = DEFAULT_EPS, full_precision: bool = True):
+    def __init__(self, size: int, *, eps: float = DEFAULT_EPS, full_precision: bool = True,
+                 checkpoint_8bit: bool = False):
         super().__init__()
         if not full_precision:
             raise NotImplementedError("the MI355X RMSNorm computes in fp32 (full_precision=True)")
-        _check_d(size)
+        self.checkpoint_8bit = bool(checkpoint_8bit)
+        if not self.checkpoint_8bit:
+            _check_d(size)
         self.eps = eps
         self.full_precision = True
         self.weight = torch.nn.Parameter(torch.ones(size))
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if self.checkpoint_8bit:
+            from .act8 import rmsnorm_8bit
+
+            return rmsnorm_8bit(x, self.weight, self.eps)
         return rmsnorm(x, self.weight, self.eps)
