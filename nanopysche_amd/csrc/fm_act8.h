@@ -57,11 +57,10 @@ __device__ __forceinline__ uint2 act_encode8(const float (&v)[8], uint32_t& code
   const float inv = act_inverse(code);
   return make_uint2(act_bytes4(v, inv), act_bytes4(v + 4, inv));
 }
-// q s of four bytes: q + 128 converts as an unsigned byte.
+// q s of four bytes (the conversion takes a sign-extended byte of the word).
 __device__ __forceinline__ void act_decode4(uint32_t w, float s, float* v) {
-  w ^= 0x80808080u;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = (float((w >> (8 * i)) & 0xffu) - 128.f) * s;
+  for (int i = 0; i < 4; ++i) v[i] = float(int8_t(w >> (8 * i))) * s;
 }
 __device__ __forceinline__ void act_decode8(uint2 w, float s, float (&v)[8]) {
   act_decode4(w.x, s, v);

@@ -9,6 +9,7 @@
 #include <type_traits>
 
 #include "fm_act8.h"
+#include "fm_lanes.h"
 #include "fm_silu.h"
 #include "../../include/fm_hip.h"
 
@@ -257,10 +258,10 @@ __global__ __launch_bounds__(256) void swiglu_backward_kernel(Items t, SwigluBwd
 }
 
 // ---------------------------------------------------------------- RMSNorm ----
-// A row sits in the registers of W waves, two eights a lane at most: lane l of them holds columns 8 l .. + 8 and, past the
-// waves' first 512 W, 8 l + 512 W .. + 8.  W = 1 takes up to 1024 columns, four rows to a workgroup of four waves; wider rows
-// take a workgroup of W = ceil(D / 1024) waves each, so the lanes of any width are busy and the backward keeps w,
-// dw's share and a row's operands in about a hundred registers.
+// A row sits in the registers of W waves: lane l of them holds columns 8 l .. + 8 and, of rows wider than 512, 8 l + 512 W .. + 8
+// too.  Up to 512 columns W is 1, four rows to a workgroup of four waves; wider rows take a workgroup of W = ceil(D / 1024)
+// waves each, so the lanes of any width are busy.  (One eight a lane and twice the waves was slower, 16384 rows of 7168:
+// forward 132 us against 100, backward 162 against 129: fewer rows on a CU, and each waits for its slowest wave.)
 struct NormArgs {
   const void* x;
   int64_t ld_x, T;
@@ -276,16 +277,10 @@ struct NormArgs {
   float* rstd;
 };
 
-__device__ __forceinline__ float wave_sum64(float v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
-  return v;
-}
-
 // Sum over a row's waves, in wave order; `parity` alternates between rows, so one barrier is enough.
 template <bool ONE>
 __device__ __forceinline__ float row_sum(float v, float (*sums)[16], int parity) {
-  v = wave_sum64(v);
+  v = group_sum<64>(v);
   if constexpr (!ONE) {
     if ((threadIdx.x & 63) == 0) sums[parity][threadIdx.x >> 6] = v;
     __syncthreads();
@@ -391,33 +386,39 @@ __global__ __launch_bounds__(ONE ? 256 : 1024) void norm_backward_kernel(NormBwd
   }
   constexpr int kStep = ONE ? 4 : 1;
   int parity = 0;
-  for (int64_t row = r0 + (ONE ? wave : 0); row < r1; row += kStep, parity ^= 1) {
-    NormRow<T, NC, TAIL> n;
-    n.load(a, row, lane, step);
-    float dot = 0.f;
+  const int64_t first = r0 + (ONE ? wave : 0);
+  // the next row's loads are in flight while this one is summed, where 128 registers hold both
+  constexpr bool kNext = ONE || sizeof(T) == 2;
+  NormRow<T, NC, TAIL> n, next;
+  if (kNext && first < r1) next.load(a, first, lane, step);
+  for (int64_t row = first; row < r1; row += kStep, parity ^= 1) {
+    if constexpr (kNext) {
+      n = next;
+      if (row + kStep < r1) next.load(a, row + kStep, lane, step);
+    } else {
+      n.load(a, row, lane, step);
+    }
+    // x r from the bytes in one product (s r is exact), and dx = r (a - (sum a x r / D) x r)
+    float xr[NC][8], g[NC][8], dot = 0.f;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      float xv[8], dv[8];
-      act_decode8(n.q[c], act_scale(n.code[c]), xv);
-      n.dy[c].widen(dv);
+      act_decode8(n.q[c], act_scale(n.code[c]) * n.r, xr[c]);
+      n.dy[c].widen(g[c]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        pdw[c][j] = fmaf(dv[j], xv[j] * n.r, pdw[c][j]);
-        dot = fmaf(dv[j] * wv[c][j], xv[j], dot);
+        pdw[c][j] = fmaf(g[c][j], xr[c][j], pdw[c][j]);
+        g[c][j] *= wv[c][j];
+        dot = fmaf(g[c][j], xr[c][j], dot);
       }
     }
-    dot = row_sum<ONE>(dot, sums, parity);
-    const float k = ((n.r * n.r) * n.r) * (dot * inv_d);
+    const float m = row_sum<ONE>(dot, sums, parity) * inv_d;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int col = step * c + 8 * lane;
       if (col >= a.D) break;
-      float xv[8], dv[8];
-      act_decode8(n.q[c], act_scale(n.code[c]), xv);
-      n.dy[c].widen(dv);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) dv[j] = n.r * (dv[j] * wv[c][j]) - k * xv[j];
-      store8<T, TAIL>(static_cast<T*>(a.dx) + row * a.ld_dx + col, dv, a.D - col);
+      for (int j = 0; j < 8; ++j) g[c][j] = n.r * fmaf(-m, xr[c][j], g[c][j]);
+      store8<T, TAIL>(static_cast<T*>(a.dx) + row * a.ld_dx + col, g[c], a.D - col);
     }
   }
   if (a.part == nullptr) return;
@@ -441,16 +442,17 @@ __global__ __launch_bounds__(ONE ? 256 : 1024) void norm_backward_kernel(NormBwd
   }
 }
 
-// dw from the slices' shares: a workgroup takes 64 columns, sixteen rows of threads every sixteenth slice each, and
-// adds the sixteen sums in order.
+// dw from the slices' shares: a workgroup takes 16 columns, 64 rows of threads every 64th slice each, then the sums of
+// sixteen rows of a wave and of the four waves, in a fixed order.
 template <typename WT>
 __global__ __launch_bounds__(256) void norm_dw_kernel(const float* part, int64_t ld_p, int slices, int D, WT* dw) {
-  __shared__ float4 acc[16][16];
-  const int q = threadIdx.x & 15, g = threadIdx.x >> 4;
-  const int col = blockIdx.x * 64 + q * 4;
+  __shared__ float4 acc[4][4];
+  const int q = threadIdx.x & 3, g = threadIdx.x >> 2;
+  const int col = blockIdx.x * 16 + q * 4;
   float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
   if (col < ld_p) {
-    for (int s = g; s < slices; s += 16) {
+#pragma unroll 4
+    for (int s = g; s < slices; s += 64) {
       const float4 v = *reinterpret_cast<const float4*>(part + s * ld_p + col);
       t.x += v.x;
       t.y += v.y;
@@ -458,14 +460,20 @@ __global__ __launch_bounds__(256) void norm_dw_kernel(const float* part, int64_t
       t.w += v.w;
     }
   }
-  acc[g][q] = t;
+#pragma unroll
+  for (int off = 4; off < 64; off <<= 1) {
+    t.x += __shfl_xor(t.x, off);
+    t.y += __shfl_xor(t.y, off);
+    t.z += __shfl_xor(t.z, off);
+    t.w += __shfl_xor(t.w, off);
+  }
+  if ((threadIdx.x & 63) < 4) acc[threadIdx.x >> 6][q] = t;
   __syncthreads();
-  if (threadIdx.x >= 64) return;
-  const int c = blockIdx.x * 64 + threadIdx.x;
-  if (c >= D) return;
+  const int c = blockIdx.x * 16 + threadIdx.x;
+  if (threadIdx.x >= 16 || c >= D) return;
   float s = 0.f;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) s += reinterpret_cast<const float*>(&acc[i][0])[threadIdx.x];
+  for (int i = 0; i < 4; ++i) s += reinterpret_cast<const float*>(&acc[i][0])[threadIdx.x];
   if constexpr (sizeof(WT) == 2) st_global(dw + c, f32_to_bf16(s));
   else st_global(dw + c, s);
 }
@@ -504,9 +512,14 @@ bool kept_ok(const void* q, int64_t ld_q, const void* codes, int64_t ld_c, int64
 
 // ---- the norm's shapes
 int norm_waves(int64_t D) { return int((D + 1023) / 1024); }
+// Rows of a workgroup of the backward: one round of the workgroups that fit (sixteen waves to a CU), but no more than 1024 of them: each
+// writes D sums that the second launch reads.
 int64_t norm_rows_per_slice(int64_t T, int64_t D) {
-  const int64_t least = norm_waves(D) == 1 ? 8 : 4, r = (T + 1023) / 1024;
-  return r < least ? least : r;
+  const int w = D <= 512 ? 4 : norm_waves(D), rows = D <= 512 ? 4 : 1;
+  int64_t most = int64_t(device_cus()) * (16 / w);
+  most = most < 1024 ? most : 1024;
+  const int64_t r = (T + most - 1) / most;
+  return (r + rows - 1) / rows * rows;
 }
 
 // go(eights a lane, one wave to a row, a width that is no multiple of 8)
@@ -519,7 +532,6 @@ void for_norm(int64_t D, F go) {
     else go(nc, one, no{});
   };
   if (D <= 512) with_tail(std::integral_constant<int, 1>{}, yes{});
-  else if (D <= 1024) with_tail(std::integral_constant<int, 2>{}, yes{});
   else with_tail(std::integral_constant<int, 2>{}, no{});
 }
 
@@ -657,7 +669,7 @@ int fm_act8_rmsnorm_backward(const void* dy, int64_t ld_dy, int dtype, int64_t T
   if (dw == nullptr) return 0;
   for_dtype(w_dtype, [&](auto wt) {
     using WT = decltype(wt);
-    hipLaunchKernelGGL(norm_dw_kernel<WT>, dim3(unsigned((D + 63) / 64)), dim3(256), 0, s, part, ld_p, int(slices), int(D), static_cast<WT*>(dw));
+    hipLaunchKernelGGL(norm_dw_kernel<WT>, dim3(unsigned((D + 15) / 16)), dim3(256), 0, s, part, ld_p, int(slices), int(D), static_cast<WT*>(dw));
   });
   return check_launch("fm_act8_rmsnorm_backward");
 }

@@ -16,8 +16,8 @@
 // and leaves E cnt / n^2 for the backward, a third adds the sequences.  Backward: one pass, logits in, gradient out.
 #include <type_traits>
 
+#include "fm_lanes.h"
 #include "fm_silu.h"
-#include "fm_tile.h"
 #include "../../include/fm_hip.h"
 
 namespace fm {
@@ -27,33 +27,6 @@ constexpr int kMaxExperts = 1024;
 constexpr float kSumFloor = 1e-8f;
 
 typedef float f32x4_el __attribute__((ext_vector_type(4), aligned(4)));
-
-// lanes of a group of N (a power of two): sum and maximum, the same in every lane
-template <int N, typename F>
-__device__ __forceinline__ float group_fold(float v, F f) {
-  auto dpp = [](float x, auto ctrl) { return __builtin_bit_cast(float, dpp_move<decltype(ctrl)::value>(__builtin_bit_cast(int, x))); };
-  if constexpr (N > 1) v = f(v, dpp(v, std::integral_constant<int, kDppQuadSwap1>{}));
-  if constexpr (N > 2) v = f(v, dpp(v, std::integral_constant<int, kDppQuadSwap2>{}));
-  if constexpr (N > 4) v = f(v, dpp(v, std::integral_constant<int, kDppRowHalfMirror>{}));
-  if constexpr (N > 8) v = f(v, dpp(v, std::integral_constant<int, kDppRowRor8>{}));
-  if constexpr (N > 16) {
-    const auto a = __builtin_amdgcn_permlane16_swap(f2u(v), f2u(v), false, false);
-    v = f(u2f(a[0]), u2f(a[1]));
-  }
-  if constexpr (N > 32) {
-    const auto a = __builtin_amdgcn_permlane32_swap(f2u(v), f2u(v), false, false);
-    v = f(u2f(a[0]), u2f(a[1]));
-  }
-  return v;
-}
-template <int N>
-__device__ __forceinline__ float group_sum(float v) {
-  return group_fold<N>(v, [](float a, float b) { return a + b; });
-}
-template <int N>
-__device__ __forceinline__ float group_max(float v) {
-  return group_fold<N>(v, [](float a, float b) { return fmaxf(a, b); });
-}
 
 // e^d for d <= 0 (or NaN) to about an ulp: 2^(d log2 e) by the hardware, the product's rounding error as a factor.
 __device__ __forceinline__ float exp_below(float d) {
