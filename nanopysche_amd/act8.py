@@ -22,7 +22,6 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .decode import _same_device
 from .norm import DEFAULT_EPS
 
 ACT8_BLOCK = 32
@@ -139,17 +138,24 @@ class Activation8:
         return _restore(self, index.contiguous(), index.numel(), (index.numel(), self.cols), out_dtype or self._dtype)
 
 
-def _new(data: torch.Tensor, shape, dtype) -> Activation8:
-    """An Activation8 of a buffer made for it: fits by construction."""
+def _empty(shape: torch.Size, rows: int, dtype, dev) -> Activation8:
+    """Room for an activation of this shape; fits by construction."""
     t = Activation8.__new__(Activation8)
-    t._data, t._shape, t._dtype = data, shape, dtype
-    t._sizes = shape[:-1].numel(), shape[-1], _pitch(shape[-1])
+    cols = shape[-1]
+    pitch = (cols + 31) // 32 * 32
+    t._data = torch.empty(rows * pitch // 32 * 33, dtype=torch.uint8, device=dev)
+    t._shape, t._dtype, t._sizes = shape, dtype, (rows, cols, pitch)
     return t
 
 
-def _empty(shape: torch.Size, dtype, dev) -> Activation8:
-    cols = shape[-1]
-    return _new(torch.empty(_bytes(shape[:-1].numel(), cols), dtype=torch.uint8, device=dev), shape, dtype)
+def _like(x: torch.Tensor) -> torch.Tensor:
+    """An empty contiguous tensor like x."""
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
+def _here(index: int, what: str, t: torch.Tensor) -> None:
+    if t.get_device() != index:
+        raise ValueError(f"{what} is on {t.device}, the others on device {index}")
 
 
 def _rows(x: torch.Tensor, what: str, most: int = MAX_ACT8_COLS) -> torch.Tensor:
@@ -175,11 +181,12 @@ def _restore(t: Activation8, index, rows, shape, dtype) -> torch.Tensor:
 
 
 def _compress(x2: torch.Tensor, shape, tile_valid=None) -> Activation8:
-    t = _empty(shape, x2.dtype, x2.device)
-    if t.rows:
+    rows, cols = x2.shape
+    t = _empty(shape, rows, x2.dtype, x2.device)
+    if rows:
         q, codes, ld_q, ld_c = t.at()
         with _lib.on_device_of(x2):
-            _lib.call("fm_act8_compress", x2.data_ptr(), _DTYPES[x2.dtype], t.rows, t.cols, x2.stride(0), q, ld_q, codes, ld_c,
+            _lib.call("fm_act8_compress", x2.data_ptr(), _DTYPES[x2.dtype], rows, cols, x2.stride(0), q, ld_q, codes, ld_c,
                       _lib.addr(tile_valid), _lib.stream_of(x2))
     return t
 
@@ -200,34 +207,32 @@ class SwigluKept(NamedTuple):
 
 
 def _halves(gate: torch.Tensor, up: Optional[torch.Tensor]):
-    """Rows of gate and up; the shape of h."""
+    """(gate's and up's tensors of rows, up's address, the shape of h): up's rows may be the second half of gate's."""
     if up is None:
         g2 = _rows(gate, "gate", 2 * MAX_ACT8_COLS)
-        H, odd = divmod(gate.shape[-1], 2)
+        H, odd = divmod(g2.shape[1], 2)
         if odd:
             raise ValueError(f"gate|up must have an even number of columns, got {gate.shape[-1]}")
-        _check_cols(H)
-        return g2[:, :H], g2[:, H:], torch.Size((*gate.shape[:-1], H))
+        return g2, g2, g2.data_ptr() + H * g2.element_size(), torch.Size((*gate.shape[:-1], H))
     if up.shape != gate.shape or up.dtype != gate.dtype:
         raise ValueError(f"gate and up must be alike, got {tuple(gate.shape)} {gate.dtype} and {tuple(up.shape)} {up.dtype}")
     g2, u2 = _rows(gate, "gate"), _rows(up, "up")
-    _same_device(g2, up=u2)
-    return g2, u2, gate.shape
+    _here(g2.get_device(), "up", u2)
+    return g2, u2, u2.data_ptr(), gate.shape
 
 
 def swiglu_compress(gate: torch.Tensor, up: Optional[torch.Tensor] = None) -> SwigluKept:
     """h = silu(gate) * up (fp32 arithmetic, rounded once) and gate and up in 8 bits, in one pass.
     gate and up [..., H], bf16 or fp32, or one tensor [..., 2H] of the gate's columns and then up's."""
-    g2, u2, shape = _halves(gate, up)
-    H, dev = shape[-1], g2.device
-    rows = g2.shape[0]
-    h = torch.empty(shape, dtype=g2.dtype, device=dev)
-    kept_g, kept_u = _empty(shape, g2.dtype, dev), _empty(shape, g2.dtype, dev)
+    g2, u2, at_u, shape = _halves(gate, up)
+    H, rows, dtype, dev = shape[-1], g2.shape[0], g2.dtype, g2.device
+    h = torch.empty(shape, dtype=dtype, device=dev)
+    kept_g, kept_u = _empty(shape, rows, dtype, dev), _empty(shape, rows, dtype, dev)
     if rows:
         qg, cg, ld_q, ld_c = kept_g.at()
         qu, cu, _, _ = kept_u.at()
         with _lib.on_device_of(g2):
-            _lib.call("fm_act8_swiglu", g2.data_ptr(), g2.stride(0), u2.data_ptr(), u2.stride(0), _DTYPES[g2.dtype], rows, H,
+            _lib.call("fm_act8_swiglu", g2.data_ptr(), g2.stride(0), at_u, u2.stride(0), _DTYPES[dtype], rows, H,
                       h.data_ptr(), H, qg, cg, qu, cu, ld_q, ld_c, _lib.stream_of(g2))
     return SwigluKept(h, kept_g, kept_u)
 
@@ -238,13 +243,15 @@ def swiglu_backward_8bit(dh: torch.Tensor, gate: Activation8, up: Activation8, p
     if dh.shape != gate.shape or up.shape != gate.shape:
         raise ValueError(f"dh, gate and up must be alike, got {tuple(dh.shape)}, {tuple(gate.shape)} and {tuple(up.shape)}")
     d2 = _rows(dh, "dh")
-    _same_device(d2, gate=gate.data, up=up.data)
+    index = d2.get_device()
+    _here(index, "gate", gate._data)
+    _here(index, "up", up._data)
     rows, H = d2.shape
     if packed:
         both = torch.empty((*dh.shape[:-1], 2 * H), dtype=dh.dtype, device=dh.device)
         at_g, at_u, ld = both.data_ptr(), both.data_ptr() + H * both.element_size(), 2 * H
     else:
-        dg, du = torch.empty(dh.shape, dtype=dh.dtype, device=dh.device), torch.empty(dh.shape, dtype=dh.dtype, device=dh.device)
+        dg, du = _like(dh), _like(dh)
         at_g, at_u, ld = dg.data_ptr(), du.data_ptr(), H
     if rows:
         qg, cg, ld_q, ld_c = gate.at()
@@ -299,11 +306,11 @@ def rmsnorm_compress(x: torch.Tensor, weight: torch.Tensor, eps: float = DEFAULT
     x2 = _rows(x, "x", MAX_ACT8_NORM)
     T, D = x2.shape
     w = _norm_weight(weight, D)
-    _same_device(x2, weight=w)
+    _here(x2.get_device(), "weight", w)
     dev = x2.device
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    y = _like(x)
     rstd = torch.empty(T, dtype=torch.float32, device=dev)
-    kept = _empty(x.shape, x.dtype, dev)
+    kept = _empty(x.shape, T, x.dtype, dev)
     if T:
         q, codes, ld_q, ld_c = kept.at()
         with _lib.on_device_of(x2):
@@ -321,8 +328,11 @@ def rmsnorm_backward_8bit(dy: torch.Tensor, x: Activation8, weight: torch.Tensor
     w = _norm_weight(weight, D)
     if rstd.dtype != torch.float32 or rstd.numel() != T or not rstd.is_contiguous():
         raise ValueError(f"rstd must be {T} contiguous float32 values, got {rstd.dtype} {tuple(rstd.shape)}")
-    _same_device(d2, weight=w, rstd=rstd, kept=x.data)
-    dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
+    index = d2.get_device()
+    _here(index, "weight", w)
+    _here(index, "rstd", rstd)
+    _here(index, "x", x._data)
+    dx = _like(dy)
     dw = ws = None
     nbytes = 0
     if need_dw:

@@ -41,8 +41,7 @@ class BalanceState:
     logits: torch.Tensor               # [T, E]
     cu_seqlens: Optional[torch.Tensor]  # [S + 1] int32
     mask: Optional[torch.Tensor]       # [T] bool
-    f: torch.Tensor                    # [S, E] first: E slots / n_s^2
-    inverse: torch.Tensor              # [2]: 1 / S', 1 / tokens
+    f: torch.Tensor                    # [S * E + 2]: E slots / n_s^2, then 1 / S' and 1 / tokens
     sigmoid: bool
     z_mult: float
     shape: torch.Size                  # of the logits as given
@@ -73,7 +72,9 @@ def _check(logits, indices, cu_seqlens, token_mask, load_tracker):
     if indices.dim() < 1 or not 1 <= indices.shape[-1] <= MAX_BALANCE_TOP_K or indices.shape[:-1] != logits.shape[:-1]:
         raise ValueError(f"indices must be [..., K] for the logits' {tuple(logits.shape[:-1])} tokens, K of 1 to {MAX_BALANCE_TOP_K}, got "
                          f"{tuple(indices.shape)}")
-    idx = indices.reshape(T, indices.shape[-1]).contiguous()
+    idx = indices if indices.dim() == 2 else indices.reshape(T, indices.shape[-1])
+    if not idx.is_contiguous():
+        idx = idx.contiguous()
     cu = cu_seqlens
     if cu is not None:
         if cu.dtype != torch.int32:
@@ -88,7 +89,10 @@ def _check(logits, indices, cu_seqlens, token_mask, load_tracker):
         if mask.shape != logits.shape[:-1]:
             raise ValueError(f"token_mask must be {tuple(logits.shape[:-1])}, got {tuple(mask.shape)}")
         mask = mask.reshape(T).contiguous()
-    _same_device(l2, indices=idx, cu_seqlens=cu, token_mask=mask)
+    index = l2.get_device()
+    for name, t in (("indices", idx), ("cu_seqlens", cu), ("token_mask", mask)):
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"{name} is on {t.device}, the logits on {l2.device}")
     if load_tracker is not None:
         if load_tracker.num_experts != E:
             raise ValueError(f"load_tracker is for {load_tracker.num_experts} experts, the logits for {E}")
@@ -102,22 +106,22 @@ def balance_forward(logits: torch.Tensor, indices: torch.Tensor, *, cu_seqlens: 
     """(loss, counts, state) of ``balance_loss``'s arguments, state for ``balance_backward``; records no gradient."""
     sigmoid = _scores(scores)
     l2, idx, cu, mask = _check(logits, indices, cu_seqlens, token_mask, load_tracker)
-    l2 = l2.detach()
+    if l2.requires_grad:
+        l2 = l2.detach()
     T, E = l2.shape
     S = 1 if cu is None else cu.numel() - 1
     dev = l2.device
     z = 0.0 if z_loss_multiplier is None else float(z_loss_multiplier)
-    f = torch.empty(S * E + 2, dtype=torch.float32, device=dev)   # and the loss's two factors
-    inverse = f[S * E:]
+    f = torch.empty(S * E + 2, dtype=torch.float32, device=dev)
     loss = torch.empty((), dtype=torch.float32, device=dev)
     counts = torch.empty(E if cu is None else (S, E), dtype=torch.int32, device=dev)
     ws = torch.empty(_lib.size_of("fm_balance_workspace_bytes", T, E, S), dtype=torch.uint8, device=dev)
     acc, total = (None, None) if load_tracker is None else (load_tracker.tokens_per_expert, load_tracker.total_tokens)
     with _lib.on_device_of(l2):
         _lib.call("fm_balance_forward", l2.data_ptr(), l2.stride(0) if T > 1 else E, T, E, idx.data_ptr(), int(idx.dtype == torch.int64),
-                  idx.shape[1], _lib.addr(cu), S, _lib.addr(mask), int(sigmoid), z, f.data_ptr(), counts.data_ptr(), inverse.data_ptr(),
+                  idx.shape[1], _lib.addr(cu), S, _lib.addr(mask), int(sigmoid), z, f.data_ptr(), counts.data_ptr(), f.data_ptr() + 4 * S * E,
                   loss.data_ptr(), _lib.addr(acc), _lib.addr(total), ws.data_ptr(), ws.numel(), _lib.stream_of(l2))
-    return loss, counts, BalanceState(l2, cu, mask, f, inverse, sigmoid, z, logits.shape)
+    return loss, counts, BalanceState(l2, cu, mask, f, sigmoid, z, logits.shape)
 
 
 def balance_backward(state: BalanceState, dloss: torch.Tensor, add_to: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -125,9 +129,12 @@ def balance_backward(state: BalanceState, dloss: torch.Tensor, add_to: Optional[
     that do not count.  ``add_to`` ([T, E] fp32): added to it in place instead."""
     l2, cu = state.logits, state.cu_seqlens
     T, E = l2.shape
+    S = 1 if cu is None else cu.numel() - 1
     if dloss.dtype != torch.float32 or dloss.numel() != 1:
         raise TypeError(f"dloss must be one float32 value, got {dloss.dtype} {tuple(dloss.shape)}")
-    _same_device(l2, dloss=dloss, add_to=add_to)
+    for name, t in (("dloss", dloss), ("add_to", add_to)):
+        if t is not None and t.get_device() != l2.get_device():
+            raise ValueError(f"{name} is on {t.device}, the logits on {l2.device}")
     if add_to is None:
         out = torch.empty(state.shape, dtype=torch.float32, device=l2.device)
         ld = E
@@ -139,8 +146,8 @@ def balance_backward(state: BalanceState, dloss: torch.Tensor, add_to: Optional[
     if T:
         with _lib.on_device_of(l2):
             _lib.call("fm_balance_backward", l2.data_ptr(), l2.stride(0) if T > 1 else E, T, E, _lib.addr(cu),
-                      1 if cu is None else cu.numel() - 1, _lib.addr(state.mask), int(state.sigmoid), state.z_mult,
-                      state.f.data_ptr(), state.inverse.data_ptr(), dloss.data_ptr(), out.data_ptr(), ld, int(add_to is not None),
+                      S, _lib.addr(state.mask), int(state.sigmoid), state.z_mult,
+                      state.f.data_ptr(), state.f.data_ptr() + 4 * S * E, dloss.data_ptr(), out.data_ptr(), ld, int(add_to is not None),
                       _lib.stream_of(l2))
     return out
 
@@ -167,7 +174,7 @@ class _BalanceFunction(torch.autograd.Function):
         if l2.stride(1) != 1 or l2.stride(0) < l2.shape[1]:
             l2 = l2.contiguous()
         s = ctx.state
-        state = BalanceState(l2, cu, mask, s.f, s.inverse, s.sigmoid, s.z_mult, s.shape)
+        state = BalanceState(l2, cu, mask, s.f, s.sigmoid, s.z_mult, s.shape)
         return balance_backward(state, dloss.float()), None, None, None, None, None, None
 
 

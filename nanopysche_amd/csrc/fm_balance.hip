@@ -8,16 +8,17 @@
 // (f_se - sum_j f_sj p_tj) / (sum sigma + 1e-8) sigma (1 - sigma) in place of p (f - sum f p).
 // A token counts if it lies in a sequence and its mask says so; the others' logits may hold anything.
 //
-// Forward: one pass over the logits and indices.  A wave takes a run of C tokens; a token's logits sit in L
-// lanes (64 / L tokens side by side), whose column sums stay in registers; the slots are counted in LDS.
-// At the end of each sequence in its run the wave writes sums and counts to its own place in the workspace:
-// run c and sequence s meet at most once, and runs and sequences both ascend, so place c + s is theirs
-// alone.  A second launch adds each sequence's places in order (no float atomics: the same bits each time)
-// and leaves E cnt / n^2 for the backward, a third adds the sequences.  Backward: one pass, logits in, gradient out.
+// Forward: one pass over the logits and indices.  The batch is cut at sequence borders and into runs of tokens; run c and
+// sequence s meet at most once, and runs and sequences both ascend, so the number c + s names each piece, and a piece finds its
+// run and sequence from its number by a search of the borders.  A piece is the work of a wave, or of four where sequences are
+// long: a token's logits sit in L lanes (64 / L tokens side by side) whose column sums stay in registers, the slots are counted in
+// LDS, and both go to the piece's place in the workspace.  A second launch adds each sequence's places in order (no float
+// atomics: the same bits each time) and leaves E cnt / n^2 for the backward, a third adds the sequences; few tokens take one launch
+// for all of it.  Backward: the same pieces, logits in, gradient out; the tokens before the first border and behind the last
+// are two sequences more, of zeros.
 #include <type_traits>
 
 #include "fm_lanes.h"
-#include "fm_silu.h"
 #include "../../include/fm_hip.h"
 
 namespace fm {
@@ -50,33 +51,56 @@ struct BalanceArgs {
   const uint8_t* mask;     // [T], or null
   int sigmoid;
   int want_z;
-  int run;                 // tokens of a wave
+  int run;                 // tokens of a piece at most
+  int64_t places;          // pieces
   float* sums;             // [places, E]
   int32_t* slots;          // [places, E]
   int32_t* tokens;         // [places]
   float* z;                // [places]
 };
 
-__device__ __forceinline__ int64_t border(const BalanceArgs& a, int64_t s) {
-  if (a.cu == nullptr) return s == 0 ? 0 : a.T;
-  const int64_t b = a.cu[s];
-  return b < 0 ? 0 : (b > a.T ? a.T : b);
+// Start of sequence a - 1: a = 0 is the rest before the first border, a = S + 1 the rest behind the last.
+__device__ __forceinline__ int64_t border(const BalanceArgs& b, int64_t a) {
+  if (a <= 0) return 0;
+  if (a > b.S + 1) return b.T;
+  if (b.cu == nullptr) return a == 1 ? 0 : b.T;
+  const int64_t t = b.cu[a - 1];
+  return t < 0 ? 0 : (t > b.T ? b.T : t);
 }
 
-// The first sequence that may hold token t: the largest s with border s at or before t (0 if none).  64 candidates a round.
-__device__ __forceinline__ int64_t sequence_of(const BalanceArgs& a, int64_t t, int lane) {
-  if (a.cu == nullptr) return 0;
-  int64_t lo = 0, n = a.S + 1;   // the answer is in [lo, lo + n)
-  while (n > 1) {
-    const int64_t step = (n + 63) / 64;
-    const int64_t at = lo + lane * step;
-    const uint64_t m = __ballot(lane * step < n && a.cu[at < a.S ? at : a.S] <= t);
+// Piece p: sequence a - 1 and its tokens [lo, hi) of run p - a.  a is the largest with border(a) + a run < (p + 1) run: a sequence that meets
+// run p - a starts before the run's end, and the next one does not.  64 candidates a round; in the last they are
+// neighbours, which hold lo and hi.
+struct Piece {
+  int64_t a, lo, hi;
+};
+__device__ __forceinline__ Piece piece_of(const BalanceArgs& b, int64_t p, int lane) {
+  int64_t a = 0, lo, hi;
+  if (b.cu == nullptr) {
+    a = 1;
+    lo = 0;
+    hi = b.T;
+  } else {
+    const int64_t end = (p + 1) * b.run;
+    int64_t n = b.S + 2;   // a is in [a, a + n)
+    while (n > 63) {
+      const int64_t step = (n + 63) / 64, at = a + lane * step;
+      const uint64_t m = __ballot(lane * step < n && border(b, at) + at * b.run < end);
+      const int64_t k = m == 0 ? 0 : 63 - __builtin_clzll(m);
+      a += k * step;
+      n = n - k * step < step ? n - k * step : step;
+    }
+    const int64_t t = border(b, a + lane);
+    const uint64_t m = __ballot(lane < n && t + (a + lane) * b.run < end);
     const int k = m == 0 ? 0 : 63 - __builtin_clzll(m);
-    lo += k * step;
-    n = n - k * step < step ? n - k * step : step;
-    if (m == 0) return 0;
+    a += k;
+    lo = __builtin_amdgcn_readlane(int(t), k);
+    hi = __builtin_amdgcn_readlane(int(t), k + 1);
   }
-  return lo;
+  const int64_t c0 = (p - a) * b.run, c1 = c0 + b.run;
+  lo = lo > c0 ? lo : c0;
+  hi = hi < c1 ? hi : c1;
+  return Piece{a, lo, c0 < 0 ? lo : hi};
 }
 
 // A token's logits over L lanes, NV to a lane (quads: NV / 4 times four neighbours).
@@ -103,7 +127,10 @@ struct Row {
     }
   }
   // softmax in place; the log of the sum of exponentials
-  __device__ __forceinline__ float softmax() {
+  __device__ __forceinline__ float softmax(int E, int l) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (column(l, i) >= E) v[i] = -INFINITY;
     float m = v[0], s = 0.f;
 #pragma unroll
     for (int i = 1; i < NV; ++i) m = fmaxf(m, v[i]);
@@ -119,12 +146,14 @@ struct Row {
     for (int i = 0; i < NV; ++i) v[i] *= r;
     return m + logf(s);
   }
-  // sigmoids in place (0 behind the last expert); 1 / (their sum + floor)
+  // sigmoids in place (0 behind the last expert): 1 or e^-|l| over 1 + e^-|l|; 1 / (their sum + floor)
   __device__ __forceinline__ float sigmoids(int E, int l) {
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      v[i] = column(l, i) < E ? sigmoid_only(v[i]) : 0.f;
+      const float e = exp_below(-fabsf(v[i]));
+      v[i] = (v[i] < 0.f ? e : 1.f) * __builtin_amdgcn_rcpf(1.f + e);
+      if (column(l, i) >= E) v[i] = 0.f;
       s += v[i];
     }
     return 1.f / (group_sum<L>(s) + kSumFloor);
@@ -134,84 +163,147 @@ struct Row {
 // Steps whose loads are in flight at once: four, as long as they stay within the shortest run.
 template <int L>
 constexpr int ahead() {
-  return 32 * L / 64 >= 4 ? 4 : (32 * L / 64 >= 2 ? 2 : 1);
+  return 16 * L / 64 >= 4 ? 4 : (16 * L / 64 >= 2 ? 2 : 1);
 }
 
-template <int L, int NV, bool QUADS>
-__global__ __launch_bounds__(256) void balance_sums_kernel(BalanceArgs a) {
-  extern __shared__ int32_t hist_all[];
-  const int lane = threadIdx.x & 63, l = lane & (L - 1), sub = lane / L;
+// Piece p's sums and counts, by one wave (its own hist) or a workgroup of four (one hist; sums and small hold a row for each wave).
+template <int L, int NV, bool QUADS, int TEAM>
+__device__ __forceinline__ void sum_piece(const BalanceArgs& a, int64_t p, int32_t* hist, float* sums, float (*small)[2]) {
+  using R = Row<L, NV, QUADS>;
   constexpr int kSide = 64 / L, kAhead = ahead<L>();   // tokens side by side
-  int32_t* hist = hist_all + (threadIdx.x >> 6) * a.E;
-  const int64_t c = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  const int64_t t0 = c * a.run, t1 = t0 + a.run < a.T ? t0 + a.run : a.T;
-  if (t0 >= t1) return;
-  for (int64_t s = sequence_of(a, t0, lane); s < a.S; ++s) {
-    int64_t lo = border(a, s), hi = border(a, s + 1);
-    if (lo >= t1) break;
-    lo = lo > t0 ? lo : t0;
-    hi = hi < t1 ? hi : t1;
-    if (lo >= hi) continue;
-    for (int e = lane; e < a.E; e += 64) hist[e] = 0;
-    float acc[NV], z = 0.f;
-    int count = 0;
+  const int lane = threadIdx.x & 63, l = lane & (L - 1), sub = lane / L;
+  const int wave = TEAM == 1 ? 0 : threadIdx.x >> 6, me = TEAM == 1 ? lane : threadIdx.x;
+  const Piece piece = piece_of(a, p, lane);
+  const int64_t lo = piece.lo, hi = piece.hi;
+  if (piece.a < 1 || piece.a > a.S || lo >= hi) return;
+  auto team_sync = [] {
+    if constexpr (TEAM > 1) __syncthreads();
+    else __builtin_amdgcn_wave_barrier();
+  };
+  // the first indices come in beside the logits
+  const uint32_t n = uint32_t(hi - lo) * uint32_t(a.K);   // of one run: some hundred tokens of K <= 1024
+  auto slot = [&](uint32_t i) {
+    const int64_t at = lo * a.K + i;
+    const int64_t e = a.idx_i64 ? static_cast<const int64_t*>(a.idx)[at] : int64_t(static_cast<const int32_t*>(a.idx)[at]);
+    const bool counts = a.mask == nullptr || a.mask[lo + i / uint32_t(a.K)] != 0;
+    return counts && e >= 0 && e < a.E ? int(e) : -1;
+  };
+  const uint32_t i0 = me, i1 = me + 64 * TEAM;
+  const int e0 = i0 < n ? slot(i0) : -1, e1 = i1 < n ? slot(i1) : -1;
+  for (int e = me; e < a.E; e += 64 * TEAM) hist[e] = 0;
+  team_sync();
+  float acc[NV], z = 0.f;
+  int count = 0;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) acc[i] = 0.f;
-    for (int64_t t = lo; t < hi; t += kSide * kAhead) {
-      Row<L, NV, QUADS> row[kAhead];
-      bool in[kAhead];
+  for (int i = 0; i < NV; ++i) acc[i] = 0.f;
+  // the next steps' logits come in while these are summed; those that do not count are zeros
+  R next[kAhead];
+  bool use[kAhead];
+  auto fetch = [&](int64_t t) {
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const int64_t mine = t + k * kSide + sub, at = mine < hi ? mine : hi - 1;
-        in[k] = mine < hi && (a.mask == nullptr || a.mask[at] != 0);
-        row[k].load(a.logits + at * a.ld, a.E, l);
+    for (int k = 0; k < kAhead; ++k) {
+      const int64_t mine = t + k * TEAM * kSide + sub, at = mine < hi ? mine : hi - 1;
+      use[k] = mine < hi && (a.mask == nullptr || a.mask[at] != 0);
+      next[k].load(a.logits + at * a.ld, a.E, l);
+    }
+  };
+  int64_t t = lo + wave * kSide;
+  if (t < hi) fetch(t);
+  while (t < hi) {
+    R row[kAhead];
+    bool in[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      in[k] = use[k];
+#pragma unroll
+      for (int i = 0; i < NV; ++i) row[k].v[i] = in[k] ? next[k].v[i] : 0.f;
+    }
+    t += TEAM * kSide * kAhead;
+    if (t < hi) fetch(t);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const float one = in[k] ? 1.f : 0.f;
+      float lse = 0.f, r = one;
+      R p = row[k];
+      if (a.sigmoid) {
+        r = p.sigmoids(a.E, l) * one;
+        if (a.want_z) lse = row[k].softmax(a.E, l);
+      } else {
+        lse = p.softmax(a.E, l);
       }
+      count += in[k];
+      if (a.want_z) z = fmaf(lse * one, lse, z);
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        float lse = 0.f, r = 1.f;
-        Row<L, NV, QUADS> p = row[k];
-        if (a.sigmoid) {
-          r = p.sigmoids(a.E, l);
-          if (a.want_z) lse = row[k].softmax();
-        } else {
-          lse = p.softmax();
-        }
-        count += in[k];
-        if (a.want_z) z += in[k] ? lse * lse : 0.f;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) acc[i] += in[k] ? p.v[i] * r : 0.f;
-      }
+      for (int i = 0; i < NV; ++i) acc[i] = fmaf(p.v[i], r, acc[i]);
     }
-    const uint32_t n = uint32_t(hi - lo) * uint32_t(a.K);   // of one run: T / 4096 tokens of K <= 1024
-    for (uint32_t i = lane; i < n; i += 64) {
-      const int64_t at = lo * a.K + i;
-      const int64_t e = a.idx_i64 ? static_cast<const int64_t*>(a.idx)[at] : int64_t(static_cast<const int32_t*>(a.idx)[at]);
-      if (e >= 0 && e < a.E && (a.mask == nullptr || a.mask[lo + i / uint32_t(a.K)] != 0)) atomicAdd(&hist[e], 1);
-    }
-    __builtin_amdgcn_wave_barrier();
-    // the tokens side by side, in a fixed order
+  }
+  if (e0 >= 0) atomicAdd(&hist[e0], 1);
+  if (e1 >= 0) atomicAdd(&hist[e1], 1);
+  for (uint32_t i = me + 128 * TEAM; i < n; i += 64 * TEAM) {
+    const int e = slot(i);
+    if (e >= 0) atomicAdd(&hist[e], 1);
+  }
+  // the tokens side by side, in a fixed order
 #pragma unroll
-    for (int off = L; off < 64; off <<= 1) {
+  for (int off = L; off < 64; off <<= 1) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) acc[i] += __shfl_xor(acc[i], off);
-      z += __shfl_xor(z, off);
-      count += __shfl_xor(count, off);
-    }
-    const int64_t place = c + s;
+    for (int i = 0; i < NV; ++i) acc[i] += __shfl_xor(acc[i], off);
+    z += __shfl_xor(z, off);
+    count += __shfl_xor(count, off);
+  }
+  if constexpr (TEAM == 1) {
     if (sub == 0) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int e = Row<L, NV, QUADS>::column(l, i);
-        if (e < a.E) st_global(a.sums + place * a.E + e, acc[i]);
+        const int e = R::column(l, i);
+        if (e < a.E) st_global(a.sums + p * a.E + e, acc[i]);
       }
     }
     if (lane == 0) {
-      st_global(reinterpret_cast<uint32_t*>(a.tokens) + place, uint32_t(count));
-      st_global(a.z + place, z);
+      st_global(reinterpret_cast<uint32_t*>(a.tokens) + p, uint32_t(count));
+      st_global(a.z + p, z);
     }
-    for (int e = lane; e < a.E; e += 64) st_global(reinterpret_cast<uint32_t*>(a.slots) + place * a.E + e, uint32_t(hist[e]));
-    __builtin_amdgcn_wave_barrier();
+    team_sync();
+  } else {
+    if (sub == 0) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int e = R::column(l, i);
+        if (e < a.E) sums[wave * a.E + e] = acc[i];
+      }
+    }
+    if (lane == 0) {
+      small[wave][0] = float(count);
+      small[wave][1] = z;
+    }
+    team_sync();
+    for (int e = me; e < a.E; e += 64 * TEAM) {
+      float v = sums[e];
+#pragma unroll
+      for (int w = 1; w < TEAM; ++w) v += sums[w * a.E + e];
+      st_global(a.sums + p * a.E + e, v);
+    }
+    if (me == 0) {
+      float c = 0.f, v = 0.f;
+#pragma unroll
+      for (int w = 0; w < TEAM; ++w) {
+        c += small[w][0];
+        v += small[w][1];
+      }
+      st_global(reinterpret_cast<uint32_t*>(a.tokens) + p, uint32_t(c));   // whole numbers of a run
+      st_global(a.z + p, v);
+    }
   }
+  for (int e = me; e < a.E; e += 64 * TEAM) st_global(reinterpret_cast<uint32_t*>(a.slots) + p * a.E + e, uint32_t(hist[e]));
+}
+
+template <int L, int NV, bool QUADS, int TEAM>
+__global__ __launch_bounds__(256) void balance_sums_kernel(BalanceArgs a) {
+  extern __shared__ int32_t lds[];   // TEAM 1: four hists; else one, and the waves' sums
+  __shared__ float small[4][2];
+  const int64_t p = TEAM == 1 ? int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6) : int64_t(blockIdx.x);
+  if (p >= a.places) return;
+  sum_piece<L, NV, QUADS, TEAM>(a, p, TEAM == 1 ? lds + (threadIdx.x >> 6) * a.E : lds, reinterpret_cast<float*>(lds + a.E), small);
 }
 
 struct FoldArgs {
@@ -236,94 +328,9 @@ __device__ __forceinline__ float block_sum(float v, float* lds) {
 
 // A sequence's places, one after the other: first and how many (0 for an empty sequence).
 __device__ __forceinline__ void places_of(const BalanceArgs& b, int64_t s, int64_t& first, int64_t& n) {
-  const int64_t lo = border(b, s), hi = border(b, s + 1);
-  first = lo / b.run + s;
+  const int64_t lo = border(b, s + 1), hi = border(b, s + 2);
+  first = lo / b.run + s + 1;
   n = hi > lo ? (hi - 1) / b.run - lo / b.run + 1 : 0;
-}
-
-// Workgroup (column group, sequence): 16 columns, blockDim / 16 rows of threads that each add every so many places, then each other.
-__global__ __launch_bounds__(1024) void balance_fold_kernel(FoldArgs a) {
-  __shared__ float sum[64][16];
-  __shared__ int32_t cnt[64][16];
-  __shared__ int32_t tok[64];
-  __shared__ float lds[16];
-  const int64_t s = blockIdx.y;
-  const int q = threadIdx.x & 15, g = threadIdx.x >> 4, groups = int(blockDim.x >> 4);
-  const int e = int(blockIdx.x) * 16 + q;
-  int64_t first, n;
-  places_of(a.b, s, first, n);
-  float p = 0.f;
-  int32_t m = 0, t = 0;
-  float z = 0.f;
-  for (int64_t i = g; i < n; i += groups) {
-    const int64_t at = first + i;
-    if (e < a.b.E) {
-      p += a.b.sums[at * a.b.E + e];
-      m += a.b.slots[at * a.b.E + e];
-    }
-    if (q == 0) {
-      t += a.b.tokens[at];
-      z += a.b.z[at];
-    }
-  }
-  sum[g][q] = p;
-  cnt[g][q] = m;
-  if (q == 0) tok[g] = t;
-  const float zsum = block_sum(z, lds);   // (a barrier for the others too)
-  float part = 0.f;
-  if (threadIdx.x < 16) {
-    p = 0.f;
-    m = t = 0;
-    for (int i = 0; i < groups; ++i) {
-      p += sum[i][q];
-      m += cnt[i][q];
-      t += tok[i];
-    }
-    if (e < a.b.E) {
-      const float inv = t > 0 ? 1.f / float(t) : 0.f;
-      const float f = float(a.b.E) * float(m) * inv;
-      st_global(a.f + s * a.b.E + e, f * inv);
-      st_global(reinterpret_cast<uint32_t*>(a.counts) + s * a.b.E + e, uint32_t(m));
-      part = f * (p * inv);
-    }
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-      st_global(reinterpret_cast<uint32_t*>(a.seq_tokens) + s, uint32_t(t));
-      st_global(a.seq_z + s, zsum);
-    }
-  }
-  const float total = block_sum(part, lds);
-  if (threadIdx.x == 0) st_global(a.loss_part + s * gridDim.x + blockIdx.x, total);
-}
-
-// Sequences of a few places: one thread to a sequence's column.
-__global__ __launch_bounds__(256) void balance_fold_short_kernel(FoldArgs a) {
-  __shared__ float lds[4];
-  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  float part = 0.f;
-  if (i < a.b.S * a.b.E) {
-    const int64_t s = i / a.b.E, e = i - s * a.b.E;
-    int64_t first, n;
-    places_of(a.b, s, first, n);
-    float p = 0.f, z = 0.f;
-    int32_t m = 0, t = 0;
-    for (int64_t k = first; k < first + n; ++k) {
-      p += a.b.sums[k * a.b.E + e];
-      m += a.b.slots[k * a.b.E + e];
-      t += a.b.tokens[k];
-      if (e == 0) z += a.b.z[k];
-    }
-    const float inv = t > 0 ? 1.f / float(t) : 0.f;
-    const float f = float(a.b.E) * float(m) * inv;
-    st_global(a.f + i, f * inv);
-    st_global(reinterpret_cast<uint32_t*>(a.counts) + i, uint32_t(m));
-    part = f * (p * inv);
-    if (e == 0) {
-      st_global(reinterpret_cast<uint32_t*>(a.seq_tokens) + s, uint32_t(t));
-      st_global(a.seq_z + s, z);
-    }
-  }
-  const float total = block_sum(part, lds);
-  if (threadIdx.x == 0) st_global(a.loss_part + blockIdx.x, total);
 }
 
 // loss, and {1 / S', 1 / N} for the backward; the running totals of a load tracker.
@@ -338,13 +345,14 @@ struct FinishArgs {
   int64_t* acc_total;    // [1] or null
 };
 
-__global__ __launch_bounds__(1024) void balance_finish_kernel(FinishArgs a) {
+// By one workgroup; loss: each thread's share of the sequences' sum.
+__device__ __forceinline__ void finish(const FinishArgs& a, float loss) {
   __shared__ float lds[16];
   __shared__ int64_t ilds[16];
-  float loss = 0.f, z = 0.f, filled = 0.f;
+  float z = 0.f, filled = 0.f;
   int64_t n = 0;
-  for (int64_t i = threadIdx.x; i < a.parts; i += 1024) loss += a.loss_part[i];
-  for (int64_t i = threadIdx.x; i < a.S; i += 1024) {
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < a.S; i += blockDim.x) {
     const int32_t t = a.seq_tokens[i];
     n += t;
     filled += t > 0 ? 1.f : 0.f;
@@ -358,12 +366,144 @@ __global__ __launch_bounds__(1024) void balance_finish_kernel(FinishArgs a) {
   __syncthreads();
   if (threadIdx.x != 0) return;
   n = 0;
-  for (int i = 0; i < 16; ++i) n += ilds[i];
+  for (int i = 0; i < int(blockDim.x >> 6); ++i) n += ilds[i];
   const float inv_s = filled > 0.f ? 1.f / filled : 0.f, inv_n = n > 0 ? 1.f / float(n) : 0.f;
   st_global(a.loss, loss * inv_s + a.z_mult * (z * inv_n));
   st_global(a.inverse, inv_s);
   st_global(a.inverse + 1, inv_n);
   if (a.acc_total) *FM_GLOBAL(int64_t, a.acc_total) = a.acc_total[0] + n;
+}
+
+// Workgroup: COLS columns of a sequence, blockDim / COLS rows of threads that each add every so many places (four places' loads at
+// once), then each other's sums in order.  The only workgroup finishes the loss too.
+template <int COLS>
+__global__ __launch_bounds__(1024) void balance_fold_kernel(FoldArgs a, int column_groups, FinishArgs fin) {
+  __shared__ float sum[1024 / COLS][COLS];
+  __shared__ int32_t cnt[1024 / COLS][COLS];
+  __shared__ int32_t tok[1024 / COLS];
+  __shared__ float lds[16];
+  const int64_t s = blockIdx.x / unsigned(column_groups);
+  const int part = int(blockIdx.x % unsigned(column_groups));
+  const int q = threadIdx.x % COLS, g = threadIdx.x / COLS, groups = int(blockDim.x) / COLS;
+  const int e = part * COLS + q, col = e < a.b.E ? e : a.b.E - 1;
+  int64_t first, n;
+  places_of(a.b, s, first, n);
+  float p = 0.f;
+  int32_t m = 0, t = 0;
+  float z = 0.f;
+  for (int64_t k = g; k < n; k += 4 * groups) {
+    float pk[4], zk[4];
+    int32_t mk[4], tk[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t at = first + (k + i * groups < n ? k + i * groups : k);
+      pk[i] = a.b.sums[at * a.b.E + col];
+      mk[i] = a.b.slots[at * a.b.E + col];
+      tk[i] = a.b.tokens[at];
+      zk[i] = a.b.z[at];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (k + i * groups >= n) break;
+      p += pk[i];
+      m += mk[i];
+      t += tk[i];
+      z += zk[i];
+    }
+  }
+  sum[g][q] = p;
+  cnt[g][q] = m;
+  if (q == 0) tok[g] = t;
+  const float zsum = block_sum(q == 0 ? z : 0.f, lds);   // (a barrier for the others too)
+  float share = 0.f;
+  if (threadIdx.x < COLS) {
+    p = 0.f;
+    m = t = 0;
+    for (int i = 0; i < groups; ++i) {
+      p += sum[i][q];
+      m += cnt[i][q];
+      t += tok[i];
+    }
+    if (e < a.b.E) {
+      const float inv = t > 0 ? 1.f / float(t) : 0.f;
+      const float f = float(a.b.E) * float(m) * inv;
+      st_global(a.f + s * a.b.E + e, f * inv);
+      st_global(reinterpret_cast<uint32_t*>(a.counts) + s * a.b.E + e, uint32_t(m));
+      share = f * (p * inv);
+    }
+    if (part == 0 && threadIdx.x == 0) {
+      st_global(reinterpret_cast<uint32_t*>(a.seq_tokens) + s, uint32_t(t));
+      st_global(a.seq_z + s, zsum);
+    }
+  }
+  if (gridDim.x == 1) {
+    __syncthreads();
+    finish(fin, share);
+    return;
+  }
+  const float total = block_sum(share, lds);
+  if (threadIdx.x == 0) st_global(a.loss_part + blockIdx.x, total);
+}
+
+// Column e of sequence s, from its places in order: its share of the loss.  Four places' loads at once.
+__device__ __forceinline__ float fold_column(const FoldArgs& a, int64_t s, int e) {
+  int64_t first, n;
+  places_of(a.b, s, first, n);
+  float p = 0.f, z = 0.f;
+  int32_t m = 0, t = 0;
+  for (int64_t k = 0; k < n; k += 4) {
+    float pk[4], zk[4];
+    int32_t mk[4], tk[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t at = first + (k + i < n ? k + i : k);
+      pk[i] = a.b.sums[at * a.b.E + e];
+      mk[i] = a.b.slots[at * a.b.E + e];
+      tk[i] = a.b.tokens[at];
+      zk[i] = a.b.z[at];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (k + i >= n) break;
+      p += pk[i];
+      m += mk[i];
+      t += tk[i];
+      z += zk[i];
+    }
+  }
+  const float inv = t > 0 ? 1.f / float(t) : 0.f;
+  const float f = float(a.b.E) * float(m) * inv;
+  st_global(a.f + s * a.b.E + e, f * inv);
+  st_global(reinterpret_cast<uint32_t*>(a.counts) + s * a.b.E + e, uint32_t(m));
+  if (e == 0) {
+    st_global(reinterpret_cast<uint32_t*>(a.seq_tokens) + s, uint32_t(t));
+    st_global(a.seq_z + s, z);
+  }
+  return f * (p * inv);
+}
+
+__global__ __launch_bounds__(1024) void balance_finish_kernel(FinishArgs a) {
+  float loss = 0.f;
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < a.parts; i += 1024) loss += a.loss_part[i];
+  finish(a, loss);
+}
+
+// Few logits in few pieces: all of the forward in one workgroup, its waves taking the pieces in turn.
+constexpr int64_t kOnePieces = 32, kOneLogits = 16384, kOneColumns = 4096;
+template <int L, int NV, bool QUADS>
+__global__ __launch_bounds__(1024) void balance_one_kernel(FoldArgs a, FinishArgs fin) {
+  extern __shared__ int32_t lds[];   // a hist for each wave
+  for (int64_t p = threadIdx.x >> 6; p < a.b.places; p += blockDim.x >> 6)
+    sum_piece<L, NV, QUADS, 1>(a.b, p, lds + (threadIdx.x >> 6) * a.b.E, nullptr, nullptr);
+  __syncthreads();
+  float loss = 0.f;
+  for (int i = threadIdx.x; i < int(a.b.S) * a.b.E; i += blockDim.x) {
+    const int s = i / a.b.E;
+    loss += fold_column(a, s, i - s * a.b.E);
+  }
+  __syncthreads();
+  finish(fin, loss);
 }
 
 // acc[e] += sum of the sequences' counts: one workgroup to an expert
@@ -412,76 +552,80 @@ __device__ __forceinline__ void put(const BalanceBwdArgs& a, int64_t t, int l, f
 
 template <int L, int NV, bool QUADS>
 __global__ __launch_bounds__(256) void balance_backward_kernel(BalanceBwdArgs a) {
+  using R = Row<L, NV, QUADS>;
   const BalanceArgs& b = a.b;
   const int lane = threadIdx.x & 63, l = lane & (L - 1), sub = lane / L;
   constexpr int kSide = 64 / L, kAhead = ahead<L>();
-  const int64_t c = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  const int64_t t0 = c * b.run, t1 = t0 + b.run < b.T ? t0 + b.run : b.T;
-  if (t0 >= t1) return;
-  const float g = a.dloss[0] * a.inverse[0];
-  const float gz = 2.f * a.z_mult * (a.dloss[0] * a.inverse[1]);
+  const int64_t p = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (p >= b.places) return;
+  const Piece piece = piece_of(b, p, lane);
+  const int64_t lo = piece.lo, hi = piece.hi;
+  if (lo >= hi) return;
   float zero[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) zero[i] = 0.f;
-  int64_t done = t0;   // tokens before it are written
-  auto skip_to = [&](int64_t end) {   // tokens of no sequence
+  if (piece.a < 1 || piece.a > b.S) {   // tokens of no sequence
     if (!a.add)
-      for (int64_t t = done + sub; t < end; t += kSide) put<L, NV, QUADS>(a, t, l, zero);
-    done = end;
-  };
-  for (int64_t s = sequence_of(b, t0, lane); s < b.S; ++s) {
-    int64_t lo = border(b, s), hi = border(b, s + 1);
-    if (lo >= t1) break;
-    lo = lo > done ? lo : done;
-    hi = hi < t1 ? hi : t1;
-    if (lo >= hi) continue;
-    skip_to(lo);
-    float f[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int e = Row<L, NV, QUADS>::column(l, i);
-      f[i] = e < b.E ? g * a.f[s * b.E + e] : 0.f;
-    }
-    for (int64_t t = lo; t < hi; t += kSide * kAhead) {
-      Row<L, NV, QUADS> row[kAhead];
-      bool in[kAhead];
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const int64_t mine = t + k * kSide + sub, at = mine < hi ? mine : hi - 1;
-        in[k] = b.mask == nullptr || b.mask[at] != 0;
-        row[k].load(b.logits + at * b.ld, b.E, l);
-      }
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const int64_t mine = t + k * kSide + sub;
-        Row<L, NV, QUADS> p = row[k];
-        float out[NV], inner = 0.f;
-        if (b.sigmoid) {
-          const float r = p.sigmoids(b.E, l);
-#pragma unroll
-          for (int i = 0; i < NV; ++i) inner = fmaf(f[i], p.v[i], inner);
-          inner = group_sum<L>(inner) * r;
-#pragma unroll
-          for (int i = 0; i < NV; ++i) out[i] = (f[i] - inner) * r * (p.v[i] * (1.f - p.v[i]));
-          if (gz != 0.f) {
-            const float lse = row[k].softmax();
-#pragma unroll
-            for (int i = 0; i < NV; ++i) out[i] = fmaf(gz * lse, row[k].v[i], out[i]);
-          }
-        } else {
-          const float lse = p.softmax();
-#pragma unroll
-          for (int i = 0; i < NV; ++i) inner = fmaf(f[i], p.v[i], inner);
-          inner = group_sum<L>(inner) - gz * lse;
-#pragma unroll
-          for (int i = 0; i < NV; ++i) out[i] = p.v[i] * (f[i] - inner);
-        }
-        if (mine < hi) put<L, NV, QUADS>(a, mine, l, in[k] ? out : zero);
-      }
-    }
-    done = hi;
+      for (int64_t t = lo + sub; t < hi; t += kSide) put<L, NV, QUADS>(a, t, l, zero);
+    return;
   }
-  skip_to(t1);
+  const float g = a.dloss[0] * a.inverse[0];
+  const float gz = 2.f * a.z_mult * (a.dloss[0] * a.inverse[1]);
+  R f;
+  f.load(a.f + (piece.a - 1) * b.E, b.E, l);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) f.v[i] = R::column(l, i) < b.E ? g * f.v[i] : 0.f;
+  R next[kAhead];
+  bool use[kAhead];
+  auto fetch = [&](int64_t t) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int64_t mine = t + k * kSide + sub, at = mine < hi ? mine : hi - 1;
+      use[k] = b.mask == nullptr || b.mask[at] != 0;
+      next[k].load(b.logits + at * b.ld, b.E, l);
+    }
+  };
+  fetch(lo);
+  for (int64_t t = lo; t < hi; t += kSide * kAhead) {
+    R row[kAhead];
+    bool in[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      row[k] = next[k];
+      in[k] = use[k];
+    }
+    if (t + kSide * kAhead < hi) fetch(t + kSide * kAhead);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int64_t mine = t + k * kSide + sub;
+      R q = row[k];
+      float out[NV], inner = 0.f;
+      if (b.sigmoid) {
+        const float r = q.sigmoids(b.E, l);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) inner = fmaf(f.v[i], q.v[i], inner);
+        inner = group_sum<L>(inner) * r;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) out[i] = (f.v[i] - inner) * r * (q.v[i] * (1.f - q.v[i]));
+        if (a.z_mult != 0.f) {
+          const float lse = row[k].softmax(b.E, l);
+#pragma unroll
+          for (int i = 0; i < NV; ++i) out[i] = fmaf(gz * lse, row[k].v[i], out[i]);
+        }
+      } else {
+        const float lse = q.softmax(b.E, l);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) inner = fmaf(f.v[i], q.v[i], inner);
+        inner = group_sum<L>(inner);
+        if (a.z_mult != 0.f) inner -= gz * lse;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) out[i] = q.v[i] * (f.v[i] - inner);
+      }
+#pragma unroll
+      for (int i = 0; i < NV; ++i) out[i] = in[k] ? out[i] : 0.f;
+      if (mine < hi) put<L, NV, QUADS>(a, mine, l, out);
+    }
+  }
 }
 
 // -------------------------------------------------------------------- launches ----
@@ -509,20 +653,33 @@ void for_experts(int E, F go) {
 #undef FM_ROW
 }
 
-// Tokens of a wave: 32 at least (a place of the workspace is 8 E bytes beside the 4 E of a token's logits), and no more waves than
-// sixteen to a CU of 256.
-int run_of(int64_t T) {
-  const int64_t r = (T + 4095) / 4096;
-  return int(r < 32 ? 32 : r);
+// Tokens side by side in a wave, as for_experts takes them.
+int side_of(int E) {
+  int side = 1;
+  for_experts(E, [&](auto l, auto, auto) { side = 64 / decltype(l)::value; });
+  return side;
 }
 
+// Tokens of a wave: 16 at least (or one step of what lies side by side), the more the longer the batch: no more than 16384 waves.
+int run_of(int64_t T, int E) {
+  const int side = side_of(E), least = side < 16 ? 16 : side;
+  const int64_t r = (T + 16383) / 16384;
+  return int(r <= least ? least : (r + least - 1) / least * least);
+}
+// Four waves to a piece where a sequence has 64 waves' tokens on average: a quarter of the places to write and add.
+int team_of(int64_t T, int E, int64_t S) { return T >= 64 * S && T > 16 * run_of(T, E) ? 4 : 1; }
+
 struct Space {
-  int64_t places, sums, slots, tokens, z, seq_tokens, seq_z, loss_part, bytes;   // offsets in bytes
+  int64_t runs, places, sums, slots, tokens, z, seq_tokens, seq_z, loss_part, bytes;   // offsets in bytes
+  int team, run;
 };
 Space space_of(int64_t T, int E, int64_t S) {
   Space w{};
   w.bytes = 256;   // never none: no tokens and no sequences are a call too
-  w.places = (T + run_of(T) - 1) / run_of(T) + S;
+  w.team = team_of(T, E, S);
+  w.run = w.team * run_of(T, E);
+  w.runs = (T + w.run - 1) / w.run;
+  w.places = w.runs + S + 2;
   auto take = [&](int64_t n) {
     const int64_t at = w.bytes;
     w.bytes += (n * 4 + 255) / 256 * 256;
@@ -534,7 +691,7 @@ Space space_of(int64_t T, int E, int64_t S) {
   w.z = take(w.places);
   w.seq_tokens = take(S);
   w.seq_z = take(S);
-  w.loss_part = take((S * E + 255) / 256 + S * ((E + 15) / 16));
+  w.loss_part = take(S * ((E + 15) / 16));
   return w;
 }
 
@@ -562,40 +719,50 @@ int fm_balance_forward(const float* logits, int64_t ld, int64_t T, int E, const 
                        int64_t S, const uint8_t* mask, int sigmoid, float z_mult, float* f, int32_t* counts, float* inverse, float* loss,
                        int64_t* acc, int64_t* acc_total, void* workspace, int64_t workspace_bytes, void* stream) {
   char* ws = static_cast<char*>(workspace);
-  BalanceArgs b{logits, ld, T, E, K, indices, indices_i64, cu, S, mask, sigmoid, z_mult != 0.f, run_of(T), nullptr, nullptr, nullptr, nullptr};
+  BalanceArgs b{logits, ld, T, E, K, indices, indices_i64, cu, S, mask, sigmoid, z_mult != 0.f, 0, 0, nullptr, nullptr, nullptr, nullptr};
   if (int rc = check_balance(b, "fm_balance_forward")) return rc;
   FM_REQUIRE(K >= 1 && K <= 1024 && (T == 0 || indices), "fm_balance_forward: null indices or bad K");
   FM_REQUIRE(inverse && loss && (S == 0 || (f && counts)), "fm_balance_forward: null output");
   const Space w = space_of(T, E, S);
   FM_REQUIRE(ws && aligned16(ws) && workspace_bytes >= w.bytes, "fm_balance_forward: the workspace must hold fm_balance_workspace_bytes(T, E, S) "
              "bytes on 16");
+  b.run = w.run;
+  b.places = w.places;
   b.sums = reinterpret_cast<float*>(ws + w.sums);
   b.slots = reinterpret_cast<int32_t*>(ws + w.slots);
   b.tokens = reinterpret_cast<int32_t*>(ws + w.tokens);
   b.z = reinterpret_cast<float*>(ws + w.z);
   const FoldArgs fold{b, f, counts, reinterpret_cast<int32_t*>(ws + w.seq_tokens), reinterpret_cast<float*>(ws + w.seq_z),
                       reinterpret_cast<float*>(ws + w.loss_part)};
+  FinishArgs fin{fold.loss_part, 0, S, fold.seq_tokens, fold.seq_z, z_mult, loss, inverse, acc_total};
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const int64_t runs = (T + b.run - 1) / b.run;
-  if (runs > 0 && S > 0)
+  // a few pieces in one workgroup: 512 tokens of 8 experts 9.0 us (three launches) -> 5.3
+  if (w.places <= kOnePieces && T * E <= kOneLogits && E <= 256 && S * E <= kOneColumns) {
+    const int64_t waves = w.places < 16 ? w.places : 16;
     for_experts(E, [&](auto l, auto n, auto q) {
-      hipLaunchKernelGGL((balance_sums_kernel<decltype(l)::value, decltype(n)::value, decltype(q)::value>), dim3(unsigned((runs + 3) / 4)),
-                         dim3(256), unsigned(4 * E * sizeof(int32_t)), s, b);
+      if constexpr (decltype(n)::value <= 4)
+        hipLaunchKernelGGL((balance_one_kernel<decltype(l)::value, decltype(n)::value, decltype(q)::value>), dim3(1), dim3(unsigned(64 * waves)),
+                           unsigned(waves * E * sizeof(int32_t)), s, fold, fin);
     });
-  int64_t parts = 0;
-  if (S > 0) {
-    // sequences of eight places or fewer on average: a thread to a column; of many, a workgroup of 1024
-    if (w.places <= 8 * S || S > 65535) {
-      parts = (S * E + 255) / 256;
-      hipLaunchKernelGGL(balance_fold_short_kernel, dim3(unsigned(parts)), dim3(256), 0, s, fold);
-    } else {
-      const unsigned groups = unsigned((E + 15) / 16);
-      parts = S * groups;
-      hipLaunchKernelGGL(balance_fold_kernel, dim3(groups, unsigned(S)), dim3(w.places > 64 * S ? 1024 : 256), 0, s, fold);
-    }
+  } else {
+    if (w.runs > 0 && S > 0)
+      for_experts(E, [&](auto l, auto n, auto q) {
+        constexpr int L = decltype(l)::value, N = decltype(n)::value;
+        constexpr bool Q = decltype(q)::value;
+        if (w.team == 4) hipLaunchKernelGGL((balance_sums_kernel<L, N, Q, 4>), dim3(unsigned(w.places)), dim3(256), unsigned(5 * E * 4), s, b);
+        else hipLaunchKernelGGL((balance_sums_kernel<L, N, Q, 1>), dim3(unsigned((w.places + 3) / 4)), dim3(256), unsigned(4 * E * 4), s, b);
+      });
+    // a sequence's 16 columns to a workgroup, of four rows of threads for a few places, more for longer sequences; one sequence of up to 64
+    // experts is one workgroup's work, the loss with it
+    const bool one = S == 1 && E <= 64;
+    const int groups = one ? 1 : (E + 15) / 16;
+    fin.parts = S * groups;
+    if (one) hipLaunchKernelGGL(balance_fold_kernel<64>, dim3(1), dim3(1024), 0, s, fold, 1, fin);
+    else if (S > 0)
+      hipLaunchKernelGGL(balance_fold_kernel<16>, dim3(unsigned(fin.parts)), dim3(w.runs <= 8 * S ? 64 : w.runs <= 64 * S ? 256 : 1024), 0, s,
+                         fold, groups, fin);
+    if (fin.parts != 1) hipLaunchKernelGGL(balance_finish_kernel, dim3(1), dim3(1024), 0, s, fin);
   }
-  const FinishArgs fin{fold.loss_part, parts, S, fold.seq_tokens, fold.seq_z, z_mult, loss, inverse, acc_total};
-  hipLaunchKernelGGL(balance_finish_kernel, dim3(1), dim3(1024), 0, s, fin);
   if (acc && S > 0) hipLaunchKernelGGL(balance_track_kernel, dim3(unsigned(E)), dim3(256), 0, s, counts, S, E, acc);
   return check_launch("fm_balance_forward");
 }
@@ -603,14 +770,15 @@ int fm_balance_forward(const float* logits, int64_t ld, int64_t T, int E, const 
 int fm_balance_backward(const float* logits, int64_t ld, int64_t T, int E, const int32_t* cu, int64_t S, const uint8_t* mask, int sigmoid,
                         float z_mult, const float* f, const float* inverse, const float* dloss, float* dlogits, int64_t ld_d, int add,
                         void* stream) {
-  const BalanceArgs b{logits, ld, T, E, 1, nullptr, 0, cu, S, mask, sigmoid, z_mult != 0.f, run_of(T), nullptr, nullptr, nullptr, nullptr};
+  BalanceArgs b{logits, ld, T, E, 1, nullptr, 0, cu, S, mask, sigmoid, z_mult != 0.f, 0, 0, nullptr, nullptr, nullptr, nullptr};
   if (int rc = check_balance(b, "fm_balance_backward")) return rc;
   if (T == 0) return 0;
   FM_REQUIRE(inverse && dloss && dlogits && ld_d >= E && (S == 0 || f), "fm_balance_backward: null pointer or a pitch below E");
+  b.run = run_of(T, E);
+  b.places = (T + b.run - 1) / b.run + S + 2;
   const BalanceBwdArgs a{b, f, inverse, dloss, z_mult, dlogits, ld_d, add};
-  const int64_t runs = (T + b.run - 1) / b.run;
   for_experts(E, [&](auto l, auto n, auto q) {
-    hipLaunchKernelGGL((balance_backward_kernel<decltype(l)::value, decltype(n)::value, decltype(q)::value>), dim3(unsigned((runs + 3) / 4)),
+    hipLaunchKernelGGL((balance_backward_kernel<decltype(l)::value, decltype(n)::value, decltype(q)::value>), dim3(unsigned((b.places + 3) / 4)),
                        dim3(256), 0, static_cast<hipStream_t>(stream), a);
   });
   return check_launch("fm_balance_backward");

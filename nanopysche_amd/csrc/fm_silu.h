@@ -38,15 +38,6 @@ __device__ __forceinline__ float silu_only(float g) {
   return d <= 3.40282347e38f ? q : g * 0.f;
 }
 
-// 1 / (1 + e^-g), as sig_silu's.
-__device__ __forceinline__ float sigmoid_only(float g) {
-#pragma clang fp contract(off)
-  const float d = 1.f + exp_neg(g);
-  const float r = __builtin_amdgcn_rcpf(d);
-  const float s = d <= 3.40282347e38f ? fmaf(fmaf(-d, r, 1.f), r, r) : 0.f;
-  return g == g ? s : g;
-}
-
 struct SigSilu {
   float s, silu;
 };

@@ -162,7 +162,7 @@ def test_balance_refuses(launched, error, match, change):  # noqa: F811
 
 def test_balance_backward_refuses(launched):  # noqa: F811
     l, _ = logits()
-    state = fm.BalanceState(l, None, None, torch.zeros(6), torch.zeros(2), False, 0.0, l.shape)
+    state = fm.BalanceState(l, None, None, torch.zeros(6), False, 0.0, l.shape)
     for bad in (torch.zeros(2), torch.zeros((), dtype=BF)):
         with pytest.raises(TypeError, match="dloss"):
             fm.balance_backward(state, bad)
