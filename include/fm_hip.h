@@ -725,6 +725,22 @@ int fm_act8_rmsnorm_backward(const void* dy, int64_t ld_dy, int dtype, int64_t T
                              const void* codes, int64_t ld_c, const void* w, int w_dtype, const float* rstd, void* dx,
                              int64_t ld_dx, void* dw, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* The expert block's operands from 8 bits, in the layouts and kinds of fm_permute, fm_swiglu_quantize and fm_swiglu_backward (either output
+ * may be NULL): the rows of the tokens [T, D], h of the kept gate|up [rows, 2H], [dg | du] of it and dh [rows, H] (bf16); and
+ * fm_router_weight_grad of kept expert outputs [rows, D]. */
+int fm_act8_permute(const void* xq, int64_t ld_xq, const void* codes, int64_t ld_c, int64_t T, int64_t D,
+                    const int32_t* assign_of_row, int64_t rows, int K, int kind, void* q, int64_t ld_q, void* s, int64_t ld_s,
+                    void* qt, int64_t ld_qt, void* st, int64_t ld_st, const int32_t* tile_valid, void* stream);
+int fm_act8_swiglu_quantize(const void* gu, int64_t ld_gu, const void* codes, int64_t ld_c, int64_t rows, int64_t H, int kind,
+                            void* q, int64_t ld_q, void* s, int64_t ld_s, void* qt, int64_t ld_qt, void* st, int64_t ld_st,
+                            const int32_t* tile_valid, void* stream);
+int fm_act8_swiglu_backward_quantize(const void* gu, int64_t ld_gu, const void* codes, int64_t ld_c, const void* dh,
+                                     int64_t ld_dh, int64_t rows, int64_t H, int kind, void* q, int64_t ld_q, void* s,
+                                     int64_t ld_s, void* qt, int64_t ld_qt, void* st, int64_t ld_st, const int32_t* tile_valid,
+                                     void* stream);
+int fm_act8_router_weight_grad(const void* dout, int64_t ld_do, const void* y, int64_t ld_y, const void* codes, int64_t ld_c,
+                               const int32_t* row_of, int64_t T, int K, int64_t D, float* dw, void* stream);
+
 /* ------------------------------- balance loss of packed and padded sequences ----
  * The load-balancing loss (reference model/moe.py:267-281) of each sequence, averaged, over the tokens that count:
  *   f_se = slots of sequence s at expert e / n_s, P_se = mean of its p_te, loss = (E / S') sum_s sum_e f_se P_se

@@ -189,6 +189,13 @@ SIGNATURES = {
     "fm_act8_rmsnorm_backward_workspace_bytes": (_i64, [_i64, _i64]),
     "fm_act8_rmsnorm_backward": (_i32, [_vp, _i64, _i32, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _vp, _vp, _i64, _vp, _vp,
                                         _i64, _vp]),
+    "fm_act8_permute": (_i32, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i32, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp,
+                               _i64, _vp, _vp]),
+    "fm_act8_swiglu_quantize": (_i32, [_vp, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp,
+                                       _vp]),
+    "fm_act8_swiglu_backward_quantize": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _i64, _vp,
+                                                _i64, _vp, _i64, _vp, _vp]),
+    "fm_act8_router_weight_grad": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i32, _i64, _vp, _vp]),
     "fm_balance_workspace_bytes": (_i64, [_i64, _i32, _i64]),
     "fm_balance_forward": (_i32, [_vp, _i64, _i64, _i32, _vp, _i32, _i32, _vp, _i64, _vp, _i32, C.c_float, _vp, _vp, _vp, _vp,
                                   _vp, _vp, _vp, _i64, _vp]),

@@ -20,7 +20,6 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .decode import _same_device
 
 MAX_BALANCE_EXPERTS = 1024
 MAX_BALANCE_TOP_K = 1024
@@ -96,7 +95,8 @@ def _check(logits, indices, cu_seqlens, token_mask, load_tracker):
     if load_tracker is not None:
         if load_tracker.num_experts != E:
             raise ValueError(f"load_tracker is for {load_tracker.num_experts} experts, the logits for {E}")
-        _same_device(l2, load_tracker=load_tracker.tokens_per_expert)
+        if load_tracker.tokens_per_expert.get_device() != index:
+            raise ValueError(f"load_tracker is on {load_tracker.tokens_per_expert.device}, the logits on {l2.device}")
     return l2, idx, cu, mask
 
 

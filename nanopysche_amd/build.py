@@ -20,7 +20,8 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libfm_hip.so"
 SOURCES = ["fm_api.cpp", "fm_quant.hip", "fm_route.hip", "fm_swiglu.hip", "fm_gemm.hip", "fm_router.hip",
-           "fm_norm.hip", "fm_few.hip", "fm_decode.hip", "fm_int8.hip", "fm_act8.hip", "fm_balance.hip"]
+           "fm_norm.hip", "fm_few.hip", "fm_decode.hip", "fm_int8.hip", "fm_act8.hip",
+           "fm_act8_block.hip", "fm_balance.hip"]
 ARCH = "gfx950"
 
 

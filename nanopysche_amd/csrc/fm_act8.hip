@@ -205,8 +205,7 @@ __global__ __launch_bounds__(256) void swiglu_kernel(Items t, SwigluArgs a) {
     float gv[8], uv[8], h[8];
     g[u].widen(gv);
     up[u].widen(uv);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] = silu_only(gv[i]) * uv[i];
+    swiglu8(gv, uv, h);
     uint32_t gc, uc;
     const uint2 gb = act_encode8(gv, gc), ub = act_encode8(uv, uc);
     if (!it[u].in) continue;
@@ -241,19 +240,14 @@ __global__ __launch_bounds__(256) void swiglu_backward_kernel(Items t, SwigluBwd
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    float gv[8], uv[8], dv[8];
+    float gv[8], uv[8], dv[8], dg[8], du[8];
     act_decode8(g[u], act_scale(gc[u]), gv);
     act_decode8(up[u], act_scale(uc[u]), uv);
     dh[u].widen(dv);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const SigSilu s = sig_silu(gv[i]);
-      gv[i] = ((dv[i] * uv[i]) * s.s) * (1.f + gv[i] * (1.f - s.s));
-      uv[i] = dv[i] * s.silu;
-    }
+    swiglu8_backward(gv, uv, dv, dg, du);
     if (!it[u].in) continue;
-    store8(static_cast<T*>(a.dg) + it[u].row * a.ld_dg + it[u].col, gv, it[u].n);
-    store8(static_cast<T*>(a.du) + it[u].row * a.ld_du + it[u].col, uv, it[u].n);
+    store8(static_cast<T*>(a.dg) + it[u].row * a.ld_dg + it[u].col, dg, it[u].n);
+    store8(static_cast<T*>(a.du) + it[u].row * a.ld_du + it[u].col, du, it[u].n);
   }
 }
 

@@ -52,4 +52,22 @@ __device__ __forceinline__ SigSilu sig_silu(float g) {
   return SigSilu{fin ? r : 0.f, fin ? q : g * 0.f};
 }
 
+// SwiGLU of eight values and its backward, every product and sum rounded (the same values in every kernel that inlines them):
+// h = silu(g) u; torch autograd of it: dg = (dh u) s (1 + g (1 - s)), du = dh silu(g), each operation rounded in this order.
+__device__ __forceinline__ void swiglu8(const float (&g)[8], const float (&u)[8], float (&h)[8]) {
+#pragma clang fp contract(off)
+#pragma unroll
+  for (int i = 0; i < 8; ++i) h[i] = silu_only(g[i]) * u[i];
+}
+__device__ __forceinline__ void swiglu8_backward(const float (&g)[8], const float (&u)[8], const float (&dh)[8], float (&dg)[8],
+                                                 float (&du)[8]) {
+#pragma clang fp contract(off)
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const SigSilu s = sig_silu(g[i]);
+    dg[i] = ((dh[i] * u[i]) * s.s) * (1.f + g[i] * (1.f - s.s));
+    du[i] = dh[i] * s.silu;
+  }
+}
+
 }  // namespace fm

@@ -27,12 +27,10 @@ struct SwigluSrc {
                *reinterpret_cast<const uint4*>(u + row * ld_u + col)};
   }
   __device__ __forceinline__ void compute(const Raw& r, float v[][8]) const {
-#pragma clang fp contract(off)   // every product rounded: the same values in every kernel that inlines this
     float gv[8], uv[8];
     unpack8_bf16(r.g, gv);
     unpack8_bf16(r.u, uv);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[0][i] = silu_only(gv[i]) * uv[i];
+    swiglu8(gv, uv, v[0]);
   }
 };
 
@@ -53,19 +51,11 @@ struct SwigluBwdSrc {
                *reinterpret_cast<const uint4*>(dh + row * ld_dh + col)};
   }
   __device__ __forceinline__ void compute(const Raw& r, float v[][8]) const {
-#pragma clang fp contract(off)   // every product and sum rounded, as in the other kernels inlining this
     float gv[8], uv[8], dv[8];
     unpack8_bf16(r.g, gv);
     unpack8_bf16(r.u, uv);
     unpack8_bf16(r.dh, dv);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      // torch autograd of silu(g) * u: dy = dh * u, dg = dy * s * (1 + g (1 - s)),
-      // du = dh * silu(g), each operation rounded in this order
-      const SigSilu ss = sig_silu(gv[i]);
-      v[0][i] = ((dv[i] * uv[i]) * ss.s) * (1.f + gv[i] * (1.f - ss.s));
-      v[1][i] = dv[i] * ss.silu;
-    }
+    swiglu8_backward(gv, uv, dv, v[0], v[1]);
   }
 };
 

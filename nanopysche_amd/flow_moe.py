@@ -24,6 +24,7 @@ from typing import Optional
 import torch
 
 from . import _lib
+from .act8 import Activation8, _compress
 from .recipes import BlockScalingGranularity, FP8RecipeConfig, FP8RecipeType
 from .routing import PAD_ROWS, RouterDotInputs, RoutingPlan, route_tokens
 
@@ -276,6 +277,19 @@ def _permute_act(x, plan, kind, col, weights, tile_valid, paired, col_paired):
     _lib.call("fm_permute", x.data_ptr(), T, D, D, plan.assign_of_row.data_ptr(), plan.rows_max, plan.top_k,
               _lib.addr(weights), *args, _lib.ptr(tile_valid), _lib.stream_of(x))
     return row, c
+
+
+def _alloc_cols(rows, cols, kind, dev, paired):
+    """The column operand alone: (its _Act, the producer's kind .. ld_st arguments)."""
+    n = rows * cols
+    if kind == _lib.QUANT_BF16:
+        qt = torch.empty(n, dtype=torch.bfloat16, device=dev)
+        return _Act(qt, rows, None, 0, False), (kind, None, 0, None, 0, qt.data_ptr(), rows, None, 0)
+    blk, size = _ACT_BLOCK[kind]
+    qt = torch.empty(n + n // blk * size, dtype=torch.uint8, device=dev)
+    at = qt.data_ptr()
+    return (_Act(qt, rows, n, cols, paired),
+            (kind | (_lib.COLS_PAIRED if paired else 0), None, 0, None, 0, at, rows, at + n, cols))
 
 
 def _swiglu(g, u, rows, H, kind, row, col, dev, tile_valid=None, kmajor=False, paired=False, col_paired=False):
@@ -1105,10 +1119,18 @@ class FP8FlowMoECompute:
     the FP8 GEMMs, the others BF16 (0 forces FP8 for all).  The object owns no
     parameters and adds no state_dict keys; weights are borrowed via
     ``set_weights``.
+
+    ``checkpoint_8bit``: what the forward keeps for the backward is kept in 8
+    bits (``Activation8``): the gate|up product, the expert outputs (for the
+    router weights' gradient) and x once per token; the backward makes h and
+    the permuted x of the weight gradients from them.  The outputs are the
+    same, the gradients are those of activations rounded to a 64th of their
+    block's largest at most.  Per assignment 2H + D bytes instead of BF16's
+    6H + 4D (the FP8 recipes' 5H + 3D), and D per token.
     """
 
     def __init__(self, config: FP8FlowMoEConfig, d_model: int, hidden_size: int,
-                 num_experts: int, fp8_gemm_threshold: int = 1000000):
+                 num_experts: int, fp8_gemm_threshold: int = 1000000, *, checkpoint_8bit: bool = False):
         if d_model % 128 or hidden_size % 128:
             raise ValueError(f"d_model ({d_model}) and hidden_size ({hidden_size}) must be "
                              "multiples of 128")
@@ -1132,6 +1154,7 @@ class FP8FlowMoECompute:
         # grid) on a second stream beside the main stream's work (False keeps
         # every launch on the caller's stream).
         self.overlap_streams = True
+        self.checkpoint_8bit = bool(checkpoint_8bit)
         # One group, every token in it with weight 1 (set by
         # FP8SharedExpertCompute): the routing plan is the identity, built once
         # per token count, and the outputs are the padded buffers' first rows
@@ -1245,6 +1268,8 @@ class FP8FlowMoECompute:
         del side, batches   # the launches are enqueued: their sources may go
         wts = weights.to(torch.float32).contiguous()
         R = plan.rows_max
+        keep8 = self.checkpoint_8bit and self._record
+        cols_now = self._record and not keep8   # the weight gradients' operands; else made in the backward
         GU = torch.empty(R, 2 * H, dtype=torch.bfloat16, device=dev)
         Y = torch.empty(R, D, dtype=torch.bfloat16, device=dev)
         mask = plan.use_fp8 if (fp8_kind is not None and use_bf16) else None
@@ -1259,7 +1284,7 @@ class FP8FlowMoECompute:
             if kind is None:
                 continue
             ew = ews[kind]
-            rows, cols = _permute_act(x, plan, kind, self._record, None, tiles.get(kind, plan.tile_expert),
+            rows, cols = _permute_act(x, plan, kind, cols_now, None, tiles.get(kind, plan.tile_expert),
                                       self._paired(kind), pcols.get(kind, False))
             _gemm_m(kind, rows, ew.w13, plan, GU, mask, want)
             saved[kind] = (cols, ew)
@@ -1268,7 +1293,7 @@ class FP8FlowMoECompute:
             if kind is None:
                 continue
             # row blocks feed the down GEMM; the column blocks are kept for dW2
-            hrow, h_cols[kind], args = _alloc_act(R, H, kind, self._record, dev, self._paired(kind),
+            hrow, h_cols[kind], args = _alloc_act(R, H, kind, cols_now, dev, self._paired(kind),
                                                   pcols.get(kind, False))
             gu = GU.data_ptr()   # gate columns, then up columns (bf16)
             _lib.call("fm_swiglu_quantize", gu, 2 * H, gu + 2 * H, 2 * H, R, H, *args,
@@ -1298,7 +1323,15 @@ class FP8FlowMoECompute:
         ctx.wdtypes = (w1.dtype, w2.dtype, w3.dtype)
         # Y only feeds the router-weight gradient (the dense path's outputs are
         # views of Y: not saving it leaves them free for in-place use)
-        ctx.save_for_backward(wts, GU, Y if ctx.needs_input_grad[1] else None)
+        keep_y = ctx.needs_input_grad[1]
+        ctx.keep8 = keep8
+        if keep8:
+            # rows of tiles past the last group hold nothing
+            GU8 = _compress(GU, GU.shape, plan.tile_expert).data
+            Y8 = _compress(Y, Y.shape, plan.tile_expert).data if keep_y else None
+            ctx.save_for_backward(wts, GU8, Y8, _compress(x, x.shape).data)
+        else:
+            ctx.save_for_backward(wts, GU, Y if keep_y else None)
         return out if ctx.x_dtype == torch.bfloat16 else out.to(ctx.x_dtype)
 
     # ----------------------------------------------------------------- backward ----
@@ -1312,7 +1345,7 @@ class FP8FlowMoECompute:
         router's share of the input gradient, summed in the unpermute:
         {"addend": bf16 [T, D]}, or with ``can_fold`` {"dlogits": [T, E],
         "gate_w": [E, D]} (E <= 8) for the unpermute to form it itself."""
-        wts, GU, Y = ctx.saved_tensors
+        wts, GU, Y, *X = ctx.saved_tensors
         wts = wts.to(torch.float32).contiguous()   # as saved, unless a saved-tensor hook returned it otherwise
         if any(w._version != version for w, version in ctx.in_place):
             raise RuntimeError("expert weights that the backward reads in place (BF16) were changed by an in-place "
@@ -1323,12 +1356,21 @@ class FP8FlowMoECompute:
         T, K = plan.num_tokens, plan.top_k
         R = plan.rows_max
         dev = GU.device
+        keep8 = ctx.keep8
+        if keep8:
+            GU, X = Activation8(GU, (R, 2 * H)), Activation8(X[0], (T, D))
+            Y = None if Y is None else Activation8(Y, (R, D))
         dO = grad_out.reshape(T, D).to(torch.bfloat16).contiguous()
         mask = plan.use_fp8 if (fp8_kind is not None and use_bf16) else None
         # router-weight gradient from the saved expert outputs (skipped when
         # the weights need none, e.g. the constant weights of a shared expert)
         dw = dot = None
-        if ctx.needs_input_grad[1] and getattr(on_router_grad, "fused_dot", False) and K <= 8 and not self._dense:
+        if ctx.needs_input_grad[1] and keep8:
+            dw = torch.empty(T * K, dtype=torch.float32, device=dev)
+            q, codes, ld_q, ld_c = Y.at()
+            _lib.call("fm_act8_router_weight_grad", _lib.addr(dO), dO.stride(0), q, ld_q, codes, ld_c,
+                      _lib.addr(plan.row_of), T, K, D, _lib.addr(dw), _lib.stream_of(dO))
+        elif ctx.needs_input_grad[1] and getattr(on_router_grad, "fused_dot", False) and K <= 8 and not self._dense:
             dot = RouterDotInputs(dO, Y, plan.row_of)
         elif ctx.needs_input_grad[1]:
             dw = torch.empty(T * K, dtype=torch.float32, device=dev)
@@ -1365,6 +1407,14 @@ class FP8FlowMoECompute:
         dy = {kind: _permute_act(dO, plan, kind, True, None if self._dense else wts,
                                  tiles.get(kind, plan.tile_expert), self._paired(kind), pcols.get(kind, False))
               for kind, _ in runs}
+        hcols = ctx.saved_hcols
+        if keep8:   # h of the kept gate|up
+            hcols = {}
+            for kind, _ in runs:
+                hcols[kind], args = _alloc_cols(R, H, kind, dev, pcols.get(kind, False))
+                q, codes, ld_q, ld_c = GU.at()
+                _lib.call("fm_act8_swiglu_quantize", q, ld_q, codes, ld_c, R, H, *args,
+                          _lib.ptr(tiles.get(kind, plan.tile_expert)), _lib.stream_of(dO))
         # dH and dW2 (contraction over each expert's tokens) both read the
         # permuted dY: each alone leaves its last round of workgroups
         # part-empty when the hidden size is not a multiple of the 256-wide
@@ -1384,24 +1434,35 @@ class FP8FlowMoECompute:
             side.wait_stream(main)
             with torch.cuda.stream(side):
                 for kind, want in two_streams:
-                    _gemm_k(kind, ctx.saved_hcols[kind], dy[kind][1], plan, H, D, dW2, H * D, mask=mask,
-                            want=want, may_split=side is main, a_cold=True)
+                    _gemm_k(kind, hcols[kind], dy[kind][1], plan, H, D, dW2, H * D, mask=mask,
+                            want=want, may_split=side is main, a_cold=not keep8)
         if ctx.dgrad_ops is None:
             raise RuntimeError("the expert block's forward did not record a backward")
         for kind, want in one_grid:
-            _gemm_mk(kind, dy[kind][0], ctx.dgrad_ops[kind][0], plan, dH, ctx.saved_hcols[kind],
-                     dy[kind][1], H, D, dW2, H * D, mask, want, a_cold=True)
+            _gemm_mk(kind, dy[kind][0], ctx.dgrad_ops[kind][0], plan, dH, hcols[kind],
+                     dy[kind][1], H, D, dW2, H * D, mask, want, a_cold=not keep8)
         for kind, want in two_streams:
             _gemm_m(kind, dy[kind][0], ctx.dgrad_ops[kind][0], plan, dH, mask, want)
         if self.capture_intermediates is not None:
             self.capture_intermediates["dh"] = dH.detach().clone()
         for kind, want in runs:
             dgu_row, dgu_col, args = _alloc_act(R, 2 * H, kind, True, dev, self._paired(kind), pcols.get(kind, False))
-            gu = GU.data_ptr()
-            _lib.call("fm_swiglu_backward", gu, GU.stride(0), gu + 2 * H, GU.stride(0), dH.data_ptr(), H, R, H, *args,
-                      _lib.ptr(tiles.get(kind, plan.tile_expert)), _lib.stream_of(GU))
+            valid = _lib.ptr(tiles.get(kind, plan.tile_expert))
+            if keep8:
+                q, codes, ld_q, ld_c = GU.at()
+                _lib.call("fm_act8_swiglu_backward_quantize", q, ld_q, codes, ld_c, dH.data_ptr(), H, R, H, *args, valid,
+                          _lib.stream_of(dO))
+                xcols, args = _alloc_cols(R, D, kind, dev, pcols.get(kind, False))
+                q, codes, ld_q, ld_c = X.at()
+                _lib.call("fm_act8_permute", q, ld_q, codes, ld_c, T, D, plan.assign_of_row.data_ptr(), R, K, *args,
+                          valid, _lib.stream_of(dO))
+            else:
+                gu = GU.data_ptr()
+                _lib.call("fm_swiglu_backward", gu, GU.stride(0), gu + 2 * H, GU.stride(0), dH.data_ptr(), H, R, H, *args,
+                          valid, _lib.stream_of(GU))
+                xcols = ctx.saved_cols[kind]
             # dW1 | dW3: contraction over each expert's tokens
-            _gemm_k(kind, dgu_col, ctx.saved_cols[kind], plan, 2 * H, D, dW1, H * D, dW3, H * D, split=H,
+            _gemm_k(kind, dgu_col, xcols, plan, 2 * H, D, dW1, H * D, dW3, H * D, split=H,
                     mask=mask, want=want)
             # input gradient
             _gemm_m(kind, dgu_row, ctx.dgrad_ops[kind][1], plan, dXp, mask, want)
@@ -1438,12 +1499,14 @@ class FP8SharedExpertCompute:
     ``set_weights(w1 [H, D], w2 [H, D], w3 [H, D])`` borrows the weights
     (``w2`` stored as ``[H, D]``, i.e. the transpose of ``nn.Linear(H, D)``'s
     weight, like the expert block's); ``__call__(x [..., D]) -> [..., D]`` is
-    differentiable with respect to x, w1, w2 and w3.
+    differentiable with respect to x, w1, w2 and w3.  ``checkpoint_8bit`` as the
+    expert block's.
     """
 
     def __init__(self, config: FP8FlowMoEConfig, d_model: int, hidden_size: int,
-                 fp8_gemm_threshold: int = 0):
-        self._block = FP8FlowMoECompute(config, d_model, hidden_size, 1, fp8_gemm_threshold)
+                 fp8_gemm_threshold: int = 0, *, checkpoint_8bit: bool = False):
+        self._block = FP8FlowMoECompute(config, d_model, hidden_size, 1, fp8_gemm_threshold,
+                                        checkpoint_8bit=checkpoint_8bit)
         self._block._dense = True
         self._route = {}
 

@@ -19,10 +19,11 @@ from typing import Optional
 import torch
 
 from . import _lib
+from .act8 import Activation8, _compress, rmsnorm_8bit
 from .decode import DecodeOutput, moe_decode
 from .flow_moe import FP8FlowMoECompute, FP8FlowMoEConfig, FP8SharedExpertCompute
 from .norm import DEFAULT_EPS, rmsnorm
-from .routing import (ExpertLoadTracker, capacity_select, gather_rows, route, route_tokens, router_backward,
+from .routing import (ExpertLoadTracker, _balance_args, capacity_select, gather_rows, route, route_tokens, router_backward,
                       router_forward, select_rows)
 
 
@@ -40,18 +41,22 @@ class _BlockCtx:
 
 class _MoELayerFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, gate_weight, gate_bias, w1, w2, w3, layer, replay, tracker, noise):
+    def forward(ctx, x, gate_weight, gate_bias, w1, w2, w3, layer, replay, tracker, noise, balance):
         lead = x.shape[:-1]
         D = x.shape[-1]
         x2 = _bf16_rows(x)
         # the router's input: x, or x + noise (jitter) in x's dtype
         xr = x2 if noise is None else _bf16_rows(x + noise)
         w, idx, aux, state = router_forward(xr, gate_weight, gate_bias, layer.score_bias, layer.top_k, layer.gating,
-                                            replay, layer.normalize_expert_weights, layer.z_loss_multiplier, tracker)
+                                            replay, layer.normalize_expert_weights, layer.z_loss_multiplier, tracker, balance)
         need_x, need_gw, need_gb = ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[2]
         bctx = _BlockCtx((need_x, need_x or need_gw or need_gb, *ctx.needs_input_grad[3:6], False, False))
         out = layer.block._forward(bctx, x2, w, w1, w2, w3, idx)
-        ctx.save_for_backward(xr, gate_weight)
+        keep8 = layer.block.checkpoint_8bit and layer.block._record
+        if keep8:   # the block's x in 8 bits, unless the router saw another
+            kept = bctx.saved_tensors[3] if noise is None else _compress(xr, xr.shape).data
+        ctx.save_for_backward(kept if keep8 else xr, gate_weight, *state.release())
+        ctx.kept_shape = xr.shape if keep8 else None
         ctx.state = state
         ctx.bctx = bctx
         ctx.layer = layer
@@ -64,7 +69,10 @@ class _MoELayerFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout, daux):
-        x2, gate_weight = ctx.saved_tensors
+        x2, gate_weight, *callers = ctx.saved_tensors
+        ctx.state.restore(callers)
+        if ctx.kept_shape is not None:
+            x2 = Activation8(x2, ctx.kept_shape).restore()
         T, D = x2.shape
         need_x, need_gw, need_gb = ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[2]
         if dout is None:
@@ -92,7 +100,7 @@ class _MoELayerFunction(torch.autograd.Function):
         dgw = grads.get("gw")
         if dgw is not None:
             dgw = dgw.to(gate_weight.dtype)
-        return dx, dgw, grads.get("gb"), dW1, dW2, dW3, None, None, None, None
+        return dx, dgw, grads.get("gb"), dW1, dW2, dW3, None, None, None, None, None
 
 
 def _bf16_rows(x):
@@ -130,7 +138,14 @@ class FP8FlowMoELayer:
     ``:1351-1356``, ``:1386-1391``, ``:1395-1498``; drop statistics as
     ``:1787-1825`` keeps them).  With a capacity factor the layer runs the
     router, the expert block and the shared expert as separate autograd
-    nodes on the kept tokens."""
+    nodes on the kept tokens.
+
+    Beyond the reference, also off by default: ``checkpoint_8bit`` keeps what the
+    backward needs in 8 bits (the pre-norm's input, the tokens, the gate|up
+    product and the expert outputs; the expert block's and shared expert's
+    option, ``rmsnorm_8bit``; with a capacity factor the router keeps its input as
+    it is), and ``layer(x, token_mask=..., cu_seqlens=...)`` with ``balance_scores`` takes the
+    load-balancing loss per sequence over the tokens that count (``balance_loss``)."""
 
     def __init__(self, config: FP8FlowMoEConfig, d_model: int, hidden_size: int, num_experts: int, top_k: int,
                  gating: str = "softmax", fp8_gemm_threshold: int = 0,
@@ -138,14 +153,20 @@ class FP8FlowMoELayer:
                  shared_hidden_size: Optional[int] = None, pre_norm: bool = False, norm_eps: float = DEFAULT_EPS,
                  jitter_eps: Optional[float] = None, capacity_factor: Optional[float] = None,
                  adaptive_capacity: bool = False, adaptive_capacity_target: float = 0.01,
-                 adaptive_capacity_ema: float = 0.3):
-        self.block = FP8FlowMoECompute(config, d_model, hidden_size, num_experts, fp8_gemm_threshold)
+                 adaptive_capacity_ema: float = 0.3, checkpoint_8bit: bool = False, balance_scores: str = "softmax"):
+        self.block = FP8FlowMoECompute(config, d_model, hidden_size, num_experts, fp8_gemm_threshold,
+                                       checkpoint_8bit=checkpoint_8bit)
+        self.checkpoint_8bit = bool(checkpoint_8bit)
+        if balance_scores not in ("softmax", "sigmoid"):
+            raise ValueError(f"balance_scores must be 'softmax' or 'sigmoid', got {balance_scores!r}")
+        self.balance_scores = balance_scores
         self.num_experts = num_experts
         self.top_k = int(top_k)
         self.gating = gating
         self.normalize_expert_weights = normalize_expert_weights
         self.z_loss_multiplier = 0.0 if z_loss_multiplier is None else float(z_loss_multiplier)
-        self.shared = (FP8SharedExpertCompute(config, d_model, shared_hidden_size, fp8_gemm_threshold)
+        self.shared = (FP8SharedExpertCompute(config, d_model, shared_hidden_size, fp8_gemm_threshold,
+                                              checkpoint_8bit=checkpoint_8bit)
                        if shared_hidden_size else None)
         self.gate_weight = self.gate_bias = self.score_bias = None
         self.pre_norm = bool(pre_norm)
@@ -244,22 +265,25 @@ class FP8FlowMoELayer:
         self.norm_weight = norm_weight
 
     def __call__(self, x: torch.Tensor, replay_indices: Optional[torch.Tensor] = None,
-                 load_tracker: Optional[ExpertLoadTracker] = None):
+                 load_tracker: Optional[ExpertLoadTracker] = None, token_mask: Optional[torch.Tensor] = None,
+                 cu_seqlens: Optional[torch.Tensor] = None):
         if self.gate_weight is None:
             raise RuntimeError("set_weights() must be called before the layer runs")
         _lib.require_device(x, "x")
+        balance = _balance_args(x, token_mask, cu_seqlens, self.balance_scores)
         if self.pre_norm:
-            x = rmsnorm(x if x.dtype == torch.bfloat16 else x.to(torch.bfloat16), self.norm_weight, self.norm_eps)
+            norm = rmsnorm_8bit if self.checkpoint_8bit else rmsnorm
+            x = norm(x if x.dtype == torch.bfloat16 else x.to(torch.bfloat16), self.norm_weight, self.norm_eps)
         noise = None
         if self.jitter_eps is not None and self.training:
             noise = torch.randn_like(x) * self.jitter_eps
         if self.capacity_factor is not None:
-            return self._forward_with_capacity(x, noise, replay_indices, load_tracker)
+            return self._forward_with_capacity(x, noise, replay_indices, load_tracker, token_mask, cu_seqlens)
         w1, w2, w3 = self.block._w
         self.block._record = torch.is_grad_enabled() and any(
             t is not None and t.requires_grad for t in (x, self.gate_weight, self.gate_bias, w1, w2, w3))
         out, aux = _MoELayerFunction.apply(x, self.gate_weight, self.gate_bias, w1, w2, w3, self, replay_indices,
-                                           load_tracker, noise)
+                                           load_tracker, noise, balance)
         if self.shared is not None:
             out = out + self.shared(x)
         return out, aux
@@ -285,7 +309,7 @@ class FP8FlowMoELayer:
                           normalize_expert_weights=self.normalize_expert_weights, norm_weight=self.norm_weight,
                           norm_eps=self.norm_eps, shared=shared)
 
-    def _forward_with_capacity(self, x, noise, replay_indices, load_tracker):
+    def _forward_with_capacity(self, x, noise, replay_indices, load_tracker, token_mask, cu_seqlens):
         """MoEBase.forward with ``capacity_factor`` (reference ``model/moe.py:1338-1393``):
         route all tokens, drop those over capacity (``_apply_capacity``), run
         the experts and the shared expert on the kept tokens and scatter
@@ -296,7 +320,9 @@ class FP8FlowMoELayer:
         w, idx, aux = route(_bf16_rows(xr), self.gate_weight, self.gate_bias, top_k=self.top_k,
                             gating=self.gating, score_bias=self.score_bias, replay_indices=replay_indices,
                             normalize_expert_weights=self.normalize_expert_weights,
-                            z_loss_multiplier=self.z_loss_multiplier, load_tracker=load_tracker)
+                            z_loss_multiplier=self.z_loss_multiplier, load_tracker=load_tracker,
+                            token_mask=None if token_mask is None else token_mask.reshape(-1), cu_seqlens=cu_seqlens,
+                            balance_scores=self.balance_scores)
         T, E = x2.shape[0], self.num_experts
         plan = route_tokens(idx, E)
         if self.adaptive_capacity:

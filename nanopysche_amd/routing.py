@@ -16,6 +16,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
+from .balance import BalanceState, balance_backward, balance_forward
 
 PAD_ROWS = 128  # every expert group is padded to a multiple of this many rows
 
@@ -357,15 +358,31 @@ class RouterState:
     flags: int
     replay: bool
     z_mult: float
+    balance: "BalanceState | None" = None   # the loss of sequences and masks, in place of the batch's
+
+    def release(self):
+        """The caller's tensors that the loss's backward reads, for autograd to keep (it notices changes in place)."""
+        if self.balance is None:
+            return ()
+        b = self.balance
+        kept = b.cu_seqlens, b.mask
+        b.cu_seqlens = b.mask = None
+        return kept
+
+    def restore(self, kept) -> None:
+        if self.balance is not None:
+            self.balance.cu_seqlens, self.balance.mask = kept
 
 
 def router_forward(x2, gate_weight, gate_bias, score_bias, top_k, gating, replay=None, normalize=None,
-                   z_mult=0.0, tracker=None):
+                   z_mult=0.0, tracker=None, balance=None):
     """Gate, gating, counts and aux loss of MoERouter.forward (reference
     model/moe.py:133-184) on x2 [T, D]: (weights [T, K], indices [T, K], aux, state).
     One library call (fm_router_forward): for E <= 8 and D = 512 n <= 2048 a
     single pass over x forms the logits, the gating, the loss partials and the
-    expert histograms, and one small kernel the counts and the loss."""
+    expert histograms, and one small kernel the counts and the loss.
+    ``balance`` (``balance_forward``'s keyword arguments) takes the loss and the
+    tracker's counts of its sequences and tokens instead."""
     T, D = x2.shape
     if T == 0:
         raise ValueError("the router needs at least one token")
@@ -389,7 +406,7 @@ def router_forward(x2, gate_weight, gate_bias, score_bias, top_k, gating, replay
             raise TypeError("replay_indices must be int64 or int32")
         rep = rep.contiguous()
     acc = tot = None
-    if tracker is not None:
+    if tracker is not None and balance is None:
         acc, tot = tracker.tokens_per_expert, tracker.total_tokens
     _lib.call("fm_router_forward", _lib.addr(x2), _x_dtype(x2), x2.stride(0), T, D, _lib.addr(w_), _dt_code(w_),
               w_.stride(0), _lib.addr(b), _lib.addr(sb), E, K, _gating_code(gating), _norm_flags(normalize),
@@ -398,7 +415,20 @@ def router_forward(x2, gate_weight, gate_bias, score_bias, top_k, gating, replay
               _lib.addr(aux), _lib.addr(ws), ws.numel(), _lib.stream_of(x2))
     state = RouterState(logits, idx, counts, _gating_code(gating), _norm_flags(normalize), replay is not None,
                         float(z_mult))
+    if balance is not None:
+        aux, _, state.balance = balance_forward(logits, idx, z_loss_multiplier=z_mult, load_tracker=tracker, **balance)
     return w, idx, aux, state
+
+
+def _balance_args(x, token_mask, cu_seqlens, scores):
+    """``router_forward``'s ``balance`` for x [..., D]: None for the loss of the batch as one sequence."""
+    if token_mask is None and cu_seqlens is None and scores == "softmax":
+        return None
+    if token_mask is not None:
+        if token_mask.shape != x.shape[:-1]:
+            raise ValueError(f"token_mask must be {tuple(x.shape[:-1])}, got {tuple(token_mask.shape)}")
+        token_mask = token_mask.reshape(-1)
+    return {"token_mask": token_mask, "cu_seqlens": cu_seqlens, "scores": scores}
 
 
 @dataclass
@@ -428,17 +458,20 @@ def router_backward(state: RouterState, x2, gate_weight, dweights, daux, need_x=
     dwts = None if dweights is None else dweights.reshape(T, K).float().contiguous()
     da = None if daux is None else daux.reshape(1).float().contiguous()
     dlogits = torch.empty(T, E, dtype=torch.float32, device=dev)
+    aux = None if state.balance is not None else da   # the batch's loss: its gradient is formed with the gating's
     if dot is not None:
         _lib.call("fm_gating_grad_dot", _lib.addr(logits), T, E, logits.stride(0), K, state.gating, state.flags,
                   int(state.replay), _lib.addr(idx), int(idx.dtype == torch.int64), None, _lib.addr(dot.dout),
-                  dot.dout.stride(0), _lib.addr(dot.y), dot.y.stride(0), _lib.addr(dot.row_of), D, None, _lib.addr(da),
+                  dot.dout.stride(0), _lib.addr(dot.y), dot.y.stride(0), _lib.addr(dot.row_of), D, None, _lib.addr(aux),
                   _lib.addr(state.counts), state.z_mult, _lib.addr(dlogits), dlogits.stride(0), st)
-    elif dwts is None and da is None:
+    elif dwts is None and aux is None:
         dlogits.zero_()
     else:
         _lib.call("fm_gating_grad", _lib.addr(logits), T, E, logits.stride(0), K, state.gating, state.flags,
-                  int(state.replay), _lib.addr(idx), int(idx.dtype == torch.int64), _lib.addr(dwts), _lib.addr(da),
+                  int(state.replay), _lib.addr(idx), int(idx.dtype == torch.int64), _lib.addr(dwts), _lib.addr(aux),
                   _lib.addr(state.counts), state.z_mult, _lib.addr(dlogits), dlogits.stride(0), st)
+    if state.balance is not None and da is not None:
+        balance_backward(state.balance, da, add_to=dlogits)
     w, _, _ = _gate_params(gate_weight, None, None)
     dx = torch.empty_like(x2) if need_x else None
     dW = torch.empty(E, D, dtype=w.dtype, device=dev) if need_w else None
@@ -458,12 +491,12 @@ class _RouterFunction(torch.autograd.Function):
     forward and backward on the GPU."""
 
     @staticmethod
-    def forward(ctx, x, gate_weight, gate_bias, score_bias, top_k, gating, replay, normalize, z_mult, tracker):
+    def forward(ctx, x, gate_weight, gate_bias, score_bias, top_k, gating, replay, normalize, z_mult, tracker, balance):
         lead = x.shape[:-1]
         x2 = x.reshape(-1, x.shape[-1]).contiguous()
         w, idx, aux, state = router_forward(x2, gate_weight, gate_bias, score_bias, top_k, gating, replay,
-                                            normalize, z_mult, tracker)
-        ctx.save_for_backward(x2, gate_weight)
+                                            normalize, z_mult, tracker, balance)
+        ctx.save_for_backward(x2, gate_weight, *state.release())
         ctx.state = state
         ctx.has_bias = gate_bias is not None
         ctx.bias_dtype = None if gate_bias is None else gate_bias.dtype
@@ -474,7 +507,8 @@ class _RouterFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dweights, _dindices, daux):
-        x2, gate_weight = ctx.saved_tensors
+        x2, gate_weight, *callers = ctx.saved_tensors
+        ctx.state.restore(callers)
         need_x, need_w, need_b = ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[2]
         dx, dW, db, _ = router_backward(ctx.state, x2, gate_weight, dweights, daux, need_x, need_w,
                                         need_b and ctx.has_bias, bias_dtype=ctx.bias_dtype)
@@ -482,12 +516,13 @@ class _RouterFunction(torch.autograd.Function):
             dx = dx.reshape(*ctx.lead, x2.shape[1])
         if dW is not None:
             dW = dW.to(gate_weight.dtype)
-        return dx, dW, db, None, None, None, None, None, None, None
+        return dx, dW, db, None, None, None, None, None, None, None, None
 
 
 def route(x: torch.Tensor, gate_weight: torch.Tensor, gate_bias=None, *, top_k: int, gating: str = "softmax",
           score_bias=None, replay_indices=None, normalize_expert_weights=None, z_loss_multiplier=None,
-          load_tracker: ExpertLoadTracker = None, jitter_eps=None, training: bool = True):
+          load_tracker: ExpertLoadTracker = None, jitter_eps=None, training: bool = True, token_mask=None,
+          cu_seqlens=None, balance_scores: str = "softmax"):
     """MoERouter.forward on the GPU (reference model/moe.py:133-184): with
     ``jitter_eps`` and ``training``, x + randn_like(x) * jitter_eps first
     (:145-148, torch's generator, so a seeded run draws the reference's
@@ -499,10 +534,17 @@ def route(x: torch.Tensor, gate_weight: torch.Tensor, gate_bias=None, *, top_k: 
     accumulates the per-expert counts for ``ExpertLoadTracker.post_batch``
     (``_update_expert_counts``, :284-292; the reference does this whenever it
     has a score bias).  Differentiable in x, gate_weight and gate_bias through
-    the weights and the loss."""
+    the weights and the loss.
+
+    ``token_mask`` [...] (bool: the token counts), ``cu_seqlens`` [S + 1] (int32
+    borders of the flattened tokens' sequences) and ``balance_scores``
+    ("softmax" or "sigmoid"): the loss and the tracker's counts are
+    ``balance_loss``'s, per sequence and without the tokens that do not count.
+    Those are routed all the same."""
     _lib.require_device(x, "x")
+    balance = _balance_args(x, token_mask, cu_seqlens, balance_scores)
     if jitter_eps is not None and training:
         x = x + torch.randn_like(x) * jitter_eps
     z = 0.0 if z_loss_multiplier is None else float(z_loss_multiplier)
     return _RouterFunction.apply(x, gate_weight, gate_bias, score_bias, int(top_k), gating, replay_indices,
-                                 normalize_expert_weights, z, load_tracker)
+                                 normalize_expert_weights, z, load_tracker, balance)
