@@ -16,18 +16,29 @@
 namespace fm {
 namespace {
 
+// How a call passes the caches, by the bytes of its widest tensor (STREAM of the kernels; wide: of 16- or 32-bit values).
+//   0  as usual
+//   1  from 32 MiB on, the second-level caches together: wide outputs are stored past them.  2999 x 2831 fp32: the norm's three
+//      launches 45.3 -> 38.2 us; 16384 x 4096 bf16 kept and restored in 33792 rows 107.7 -> 95.5.  (The payload, which
+//      the backward wants, is stored as usual: past the caches the latter takes 107.3.)
+//   2  from 128 MiB on, half of the last-level cache: the backward's gradients and the compressed activation are loaded past them
+//      too, so that what was kept stays: norm of 16384 x 7168 228 -> 204 us, SwiGLU of 16384 x 14336 667 -> 654.  At 34 MB
+//      that costs: 38.2 -> 42.5 us.
+constexpr int64_t kStreamOut = int64_t(32) << 20, kStreamIn = int64_t(128) << 20;
+inline int stream_level(int64_t bytes) { return bytes >= kStreamIn ? 2 : bytes >= kStreamOut ? 1 : 0; }
+
 // ------------------------------------------------------------ rows of eight ----
 // Eight neighbours of a row as they are stored, n of them in the row (zeros behind).  TAIL: n may lie between 0 and 8.
 template <typename T>
 struct Eight {
   static constexpr int kWords = sizeof(T) * 2;
   uint32_t w[kWords];
-  template <bool TAIL = true>
+  template <bool TAIL = true, bool NT = false>
   __device__ __forceinline__ void load(const T* p, int n) {
     if (n >= 8) {
 #pragma unroll
       for (int i = 0; i < kWords / 4; ++i) {
-        const u32x4_el v = reinterpret_cast<const u32x4_el*>(p)[i];
+        const u32x4_el v = NT ? __builtin_nontemporal_load(FM_GLOBAL(const u32x4_el, p) + i) : *(FM_GLOBAL(const u32x4_el, p) + i);
 #pragma unroll
         for (int j = 0; j < 4; ++j) w[4 * i + j] = v[j];
       }
@@ -52,7 +63,7 @@ struct Eight {
 };
 
 // The first n of eight values, rounded to T.
-template <typename T, bool TAIL = true>
+template <typename T, bool TAIL = true, bool NT = false>
 __device__ __forceinline__ void store8(T* p, const float (&v)[8], int n) {
   uint32_t w[Eight<T>::kWords];
 #pragma unroll
@@ -62,8 +73,11 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8], int n) {
   }
   if (n >= 8) {
 #pragma unroll
-    for (int i = 0; i < Eight<T>::kWords / 4; ++i)
-      *FM_GLOBAL(u32x4_el, reinterpret_cast<u32x4_el*>(p) + i) = u32x4_el{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+    for (int i = 0; i < Eight<T>::kWords / 4; ++i) {
+      const u32x4_el v = {w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+      if constexpr (NT) __builtin_nontemporal_store(v, FM_GLOBAL(u32x4_el, p) + i);
+      else *(FM_GLOBAL(u32x4_el, p) + i) = v;
+    }
     return;
   }
   if constexpr (!TAIL) return;
@@ -126,7 +140,7 @@ struct CompressArgs {
   const int32_t* tile_valid;   // rows of 128-row tiles with a negative entry are left alone; null: none
 };
 
-template <typename T, int U>
+template <typename T, int U, int STREAM>
 __global__ __launch_bounds__(256) void compress_kernel(Items t, CompressArgs a) {
   Item it[U];
   Eight<T> x[U];
@@ -134,7 +148,7 @@ __global__ __launch_bounds__(256) void compress_kernel(Items t, CompressArgs a) 
   for (int u = 0; u < U; ++u) {
     it[u] = item_of<U>(t, u);
     if (a.tile_valid && a.tile_valid[it[u].row >> 7] < 0) it[u].in = false;
-    x[u].load(static_cast<const T*>(a.x) + it[u].row * a.ld_x + it[u].col, it[u].in ? it[u].n : 0);
+    x[u].template load<true, (STREAM > 1)>(static_cast<const T*>(a.x) + it[u].row * a.ld_x + it[u].col, it[u].in ? it[u].n : 0);
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -155,7 +169,7 @@ struct RestoreArgs {
   int64_t ld_out;
 };
 
-template <typename T, int U, bool GATHER>
+template <typename T, int U, bool GATHER, int STREAM>
 __global__ __launch_bounds__(256) void restore_kernel(Items t, RestoreArgs a) {
   Item it[U];
   uint2 b[U];
@@ -176,7 +190,7 @@ __global__ __launch_bounds__(256) void restore_kernel(Items t, RestoreArgs a) {
   for (int u = 0; u < U; ++u) {
     float v[8];
     act_decode8(b[u], act_scale(code[u]), v);
-    if (it[u].in) store8(static_cast<T*>(a.out) + it[u].row * a.ld_out + it[u].col, v, it[u].n);
+    if (it[u].in) store8<T, true, (STREAM > 0)>(static_cast<T*>(a.out) + it[u].row * a.ld_out + it[u].col, v, it[u].n);
   }
 }
 
@@ -190,15 +204,15 @@ struct SwigluArgs {
   int64_t ld_q, ld_c;
 };
 
-template <typename T, int U>
+template <typename T, int U, int STREAM>
 __global__ __launch_bounds__(256) void swiglu_kernel(Items t, SwigluArgs a) {
   Item it[U];
   Eight<T> g[U], up[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     it[u] = item_of<U>(t, u);
-    g[u].load(static_cast<const T*>(a.g) + it[u].row * a.ld_g + it[u].col, it[u].n);
-    up[u].load(static_cast<const T*>(a.u) + it[u].row * a.ld_u + it[u].col, it[u].n);
+    g[u].template load<true>(static_cast<const T*>(a.g) + it[u].row * a.ld_g + it[u].col, it[u].n);
+    up[u].template load<true>(static_cast<const T*>(a.u) + it[u].row * a.ld_u + it[u].col, it[u].n);
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -209,7 +223,7 @@ __global__ __launch_bounds__(256) void swiglu_kernel(Items t, SwigluArgs a) {
     uint32_t gc, uc;
     const uint2 gb = act_encode8(gv, gc), ub = act_encode8(uv, uc);
     if (!it[u].in) continue;
-    store8(static_cast<T*>(a.h) + it[u].row * a.ld_h + it[u].col, h, it[u].n);
+    store8<T, true, (STREAM > 0)>(static_cast<T*>(a.h) + it[u].row * a.ld_h + it[u].col, h, it[u].n);
     store_kept(a.qg, a.ld_q, a.cg, a.ld_c, it[u].row, it[u].col, gb, gc);
     store_kept(a.qu, a.ld_q, a.cu, a.ld_c, it[u].row, it[u].col, ub, uc);
   }
@@ -223,7 +237,7 @@ struct SwigluBwdArgs {
   int64_t ld_dg, ld_du;
 };
 
-template <typename T, int U>
+template <typename T, int U, int STREAM>
 __global__ __launch_bounds__(256) void swiglu_backward_kernel(Items t, SwigluBwdArgs a) {
   Item it[U];
   Eight<T> dh[U];
@@ -236,7 +250,7 @@ __global__ __launch_bounds__(256) void swiglu_backward_kernel(Items t, SwigluBwd
     up[u] = a.u.bytes(it[u].row, it[u].col);
     gc[u] = a.g.code(it[u].row, it[u].col);
     uc[u] = a.u.code(it[u].row, it[u].col);
-    dh[u].load(static_cast<const T*>(a.dh) + it[u].row * a.ld_dh + it[u].col, it[u].n);
+    dh[u].template load<true, (STREAM > 1)>(static_cast<const T*>(a.dh) + it[u].row * a.ld_dh + it[u].col, it[u].n);
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -246,8 +260,8 @@ __global__ __launch_bounds__(256) void swiglu_backward_kernel(Items t, SwigluBwd
     dh[u].widen(dv);
     swiglu8_backward(gv, uv, dv, dg, du);
     if (!it[u].in) continue;
-    store8(static_cast<T*>(a.dg) + it[u].row * a.ld_dg + it[u].col, dg, it[u].n);
-    store8(static_cast<T*>(a.du) + it[u].row * a.ld_du + it[u].col, du, it[u].n);
+    store8<T, true, (STREAM > 0)>(static_cast<T*>(a.dg) + it[u].row * a.ld_dg + it[u].col, dg, it[u].n);
+    store8<T, true, (STREAM > 0)>(static_cast<T*>(a.du) + it[u].row * a.ld_du + it[u].col, du, it[u].n);
   }
 }
 
@@ -285,7 +299,7 @@ __device__ __forceinline__ float row_sum(float v, float (*sums)[16], int parity)
   return v;
 }
 
-template <typename T, typename WT, int NC, bool ONE, bool TAIL>
+template <typename T, typename WT, int NC, bool ONE, bool TAIL, int STREAM>
 __global__ __launch_bounds__(ONE ? 256 : 1024) void norm_kernel(NormArgs a) {
   __shared__ float sums[1][16];
   const int lane = ONE ? threadIdx.x & 63 : threadIdx.x;
@@ -322,7 +336,7 @@ __global__ __launch_bounds__(ONE ? 256 : 1024) void norm_kernel(NormArgs a) {
     for (int j = 0; j < 8; ++j) yv[j] = (v[j] * r) * wv[j];
     uint32_t code;
     const uint2 b = act_encode8(v, code);
-    store8<T, TAIL>(static_cast<T*>(a.y) + row * a.ld_y + col, yv, a.D - col);
+    store8<T, TAIL, (STREAM > 0)>(static_cast<T*>(a.y) + row * a.ld_y + col, yv, a.D - col);
     store_kept(a.q, a.ld_q, a.codes, a.ld_c, row, col, b, code);
   }
 }
@@ -342,7 +356,7 @@ struct NormBwdArgs {
   int64_t ld_p, rps;
 };
 
-template <typename T, int NC, bool TAIL>
+template <typename T, int NC, bool TAIL, int STREAM>
 struct NormRow {
   uint2 q[NC];
   uint32_t code[NC];
@@ -355,13 +369,13 @@ struct NormRow {
       const int at = col < a.x.ld_q ? col : 0;   // behind the row: its first bytes, with a dy of zeros
       q[c] = a.x.bytes(row, at);
       code[c] = a.x.code(row, at);
-      dy[c].template load<TAIL>(static_cast<const T*>(a.dy) + row * a.ld_dy + col, a.D - col);
+      dy[c].template load<TAIL, (STREAM > 1)>(static_cast<const T*>(a.dy) + row * a.ld_dy + col, a.D - col);
     }
     r = a.rstd[row];
   }
 };
 
-template <typename T, typename WT, int NC, bool ONE, bool TAIL>
+template <typename T, typename WT, int NC, bool ONE, bool TAIL, int STREAM>
 __global__ __launch_bounds__(ONE ? 256 : 1024) void norm_backward_kernel(NormBwdArgs a) {
   __shared__ float sums[2][16];
   const int lane = ONE ? threadIdx.x & 63 : threadIdx.x, wave = threadIdx.x >> 6;
@@ -383,7 +397,7 @@ __global__ __launch_bounds__(ONE ? 256 : 1024) void norm_backward_kernel(NormBwd
   const int64_t first = r0 + (ONE ? wave : 0);
   // the next row's loads are in flight while this one is summed, where 128 registers hold both
   constexpr bool kNext = ONE || sizeof(T) == 2;
-  NormRow<T, NC, TAIL> n, next;
+  NormRow<T, NC, TAIL, STREAM> n, next;
   if (kNext && first < r1) next.load(a, first, lane, step);
   for (int64_t row = first; row < r1; row += kStep, parity ^= 1) {
     if constexpr (kNext) {
@@ -412,7 +426,7 @@ __global__ __launch_bounds__(ONE ? 256 : 1024) void norm_backward_kernel(NormBwd
       if (col >= a.D) break;
 #pragma unroll
       for (int j = 0; j < 8; ++j) g[c][j] = n.r * fmaf(-m, xr[c][j], g[c][j]);
-      store8<T, TAIL>(static_cast<T*>(a.dx) + row * a.ld_dx + col, g[c], a.D - col);
+      store8<T, TAIL, (STREAM > 0)>(static_cast<T*>(a.dx) + row * a.ld_dx + col, g[c], a.D - col);
     }
   }
   if (a.part == nullptr) return;
@@ -493,6 +507,15 @@ int for_items(int64_t rows, int64_t cols, F go) {
   return 0;
 }
 
+// go(tag of the level, one of LEVELS)
+template <int... LEVELS, typename F>
+void for_stream(int64_t bytes, F go) {
+  const int level = stream_level(bytes);
+  int best = 0;
+  ((best = LEVELS <= level ? LEVELS : best), ...);
+  ((best == LEVELS ? go(std::integral_constant<int, LEVELS>{}) : void()), ...);
+}
+
 template <typename F>
 void for_dtype(int dtype, F go) {
   if (dtype == FM_DTYPE_BF16) go(uint16_t{});
@@ -547,8 +570,10 @@ int fm_act8_compress(const void* x, int x_dtype, int64_t rows, int64_t cols, int
   const CompressArgs a{x, ld_x, static_cast<uint8_t*>(q), ld_q, static_cast<uint8_t*>(codes), ld_c, tile_valid};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   for_dtype(x_dtype, [&](auto t) {
-    for_items<4>(rows, cols, [&](const Items& items, auto u, unsigned wgs) {
-      hipLaunchKernelGGL((compress_kernel<decltype(t), decltype(u)::value>), dim3(wgs), dim3(256), 0, s, items, a);
+    for_stream<0, 2>(rows * cols * int64_t(sizeof(t)), [&](auto stream_) {
+      for_items<4>(rows, cols, [&](const Items& items, auto u, unsigned wgs) {
+        hipLaunchKernelGGL((compress_kernel<decltype(t), decltype(u)::value, decltype(stream_)::value>), dim3(wgs), dim3(256), 0, s, items, a);
+      });
     });
   });
   return check_launch("fm_act8_compress");
@@ -565,9 +590,13 @@ int fm_act8_restore(const void* q, int64_t ld_q, const void* codes, int64_t ld_c
   const RestoreArgs a{Act8{static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(codes), ld_q, ld_c}, index, src_rows, out, ld_out};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   for_dtype(out_dtype, [&](auto t) {
-    for_items<4>(rows, cols, [&](const Items& items, auto u, unsigned wgs) {
-      if (index) hipLaunchKernelGGL((restore_kernel<decltype(t), decltype(u)::value, true>), dim3(wgs), dim3(256), 0, s, items, a);
-      else hipLaunchKernelGGL((restore_kernel<decltype(t), decltype(u)::value, false>), dim3(wgs), dim3(256), 0, s, items, a);
+    for_stream<0, 1>(rows * cols * int64_t(sizeof(t)), [&](auto stream_) {
+      constexpr int kStream = decltype(stream_)::value;
+      for_items<4>(rows, cols, [&](const Items& items, auto u, unsigned wgs) {
+        constexpr int U = decltype(u)::value;
+        if (index) hipLaunchKernelGGL((restore_kernel<decltype(t), U, true, kStream>), dim3(wgs), dim3(256), 0, s, items, a);
+        else hipLaunchKernelGGL((restore_kernel<decltype(t), U, false, kStream>), dim3(wgs), dim3(256), 0, s, items, a);
+      });
     });
   });
   return check_launch("fm_act8_restore");
@@ -584,8 +613,10 @@ int fm_act8_swiglu(const void* g, int64_t ld_g, const void* u, int64_t ld_u, int
                      static_cast<uint8_t*>(cu), ld_q, ld_c};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   for_dtype(dtype, [&](auto t) {
-    for_items<2>(rows, H, [&](const Items& items, auto n, unsigned wgs) {
-      hipLaunchKernelGGL((swiglu_kernel<decltype(t), decltype(n)::value>), dim3(wgs), dim3(256), 0, s, items, a);
+    for_stream<0, 1>(rows * H * int64_t(sizeof(t)), [&](auto stream_) {
+      for_items<2>(rows, H, [&](const Items& items, auto n, unsigned wgs) {
+        hipLaunchKernelGGL((swiglu_kernel<decltype(t), decltype(n)::value, decltype(stream_)::value>), dim3(wgs), dim3(256), 0, s, items, a);
+      });
     });
   });
   return check_launch("fm_act8_swiglu");
@@ -602,8 +633,11 @@ int fm_act8_swiglu_backward(const void* dh, int64_t ld_dh, int dtype, int64_t ro
                         Act8{static_cast<const uint8_t*>(qu), static_cast<const uint8_t*>(cu), ld_q, ld_c}, dg, du, ld_dg, ld_du};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   for_dtype(dtype, [&](auto t) {
-    for_items<2>(rows, H, [&](const Items& items, auto n, unsigned wgs) {
-      hipLaunchKernelGGL((swiglu_backward_kernel<decltype(t), decltype(n)::value>), dim3(wgs), dim3(256), 0, s, items, a);
+    for_stream<0, 1, 2>(rows * H * int64_t(sizeof(t)), [&](auto stream_) {
+      for_items<2>(rows, H, [&](const Items& items, auto n, unsigned wgs) {
+        hipLaunchKernelGGL((swiglu_backward_kernel<decltype(t), decltype(n)::value, decltype(stream_)::value>), dim3(wgs), dim3(256), 0, s,
+                           items, a);
+      });
     });
   });
   return check_launch("fm_act8_swiglu_backward");
@@ -622,8 +656,10 @@ int fm_act8_rmsnorm(const void* x, int dtype, int64_t ld_x, int64_t T, int64_t D
     for_dtype(w_dtype, [&](auto wt) {
       for_norm(D, [&](auto nc, auto one, auto tail) {
         constexpr bool kOne = decltype(one)::value;
-        hipLaunchKernelGGL((norm_kernel<decltype(t), decltype(wt), decltype(nc)::value, kOne, decltype(tail)::value>),
-                           dim3(unsigned(kOne ? (T + 3) / 4 : T)), dim3(kOne ? 256 : 64 * norm_waves(D)), 0, s, a);
+        for_stream<0, 1>(T * D * int64_t(sizeof(t)), [&](auto stream_) {
+          hipLaunchKernelGGL((norm_kernel<decltype(t), decltype(wt), decltype(nc)::value, kOne, decltype(tail)::value, decltype(stream_)::value>),
+                             dim3(unsigned(kOne ? (T + 3) / 4 : T)), dim3(kOne ? 256 : 64 * norm_waves(D)), 0, s, a);
+        });
       });
     });
   });
@@ -654,8 +690,11 @@ int fm_act8_rmsnorm_backward(const void* dy, int64_t ld_dy, int dtype, int64_t T
     for_dtype(w_dtype, [&](auto wt) {
       for_norm(D, [&](auto nc, auto one, auto tail) {
         constexpr bool kOne = decltype(one)::value;
-        hipLaunchKernelGGL((norm_backward_kernel<decltype(t), decltype(wt), decltype(nc)::value, kOne, decltype(tail)::value>),
-                           dim3(unsigned(slices)), dim3(kOne ? 256 : 64 * norm_waves(D)), 0, s, a);
+        for_stream<0, 1, 2>(T * D * int64_t(sizeof(t)), [&](auto stream_) {
+          hipLaunchKernelGGL((norm_backward_kernel<decltype(t), decltype(wt), decltype(nc)::value, kOne, decltype(tail)::value,
+                                                   decltype(stream_)::value>),
+                             dim3(unsigned(slices)), dim3(kOne ? 256 : 64 * norm_waves(D)), 0, s, a);
+        });
       });
     });
   });
