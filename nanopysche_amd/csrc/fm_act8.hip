@@ -534,7 +534,7 @@ int norm_waves(int64_t D) { return int((D + 1023) / 1024); }
 int64_t norm_rows_per_slice(int64_t T, int64_t D) {
   const int w = D <= 512 ? 4 : norm_waves(D), rows = D <= 512 ? 4 : 1;
   int64_t most = int64_t(device_cus()) * (16 / w);
-  most = most < 1024 ? most : 1024;
+  most = most < 512 ? most : 512;
   const int64_t r = (T + most - 1) / most;
   return (r + rows - 1) / rows * rows;
 }
