@@ -727,7 +727,11 @@ int fm_act8_rmsnorm_backward(const void* dy, int64_t ld_dy, int dtype, int64_t T
 
 /* The expert block's operands from 8 bits, in the layouts and kinds of fm_permute, fm_swiglu_quantize and fm_swiglu_backward (either output
  * may be NULL): the rows of the tokens [T, D], h of the kept gate|up [rows, 2H], [dg | du] of it and dh [rows, H] (bf16); and
- * fm_router_weight_grad of kept expert outputs [rows, D]. */
+ * fm_router_weight_grad of kept expert outputs [rows, D].  fm_act8_swiglu_keep_quantize is the forward's fm_swiglu_quantize (rows a multiple
+ * of 128, row output only) that keeps its bf16 gate|up [rows, 2H] in the same pass. */
+int fm_act8_swiglu_keep_quantize(const void* gu, int64_t ld_gu, int64_t rows, int64_t H, void* q8, int64_t ld_q8, void* codes,
+                                 int64_t ld_c, int kind, void* q, int64_t ld_q, void* s, int64_t ld_s,
+                                 const int32_t* tile_valid, void* stream);
 int fm_act8_permute(const void* xq, int64_t ld_xq, const void* codes, int64_t ld_c, int64_t T, int64_t D,
                     const int32_t* assign_of_row, int64_t rows, int K, int kind, void* q, int64_t ld_q, void* s, int64_t ld_s,
                     void* qt, int64_t ld_qt, void* st, int64_t ld_st, const int32_t* tile_valid, void* stream);

@@ -191,6 +191,7 @@ SIGNATURES = {
                                         _i64, _vp]),
     "fm_act8_permute": (_i32, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i32, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp,
                                _i64, _vp, _vp]),
+    "fm_act8_swiglu_keep_quantize": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _i32, _vp, _i64, _vp, _i64, _vp, _vp]),
     "fm_act8_swiglu_quantize": (_i32, [_vp, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp,
                                        _vp]),
     "fm_act8_swiglu_backward_quantize": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _i64, _vp,

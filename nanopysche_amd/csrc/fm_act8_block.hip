@@ -1,5 +1,6 @@
 // The expert block's backward from activations in 8 bits (fm_act8.h): the operands of its grouped products, made from the
 // kept gate|up, tokens and expert outputs in the passes that the 16-bit ones take.
+//   fm_act8_swiglu_keep_quantize      the forward's h, as fm_swiglu_quantize, keeping gate|up on the way
 //   fm_act8_permute                   the tokens in expert order, as fm_permute
 //   fm_act8_swiglu_quantize           h = silu(g) u of the kept g and u, as fm_swiglu_quantize
 //   fm_act8_swiglu_backward_quantize  [dg | du], as fm_swiglu_backward
@@ -62,6 +63,40 @@ struct KeptSwigluSrc {
     float g[8], u[8];
     act_decode8(r.g, act_scale(r.gc), g);
     act_decode8(r.u, act_scale(r.uc), u);
+    swiglu8(g, u, v[0]);
+  }
+};
+
+// The forward: h of bf16 gate|up, which compute stores in 8 bits as well.  Row outputs only: the producer then computes every row
+// in range once, its quads of lanes together.
+struct KeepSwigluSrc {
+  static constexpr int kOut = 1;
+  const uint16_t* gu;   // bf16 [rows, ld]
+  int64_t ld, H;
+  uint8_t* q;
+  int64_t ld_q;
+  uint8_t* codes;
+  int64_t ld_c;
+  struct Raw {
+    uint4 g, u;
+    int64_t row, col;
+  };
+  __device__ __forceinline__ Raw fetch(int64_t row, int64_t col) const {
+    const uint16_t* p = gu + row * ld + col;
+    return Raw{*reinterpret_cast<const uint4*>(p), *reinterpret_cast<const uint4*>(p + H), row, col};
+  }
+  __device__ __forceinline__ void keep(const float (&v)[8], int64_t row, int64_t col) const {
+    uint32_t code;
+    const uint2 b = act_encode8(v, code);
+    st_global(q + row * ld_q + col, b);
+    if ((threadIdx.x & 3) == 0) st_global(codes + row * ld_c + (col >> 5), uint8_t(code));
+  }
+  __device__ __forceinline__ void compute(const Raw& r, float v[][8]) const {
+    float g[8], u[8];
+    unpack8_bf16(r.g, g);
+    unpack8_bf16(r.u, u);
+    keep(g, r.row, r.col);
+    keep(u, r.row, r.col + H);
     swiglu8(g, u, v[0]);
   }
 };
@@ -146,6 +181,18 @@ int fm_act8_permute(const void* xq, int64_t ld_xq, const void* codes, int64_t ld
   if (T == 0) return launch_tile_producer(NoTokensSrc{}, o, rows, D, static_cast<hipStream_t>(stream), "fm_act8_permute");
   return launch_tile_producer(KeptGatherSrc{kept_of(xq, ld_xq, codes, ld_c), assign_of_row, K}, o, rows, D,
                               static_cast<hipStream_t>(stream), "fm_act8_permute");
+}
+
+int fm_act8_swiglu_keep_quantize(const void* gu, int64_t ld_gu, int64_t rows, int64_t H, void* q8, int64_t ld_q8, void* codes, int64_t ld_c,
+                                 int kind, void* q, int64_t ld_q, void* s, int64_t ld_s, const int32_t* tile_valid, void* stream) {
+  FM_REQUIRE(H >= 128 && H % 128 == 0 && rows % 128 == 0, "fm_act8_swiglu_keep_quantize: H and rows must be multiples of 128");
+  FM_REQUIRE(rows == 0 || (gu && aligned16(gu) && ld_gu >= 2 * H && ld_gu % 8 == 0),
+             "fm_act8_swiglu_keep_quantize: gate|up must lie on 16 bytes, its pitch a multiple of 8");
+  FM_REQUIRE(rows == 0 || kept_ok(q8, ld_q8, codes, ld_c, 2 * H), "fm_act8_swiglu_keep_quantize: bad payload, codes or pitches");
+  const TileOut o = make_tile_out(kind, q, ld_q, s, ld_s, nullptr, 0, nullptr, 0, 0, 0, tile_valid);
+  return launch_tile_producer(KeepSwigluSrc{static_cast<const uint16_t*>(gu), ld_gu, H, static_cast<uint8_t*>(q8), ld_q8,
+                                            static_cast<uint8_t*>(codes), ld_c},
+                              o, rows, H, static_cast<hipStream_t>(stream), "fm_act8_swiglu_keep_quantize");
 }
 
 int fm_act8_swiglu_quantize(const void* gu, int64_t ld_gu, const void* codes, int64_t ld_c, int64_t rows, int64_t H, int kind, void* q,

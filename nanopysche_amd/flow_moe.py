@@ -24,7 +24,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .act8 import Activation8, _compress
+from .act8 import Activation8, _compress, _empty
 from .recipes import BlockScalingGranularity, FP8RecipeConfig, FP8RecipeType
 from .routing import PAD_ROWS, RouterDotInputs, RoutingPlan, route_tokens
 
@@ -1289,6 +1289,7 @@ class FP8FlowMoECompute:
             _gemm_m(kind, rows, ew.w13, plan, GU, mask, want)
             saved[kind] = (cols, ew)
         h_cols = {}
+        GU8 = _empty(GU.shape, R, torch.bfloat16, dev) if keep8 else None   # rows of tiles past the last group hold nothing
         for kind, want in ((fp8_kind, 1), (_lib.QUANT_BF16 if use_bf16 else None, 0)):
             if kind is None:
                 continue
@@ -1296,8 +1297,13 @@ class FP8FlowMoECompute:
             hrow, h_cols[kind], args = _alloc_act(R, H, kind, cols_now, dev, self._paired(kind),
                                                   pcols.get(kind, False))
             gu = GU.data_ptr()   # gate columns, then up columns (bf16)
-            _lib.call("fm_swiglu_quantize", gu, 2 * H, gu + 2 * H, 2 * H, R, H, *args,
-                      _lib.ptr(tiles.get(kind, plan.tile_expert)), _lib.stream_of(GU))
+            valid = _lib.ptr(tiles.get(kind, plan.tile_expert))
+            if keep8:
+                q, codes, ld_q, ld_c = GU8.at()
+                _lib.call("fm_act8_swiglu_keep_quantize", gu, 2 * H, R, H, q, ld_q, codes, ld_c, *args[:5], valid,
+                          _lib.stream_of(GU))
+            else:
+                _lib.call("fm_swiglu_quantize", gu, 2 * H, gu + 2 * H, 2 * H, R, H, *args, valid, _lib.stream_of(GU))
             _gemm_m(kind, hrow, saved[kind][1].w2t, plan, Y, mask, want)
         if self._dense:
             # the output must not be a view made inside this Function (callers
@@ -1326,10 +1332,8 @@ class FP8FlowMoECompute:
         keep_y = ctx.needs_input_grad[1]
         ctx.keep8 = keep8
         if keep8:
-            # rows of tiles past the last group hold nothing
-            GU8 = _compress(GU, GU.shape, plan.tile_expert).data
             Y8 = _compress(Y, Y.shape, plan.tile_expert).data if keep_y else None
-            ctx.save_for_backward(wts, GU8, Y8, _compress(x, x.shape).data)
+            ctx.save_for_backward(wts, GU8.data, Y8, _compress(x, x.shape).data)
         else:
             ctx.save_for_backward(wts, GU, Y if keep_y else None)
         return out if ctx.x_dtype == torch.bfloat16 else out.to(ctx.x_dtype)
