@@ -751,7 +751,7 @@ int fm_act8_router_weight_grad(const void* dout, int64_t ld_do, const void* y, i
  *   + z_mult mean_t logsumexp(l_t)^2; S': sequences with n_s > 0; p = softmax(l), or (sigmoid) sigma / (sum sigma + 1e-8).
  * Sequence s is tokens [cu[s], cu[s + 1]) (ascending int32 in [0, T]; null: one sequence of all), of which those count whose mask
  * byte is not 0 (null: all).  The logits [T, E] fp32 of others may hold anything, indices [T, K] outside [0, E) fill no slot.
- * E up to 1024.
+ * E up to 1024, S below 2^20.
  * fm_balance_forward: f [S, E] = E slots / n_s^2 and inverse [2] = {1 / S', 1 / N} for the backward, counts [S, E], loss; acc [E] and
  *   acc_total [1] (int64 or null) are raised by the counts and the tokens that count.  Workspace on 16 bytes.
  * fm_balance_backward: dlogits [T, E] = dloss times the gradient, zeros for tokens that do not count (add: added to what

@@ -23,7 +23,7 @@ from . import _lib
 
 MAX_BALANCE_EXPERTS = 1024
 MAX_BALANCE_TOP_K = 1024
-MAX_SEQUENCES = 2 ** 24 - 1
+MAX_SEQUENCES = 2 ** 20 - 1
 
 
 class BalanceOutput(NamedTuple):
@@ -130,6 +130,8 @@ def balance_backward(state: BalanceState, dloss: torch.Tensor, add_to: Optional[
     l2, cu = state.logits, state.cu_seqlens
     T, E = l2.shape
     S = 1 if cu is None else cu.numel() - 1
+    if state.f.numel() != S * E + 2 or (state.mask is not None and state.mask.numel() != T):
+        raise ValueError(f"the state's f and mask do not fit {T} tokens, {E} experts and {S} sequences")
     if dloss.dtype != torch.float32 or dloss.numel() != 1:
         raise TypeError(f"dloss must be one float32 value, got {dloss.dtype} {tuple(dloss.shape)}")
     for name, t in (("dloss", dloss), ("add_to", add_to)):

@@ -650,19 +650,26 @@ int fm_act8_rmsnorm(const void* x, int dtype, int64_t ld_x, int64_t T, int64_t D
   if (T == 0) return 0;
   FM_REQUIRE(x && w && y && rstd && ld_x >= 0 && ld_y >= D, "fm_act8_rmsnorm: null pointer or bad pitch");
   FM_REQUIRE(kept_ok(q, ld_q, codes, ld_c, D) && ld_q == (D + 31) / 32 * 32, "fm_act8_rmsnorm: bad payload, codes or pitches");
-  const NormArgs a{x, ld_x, T, int(D), w, eps, y, ld_y, static_cast<uint8_t*>(q), ld_q, static_cast<uint8_t*>(codes), ld_c, rstd};
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  for_dtype(dtype, [&](auto t) {
-    for_dtype(w_dtype, [&](auto wt) {
-      for_norm(D, [&](auto nc, auto one, auto tail) {
-        constexpr bool kOne = decltype(one)::value;
-        for_stream<0, 1>(T * D * int64_t(sizeof(t)), [&](auto stream_) {
-          hipLaunchKernelGGL((norm_kernel<decltype(t), decltype(wt), decltype(nc)::value, kOne, decltype(tail)::value, decltype(stream_)::value>),
-                             dim3(unsigned(kOne ? (T + 3) / 4 : T)), dim3(kOne ? 256 : 64 * norm_waves(D)), 0, s, a);
+  // a launch has fewer than 2^32 threads
+  const int64_t each = D <= 512 ? 64 : 64 * norm_waves(D), run = (int64_t(1) << 31) / each;
+  for (int64_t r = 0; r < T; r += run) {
+    const int64_t n = T - r < run ? T - r : run;
+    for_dtype(dtype, [&](auto t) {
+      const NormArgs a{static_cast<const decltype(t)*>(x) + r * ld_x, ld_x, n, int(D), w, eps, static_cast<decltype(t)*>(y) + r * ld_y, ld_y,
+                       static_cast<uint8_t*>(q) + r * ld_q, ld_q, static_cast<uint8_t*>(codes) + r * ld_c, ld_c, rstd + r};
+      for_dtype(w_dtype, [&](auto wt) {
+        for_norm(D, [&](auto nc, auto one, auto tail) {
+          constexpr bool kOne = decltype(one)::value;
+          for_stream<0, 1>(T * D * int64_t(sizeof(t)), [&](auto stream_) {
+            hipLaunchKernelGGL((norm_kernel<decltype(t), decltype(wt), decltype(nc)::value, kOne, decltype(tail)::value,
+                                            decltype(stream_)::value>),
+                               dim3(unsigned(kOne ? (n + 3) / 4 : n)), dim3(kOne ? 256 : 64 * norm_waves(D)), 0, s, a);
+          });
         });
       });
     });
-  });
+  }
   return check_launch("fm_act8_rmsnorm");
 }
 

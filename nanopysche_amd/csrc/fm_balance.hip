@@ -25,6 +25,7 @@ namespace fm {
 namespace {
 
 constexpr int kMaxExperts = 1024;
+constexpr int64_t kMaxSequences = int64_t(1) << 20;   // 64 column groups of 64 threads each stay below 2^32 threads
 constexpr float kSumFloor = 1e-8f;
 
 typedef float f32x4_el __attribute__((ext_vector_type(4), aligned(4)));
@@ -698,7 +699,7 @@ Space space_of(int64_t T, int E, int64_t S) {
 int check_balance(const BalanceArgs& a, const char* what) {
   FM_REQUIRE(a.T >= 0 && a.T < (int64_t(1) << 31), "%s: T must be below 2^31", what);
   FM_REQUIRE(a.E >= 1 && a.E <= kMaxExperts, "%s: E must be 1 to %d (got %d)", what, kMaxExperts, a.E);
-  FM_REQUIRE(a.S >= 0 && a.S < (int64_t(1) << 24), "%s: fewer than 2^24 sequences", what);
+  FM_REQUIRE(a.S >= 0 && a.S < kMaxSequences, "%s: fewer than 2^20 sequences", what);
   FM_REQUIRE(a.cu || a.S == 1, "%s: without borders there is one sequence", what);
   FM_REQUIRE(a.T == 0 || (a.logits && a.ld >= a.E), "%s: null logits or a pitch below E", what);
   return 0;

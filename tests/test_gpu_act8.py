@@ -319,6 +319,24 @@ def test_rmsnorm_strides_and_empty(dev):
     assert torch.equal(y, zero) and close(gx, torch.full_like(zero, 1e3).double(), times=16)   # 1 / sqrt(1e-6)
 
 
+def test_rmsnorm_of_more_rows_than_a_launch_takes(dev):
+    """Four rows to a workgroup of 256: 2^25 rows a launch; rows repeat, so a few stand for all."""
+    rows = activation(gen(15), 1000, 8)
+    T = 2 ** 25 + 4000
+    x = rows.repeat((T + 999) // 1000, 1)[:T]
+    w = torch.rand(8, generator=gen(16), device="cuda")
+    y, k, r = fm.rmsnorm_compress(x, w)
+    ys, ks, rs = fm.rmsnorm_compress(rows, w)
+    gx, gw = fm.rmsnorm_backward_8bit(x, k, w, r)
+    gs, _ = fm.rmsnorm_backward_8bit(rows, ks, w, rs)
+    whole = T // 1000
+    for got, one in ((y, ys), (gx, gs), (r[:, None], rs[:, None]), (k.restore(), ks.restore())):
+        assert torch.equal(got[:whole * 1000].view(whole, 1000, -1), one.expand(whole, 1000, -1))
+        assert torch.equal(got[whole * 1000:], one[:T - whole * 1000])
+    ref = (rows.double() * kept(rows.double()) * rs.double()[:, None]).sum(0) * (T / 1000)
+    assert torch.all((gw.double() - ref).abs() <= 1e-3 * ref.abs().max())   # 65,000 rows a slice, one after the other, in fp32: 2^-24 sqrt of them
+
+
 def test_rmsnorm_module(dev):
     x = activation(gen(13), 20, 1536)
     a, b = x.clone().requires_grad_(True), x.clone().requires_grad_(True)

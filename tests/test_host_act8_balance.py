@@ -147,6 +147,7 @@ def logits(T=6, E=4):
     (TypeError, "int32", dict(cu_seqlens=torch.zeros(2, dtype=torch.int64))),
     (ValueError, "cu_seqlens must be", dict(cu_seqlens=torch.zeros(2, 1, dtype=torch.int32))),
     (ValueError, "cu_seqlens must be", dict(cu_seqlens=torch.zeros(0, dtype=torch.int32))),
+    (ValueError, "cu_seqlens must be", dict(cu_seqlens=torch.zeros(2 ** 20 + 1, dtype=torch.int32))),
     (TypeError, "bool", dict(token_mask=torch.ones(6))),
     (ValueError, "token_mask must be", dict(token_mask=torch.ones(5, dtype=torch.bool))),
     (ValueError, "scores", dict(scores="relu")),
@@ -169,6 +170,12 @@ def test_balance_backward_refuses(launched):  # noqa: F811
     for bad in (torch.zeros(6, 5), torch.zeros(6, 4, dtype=BF), torch.zeros(4, 6).t(), torch.zeros(1, 4).expand(6, 4)):
         with pytest.raises(ValueError, match="add_to"):
             fm.balance_backward(state, torch.zeros(()), add_to=bad)
+    short = fm.BalanceState(l, None, None, torch.zeros(5), False, 0.0, l.shape)
+    masked = fm.BalanceState(l, None, torch.ones(5, dtype=torch.bool), torch.zeros(6), False, 0.0, l.shape)
+    borders = fm.BalanceState(l, torch.zeros(3, dtype=torch.int32), None, torch.zeros(6), False, 0.0, l.shape)
+    for state in (short, masked, borders):
+        with pytest.raises(ValueError, match="do not fit"):
+            fm.balance_backward(state, torch.zeros(()))
     assert launched == []
 
 
@@ -196,4 +203,10 @@ def test_the_library_refuses_before_a_launch():
     bad(b"workspace", lib.fm_balance_forward(p, 8, 100, 8, p, 1, 2, p, 3, None, 0, 0.0, p, p, p, p, None, None, p, need - 1, None))
     bad(b"one sequence", lib.fm_balance_forward(p, 8, 100, 8, p, 1, 2, None, 3, None, 0, 0.0, p, p, p, p, None, None, p, need, None))
     bad(b"E must be", lib.fm_balance_forward(p, 8, 100, 1025, p, 1, 2, p, 3, None, 0, 0.0, p, p, p, p, None, None, p, need, None))
+    bad(b"sequences", lib.fm_balance_forward(p, 8, 100, 8, p, 1, 2, p, 1 << 20, None, 0, 0.0, p, p, p, p, None, None, p, 1 << 40, None))
+    bad(b"multiples of 128", lib.fm_act8_swiglu_keep_quantize(p, 256, 100, 128, p, 256, p, 8, 0, p, 128, None, 0, None, None))
+    bad(b"payload", lib.fm_act8_permute(p, 256, None, 8, 4, 256, p, 128, 2, 0, p, 256, None, 0, None, 0, None, 0, None, None))
+    bad(b"H must be", lib.fm_act8_swiglu_quantize(p, 64, p, 2, 128, 32, 0, p, 32, None, 0, None, 0, None, 0, None, None))
+    bad(b"16 bytes", lib.fm_act8_swiglu_backward_quantize(p, 256, p, 8, C.c_void_p(264), 128, 128, 128, 0, p, 256, None, 0, None, 0, None, 0, None, None))
+    bad(b"16 bytes", lib.fm_act8_router_weight_grad(p, 100, p, 128, p, 4, p, 4, 2, 128, p, None))
     bad(b"pitch", lib.fm_balance_backward(p, 8, 100, 8, p, 3, None, 0, 0.0, p, p, p, p, 7, 0, None))
