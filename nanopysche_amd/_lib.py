@@ -284,6 +284,16 @@ def on_device_of(t: torch.Tensor):
 _HERE = contextlib.nullcontext()
 
 
+def call_on(t: torch.Tensor, name: str, *args) -> None:
+    """``call`` with t's current stream as the last argument, where t's device is the current one."""
+    index = t.get_device()
+    if index >= 0 and torch._C._cuda_getDevice() == index:
+        call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with on_device_of(t):
+            call(name, *args, stream_of(t))
+
+
 def ptr(t) -> C.c_void_p:
     return C.c_void_p(0 if t is None else t.data_ptr())
 

@@ -150,7 +150,7 @@ def _empty(shape: torch.Size, rows: int, dtype, dev) -> Activation8:
 
 def _like(x: torch.Tensor) -> torch.Tensor:
     """An empty contiguous tensor like x."""
-    return torch.empty_like(x, memory_format=torch.contiguous_format)
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
 def _here(index: int, what: str, t: torch.Tensor) -> None:
@@ -174,9 +174,8 @@ def _restore(t: Activation8, index, rows, shape, dtype) -> torch.Tensor:
     out = torch.empty(shape, dtype=dtype, device=t.device)
     if out.numel():
         q, codes, ld_q, ld_c = t.at()
-        with _lib.on_device_of(out):
-            _lib.call("fm_act8_restore", q, ld_q, codes, ld_c, t.rows, t.cols, _lib.addr(index), rows, out.data_ptr(), code,
-                      t.cols, _lib.stream_of(out))
+        src_rows, cols, _ = t._sizes
+        _lib.call_on(out, "fm_act8_restore", q, ld_q, codes, ld_c, src_rows, cols, _lib.addr(index), rows, out.data_ptr(), code, cols)
     return out
 
 
@@ -185,9 +184,8 @@ def _compress(x2: torch.Tensor, shape, tile_valid=None) -> Activation8:
     t = _empty(shape, rows, x2.dtype, x2.device)
     if rows:
         q, codes, ld_q, ld_c = t.at()
-        with _lib.on_device_of(x2):
-            _lib.call("fm_act8_compress", x2.data_ptr(), _DTYPES[x2.dtype], rows, cols, x2.stride(0), q, ld_q, codes, ld_c,
-                      _lib.addr(tile_valid), _lib.stream_of(x2))
+        _lib.call_on(x2, "fm_act8_compress", x2.data_ptr(), _DTYPES[x2.dtype], rows, cols, x2.stride(0), q, ld_q, codes, ld_c,
+                     _lib.addr(tile_valid))
     return t
 
 
@@ -213,7 +211,7 @@ def _halves(gate: torch.Tensor, up: Optional[torch.Tensor]):
         H, odd = divmod(g2.shape[1], 2)
         if odd:
             raise ValueError(f"gate|up must have an even number of columns, got {gate.shape[-1]}")
-        return g2, g2, g2.data_ptr() + H * g2.element_size(), torch.Size((*gate.shape[:-1], H))
+        return g2, g2, g2.data_ptr() + H * g2.element_size(), gate.shape[:-1] + (H,)
     if up.shape != gate.shape or up.dtype != gate.dtype:
         raise ValueError(f"gate and up must be alike, got {tuple(gate.shape)} {gate.dtype} and {tuple(up.shape)} {up.dtype}")
     g2, u2 = _rows(gate, "gate"), _rows(up, "up")
@@ -231,9 +229,8 @@ def swiglu_compress(gate: torch.Tensor, up: Optional[torch.Tensor] = None) -> Sw
     if rows:
         qg, cg, ld_q, ld_c = kept_g.at()
         qu, cu, _, _ = kept_u.at()
-        with _lib.on_device_of(g2):
-            _lib.call("fm_act8_swiglu", g2.data_ptr(), g2.stride(0), at_u, u2.stride(0), _DTYPES[dtype], rows, H,
-                      h.data_ptr(), H, qg, cg, qu, cu, ld_q, ld_c, _lib.stream_of(g2))
+        _lib.call_on(g2, "fm_act8_swiglu", g2.data_ptr(), g2.stride(0), at_u, u2.stride(0), _DTYPES[dtype], rows, H, h.data_ptr(), H,
+                     qg, cg, qu, cu, ld_q, ld_c)
     return SwigluKept(h, kept_g, kept_u)
 
 
@@ -248,7 +245,7 @@ def swiglu_backward_8bit(dh: torch.Tensor, gate: Activation8, up: Activation8, p
     _here(index, "up", up._data)
     rows, H = d2.shape
     if packed:
-        both = torch.empty((*dh.shape[:-1], 2 * H), dtype=dh.dtype, device=dh.device)
+        both = torch.empty(dh.shape[:-1] + (2 * H,), dtype=dh.dtype, device=dh.device)
         at_g, at_u, ld = both.data_ptr(), both.data_ptr() + H * both.element_size(), 2 * H
     else:
         dg, du = _like(dh), _like(dh)
@@ -256,9 +253,8 @@ def swiglu_backward_8bit(dh: torch.Tensor, gate: Activation8, up: Activation8, p
     if rows:
         qg, cg, ld_q, ld_c = gate.at()
         qu, cu, _, _ = up.at()
-        with _lib.on_device_of(d2):
-            _lib.call("fm_act8_swiglu_backward", d2.data_ptr(), d2.stride(0), _DTYPES[d2.dtype], rows, H, qg, cg, qu, cu, ld_q, ld_c,
-                      at_g, ld, at_u, ld, _lib.stream_of(d2))
+        _lib.call_on(d2, "fm_act8_swiglu_backward", d2.data_ptr(), d2.stride(0), _DTYPES[d2.dtype], rows, H, qg, cg, qu, cu, ld_q, ld_c,
+                     at_g, ld, at_u, ld)
     return both if packed else (dg, du)
 
 
@@ -295,7 +291,7 @@ class RMSNormKept(NamedTuple):
 
 def _norm_weight(weight: torch.Tensor, D: int) -> torch.Tensor:
     _dtype(weight.dtype, "weight")
-    if tuple(weight.shape) != (D,):
+    if weight.dim() != 1 or weight.numel() != D:
         raise ValueError(f"weight must be [{D}], got {tuple(weight.shape)}")
     return weight if weight.is_contiguous() else weight.contiguous()
 
@@ -313,9 +309,8 @@ def rmsnorm_compress(x: torch.Tensor, weight: torch.Tensor, eps: float = DEFAULT
     kept = _empty(x.shape, T, x.dtype, dev)
     if T:
         q, codes, ld_q, ld_c = kept.at()
-        with _lib.on_device_of(x2):
-            _lib.call("fm_act8_rmsnorm", x2.data_ptr(), _DTYPES[x2.dtype], x2.stride(0), T, D, w.data_ptr(), _DTYPES[w.dtype], float(eps),
-                      y.data_ptr(), D, q, ld_q, codes, ld_c, rstd.data_ptr(), _lib.stream_of(x2))
+        _lib.call_on(x2, "fm_act8_rmsnorm", x2.data_ptr(), _DTYPES[x2.dtype], x2.stride(0), T, D, w.data_ptr(), _DTYPES[w.dtype], eps,
+                     y.data_ptr(), D, q, ld_q, codes, ld_c, rstd.data_ptr())
     return RMSNormKept(y, kept, rstd)
 
 
@@ -343,9 +338,8 @@ def rmsnorm_backward_8bit(dy: torch.Tensor, x: Activation8, weight: torch.Tensor
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dy.device)
     if T:
         q, codes, ld_q, ld_c = x.at()
-        with _lib.on_device_of(d2):
-            _lib.call("fm_act8_rmsnorm_backward", d2.data_ptr(), d2.stride(0), _DTYPES[d2.dtype], T, D, q, ld_q, codes, ld_c, w.data_ptr(),
-                      _DTYPES[w.dtype], rstd.data_ptr(), dx.data_ptr(), D, _lib.addr(dw), _lib.addr(ws), nbytes, _lib.stream_of(d2))
+        _lib.call_on(d2, "fm_act8_rmsnorm_backward", d2.data_ptr(), d2.stride(0), _DTYPES[d2.dtype], T, D, q, ld_q, codes, ld_c, w.data_ptr(),
+                     _DTYPES[w.dtype], rstd.data_ptr(), dx.data_ptr(), D, _lib.addr(dw), _lib.addr(ws), nbytes)
     return dx, dw
 
 

@@ -115,12 +115,12 @@ def balance_forward(logits: torch.Tensor, indices: torch.Tensor, *, cu_seqlens: 
     f = torch.empty(S * E + 2, dtype=torch.float32, device=dev)
     loss = torch.empty((), dtype=torch.float32, device=dev)
     counts = torch.empty(E if cu is None else (S, E), dtype=torch.int32, device=dev)
-    ws = torch.empty(_lib.size_of("fm_balance_workspace_bytes", T, E, S), dtype=torch.uint8, device=dev)
+    nbytes = _lib.size_of("fm_balance_workspace_bytes", T, E, S)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     acc, total = (None, None) if load_tracker is None else (load_tracker.tokens_per_expert, load_tracker.total_tokens)
-    with _lib.on_device_of(l2):
-        _lib.call("fm_balance_forward", l2.data_ptr(), l2.stride(0) if T > 1 else E, T, E, idx.data_ptr(), int(idx.dtype == torch.int64),
-                  idx.shape[1], _lib.addr(cu), S, _lib.addr(mask), int(sigmoid), z, f.data_ptr(), counts.data_ptr(), f.data_ptr() + 4 * S * E,
-                  loss.data_ptr(), _lib.addr(acc), _lib.addr(total), ws.data_ptr(), ws.numel(), _lib.stream_of(l2))
+    _lib.call_on(l2, "fm_balance_forward", l2.data_ptr(), l2.stride(0) if T > 1 else E, T, E, idx.data_ptr(), int(idx.dtype == torch.int64),
+                 idx.shape[1], _lib.addr(cu), S, _lib.addr(mask), int(sigmoid), z, f.data_ptr(), counts.data_ptr(), f.data_ptr() + 4 * S * E,
+                 loss.data_ptr(), _lib.addr(acc), _lib.addr(total), ws.data_ptr(), nbytes)
     return loss, counts, BalanceState(l2, cu, mask, f, sigmoid, z, logits.shape)
 
 
@@ -146,11 +146,9 @@ def balance_backward(state: BalanceState, dloss: torch.Tensor, add_to: Optional[
             raise ValueError(f"add_to must be a float32 [{T}, {E}] of rows, got {add_to.dtype} {tuple(add_to.shape)} of strides {add_to.stride()}")
         out, ld = add_to, add_to.stride(0) if T > 1 else E
     if T:
-        with _lib.on_device_of(l2):
-            _lib.call("fm_balance_backward", l2.data_ptr(), l2.stride(0) if T > 1 else E, T, E, _lib.addr(cu),
-                      S, _lib.addr(state.mask), int(state.sigmoid), state.z_mult,
-                      state.f.data_ptr(), state.f.data_ptr() + 4 * S * E, dloss.data_ptr(), out.data_ptr(), ld, int(add_to is not None),
-                      _lib.stream_of(l2))
+        _lib.call_on(l2, "fm_balance_backward", l2.data_ptr(), l2.stride(0) if T > 1 else E, T, E, _lib.addr(cu), S, _lib.addr(state.mask),
+                     int(state.sigmoid), state.z_mult, state.f.data_ptr(), state.f.data_ptr() + 4 * S * E, dloss.data_ptr(), out.data_ptr(),
+                     ld, int(add_to is not None))
     return out
 
 
