@@ -25,7 +25,7 @@ namespace fm {
 namespace {
 
 constexpr int kMaxExperts = 1024;
-constexpr int64_t kMaxSequences = int64_t(1) << 20;   // 64 column groups of 64 threads each stay below 2^32 threads
+constexpr int64_t kMaxSequences = int64_t(1) << 20;   // 64 column groups of a wave each stay below 2^32 threads
 constexpr float kSumFloor = 1e-8f;
 
 typedef float f32x4_el __attribute__((ext_vector_type(4), aligned(4)));
@@ -38,6 +38,12 @@ __device__ __forceinline__ float exp_below(float d) {
   const float h = d * kL;
   const float e = __builtin_amdgcn_exp2f(h);
   return fmaf(e, fmaf(d, kLlo, fmaf(d, kL, -h)) * kLn2, e);
+}
+
+// 1 / d of a normal d to about an ulp.
+__device__ __forceinline__ float reciprocal(float d) {
+  const float r = __builtin_amdgcn_rcpf(d);
+  return fmaf(fmaf(-d, r, 1.f), r, r);
 }
 
 struct BalanceArgs {
@@ -127,11 +133,9 @@ struct Row {
       }
     }
   }
-  // softmax in place; the log of the sum of exponentials
-  __device__ __forceinline__ float softmax(int E, int l) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (column(l, i) >= E) v[i] = -INFINITY;
+  // Columns behind the last expert hold -infinity: exponentials and sigmoids of 0.
+  // softmax in place; the log of the sum of exponentials, where wanted
+  __device__ __forceinline__ float softmax(bool want_log) {
     float m = v[0], s = 0.f;
 #pragma unroll
     for (int i = 1; i < NV; ++i) m = fmaxf(m, v[i]);
@@ -142,22 +146,21 @@ struct Row {
       s += v[i];
     }
     s = group_sum<L>(s);
-    const float r = 1.f / s;
+    const float r = reciprocal(s);
 #pragma unroll
     for (int i = 0; i < NV; ++i) v[i] *= r;
-    return m + logf(s);
+    return want_log ? m + logf(s) : 0.f;
   }
-  // sigmoids in place (0 behind the last expert): 1 or e^-|l| over 1 + e^-|l|; 1 / (their sum + floor)
-  __device__ __forceinline__ float sigmoids(int E, int l) {
+  // sigmoids in place: 1 or e^-|l| over 1 + e^-|l|; 1 / (their sum + floor)
+  __device__ __forceinline__ float sigmoids() {
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const float e = exp_below(-fabsf(v[i]));
       v[i] = (v[i] < 0.f ? e : 1.f) * __builtin_amdgcn_rcpf(1.f + e);
-      if (column(l, i) >= E) v[i] = 0.f;
       s += v[i];
     }
-    return 1.f / (group_sum<L>(s) + kSumFloor);
+    return reciprocal(group_sum<L>(s) + kSumFloor);
   }
 };
 
@@ -197,7 +200,7 @@ __device__ __forceinline__ void sum_piece(const BalanceArgs& a, int64_t p, int32
   int count = 0;
 #pragma unroll
   for (int i = 0; i < NV; ++i) acc[i] = 0.f;
-  // the next steps' logits come in while these are summed; those that do not count are zeros
+  // the next steps' logits come in while these are summed
   R next[kAhead];
   bool use[kAhead];
   auto fetch = [&](int64_t t) {
@@ -215,27 +218,29 @@ __device__ __forceinline__ void sum_piece(const BalanceArgs& a, int64_t p, int32
     bool in[kAhead];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
+      row[k] = next[k];
       in[k] = use[k];
-#pragma unroll
-      for (int i = 0; i < NV; ++i) row[k].v[i] = in[k] ? next[k].v[i] : 0.f;
     }
     t += TEAM * kSide * kAhead;
     if (t < hi) fetch(t);
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const float one = in[k] ? 1.f : 0.f;
-      float lse = 0.f, r = one;
+    for (int k = 0; k < kAhead; ++k) {   // what does not count may be a NaN: it is left out by a select
       R p = row[k];
-      if (a.sigmoid) {
-        r = p.sigmoids(a.E, l) * one;
-        if (a.want_z) lse = row[k].softmax(a.E, l);
-      } else {
-        lse = p.softmax(a.E, l);
-      }
       count += in[k];
-      if (a.want_z) z = fmaf(lse * one, lse, z);
+      if (a.sigmoid) {
+        const float r = p.sigmoids();
 #pragma unroll
-      for (int i = 0; i < NV; ++i) acc[i] = fmaf(p.v[i], r, acc[i]);
+        for (int i = 0; i < NV; ++i) acc[i] += in[k] ? p.v[i] * r : 0.f;
+        if (a.want_z) {
+          const float lse = row[k].softmax(true);
+          z += in[k] ? lse * lse : 0.f;
+        }
+      } else {
+        const float lse = p.softmax(a.want_z);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) acc[i] += in[k] ? p.v[i] : 0.f;
+        z += in[k] ? lse * lse : 0.f;
+      }
     }
   }
   if (e0 >= 0) atomicAdd(&hist[e0], 1);
@@ -307,24 +312,78 @@ __global__ __launch_bounds__(256) void balance_sums_kernel(BalanceArgs a) {
   sum_piece<L, NV, QUADS, TEAM>(a, p, TEAM == 1 ? lds + (threadIdx.x >> 6) * a.E : lds, reinterpret_cast<float*>(lds + a.E), small);
 }
 
+// A workgroup's share of the loss: sum_e f P of its columns; its sequences' tokens, how many of them have any, and their z
+// (with the first columns alone).
+struct alignas(16) Share {
+  float loss, z;
+  int32_t tokens, filled;   // of one workgroup: T < 2^31
+};
+
 struct FoldArgs {
   BalanceArgs b;
   float* f;             // [S, E]: E cnt / n^2
   int32_t* counts;      // [S, E]
-  int32_t* seq_tokens;  // [S]
-  float* seq_z;         // [S]
-  float* loss_part;     // [workgroups of the fold]
+  Share* shares;        // [workgroups of the fold]
 };
 
-// Sum of v over a workgroup of up to 1024 threads, in a fixed order; valid in thread 0.
-__device__ __forceinline__ float block_sum(float v, float* lds) {
-  v = group_sum<64>(v);
+// Sum of v over a workgroup of up to 1024 threads, in a fixed order, the same in every thread.
+template <typename V>
+__device__ __forceinline__ V block_sum(V v, V* lds) {
+  if constexpr (sizeof(V) == 4) {
+    if constexpr (std::is_same<V, float>::value) v = group_sum<64>(v);
+    else
+      for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
+  } else {
+    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
+  }
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
-  float s = 0.f;
+  V s = 0;
   for (int i = 0; i < int(blockDim.x >> 6); ++i) s += lds[i];
   __syncthreads();
   return s;
+}
+
+// loss, and {1 / S', 1 / N} for the backward; the running totals of a load tracker.
+struct FinishArgs {
+  const Share* shares;
+  int64_t parts;
+  float z_mult;
+  float* loss;
+  float* inverse;        // [2]
+  int64_t* acc_total;    // [1] or null
+};
+
+// By one workgroup, from each thread's share of the sums.
+__device__ __forceinline__ void finish(const FinishArgs& a, float loss, float z, int64_t tokens, int32_t filled) {
+  __shared__ float lds[16];
+  __shared__ int32_t ilds[16];
+  __shared__ int64_t llds[16];
+  loss = block_sum(loss, lds);
+  z = block_sum(z, lds);
+  filled = block_sum(filled, ilds);
+  tokens = block_sum(tokens, llds);
+  if (threadIdx.x != 0) return;
+  const float inv_s = filled > 0 ? 1.f / float(filled) : 0.f, inv_n = tokens > 0 ? 1.f / float(tokens) : 0.f;
+  st_global(a.loss, loss * inv_s + a.z_mult * (z * inv_n));
+  st_global(a.inverse, inv_s);
+  st_global(a.inverse + 1, inv_n);
+  if (a.acc_total) *FM_GLOBAL(int64_t, a.acc_total) = a.acc_total[0] + tokens;
+}
+
+__global__ __launch_bounds__(1024) void balance_finish_kernel(FinishArgs a) {
+  float loss = 0.f, z = 0.f;
+  int64_t tokens = 0;
+  int32_t filled = 0;
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < a.parts; i += 1024) {
+    const Share s = a.shares[i];
+    loss += s.loss;
+    z += s.z;
+    tokens += s.tokens;
+    filled += s.filled;
+  }
+  finish(a, loss, z, tokens, filled);
 }
 
 // A sequence's places, one after the other: first and how many (0 for an empty sequence).
@@ -334,160 +393,97 @@ __device__ __forceinline__ void places_of(const BalanceArgs& b, int64_t s, int64
   n = hi > lo ? (hi - 1) / b.run - lo / b.run + 1 : 0;
 }
 
-// loss, and {1 / S', 1 / N} for the backward; the running totals of a load tracker.
-struct FinishArgs {
-  const float* loss_part;
-  int64_t parts, S;
-  const int32_t* seq_tokens;
-  const float* seq_z;
-  float z_mult;
-  float* loss;
-  float* inverse;        // [2]
-  int64_t* acc_total;    // [1] or null
+// What a sequence's places add up to, of one column.
+struct Column {
+  float p, z;
+  int32_t slots, tokens;
+  // places first + g, first + g + step, ..: four places' loads at once
+  __device__ __forceinline__ void add(const BalanceArgs& b, int64_t first, int64_t n, int g, int step, int col) {
+    for (int64_t k = g; k < n; k += 4 * step) {
+      float pk[4], zk[4];
+      int32_t mk[4], tk[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t at = first + (k + i * step < n ? k + i * step : k);
+        pk[i] = b.sums[at * b.E + col];
+        mk[i] = b.slots[at * b.E + col];
+        tk[i] = b.tokens[at];
+        zk[i] = b.z[at];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (k + i * step >= n) break;
+        p += pk[i];
+        slots += mk[i];
+        tokens += tk[i];
+        z += zk[i];
+      }
+    }
+  }
+  // writes f and the count; this column's share of the loss
+  __device__ __forceinline__ float write(const FoldArgs& a, int64_t at) const {
+    const float inv = tokens > 0 ? 1.f / float(tokens) : 0.f;
+    const float f = float(a.b.E) * float(slots) * inv;
+    st_global(a.f + at, f * inv);
+    st_global(reinterpret_cast<uint32_t*>(a.counts) + at, uint32_t(slots));
+    return f * (p * inv);
+  }
 };
 
-// By one workgroup; loss: each thread's share of the sequences' sum.
-__device__ __forceinline__ void finish(const FinishArgs& a, float loss) {
-  __shared__ float lds[16];
-  __shared__ int64_t ilds[16];
-  float z = 0.f, filled = 0.f;
-  int64_t n = 0;
-#pragma unroll 4
-  for (int64_t i = threadIdx.x; i < a.S; i += blockDim.x) {
-    const int32_t t = a.seq_tokens[i];
-    n += t;
-    filled += t > 0 ? 1.f : 0.f;
-    z += a.seq_z[i];
-  }
-  loss = block_sum(loss, lds);
-  z = block_sum(z, lds);
-  filled = block_sum(filled, lds);   // whole numbers below 2^24
-  for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off);
-  if ((threadIdx.x & 63) == 0) ilds[threadIdx.x >> 6] = n;
-  __syncthreads();
-  if (threadIdx.x != 0) return;
-  n = 0;
-  for (int i = 0; i < int(blockDim.x >> 6); ++i) n += ilds[i];
-  const float inv_s = filled > 0.f ? 1.f / filled : 0.f, inv_n = n > 0 ? 1.f / float(n) : 0.f;
-  st_global(a.loss, loss * inv_s + a.z_mult * (z * inv_n));
-  st_global(a.inverse, inv_s);
-  st_global(a.inverse + 1, inv_n);
-  if (a.acc_total) *FM_GLOBAL(int64_t, a.acc_total) = a.acc_total[0] + n;
-}
-
-// Workgroup: COLS columns of a sequence, blockDim / COLS rows of threads that each add every so many places (four places' loads at
-// once), then each other's sums in order.  The only workgroup finishes the loss too.
-template <int COLS>
+// WHOLE: a workgroup to 16 columns of a sequence, of 64 rows of threads; else a wave, of four rows, and sixteen of them to a
+// workgroup.  Each row adds every so many places, then the rows' sums meet in order.  The only workgroup finishes the loss too.
+template <bool WHOLE>
 __global__ __launch_bounds__(1024) void balance_fold_kernel(FoldArgs a, int column_groups, FinishArgs fin) {
-  __shared__ float sum[1024 / COLS][COLS];
-  __shared__ int32_t cnt[1024 / COLS][COLS];
-  __shared__ int32_t tok[1024 / COLS];
   __shared__ float lds[16];
-  const int64_t s = blockIdx.x / unsigned(column_groups);
-  const int part = int(blockIdx.x % unsigned(column_groups));
-  const int q = threadIdx.x % COLS, g = threadIdx.x / COLS, groups = int(blockDim.x) / COLS;
-  const int e = part * COLS + q, col = e < a.b.E ? e : a.b.E - 1;
-  int64_t first, n;
-  places_of(a.b, s, first, n);
-  float p = 0.f;
-  int32_t m = 0, t = 0;
-  float z = 0.f;
-  for (int64_t k = g; k < n; k += 4 * groups) {
-    float pk[4], zk[4];
-    int32_t mk[4], tk[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t at = first + (k + i * groups < n ? k + i * groups : k);
-      pk[i] = a.b.sums[at * a.b.E + col];
-      mk[i] = a.b.slots[at * a.b.E + col];
-      tk[i] = a.b.tokens[at];
-      zk[i] = a.b.z[at];
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (k + i * groups >= n) break;
-      p += pk[i];
-      m += mk[i];
-      t += tk[i];
-      z += zk[i];
-    }
+  __shared__ int32_t ilds[16];
+  const int64_t unit = WHOLE ? int64_t(blockIdx.x) : int64_t(blockIdx.x) * 16 + (threadIdx.x >> 6);
+  const int64_t s = unit / column_groups;
+  const int part = int(unit - s * column_groups);
+  const int q = threadIdx.x & 15, e = part * 16 + q, col = e < a.b.E ? e : a.b.E - 1;
+  Column c{0.f, 0.f, 0, 0};
+  if (WHOLE || s < a.b.S) {
+    int64_t first, n;
+    places_of(a.b, s, first, n);
+    c.add(a.b, first, n, WHOLE ? threadIdx.x >> 4 : (threadIdx.x >> 4) & 3, WHOLE ? 64 : 4, col);
   }
-  sum[g][q] = p;
-  cnt[g][q] = m;
-  if (q == 0) tok[g] = t;
-  const float zsum = block_sum(q == 0 ? z : 0.f, lds);   // (a barrier for the others too)
-  float share = 0.f;
-  if (threadIdx.x < COLS) {
-    p = 0.f;
-    m = t = 0;
-    for (int i = 0; i < groups; ++i) {
-      p += sum[i][q];
-      m += cnt[i][q];
-      t += tok[i];
-    }
-    if (e < a.b.E) {
-      const float inv = t > 0 ? 1.f / float(t) : 0.f;
-      const float f = float(a.b.E) * float(m) * inv;
-      st_global(a.f + s * a.b.E + e, f * inv);
-      st_global(reinterpret_cast<uint32_t*>(a.counts) + s * a.b.E + e, uint32_t(m));
-      share = f * (p * inv);
-    }
-    if (part == 0 && threadIdx.x == 0) {
-      st_global(reinterpret_cast<uint32_t*>(a.seq_tokens) + s, uint32_t(t));
-      st_global(a.seq_z + s, zsum);
-    }
+  // the four rows of a wave
+#pragma unroll
+  for (int off = 16; off < 64; off <<= 1) {
+    c.p += __shfl_xor(c.p, off);
+    c.z += __shfl_xor(c.z, off);
+    c.slots += __shfl_xor(c.slots, off);
+    c.tokens += __shfl_xor(c.tokens, off);
   }
-  if (gridDim.x == 1) {
+  bool mine = (threadIdx.x & 63) < 16 && s < a.b.S;
+  if constexpr (WHOLE) {   // and the sixteen waves
+    __shared__ Column waves[16][16];
+    if ((threadIdx.x & 63) < 16) waves[threadIdx.x >> 6][q] = c;
     __syncthreads();
-    finish(fin, share);
+    mine = threadIdx.x < 16;
+    if (mine) {
+      c = waves[0][q];
+      for (int i = 1; i < 16; ++i) {
+        c.p += waves[i][q].p;
+        c.z += waves[i][q].z;
+        c.slots += waves[i][q].slots;
+        c.tokens += waves[i][q].tokens;
+      }
+    }
+  }
+  const float loss = mine && e < a.b.E ? c.write(a, s * a.b.E + e) : 0.f;
+  const bool first_column = mine && e == 0;
+  const float z = first_column ? c.z : 0.f;
+  const int32_t tokens = first_column ? c.tokens : 0, filled = first_column && c.tokens > 0 ? 1 : 0;
+  if (gridDim.x == 1) {
+    finish(fin, loss, z, tokens, filled);
     return;
   }
-  const float total = block_sum(share, lds);
-  if (threadIdx.x == 0) st_global(a.loss_part + blockIdx.x, total);
-}
-
-// Column e of sequence s, from its places in order: its share of the loss.  Four places' loads at once.
-__device__ __forceinline__ float fold_column(const FoldArgs& a, int64_t s, int e) {
-  int64_t first, n;
-  places_of(a.b, s, first, n);
-  float p = 0.f, z = 0.f;
-  int32_t m = 0, t = 0;
-  for (int64_t k = 0; k < n; k += 4) {
-    float pk[4], zk[4];
-    int32_t mk[4], tk[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t at = first + (k + i < n ? k + i : k);
-      pk[i] = a.b.sums[at * a.b.E + e];
-      mk[i] = a.b.slots[at * a.b.E + e];
-      tk[i] = a.b.tokens[at];
-      zk[i] = a.b.z[at];
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (k + i >= n) break;
-      p += pk[i];
-      m += mk[i];
-      t += tk[i];
-      z += zk[i];
-    }
-  }
-  const float inv = t > 0 ? 1.f / float(t) : 0.f;
-  const float f = float(a.b.E) * float(m) * inv;
-  st_global(a.f + s * a.b.E + e, f * inv);
-  st_global(reinterpret_cast<uint32_t*>(a.counts) + s * a.b.E + e, uint32_t(m));
-  if (e == 0) {
-    st_global(reinterpret_cast<uint32_t*>(a.seq_tokens) + s, uint32_t(t));
-    st_global(a.seq_z + s, z);
-  }
-  return f * (p * inv);
-}
-
-__global__ __launch_bounds__(1024) void balance_finish_kernel(FinishArgs a) {
-  float loss = 0.f;
-#pragma unroll 4
-  for (int64_t i = threadIdx.x; i < a.parts; i += 1024) loss += a.loss_part[i];
-  finish(a, loss);
+  Share total;
+  total.loss = block_sum(loss, lds);
+  total.z = block_sum(z, lds);
+  total.tokens = block_sum(tokens, ilds);
+  total.filled = block_sum(filled, ilds);
+  if (threadIdx.x == 0) st_global(a.shares + blockIdx.x, make_uint4(f2u(total.loss), f2u(total.z), uint32_t(total.tokens), uint32_t(total.filled)));
 }
 
 // Few logits in few pieces: all of the forward in one workgroup, its waves taking the pieces in turn.
@@ -498,13 +494,22 @@ __global__ __launch_bounds__(1024) void balance_one_kernel(FoldArgs a, FinishArg
   for (int64_t p = threadIdx.x >> 6; p < a.b.places; p += blockDim.x >> 6)
     sum_piece<L, NV, QUADS, 1>(a.b, p, lds + (threadIdx.x >> 6) * a.b.E, nullptr, nullptr);
   __syncthreads();
-  float loss = 0.f;
+  float loss = 0.f, z = 0.f;
+  int32_t tokens = 0, filled = 0;
   for (int i = threadIdx.x; i < int(a.b.S) * a.b.E; i += blockDim.x) {
-    const int s = i / a.b.E;
-    loss += fold_column(a, s, i - s * a.b.E);
+    const int s = i / a.b.E, e = i - s * a.b.E;
+    Column c{0.f, 0.f, 0, 0};
+    int64_t first, n;
+    places_of(a.b, s, first, n);
+    c.add(a.b, first, n, 0, 1, e);
+    loss += c.write(a, i);
+    if (e == 0) {
+      z += c.z;
+      tokens += c.tokens;
+      filled += c.tokens > 0;
+    }
   }
-  __syncthreads();
-  finish(fin, loss);
+  finish(fin, loss, z, tokens, filled);
 }
 
 // acc[e] += sum of the sequences' counts: one workgroup to an expert
@@ -602,19 +607,19 @@ __global__ __launch_bounds__(256) void balance_backward_kernel(BalanceBwdArgs a)
       R q = row[k];
       float out[NV], inner = 0.f;
       if (b.sigmoid) {
-        const float r = q.sigmoids(b.E, l);
+        const float r = q.sigmoids();
 #pragma unroll
         for (int i = 0; i < NV; ++i) inner = fmaf(f.v[i], q.v[i], inner);
         inner = group_sum<L>(inner) * r;
 #pragma unroll
         for (int i = 0; i < NV; ++i) out[i] = (f.v[i] - inner) * r * (q.v[i] * (1.f - q.v[i]));
         if (a.z_mult != 0.f) {
-          const float lse = row[k].softmax(b.E, l);
+          const float lse = row[k].softmax(true);
 #pragma unroll
           for (int i = 0; i < NV; ++i) out[i] = fmaf(gz * lse, row[k].v[i], out[i]);
         }
       } else {
-        const float lse = q.softmax(b.E, l);
+        const float lse = q.softmax(a.z_mult != 0.f);
 #pragma unroll
         for (int i = 0; i < NV; ++i) inner = fmaf(f.v[i], q.v[i], inner);
         inner = group_sum<L>(inner);
@@ -661,17 +666,18 @@ int side_of(int E) {
   return side;
 }
 
-// Tokens of a wave: 16 at least (or one step of what lies side by side), the more the longer the batch: no more than 16384 waves.
+// Tokens of a wave: 16 at least (or one step of what lies side by side), the more the longer the batch: no more than 4096 waves, sixteen
+// to a CU.
 int run_of(int64_t T, int E) {
   const int side = side_of(E), least = side < 16 ? 16 : side;
-  const int64_t r = (T + 16383) / 16384;
+  const int64_t r = (T + 4095) / 4096;
   return int(r <= least ? least : (r + least - 1) / least * least);
 }
 // Four waves to a piece where a sequence has 64 waves' tokens on average: a quarter of the places to write and add.
 int team_of(int64_t T, int E, int64_t S) { return T >= 64 * S && T > 16 * run_of(T, E) ? 4 : 1; }
 
 struct Space {
-  int64_t runs, places, sums, slots, tokens, z, seq_tokens, seq_z, loss_part, bytes;   // offsets in bytes
+  int64_t runs, places, sums, slots, tokens, z, shares, bytes;   // offsets in bytes
   int team, run;
 };
 Space space_of(int64_t T, int E, int64_t S) {
@@ -690,9 +696,7 @@ Space space_of(int64_t T, int E, int64_t S) {
   w.slots = take(w.places * E);
   w.tokens = take(w.places);
   w.z = take(w.places);
-  w.seq_tokens = take(S);
-  w.seq_z = take(S);
-  w.loss_part = take(S * ((E + 15) / 16));
+  w.shares = take(4 * S * ((E + 15) / 16));
   return w;
 }
 
@@ -733,9 +737,8 @@ int fm_balance_forward(const float* logits, int64_t ld, int64_t T, int E, const 
   b.slots = reinterpret_cast<int32_t*>(ws + w.slots);
   b.tokens = reinterpret_cast<int32_t*>(ws + w.tokens);
   b.z = reinterpret_cast<float*>(ws + w.z);
-  const FoldArgs fold{b, f, counts, reinterpret_cast<int32_t*>(ws + w.seq_tokens), reinterpret_cast<float*>(ws + w.seq_z),
-                      reinterpret_cast<float*>(ws + w.loss_part)};
-  FinishArgs fin{fold.loss_part, 0, S, fold.seq_tokens, fold.seq_z, z_mult, loss, inverse, acc_total};
+  const FoldArgs fold{b, f, counts, reinterpret_cast<Share*>(ws + w.shares)};
+  FinishArgs fin{fold.shares, 0, z_mult, loss, inverse, acc_total};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   // a few pieces in one workgroup: 512 tokens of 8 experts 9.0 us (three launches) -> 5.3
   if (w.places <= kOnePieces && T * E <= kOneLogits && E <= 256 && S * E <= kOneColumns) {
@@ -753,15 +756,12 @@ int fm_balance_forward(const float* logits, int64_t ld, int64_t T, int E, const 
         if (w.team == 4) hipLaunchKernelGGL((balance_sums_kernel<L, N, Q, 4>), dim3(unsigned(w.places)), dim3(256), unsigned(5 * E * 4), s, b);
         else hipLaunchKernelGGL((balance_sums_kernel<L, N, Q, 1>), dim3(unsigned((w.places + 3) / 4)), dim3(256), unsigned(4 * E * 4), s, b);
       });
-    // a sequence's 16 columns to a workgroup, of four rows of threads for a few places, more for longer sequences; one sequence of up to 64
-    // experts is one workgroup's work, the loss with it
-    const bool one = S == 1 && E <= 64;
-    const int groups = one ? 1 : (E + 15) / 16;
-    fin.parts = S * groups;
-    if (one) hipLaunchKernelGGL(balance_fold_kernel<64>, dim3(1), dim3(1024), 0, s, fold, 1, fin);
-    else if (S > 0)
-      hipLaunchKernelGGL(balance_fold_kernel<16>, dim3(unsigned(fin.parts)), dim3(w.runs <= 8 * S ? 64 : w.runs <= 64 * S ? 256 : 1024), 0, s,
-                         fold, groups, fin);
+    // 16 columns of a sequence to a wave while sequences have 64 places or fewer on average, then to a workgroup
+    const int groups = (E + 15) / 16;
+    const bool whole = w.runs > 64 * S;
+    fin.parts = whole ? S * groups : (S * groups + 15) / 16;
+    if (whole && S > 0) hipLaunchKernelGGL(balance_fold_kernel<true>, dim3(unsigned(fin.parts)), dim3(1024), 0, s, fold, groups, fin);
+    else if (S > 0) hipLaunchKernelGGL(balance_fold_kernel<false>, dim3(unsigned(fin.parts)), dim3(1024), 0, s, fold, groups, fin);
     if (fin.parts != 1) hipLaunchKernelGGL(balance_finish_kernel, dim3(1), dim3(1024), 0, s, fin);
   }
   if (acc && S > 0) hipLaunchKernelGGL(balance_track_kernel, dim3(unsigned(E)), dim3(256), 0, s, counts, S, E, acc);
