@@ -30,14 +30,14 @@ constexpr float kSumFloor = 1e-8f;
 
 typedef float f32x4_el __attribute__((ext_vector_type(4), aligned(4)));
 
-// e^d for d <= 0 (or NaN) to about an ulp: 2^(d log2 e) by the hardware, the product's rounding error as a factor.
+// e^d for -110 <= d <= 0: 2^(d log2 e) by the hardware, with the product's rounding error as a factor (without it an ulp more for each
+// 2^k <= |d|).
 __device__ __forceinline__ float exp_below(float d) {
 #pragma clang fp contract(off)
-  constexpr float kL = 1.44269502162933349609375f, kLlo = 1.925963033500011e-08f, kLn2 = 0.693147180559945f;
-  d = d < -110.f ? -110.f : d;   // 0 there; an infinity has no product error to speak of
+  constexpr float kL = 1.44269502162933349609375f, kLn2 = 0.693147180559945f;
   const float h = d * kL;
   const float e = __builtin_amdgcn_exp2f(h);
-  return fmaf(e, fmaf(d, kLlo, fmaf(d, kL, -h)) * kLn2, e);
+  return fmaf(e, fmaf(d, kL, -h) * kLn2, e);
 }
 
 // 1 / d of a normal d to about an ulp.
@@ -135,28 +135,29 @@ struct Row {
   }
   // Columns behind the last expert hold -infinity: exponentials and sigmoids of 0.
   // softmax in place; the log of the sum of exponentials, where wanted
+  // A NaN, or a largest logit of +-infinity, makes the factor NaN: the bound below would hide the NaN's own exponential.
   __device__ __forceinline__ float softmax(bool want_log) {
     float m = v[0], s = 0.f;
 #pragma unroll
-    for (int i = 1; i < NV; ++i) m = fmaxf(m, v[i]);
-    m = group_max<L>(m);
+    for (int i = 1; i < NV; ++i) m = __builtin_elementwise_maximum(m, v[i]);
+    m = group_fold<L>(m, [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      v[i] = exp_below(v[i] - m);
+      v[i] = exp_below(fmaxf(v[i] - m, -110.f));
       s += v[i];
     }
     s = group_sum<L>(s);
-    const float r = reciprocal(s);
+    const float r = fmaf(m, 0.f, reciprocal(s));
 #pragma unroll
     for (int i = 0; i < NV; ++i) v[i] *= r;
     return want_log ? m + logf(s) : 0.f;
   }
-  // sigmoids in place: 1 or e^-|l| over 1 + e^-|l|; 1 / (their sum + floor)
+  // sigmoids in place: 1 or e^-|l| over 1 + e^-|l| (half an ulp of l's exponent and two more of the sigmoid); 1 / (their sum + floor)
   __device__ __forceinline__ float sigmoids() {
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const float e = exp_below(-fabsf(v[i]));
+      const float e = __builtin_amdgcn_exp2f(-fabsf(v[i]) * 1.44269502162933349609375f);
       v[i] = (v[i] < 0.f ? e : 1.f) * __builtin_amdgcn_rcpf(1.f + e);
       s += v[i];
     }
@@ -223,23 +224,30 @@ __device__ __forceinline__ void sum_piece(const BalanceArgs& a, int64_t p, int32
     }
     t += TEAM * kSide * kAhead;
     if (t < hi) fetch(t);
+    if (a.mask) {   // what a mask leaves out may be a NaN; a row past the end is the last one again
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {   // what does not count may be a NaN: it is left out by a select
+      for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+        for (int i = 0; i < NV; ++i) row[k].v[i] = in[k] ? row[k].v[i] : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const float one = in[k] ? 1.f : 0.f;
       R p = row[k];
       count += in[k];
       if (a.sigmoid) {
-        const float r = p.sigmoids();
+        const float r = p.sigmoids() * one;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) acc[i] += in[k] ? p.v[i] * r : 0.f;
+        for (int i = 0; i < NV; ++i) acc[i] = fmaf(p.v[i], r, acc[i]);
         if (a.want_z) {
           const float lse = row[k].softmax(true);
-          z += in[k] ? lse * lse : 0.f;
+          z = fmaf(lse * one, lse, z);
         }
       } else {
         const float lse = p.softmax(a.want_z);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) acc[i] += in[k] ? p.v[i] : 0.f;
-        z += in[k] ? lse * lse : 0.f;
+        for (int i = 0; i < NV; ++i) acc[i] = fmaf(p.v[i], one, acc[i]);
+        z = fmaf(lse * one, lse, z);
       }
     }
   }
