@@ -10,7 +10,7 @@
 //
 // Forward: one pass over the logits and indices.  The batch is cut at sequence borders and into runs of tokens; run c and
 // sequence s meet at most once, and runs and sequences both ascend, so the number c + s names each piece, and a piece finds its
-// run and sequence from its number by a search of the borders.  A piece is the work of a wave, or of four where sequences are
+// run and sequence from its number by a search of the borders.  A piece is the work of a wave, or of four or sixteen where sequences are
 // long: a token's logits sit in L lanes (64 / L tokens side by side) whose column sums stay in registers, the slots are counted in
 // LDS, and both go to the piece's place in the workspace.  A second launch adds each sequence's places in order (no float
 // atomics: the same bits each time) and leaves E cnt / n^2 for the backward, a third adds the sequences; few tokens take one launch
@@ -171,7 +171,7 @@ constexpr int ahead() {
   return 16 * L / 64 >= 4 ? 4 : (16 * L / 64 >= 2 ? 2 : 1);
 }
 
-// Piece p's sums and counts, by one wave (its own hist) or a workgroup of four (one hist; sums and small hold a row for each wave).
+// Piece p's sums and counts, by one wave (its own hist) or a workgroup of TEAM (one hist; sums and small hold a row for each wave).
 template <int L, int NV, bool QUADS, int TEAM>
 __device__ __forceinline__ void sum_piece(const BalanceArgs& a, int64_t p, int32_t* hist, float* sums, float (*small)[2]) {
   using R = Row<L, NV, QUADS>;
@@ -312,9 +312,9 @@ __device__ __forceinline__ void sum_piece(const BalanceArgs& a, int64_t p, int32
 }
 
 template <int L, int NV, bool QUADS, int TEAM>
-__global__ __launch_bounds__(256) void balance_sums_kernel(BalanceArgs a) {
+__global__ __launch_bounds__(TEAM == 16 ? 1024 : 256) void balance_sums_kernel(BalanceArgs a) {
   extern __shared__ int32_t lds[];   // TEAM 1: four hists; else one, and the waves' sums
-  __shared__ float small[4][2];
+  __shared__ float small[TEAM][2];
   const int64_t p = TEAM == 1 ? int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6) : int64_t(blockIdx.x);
   if (p >= a.places) return;
   sum_piece<L, NV, QUADS, TEAM>(a, p, TEAM == 1 ? lds + (threadIdx.x >> 6) * a.E : lds, reinterpret_cast<float*>(lds + a.E), small);
@@ -324,7 +324,7 @@ __global__ __launch_bounds__(256) void balance_sums_kernel(BalanceArgs a) {
 // (with the first columns alone).
 struct alignas(16) Share {
   float loss, z;
-  int32_t tokens, filled;   // of one workgroup: T < 2^31
+  int32_t tokens, filled;   // below T < 2^31 in any sum
 };
 
 struct FoldArgs {
@@ -334,22 +334,26 @@ struct FoldArgs {
   Share* shares;        // [workgroups of the fold]
 };
 
-// Sum of v over a workgroup of up to 1024 threads, in a fixed order, the same in every thread.
-template <typename V>
-__device__ __forceinline__ V block_sum(V v, V* lds) {
-  if constexpr (sizeof(V) == 4) {
-    if constexpr (std::is_same<V, float>::value) v = group_sum<64>(v);
-    else
-      for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
-  } else {
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
+// The sum over a workgroup's threads, in a fixed order; valid in thread 0.
+__device__ __forceinline__ Share block_sum(Share v) {
+  __shared__ Share waves[16];
+  v.loss = group_sum<64>(v.loss);
+  v.z = group_sum<64>(v.z);
+  for (int off = 32; off > 0; off >>= 1) {
+    v.tokens += __shfl_xor(v.tokens, off);
+    v.filled += __shfl_xor(v.filled, off);
   }
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
   __syncthreads();
-  V s = 0;
-  for (int i = 0; i < int(blockDim.x >> 6); ++i) s += lds[i];
-  __syncthreads();
-  return s;
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < int(blockDim.x >> 6); ++i) {
+      v.loss += waves[i].loss;
+      v.z += waves[i].z;
+      v.tokens += waves[i].tokens;
+      v.filled += waves[i].filled;
+    }
+  }
+  return v;
 }
 
 // loss, and {1 / S', 1 / N} for the backward; the running totals of a load tracker.
@@ -363,35 +367,27 @@ struct FinishArgs {
 };
 
 // By one workgroup, from each thread's share of the sums.
-__device__ __forceinline__ void finish(const FinishArgs& a, float loss, float z, int64_t tokens, int32_t filled) {
-  __shared__ float lds[16];
-  __shared__ int32_t ilds[16];
-  __shared__ int64_t llds[16];
-  loss = block_sum(loss, lds);
-  z = block_sum(z, lds);
-  filled = block_sum(filled, ilds);
-  tokens = block_sum(tokens, llds);
+__device__ __forceinline__ void finish(const FinishArgs& a, Share v) {
+  v = block_sum(v);
   if (threadIdx.x != 0) return;
-  const float inv_s = filled > 0 ? 1.f / float(filled) : 0.f, inv_n = tokens > 0 ? 1.f / float(tokens) : 0.f;
-  st_global(a.loss, loss * inv_s + a.z_mult * (z * inv_n));
+  const float inv_s = v.filled > 0 ? 1.f / float(v.filled) : 0.f, inv_n = v.tokens > 0 ? 1.f / float(v.tokens) : 0.f;
+  st_global(a.loss, v.loss * inv_s + a.z_mult * (v.z * inv_n));
   st_global(a.inverse, inv_s);
   st_global(a.inverse + 1, inv_n);
-  if (a.acc_total) *FM_GLOBAL(int64_t, a.acc_total) = a.acc_total[0] + tokens;
+  if (a.acc_total) *FM_GLOBAL(int64_t, a.acc_total) = a.acc_total[0] + v.tokens;
 }
 
 __global__ __launch_bounds__(1024) void balance_finish_kernel(FinishArgs a) {
-  float loss = 0.f, z = 0.f;
-  int64_t tokens = 0;
-  int32_t filled = 0;
+  Share v{0.f, 0.f, 0, 0};
 #pragma unroll 4
   for (int64_t i = threadIdx.x; i < a.parts; i += 1024) {
     const Share s = a.shares[i];
-    loss += s.loss;
-    z += s.z;
-    tokens += s.tokens;
-    filled += s.filled;
+    v.loss += s.loss;
+    v.z += s.z;
+    v.tokens += s.tokens;
+    v.filled += s.filled;
   }
-  finish(a, loss, z, tokens, filled);
+  finish(a, v);
 }
 
 // A sequence's places, one after the other: first and how many (0 for an empty sequence).
@@ -442,8 +438,6 @@ struct Column {
 // workgroup.  Each row adds every so many places, then the rows' sums meet in order.  The only workgroup finishes the loss too.
 template <bool WHOLE>
 __global__ __launch_bounds__(1024) void balance_fold_kernel(FoldArgs a, int column_groups, FinishArgs fin) {
-  __shared__ float lds[16];
-  __shared__ int32_t ilds[16];
   const int64_t unit = WHOLE ? int64_t(blockIdx.x) : int64_t(blockIdx.x) * 16 + (threadIdx.x >> 6);
   const int64_t s = unit / column_groups;
   const int part = int(unit - s * column_groups);
@@ -478,20 +472,18 @@ __global__ __launch_bounds__(1024) void balance_fold_kernel(FoldArgs a, int colu
       }
     }
   }
-  const float loss = mine && e < a.b.E ? c.write(a, s * a.b.E + e) : 0.f;
-  const bool first_column = mine && e == 0;
-  const float z = first_column ? c.z : 0.f;
-  const int32_t tokens = first_column ? c.tokens : 0, filled = first_column && c.tokens > 0 ? 1 : 0;
+  Share v{mine && e < a.b.E ? c.write(a, s * a.b.E + e) : 0.f, 0.f, 0, 0};
+  if (mine && e == 0) {
+    v.z = c.z;
+    v.tokens = c.tokens;
+    v.filled = c.tokens > 0;
+  }
   if (gridDim.x == 1) {
-    finish(fin, loss, z, tokens, filled);
+    finish(fin, v);
     return;
   }
-  Share total;
-  total.loss = block_sum(loss, lds);
-  total.z = block_sum(z, lds);
-  total.tokens = block_sum(tokens, ilds);
-  total.filled = block_sum(filled, ilds);
-  if (threadIdx.x == 0) st_global(a.shares + blockIdx.x, make_uint4(f2u(total.loss), f2u(total.z), uint32_t(total.tokens), uint32_t(total.filled)));
+  v = block_sum(v);
+  if (threadIdx.x == 0) st_global(a.shares + blockIdx.x, make_uint4(f2u(v.loss), f2u(v.z), uint32_t(v.tokens), uint32_t(v.filled)));
 }
 
 // Few logits in few pieces: all of the forward in one workgroup, its waves taking the pieces in turn.
@@ -502,22 +494,21 @@ __global__ __launch_bounds__(1024) void balance_one_kernel(FoldArgs a, FinishArg
   for (int64_t p = threadIdx.x >> 6; p < a.b.places; p += blockDim.x >> 6)
     sum_piece<L, NV, QUADS, 1>(a.b, p, lds + (threadIdx.x >> 6) * a.b.E, nullptr, nullptr);
   __syncthreads();
-  float loss = 0.f, z = 0.f;
-  int32_t tokens = 0, filled = 0;
+  Share v{0.f, 0.f, 0, 0};
   for (int i = threadIdx.x; i < int(a.b.S) * a.b.E; i += blockDim.x) {
     const int s = i / a.b.E, e = i - s * a.b.E;
     Column c{0.f, 0.f, 0, 0};
     int64_t first, n;
     places_of(a.b, s, first, n);
     c.add(a.b, first, n, 0, 1, e);
-    loss += c.write(a, i);
+    v.loss += c.write(a, i);
     if (e == 0) {
-      z += c.z;
-      tokens += c.tokens;
-      filled += c.tokens > 0;
+      v.z += c.z;
+      v.tokens += c.tokens;
+      v.filled += c.tokens > 0;
     }
   }
-  finish(fin, loss, z, tokens, filled);
+  finish(fin, v);
 }
 
 // acc[e] += sum of the sequences' counts: one workgroup to an expert
@@ -681,8 +672,13 @@ int run_of(int64_t T, int E) {
   const int64_t r = (T + 4095) / 4096;
   return int(r <= least ? least : (r + least - 1) / least * least);
 }
-// Four waves to a piece where a sequence has 64 waves' tokens on average: a quarter of the places to write and add.
-int team_of(int64_t T, int E, int64_t S) { return T >= 64 * S && T > 16 * run_of(T, E) ? 4 : 1; }
+// Waves to a piece: four where sequences have 64 tokens on average, sixteen from 1024 on; the fewer places to write and add.  One
+// sequence of 65536 tokens, 256 experts: fold 11.5 us of 1024 places, 7.0 of 256.
+// (Beyond 512 experts sixteen waves of a row's registers do not fit.)
+int team_of(int64_t T, int E, int64_t S) {
+  if (T <= 16 * run_of(T, E) || T < 64 * S) return 1;
+  return T < 1024 * S || E > 512 ? 4 : 16;
+}
 
 struct Space {
   int64_t runs, places, sums, slots, tokens, z, shares, bytes;   // offsets in bytes
@@ -761,6 +757,12 @@ int fm_balance_forward(const float* logits, int64_t ld, int64_t T, int E, const 
       for_experts(E, [&](auto l, auto n, auto q) {
         constexpr int L = decltype(l)::value, N = decltype(n)::value;
         constexpr bool Q = decltype(q)::value;
+        if constexpr (N <= 8) {
+          if (w.team == 16) {
+            hipLaunchKernelGGL((balance_sums_kernel<L, N, Q, 16>), dim3(unsigned(w.places)), dim3(1024), unsigned(17 * E * 4), s, b);
+            return;
+          }
+        }
         if (w.team == 4) hipLaunchKernelGGL((balance_sums_kernel<L, N, Q, 4>), dim3(unsigned(w.places)), dim3(256), unsigned(5 * E * 4), s, b);
         else hipLaunchKernelGGL((balance_sums_kernel<L, N, Q, 1>), dim3(unsigned((w.places + 3) / 4)), dim3(256), unsigned(4 * E * 4), s, b);
       });
