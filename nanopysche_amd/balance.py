@@ -40,7 +40,7 @@ class BalanceState:
     logits: torch.Tensor               # [T, E]
     cu_seqlens: Optional[torch.Tensor]  # [S + 1] int32
     mask: Optional[torch.Tensor]       # [T] bool
-    f: torch.Tensor                    # [S * E + 2]: E slots / n_s^2, then 1 / S' and 1 / tokens
+    f: torch.Tensor                    # fp32, S * E + 2 at least: E slots / n_s^2, then 1 / S' and 1 / tokens
     sigmoid: bool
     z_mult: float
     shape: torch.Size                  # of the logits as given
@@ -112,15 +112,16 @@ def balance_forward(logits: torch.Tensor, indices: torch.Tensor, *, cu_seqlens: 
     S = 1 if cu is None else cu.numel() - 1
     dev = l2.device
     z = 0.0 if z_loss_multiplier is None else float(z_loss_multiplier)
-    f = torch.empty(S * E + 2, dtype=torch.float32, device=dev)
+    nbytes = _lib.size_of("fm_balance_workspace_bytes", T, E, S)
+    room = (S * E + 65) // 64 * 64   # f and its two factors, then the workspace, on 256 bytes: an allocation less a call
+    f = torch.empty(room + nbytes // 4, dtype=torch.float32, device=dev)
     loss = torch.empty((), dtype=torch.float32, device=dev)
     counts = torch.empty(E if cu is None else (S, E), dtype=torch.int32, device=dev)
-    nbytes = _lib.size_of("fm_balance_workspace_bytes", T, E, S)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    at = f.data_ptr()
     acc, total = (None, None) if load_tracker is None else (load_tracker.tokens_per_expert, load_tracker.total_tokens)
     _lib.call_on(l2, "fm_balance_forward", l2.data_ptr(), l2.stride(0) if T > 1 else E, T, E, idx.data_ptr(), int(idx.dtype == torch.int64),
-                 idx.shape[1], _lib.addr(cu), S, _lib.addr(mask), int(sigmoid), z, f.data_ptr(), counts.data_ptr(), f.data_ptr() + 4 * S * E,
-                 loss.data_ptr(), _lib.addr(acc), _lib.addr(total), ws.data_ptr(), nbytes)
+                 idx.shape[1], _lib.addr(cu), S, _lib.addr(mask), int(sigmoid), z, at, counts.data_ptr(), at + 4 * S * E, loss.data_ptr(),
+                 _lib.addr(acc), _lib.addr(total), at + 4 * room, nbytes)
     return loss, counts, BalanceState(l2, cu, mask, f, sigmoid, z, logits.shape)
 
 
@@ -130,7 +131,7 @@ def balance_backward(state: BalanceState, dloss: torch.Tensor, add_to: Optional[
     l2, cu = state.logits, state.cu_seqlens
     T, E = l2.shape
     S = 1 if cu is None else cu.numel() - 1
-    if state.f.numel() != S * E + 2 or (state.mask is not None and state.mask.numel() != T):
+    if state.f.numel() < S * E + 2 or (state.mask is not None and state.mask.numel() != T):
         raise ValueError(f"the state's f and mask do not fit {T} tokens, {E} experts and {S} sequences")
     if dloss.dtype != torch.float32 or dloss.numel() != 1:
         raise TypeError(f"dloss must be one float32 value, got {dloss.dtype} {tuple(dloss.shape)}")
