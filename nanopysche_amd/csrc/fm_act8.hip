@@ -285,16 +285,15 @@ struct NormArgs {
   float* rstd;
 };
 
-// Sum over a row's waves, in wave order; `parity` alternates between rows, so one barrier is enough.
+// Sum over a row's waves [first, + waves) of the workgroup's, in wave order; `parity` alternates between rows, so one barrier is enough.
 template <bool ONE>
-__device__ __forceinline__ float row_sum(float v, float (*sums)[16], int parity) {
+__device__ __forceinline__ float row_sum(float v, float (*sums)[16], int parity, int first, int waves) {
   v = group_sum<64>(v);
   if constexpr (!ONE) {
     if ((threadIdx.x & 63) == 0) sums[parity][threadIdx.x >> 6] = v;
     __syncthreads();
-    const int waves = int(blockDim.x >> 6);
-    v = sums[parity][0];
-    for (int i = 1; i < waves; ++i) v += sums[parity][i];
+    v = sums[parity][first];
+    for (int i = 1; i < waves; ++i) v += sums[parity][first + i];
   }
   return v;
 }
@@ -322,7 +321,7 @@ __global__ __launch_bounds__(ONE ? 256 : 1024) void norm_kernel(NormArgs a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
   }
-  ss = row_sum<ONE>(ss, sums, 0);
+  ss = row_sum<ONE>(ss, sums, 0, 0, int(blockDim.x >> 6));
   const float r = 1.0f / sqrtf(ss / float(a.D) + a.eps);
   if (lane == 0) st_global(a.rstd + row, r);
 #pragma unroll
@@ -341,7 +340,9 @@ __global__ __launch_bounds__(ONE ? 256 : 1024) void norm_kernel(NormArgs a) {
   }
 }
 
-// A workgroup takes the rows [slice * rps, + rps) (W = 1: its waves every fourth of them) and writes the slice's share of dw.
+// A workgroup of G teams of W waves takes the rows [slice * rps, + rps), a team every G-th of them, and writes the slice's share of
+// dw: the teams' shares, added in order.  Eight waves or so to a workgroup, two of them to a CU: 16384 rows of 2048 take 65 us with one
+// team to a workgroup (four waves to a CU), 35 with four.
 struct NormBwdArgs {
   const void* dy;
   int64_t ld_dy;
@@ -354,6 +355,7 @@ struct NormBwdArgs {
   int64_t ld_dx;
   float* part;      // [slices, ld_p], or null: no dw
   int64_t ld_p, rps;
+  int waves, teams;  // W and G
 };
 
 template <typename T, int NC, bool TAIL, int STREAM>
@@ -362,24 +364,27 @@ struct NormRow {
   uint32_t code[NC];
   Eight<T> dy[NC];
   float r;
-  __device__ __forceinline__ void load(const NormBwdArgs& a, int64_t row, int lane, int step) {
+  // in: else a dy of zeros
+  __device__ __forceinline__ void load(const NormBwdArgs& a, int64_t row, bool in, int lane, int step) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int col = step * c + 8 * lane;
       const int at = col < a.x.ld_q ? col : 0;   // behind the row: its first bytes, with a dy of zeros
       q[c] = a.x.bytes(row, at);
       code[c] = a.x.code(row, at);
-      dy[c].template load<TAIL, (STREAM > 1)>(static_cast<const T*>(a.dy) + row * a.ld_dy + col, a.D - col);
+      dy[c].template load<TAIL, (STREAM > 1)>(static_cast<const T*>(a.dy) + row * a.ld_dy + col, in ? a.D - col : 0);
     }
     r = a.rstd[row];
   }
 };
 
 template <typename T, typename WT, int NC, bool ONE, bool TAIL, int STREAM>
-__global__ __launch_bounds__(ONE ? 256 : 1024) void norm_backward_kernel(NormBwdArgs a) {
+__global__ __launch_bounds__(ONE ? 512 : 1024) void norm_backward_kernel(NormBwdArgs a) {
+  extern __shared__ float4 shares4[];   // a team's dw [ld_p], if there are several
   __shared__ float sums[2][16];
-  const int lane = ONE ? threadIdx.x & 63 : threadIdx.x, wave = threadIdx.x >> 6;
-  const int step = ONE ? 512 : int(blockDim.x) * 8;
+  const int width = ONE ? 64 : 64 * a.waves;   // threads of a team
+  const int team = ONE ? int(threadIdx.x >> 6) : int(threadIdx.x) / width, lane = int(threadIdx.x) - team * width;
+  const int step = 8 * width;
   const int64_t r0 = int64_t(blockIdx.x) * a.rps, r1 = r0 + a.rps < a.T ? r0 + a.rps : a.T;
   const float inv_d = 1.0f / float(a.D);
   float wv[NC][8], pdw[NC][8];
@@ -392,19 +397,23 @@ __global__ __launch_bounds__(ONE ? 256 : 1024) void norm_backward_kernel(NormBwd
 #pragma unroll
     for (int j = 0; j < 8; ++j) pdw[c][j] = 0.f;
   }
-  constexpr int kStep = ONE ? 4 : 1;
   int parity = 0;
-  const int64_t first = r0 + (ONE ? wave : 0);
   // the next row's loads are in flight while this one is summed, where 128 registers hold both
-  constexpr bool kNext = ONE || sizeof(T) == 2;
+  constexpr bool kNext = ONE || (sizeof(T) == 2 && !TAIL);
   NormRow<T, NC, TAIL, STREAM> n, next;
-  if (kNext && first < r1) next.load(a, first, lane, step);
-  for (int64_t row = first; row < r1; row += kStep, parity ^= 1) {
+  // a team without a row of its own reads the slice's last one again, with a dy of zeros
+  auto load = [&](NormRow<T, NC, TAIL, STREAM>& to, int64_t i) {
+    const bool in = i + team < r1;
+    to.load(a, in ? i + team : r1 - 1, in, lane, step);
+  };
+  if constexpr (kNext) load(next, r0);
+  for (int64_t i = r0; i < r1; i += a.teams, parity ^= 1) {
+    const int64_t row = i + team;
     if constexpr (kNext) {
       n = next;
-      if (row + kStep < r1) next.load(a, row + kStep, lane, step);
+      if (i + a.teams < r1) load(next, i + a.teams);
     } else {
-      n.load(a, row, lane, step);
+      load(n, i);
     }
     // x r from the bytes in one product (s r is exact), and dx = r (a - (sum a x r / D) x r)
     float xr[NC][8], g[NC][8], dot = 0.f;
@@ -419,7 +428,8 @@ __global__ __launch_bounds__(ONE ? 256 : 1024) void norm_backward_kernel(NormBwd
         dot = fmaf(g[c][j], xr[c][j], dot);
       }
     }
-    const float m = row_sum<ONE>(dot, sums, parity) * inv_d;
+    const float m = row_sum<ONE>(dot, sums, parity, team * a.waves, a.waves) * inv_d;
+    if (row >= r1) continue;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int col = step * c + 8 * lane;
@@ -430,24 +440,35 @@ __global__ __launch_bounds__(ONE ? 256 : 1024) void norm_backward_kernel(NormBwd
     }
   }
   if (a.part == nullptr) return;
-  if constexpr (ONE) {   // the four waves' shares, in wave order
-    __shared__ float acc[4][NC * 512];
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) acc[wave][(c * 8 + j) * 64 + lane] = pdw[c][j];
-    __syncthreads();
-    for (int i = threadIdx.x; i < NC * 512; i += 256) {
-      const int col = (i >> 9) * 512 + (i & 63) * 8 + ((i >> 6) & 7);
-      if (col < a.D) st_global(a.part + blockIdx.x * a.ld_p + col, ((acc[0][i] + acc[1][i]) + acc[2][i]) + acc[3][i]);
-    }
-  } else {
+  float* part = a.part + blockIdx.x * a.ld_p;   // ld_p is D rounded up to 8
+  if (a.teams == 1) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int col = step * c + 8 * lane;
-      if (col < a.D) store8<float, false>(a.part + blockIdx.x * a.ld_p + col, pdw[c], 8);   // ld_p is D rounded up to 8
+      if (col < a.D) store8<float, false>(part + col, pdw[c], 8);
+    }
+    return;
+  }
+  for (int t = 0; t < a.teams; ++t) {
+    if (t > 0) __syncthreads();
+    if (team != t) continue;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int col = step * c + 8 * lane;
+      if (col >= a.D) break;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float4 v = make_float4(pdw[c][4 * h], pdw[c][4 * h + 1], pdw[c][4 * h + 2], pdw[c][4 * h + 3]);
+        if (t > 0) {
+          const float4 before = shares4[col / 4 + h];
+          v = make_float4(before.x + v.x, before.y + v.y, before.z + v.z, before.w + v.w);
+        }
+        shares4[col / 4 + h] = v;
+      }
     }
   }
+  __syncthreads();
+  for (int i = threadIdx.x; i < int(a.ld_p) / 4; i += blockDim.x) st_global(part + 4 * i, shares4[i]);
 }
 
 // dw from the slices' shares: a workgroup takes 16 columns, 64 rows of threads every 64th slice each, then the sums of
@@ -529,14 +550,20 @@ bool kept_ok(const void* q, int64_t ld_q, const void* codes, int64_t ld_c, int64
 
 // ---- the norm's shapes
 int norm_waves(int64_t D) { return int((D + 1023) / 1024); }
-// Rows of a workgroup of the backward: one round of the workgroups that fit (sixteen waves to a CU), but no more than 1024 of them: each
-// writes D sums that the second launch reads.
+// Teams of a workgroup of the backward, and its rows: one row each while 512 workgroups take all; else one round of the workgroups that fit
+// (sixteen waves to a CU), but no more than 512 of them: each writes D sums that the second launch reads.
+int norm_teams(int64_t T, int64_t D) {
+  if (T <= 512) return 1;
+  if (D <= 512) return 8;
+  const int w = norm_waves(D);
+  return w <= 4 ? 8 / w : 1;
+}
 int64_t norm_rows_per_slice(int64_t T, int64_t D) {
-  const int w = D <= 512 ? 4 : norm_waves(D), rows = D <= 512 ? 4 : 1;
-  int64_t most = int64_t(device_cus()) * (16 / w);
+  const int teams = norm_teams(T, D), waves = teams * (D <= 512 ? 1 : norm_waves(D));
+  int64_t most = int64_t(device_cus()) * (16 / waves);
   most = most < 512 ? most : 512;
   const int64_t r = (T + most - 1) / most;
-  return (r + rows - 1) / rows * rows;
+  return (r + teams - 1) / teams * teams;
 }
 
 // go(eights a lane, one wave to a row, a width that is no multiple of 8)
@@ -691,7 +718,7 @@ int fm_act8_rmsnorm_backward(const void* dy, int64_t ld_dy, int dtype, int64_t T
   const int64_t rps = norm_rows_per_slice(T, D), slices = (T + rps - 1) / rps, ld_p = (D + 7) / 8 * 8;
   float* part = static_cast<float*>(workspace);
   const NormBwdArgs a{dy, ld_dy, Act8{static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(codes), ld_q, ld_c}, T, int(D), w, rstd,
-                      dx, ld_dx, dw ? part : nullptr, ld_p, rps};
+                      dx, ld_dx, dw ? part : nullptr, ld_p, rps, D <= 512 ? 1 : norm_waves(D), norm_teams(T, D)};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   for_dtype(dtype, [&](auto t) {
     for_dtype(w_dtype, [&](auto wt) {
@@ -700,7 +727,7 @@ int fm_act8_rmsnorm_backward(const void* dy, int64_t ld_dy, int dtype, int64_t T
         for_stream<0, 1, 2>(T * D * int64_t(sizeof(t)), [&](auto stream_) {
           hipLaunchKernelGGL((norm_backward_kernel<decltype(t), decltype(wt), decltype(nc)::value, kOne, decltype(tail)::value,
                                                    decltype(stream_)::value>),
-                             dim3(unsigned(slices)), dim3(kOne ? 256 : 64 * norm_waves(D)), 0, s, a);
+                             dim3(unsigned(slices)), dim3(64 * a.waves * a.teams), a.teams > 1 && a.part ? unsigned(ld_p * 4) : 0u, s, a);
         });
       });
     });
