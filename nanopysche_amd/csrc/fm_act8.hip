@@ -100,8 +100,7 @@ struct FastDiv {
   __device__ __forceinline__ uint32_t quotient(uint32_t n) const { return (n + __umulhi(n, m)) >> l; }
 };
 
-// A matrix's eights, row by row, ld_q / 8 (a multiple of 4) to a row: eight i is columns
-// [8 (i % per), + 8) of row i / per.
+// A matrix's eights (fours, where EACH is 4), row by row, ld_q / EACH to a row: eight i is columns [8 (i % per), + 8) of row i / per.
 struct Items {
   FastDiv per;
   uint32_t n;      // fewer than 2^31
@@ -114,12 +113,12 @@ struct Item {
   bool in;
 };
 // Eights u of U of a thread; one past the last stands for the last and is not stored.
-template <int U>
+template <int U, int EACH = 8>
 __device__ __forceinline__ Item item_of(const Items& t, int u) {
   const uint32_t i = blockIdx.x * (256u * U) + u * 256u + threadIdx.x;
   const uint32_t j = i < t.n ? i : t.n - 1;
   const uint32_t r = t.per.quotient(j);
-  const int col = int(j - r * t.per.d) * 8;
+  const int col = int(j - r * t.per.d) * EACH;
   return Item{t.row0 + r, col, t.cols - col, i < t.n};
 }
 
@@ -169,28 +168,50 @@ struct RestoreArgs {
   int64_t ld_out;
 };
 
+// A lane stores 16 bytes: eight bf16 values or four fp32 ones.  (Eight fp32 values as two stores, each to every other 16 bytes, went past
+// the caches at half the rate: 65536 x 1024 108 us, of fours 49.)
 template <typename T, int U, bool GATHER, int STREAM>
 __global__ __launch_bounds__(256) void restore_kernel(Items t, RestoreArgs a) {
+  constexpr int kEach = 16 / sizeof(T);
   Item it[U];
-  uint2 b[U];
-  uint32_t code[U];
+  uint32_t b[U][kEach / 4], code[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    it[u] = item_of<U>(t, u);
+    it[u] = item_of<U, kEach>(t, u);
     int64_t r = it[u].row;
     bool zero = false;
     if constexpr (GATHER) {
       r = a.index[r];
       zero = r < 0 || r >= a.src_rows;
     }
-    b[u] = zero ? make_uint2(0, 0) : a.x.bytes(r, it[u].col);
     code[u] = zero ? 0u : a.x.code(r, it[u].col);
+    if constexpr (kEach == 8) {
+      const uint2 w = zero ? make_uint2(0, 0) : a.x.bytes(r, it[u].col);
+      b[u][0] = w.x;
+      b[u][1] = w.y;
+    } else {
+      b[u][0] = zero ? 0u : *reinterpret_cast<const uint32_t*>(a.x.q + r * a.x.ld_q + it[u].col);
+    }
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     float v[8];
-    act_decode8(b[u], act_scale(code[u]), v);
-    if (it[u].in) store8<T, true, (STREAM > 0)>(static_cast<T*>(a.out) + it[u].row * a.ld_out + it[u].col, v, it[u].n);
+    const float s = act_scale(code[u]);
+#pragma unroll
+    for (int i = 0; i < kEach / 4; ++i) act_decode4(b[u][i], s, v + 4 * i);
+    if (!it[u].in) continue;
+    T* p = static_cast<T*>(a.out) + it[u].row * a.ld_out + it[u].col;
+    if constexpr (kEach == 8) {
+      store8<T, true, (STREAM > 0)>(p, v, it[u].n);
+    } else if (it[u].n >= 4) {
+      const u32x4_el w = {f2u(v[0]), f2u(v[1]), f2u(v[2]), f2u(v[3])};
+      if constexpr (STREAM > 0) __builtin_nontemporal_store(w, FM_GLOBAL(u32x4_el, p));
+      else *FM_GLOBAL(u32x4_el, p) = w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        if (i < it[u].n) st_global(p + i, v[i]);
+    }
   }
 }
 
@@ -267,7 +288,8 @@ __global__ __launch_bounds__(256) void swiglu_backward_kernel(Items t, SwigluBwd
 
 // ---------------------------------------------------------------- RMSNorm ----
 // A row sits in the registers of W waves: lane l of them holds columns 8 l .. + 8 and, of rows wider than 512, 8 l + 512 W .. + 8
-// too.  Up to 512 columns W is 1, four rows to a workgroup of four waves; wider rows take a workgroup of W = ceil(D / 1024)
+// too.  Up to 512 columns a row takes L = 8, 16, 32 or 64 lanes of a wave, 64 / L rows side by side (1.6 M rows of 40: a whole wave to a
+// row took 385 us forward and 415 backward, eight lanes 62 and 75); wider rows take a workgroup of W = ceil(D / 1024)
 // waves each, so the lanes of any width are busy.  (One eight a lane and twice the waves was slower, 16384 rows of 7168:
 // forward 132 us against 100, backward 162 against 129: fewer rows on a CU, and each waits for its slowest wave.)
 struct NormArgs {
@@ -285,11 +307,11 @@ struct NormArgs {
   float* rstd;
 };
 
-// Sum over a row's waves [first, + waves) of the workgroup's, in wave order; `parity` alternates between rows, so one barrier is enough.
-template <bool ONE>
+// Sum over a row's L lanes, or (L 0) its waves [first, + waves) of the workgroup's, in wave order; `parity` alternates between rows, so one barrier is enough.
+template <int L>
 __device__ __forceinline__ float row_sum(float v, float (*sums)[16], int parity, int first, int waves) {
-  v = group_sum<64>(v);
-  if constexpr (!ONE) {
+  v = group_sum<L == 0 ? 64 : L>(v);
+  if constexpr (L == 0) {
     if ((threadIdx.x & 63) == 0) sums[parity][threadIdx.x >> 6] = v;
     __syncthreads();
     v = sums[parity][first];
@@ -298,13 +320,14 @@ __device__ __forceinline__ float row_sum(float v, float (*sums)[16], int parity,
   return v;
 }
 
-template <typename T, typename WT, int NC, bool ONE, bool TAIL, int STREAM>
-__global__ __launch_bounds__(ONE ? 256 : 1024) void norm_kernel(NormArgs a) {
+template <typename T, typename WT, int NC, int L, bool TAIL, int STREAM>
+__global__ __launch_bounds__(L > 0 ? 256 : 1024) void norm_kernel(NormArgs a) {
   __shared__ float sums[1][16];
-  const int lane = ONE ? threadIdx.x & 63 : threadIdx.x;
-  const int step = ONE ? 512 : int(blockDim.x) * 8;
-  const int64_t row = ONE ? int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6) : int64_t(blockIdx.x);
-  if (ONE && row >= a.T) return;
+  const int lane = L > 0 ? threadIdx.x & (L - 1) : threadIdx.x;
+  const int step = int(blockDim.x) * 8;   // (of a second eight, of wide rows alone)
+  const int64_t mine = L > 0 ? int64_t(blockIdx.x) * (256 / (L > 0 ? L : 1)) + threadIdx.x / (L > 0 ? L : 1) : int64_t(blockIdx.x);
+  const bool in = mine < a.T;
+  const int64_t row = in ? mine : a.T - 1;   // past the end: the last row again, not stored
   const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
   Eight<T> xr[NC];
 #pragma unroll
@@ -321,8 +344,9 @@ __global__ __launch_bounds__(ONE ? 256 : 1024) void norm_kernel(NormArgs a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
   }
-  ss = row_sum<ONE>(ss, sums, 0, 0, int(blockDim.x >> 6));
+  ss = row_sum<L>(ss, sums, 0, 0, int(blockDim.x >> 6));
   const float r = 1.0f / sqrtf(ss / float(a.D) + a.eps);
+  if (!in) return;
   if (lane == 0) st_global(a.rstd + row, r);
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
@@ -378,12 +402,12 @@ struct NormRow {
   }
 };
 
-template <typename T, typename WT, int NC, bool ONE, bool TAIL, int STREAM>
-__global__ __launch_bounds__(ONE ? 512 : 1024) void norm_backward_kernel(NormBwdArgs a) {
+template <typename T, typename WT, int NC, int L, bool TAIL, int STREAM>
+__global__ __launch_bounds__(L > 0 ? 512 : 1024) void norm_backward_kernel(NormBwdArgs a) {
   extern __shared__ float4 shares4[];   // a team's dw [ld_p], if there are several
   __shared__ float sums[2][16];
-  const int width = ONE ? 64 : 64 * a.waves;   // threads of a team
-  const int team = ONE ? int(threadIdx.x >> 6) : int(threadIdx.x) / width, lane = int(threadIdx.x) - team * width;
+  const int width = L > 0 ? L : 64 * a.waves;   // threads of a team
+  const int team = int(threadIdx.x) / width, lane = int(threadIdx.x) - team * width;
   const int step = 8 * width;
   const int64_t r0 = int64_t(blockIdx.x) * a.rps, r1 = r0 + a.rps < a.T ? r0 + a.rps : a.T;
   const float inv_d = 1.0f / float(a.D);
@@ -399,7 +423,7 @@ __global__ __launch_bounds__(ONE ? 512 : 1024) void norm_backward_kernel(NormBwd
   }
   int parity = 0;
   // the next row's loads are in flight while this one is summed, where 128 registers hold both
-  constexpr bool kNext = ONE || (sizeof(T) == 2 && !TAIL);
+  constexpr bool kNext = L > 0 || (sizeof(T) == 2 && !TAIL);
   NormRow<T, NC, TAIL, STREAM> n, next;
   // a team without a row of its own reads the slice's last one again, with a dy of zeros
   auto load = [&](NormRow<T, NC, TAIL, STREAM>& to, int64_t i) {
@@ -428,7 +452,7 @@ __global__ __launch_bounds__(ONE ? 512 : 1024) void norm_backward_kernel(NormBwd
         dot = fmaf(g[c][j], xr[c][j], dot);
       }
     }
-    const float m = row_sum<ONE>(dot, sums, parity, team * a.waves, a.waves) * inv_d;
+    const float m = row_sum<L>(dot, sums, parity, team * a.waves, a.waves) * inv_d;
     if (row >= r1) continue;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -441,17 +465,28 @@ __global__ __launch_bounds__(ONE ? 512 : 1024) void norm_backward_kernel(NormBwd
   }
   if (a.part == nullptr) return;
   float* part = a.part + blockIdx.x * a.ld_p;   // ld_p is D rounded up to 8
-  if (a.teams == 1) {
+  // the rows side by side in a wave, then waves (L > 0) or teams one after the other
+  if constexpr (L > 0) {
+#pragma unroll
+    for (int off = L; off < 64; off <<= 1)
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pdw[c][j] += __shfl_xor(pdw[c][j], off);
+  }
+  const int turns = L > 0 ? int(blockDim.x >> 6) : a.teams, turn = L > 0 ? int(threadIdx.x >> 6) : team;
+  const bool one = L == 0 || (threadIdx.x & 63) < (L > 0 ? L : 64);
+  if (turns == 1) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int col = step * c + 8 * lane;
-      if (col < a.D) store8<float, false>(part + col, pdw[c], 8);
+      if (one && col < a.D) store8<float, false>(part + col, pdw[c], 8);
     }
     return;
   }
-  for (int t = 0; t < a.teams; ++t) {
+  for (int t = 0; t < turns; ++t) {
     if (t > 0) __syncthreads();
-    if (team != t) continue;
+    if (turn != t || !one) continue;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int col = step * c + 8 * lane;
@@ -509,14 +544,14 @@ __global__ __launch_bounds__(256) void norm_dw_kernel(const float* part, int64_t
 
 // ----------------------------------------------------------------- launches ----
 constexpr int64_t kMaxItems = int64_t(1) << 30;   // of one launch; longer matrices go in runs of rows
-constexpr int64_t kMaxCols = (int64_t(1) << 24) - 1;   // 128 rows stay below that
+constexpr int64_t kMaxCols = (int64_t(1) << 24) - 1;   // 128 rows stay below twice that
 constexpr int kNormMaxD = 16384;
 
 // Calls go(items, unroll tag, workgroups) over the eights of a [rows, cols] matrix.  Four eights a thread keep 64
 // bytes a lane in flight; a matrix that then leaves CUs without two workgroups takes one a thread.
-template <int UMAX, typename F>
+template <int UMAX, int EACH = 8, typename F>
 int for_items(int64_t rows, int64_t cols, F go) {
-  const int64_t per = (cols + kActBlock - 1) / kActBlock * (kActBlock / 8);
+  const int64_t per = (cols + kActBlock - 1) / kActBlock * (kActBlock / EACH);
   int64_t run = kMaxItems / per;
   run = run < 128 ? run : run / 128 * 128;   // whole 128-row tiles
   for (int64_t r = 0; r < rows; r += run) {
@@ -550,33 +585,42 @@ bool kept_ok(const void* q, int64_t ld_q, const void* codes, int64_t ld_c, int64
 
 // ---- the norm's shapes
 int norm_waves(int64_t D) { return int((D + 1023) / 1024); }
-// Teams of a workgroup of the backward, and its rows: one row each while 512 workgroups take all; else one round of the workgroups that fit
-// (sixteen waves to a CU), but no more than 512 of them: each writes D sums that the second launch reads.
+// Lanes of a narrow row, 0 for a wide one's waves.
+int norm_lanes(int64_t D) { return D > 512 ? 0 : D > 256 ? 64 : D > 128 ? 32 : D > 64 ? 16 : 8; }
+// Waves of a workgroup of the backward, and its teams (rows side by side): the fewest while 512 workgroups take all rows at once; else
+// eight waves or so, one round of the workgroups that fit (sixteen waves to a CU), but no more than 512 of them: each writes D sums
+// that the second launch reads.
+int norm_group_waves(int64_t T, int64_t D) {
+  const int w = D <= 512 ? 1 : norm_waves(D);
+  return T <= 512 || w > 4 ? w : 8 / w * w;
+}
 int norm_teams(int64_t T, int64_t D) {
-  if (T <= 512) return 1;
-  if (D <= 512) return 8;
-  const int w = norm_waves(D);
-  return w <= 4 ? 8 / w : 1;
+  const int waves = norm_group_waves(T, D);
+  return D <= 512 ? waves * 64 / norm_lanes(D) : waves / norm_waves(D);
 }
 int64_t norm_rows_per_slice(int64_t T, int64_t D) {
-  const int teams = norm_teams(T, D), waves = teams * (D <= 512 ? 1 : norm_waves(D));
-  int64_t most = int64_t(device_cus()) * (16 / waves);
+  const int teams = norm_teams(T, D);
+  int64_t most = int64_t(device_cus()) * (16 / norm_group_waves(T, D));
   most = most < 512 ? most : 512;
   const int64_t r = (T + most - 1) / most;
   return (r + teams - 1) / teams * teams;
 }
 
-// go(eights a lane, one wave to a row, a width that is no multiple of 8)
+// go(eights a lane, lanes of a row (0: waves), a width that is no multiple of 8)
 template <typename F>
 void for_norm(int64_t D, F go) {
-  using yes = std::true_type;
-  using no = std::false_type;
-  auto with_tail = [&](auto nc, auto one) {
-    if (D % 8) go(nc, one, yes{});
-    else go(nc, one, no{});
+  auto with_tail = [&](auto nc, auto lanes) {
+    if (D % 8) go(nc, lanes, std::true_type{});
+    else go(nc, lanes, std::false_type{});
   };
-  if (D <= 512) with_tail(std::integral_constant<int, 1>{}, yes{});
-  else with_tail(std::integral_constant<int, 2>{}, no{});
+  using one = std::integral_constant<int, 1>;
+  switch (norm_lanes(D)) {
+    case 8: with_tail(one{}, std::integral_constant<int, 8>{}); break;
+    case 16: with_tail(one{}, std::integral_constant<int, 16>{}); break;
+    case 32: with_tail(one{}, std::integral_constant<int, 32>{}); break;
+    case 64: with_tail(one{}, std::integral_constant<int, 64>{}); break;
+    default: with_tail(std::integral_constant<int, 2>{}, std::integral_constant<int, 0>{}); break;
+  }
 }
 
 }  // namespace
@@ -619,7 +663,7 @@ int fm_act8_restore(const void* q, int64_t ld_q, const void* codes, int64_t ld_c
   for_dtype(out_dtype, [&](auto t) {
     for_stream<0, 1>(rows * cols * int64_t(sizeof(t)), [&](auto stream_) {
       constexpr int kStream = decltype(stream_)::value;
-      for_items<4>(rows, cols, [&](const Items& items, auto u, unsigned wgs) {
+      for_items<4, 16 / sizeof(t)>(rows, cols, [&](const Items& items, auto u, unsigned wgs) {
         constexpr int U = decltype(u)::value;
         if (index) hipLaunchKernelGGL((restore_kernel<decltype(t), U, true, kStream>), dim3(wgs), dim3(256), 0, s, items, a);
         else hipLaunchKernelGGL((restore_kernel<decltype(t), U, false, kStream>), dim3(wgs), dim3(256), 0, s, items, a);
@@ -678,20 +722,19 @@ int fm_act8_rmsnorm(const void* x, int dtype, int64_t ld_x, int64_t T, int64_t D
   FM_REQUIRE(x && w && y && rstd && ld_x >= 0 && ld_y >= D, "fm_act8_rmsnorm: null pointer or bad pitch");
   FM_REQUIRE(kept_ok(q, ld_q, codes, ld_c, D) && ld_q == (D + 31) / 32 * 32, "fm_act8_rmsnorm: bad payload, codes or pitches");
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  // a launch has fewer than 2^32 threads
-  const int64_t each = D <= 512 ? 64 : 64 * norm_waves(D), run = (int64_t(1) << 31) / each;
+  const int lanes = norm_lanes(D), threads = lanes ? 256 : 64 * norm_waves(D), rows = lanes ? 256 / lanes : 1;   // of a workgroup
+  const int64_t run = (int64_t(1) << 31) / threads * rows;   // a launch has fewer than 2^32 threads
   for (int64_t r = 0; r < T; r += run) {
     const int64_t n = T - r < run ? T - r : run;
     for_dtype(dtype, [&](auto t) {
       const NormArgs a{static_cast<const decltype(t)*>(x) + r * ld_x, ld_x, n, int(D), w, eps, static_cast<decltype(t)*>(y) + r * ld_y, ld_y,
                        static_cast<uint8_t*>(q) + r * ld_q, ld_q, static_cast<uint8_t*>(codes) + r * ld_c, ld_c, rstd + r};
       for_dtype(w_dtype, [&](auto wt) {
-        for_norm(D, [&](auto nc, auto one, auto tail) {
-          constexpr bool kOne = decltype(one)::value;
+        for_norm(D, [&](auto nc, auto l, auto tail) {
           for_stream<0, 1>(T * D * int64_t(sizeof(t)), [&](auto stream_) {
-            hipLaunchKernelGGL((norm_kernel<decltype(t), decltype(wt), decltype(nc)::value, kOne, decltype(tail)::value,
+            hipLaunchKernelGGL((norm_kernel<decltype(t), decltype(wt), decltype(nc)::value, decltype(l)::value, decltype(tail)::value,
                                             decltype(stream_)::value>),
-                               dim3(unsigned(kOne ? (n + 3) / 4 : n)), dim3(kOne ? 256 : 64 * norm_waves(D)), 0, s, a);
+                               dim3(unsigned((n + rows - 1) / rows)), dim3(threads), 0, s, a);
           });
         });
       });
@@ -716,18 +759,18 @@ int fm_act8_rmsnorm_backward(const void* dy, int64_t ld_dy, int dtype, int64_t T
   FM_REQUIRE(dw == nullptr || (workspace && aligned16(workspace) && workspace_bytes >= fm_act8_rmsnorm_backward_workspace_bytes(T, D)),
              "fm_act8_rmsnorm_backward: dw needs a workspace of fm_act8_rmsnorm_backward_workspace_bytes(T, D) bytes on 16");
   const int64_t rps = norm_rows_per_slice(T, D), slices = (T + rps - 1) / rps, ld_p = (D + 7) / 8 * 8;
+  const int waves = norm_group_waves(T, D), turns = D <= 512 ? waves : norm_teams(T, D);   // shares of dw that meet in LDS
   float* part = static_cast<float*>(workspace);
   const NormBwdArgs a{dy, ld_dy, Act8{static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(codes), ld_q, ld_c}, T, int(D), w, rstd,
                       dx, ld_dx, dw ? part : nullptr, ld_p, rps, D <= 512 ? 1 : norm_waves(D), norm_teams(T, D)};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   for_dtype(dtype, [&](auto t) {
     for_dtype(w_dtype, [&](auto wt) {
-      for_norm(D, [&](auto nc, auto one, auto tail) {
-        constexpr bool kOne = decltype(one)::value;
+      for_norm(D, [&](auto nc, auto l, auto tail) {
         for_stream<0, 1, 2>(T * D * int64_t(sizeof(t)), [&](auto stream_) {
-          hipLaunchKernelGGL((norm_backward_kernel<decltype(t), decltype(wt), decltype(nc)::value, kOne, decltype(tail)::value,
+          hipLaunchKernelGGL((norm_backward_kernel<decltype(t), decltype(wt), decltype(nc)::value, decltype(l)::value, decltype(tail)::value,
                                                    decltype(stream_)::value>),
-                             dim3(unsigned(slices)), dim3(64 * a.waves * a.teams), a.teams > 1 && a.part ? unsigned(ld_p * 4) : 0u, s, a);
+                             dim3(unsigned(slices)), dim3(64 * waves), dw && turns > 1 ? unsigned(ld_p * 4) : 0u, s, a);
         });
       });
     });

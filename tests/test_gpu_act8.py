@@ -253,7 +253,8 @@ def norm_ref(x, w, dy, eps):
 @pytest.mark.parametrize("wdtype", [F32, BF])
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("shape", [(1, 1), (1, 9), (3, 31), (5, 512), (9, 513), (2, 5, 1000), (33, 1024), (37, 1025), (130, 2048), (37, 2831),
-                                   (19, 7168), (3, 16384), (2, 16383), (4100, 256), (8200, 40)])
+                                   (19, 7168), (3, 16384), (2, 16383), (4100, 256), (8200, 40),
+                                   (1, 64), (7, 65), (9, 128), (600, 130), (515, 300), (513, 512), (5000, 17), (700, 4096)])
 def test_rmsnorm(dev, shape, dtype, wdtype):
     g = gen(shape[0] + shape[-1])
     x, dy = activation(g, *shape, dtype=dtype), activation(g, *shape, dtype=dtype) * 1e-2
