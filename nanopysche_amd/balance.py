@@ -71,6 +71,8 @@ def _check(logits, indices, cu_seqlens, token_mask, load_tracker):
     if indices.dim() < 1 or not 1 <= indices.shape[-1] <= MAX_BALANCE_TOP_K or indices.shape[:-1] != logits.shape[:-1]:
         raise ValueError(f"indices must be [..., K] for the logits' {tuple(logits.shape[:-1])} tokens, K of 1 to {MAX_BALANCE_TOP_K}, got "
                          f"{tuple(indices.shape)}")
+    if T * indices.shape[-1] >= 2 ** 31:   # the counts are int32
+        raise ValueError(f"fewer than 2^31 slots, got {T} tokens of {indices.shape[-1]}")
     idx = indices if indices.dim() == 2 else indices.reshape(T, indices.shape[-1])
     if not idx.is_contiguous():
         idx = idx.contiguous()

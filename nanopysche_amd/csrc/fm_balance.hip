@@ -732,6 +732,7 @@ int fm_balance_forward(const float* logits, int64_t ld, int64_t T, int E, const 
   if (int rc = check_balance(b, "fm_balance_forward")) return rc;
   FM_REQUIRE(K >= 1 && K <= 1024 && (T == 0 || indices), "fm_balance_forward: null indices or bad K");
   FM_REQUIRE(inverse && loss && (S == 0 || (f && counts)), "fm_balance_forward: null output");
+  FM_REQUIRE(T * K < (int64_t(1) << 31), "fm_balance_forward: fewer than 2^31 slots");
   const Space w = space_of(T, E, S);
   FM_REQUIRE(ws && aligned16(ws) && workspace_bytes >= w.bytes, "fm_balance_forward: the workspace must hold fm_balance_workspace_bytes(T, E, S) "
              "bytes on 16");

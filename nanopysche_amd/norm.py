@@ -174,7 +174,11 @@ class RMSNorm(torch.nn.Module):
         if not full_precision:
             raise NotImplementedError("the MI355X RMSNorm computes in fp32 (full_precision=True)")
         self.checkpoint_8bit = bool(checkpoint_8bit)
-        if not self.checkpoint_8bit:
+        if self.checkpoint_8bit:
+            from .act8 import MAX_ACT8_NORM, _check_cols
+
+            _check_cols(size, MAX_ACT8_NORM)
+        else:
             _check_d(size)
         self.eps = eps
         self.full_precision = True

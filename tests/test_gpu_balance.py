@@ -290,3 +290,16 @@ def test_tensors_elsewhere_are_refused(dev):
             call()
     with pytest.raises(ValueError, match="load_tracker"):
         fm.balance_loss(logits, idx, load_tracker=fm.ExpertLoadTracker(9, "cuda"))
+
+
+def test_offsets_past_32_bits(dev):
+    """Logits and gradients whose rows lie 2^20 apart: the last ones are past 2^31 elements."""
+    T, E, far = 2100, 8, 2 ** 20
+    logits, idx = inputs(T, E, 2, 30)
+    l = torch.empty(T * far, device="cuda").as_strided((T, E), (far, 1)).copy_(logits)
+    d = torch.empty(T * far, device="cuda").as_strided((T, E), (far, 1)).zero_()
+    one = torch.ones((), device="cuda")
+    loss, counts, state = fm.balance_forward(l, idx)
+    near, near_counts, near_state = fm.balance_forward(logits, idx)
+    assert torch.equal(loss, near) and torch.equal(counts, near_counts)
+    assert torch.equal(fm.balance_backward(state, one, add_to=d), fm.balance_backward(near_state, one))

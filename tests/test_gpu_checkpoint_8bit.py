@@ -325,3 +325,29 @@ def test_mask_changed_in_place_is_noticed(dev):
     mask[3] = False
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         aux.backward()
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(pre_norm=True, shared=128), dict(capacity_factor=8.0)])
+def test_layer_of_one_token_that_does_not_count(dev, kw):
+    layer, p = layer_of("flow_moe", 512, 128, 8, 2, 70, True, **dict(kw))
+    x = rand(torch.Generator().manual_seed(71), 1, 512).requires_grad_(True)
+    out, aux = layer(x, token_mask=torch.zeros(1, dtype=torch.bool, device="cuda"))
+    assert out.shape == (1, 512) and out.any() and aux == 0
+    torch.autograd.backward([out, aux], [torch.ones_like(out), torch.ones_like(aux)])
+    assert torch.isfinite(x.grad).all() and x.grad.any()
+    assert all(v.grad is None or torch.isfinite(v.grad).all() for v in p.values())
+    with pytest.raises(ValueError, match="at least one token"):
+        layer(x[:0], token_mask=torch.zeros(0, dtype=torch.bool, device="cuda"))
+
+
+@pytest.mark.parametrize("pre_norm", [False, True])
+def test_layer_of_fp32_tokens(dev, pre_norm):
+    """fp32 tokens are rounded to bf16 where the layer takes them in: its results are those of the rounded ones."""
+    res = []
+    for x in (rand(torch.Generator().manual_seed(81), 300, 512).float(), rand(torch.Generator().manual_seed(81), 300, 512)):
+        layer, p = layer_of("none", 512, 128, 8, 2, 80, True, pre_norm=pre_norm)
+        leaf = x.requires_grad_(True)
+        out, aux = layer(leaf)
+        torch.autograd.backward([out, aux], [torch.ones_like(out), torch.ones_like(aux)])
+        res.append((out.bfloat16(), aux, leaf.grad.bfloat16(), *(v.grad for v in p.values())))
+    assert all(torch.equal(a, b) for a, b in zip(*res))

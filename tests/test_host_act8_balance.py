@@ -210,3 +210,21 @@ def test_the_library_refuses_before_a_launch():
     bad(b"16 bytes", lib.fm_act8_swiglu_backward_quantize(p, 256, p, 8, C.c_void_p(264), 128, 128, 128, 0, p, 256, None, 0, None, 0, None, 0, None, None))
     bad(b"16 bytes", lib.fm_act8_router_weight_grad(p, 100, p, 128, p, 4, p, 4, 2, 128, p, None))
     bad(b"pitch", lib.fm_balance_backward(p, 8, 100, 8, p, 3, None, 0, 0.0, p, p, p, p, 7, 0, None))
+
+
+def test_more_slots_than_the_counts_hold_are_refused(launched):  # noqa: F811
+    l, i = torch.zeros(1, 4).expand(2 ** 21, 4), torch.zeros(1, 1, dtype=torch.int32).expand(2 ** 21, 1024)
+    with pytest.raises(ValueError, match=r"fewer than 2\^31 slots"):
+        fm.balance_loss(l, i)
+    assert launched == []
+    lib, p = _lib.load(), C.c_void_p(256)
+    need = lib.fm_balance_workspace_bytes(2 ** 21, 4, 1)
+    assert lib.fm_balance_forward(p, 4, 2 ** 21, 4, p, 0, 1024, None, 1, None, 0, 0.0, p, p, p, p, None, None, p, need, None) != 0
+    assert b"fewer than 2^31 slots" in lib.fm_last_error_string()
+
+
+def test_norm_module_checks_its_size():
+    for size in (0, MAX_ACT8_NORM + 1):
+        with pytest.raises(ValueError, match="columns"):
+            fm.RMSNorm(size, checkpoint_8bit=True)
+    assert fm.RMSNorm(1000, checkpoint_8bit=True).weight.shape == (1000,)
