@@ -165,17 +165,17 @@ struct Row {
   }
 };
 
-// Steps whose loads are in flight at once: four, as long as they stay within the shortest run.
-template <int L>
+// Steps whose loads are in flight at once: four, as long as they stay within the shortest run; two of eight values side by side.
+template <int L, int NV>
 constexpr int ahead() {
-  return 16 * L / 64 >= 4 ? 4 : (16 * L / 64 >= 2 ? 2 : 1);
+  return 16 * L / 64 >= 4 ? (NV > 4 && L < 64 ? 2 : 4) : (16 * L / 64 >= 2 ? 2 : 1);
 }
 
 // Piece p's sums and counts, by one wave (its own hist) or a workgroup of TEAM (one hist; sums and small hold a row for each wave).
 template <int L, int NV, bool QUADS, int TEAM>
 __device__ __forceinline__ void sum_piece(const BalanceArgs& a, int64_t p, int32_t* hist, float* sums, float (*small)[2]) {
   using R = Row<L, NV, QUADS>;
-  constexpr int kSide = 64 / L, kAhead = ahead<L>();   // tokens side by side
+  constexpr int kSide = 64 / L, kAhead = ahead<L, NV>();   // tokens side by side
   const int lane = threadIdx.x & 63, l = lane & (L - 1), sub = lane / L;
   const int wave = TEAM == 1 ? 0 : threadIdx.x >> 6, me = TEAM == 1 ? lane : threadIdx.x;
   const Piece piece = piece_of(a, p, lane);
@@ -401,28 +401,34 @@ __device__ __forceinline__ void places_of(const BalanceArgs& b, int64_t s, int64
 struct Column {
   float p, z;
   int32_t slots, tokens;
-  // places first + g, first + g + step, ..: four places' loads at once
+  // places first + g, first + g + step, ..: the loads of U places at once
+  template <int U>
   __device__ __forceinline__ void add(const BalanceArgs& b, int64_t first, int64_t n, int g, int step, int col) {
-    for (int64_t k = g; k < n; k += 4 * step) {
-      float pk[4], zk[4];
-      int32_t mk[4], tk[4];
+    for (int64_t k = g; k < n; k += U * step) {
+      float pk[U] = {}, zk[U] = {};
+      int32_t mk[U] = {}, tk[U] = {};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t at = first + (k + i * step < n ? k + i * step : k);
+      for (int i = 0; i < U; ++i) {
+        if (k + i * step >= n) continue;
+        const int64_t at = first + k + i * step;
         pk[i] = b.sums[at * b.E + col];
         mk[i] = b.slots[at * b.E + col];
         tk[i] = b.tokens[at];
         zk[i] = b.z[at];
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (k + i * step >= n) break;
-        p += pk[i];
-        slots += mk[i];
-        tokens += tk[i];
-        z += zk[i];
-      }
+      for (int i = 0; i < U; ++i) add(Column{pk[i], zk[i], mk[i], tk[i]});
     }
+  }
+  __device__ __forceinline__ void add(const Column& c) {
+    p += c.p;
+    z += c.z;
+    slots += c.slots;
+    tokens += c.tokens;
+  }
+  // the sum over lanes `from`, 2 from, .. below `to` apart
+  __device__ __forceinline__ void join(int from, int to) {
+    for (int off = from; off < to; off <<= 1) add(Column{__shfl_xor(p, off), __shfl_xor(z, off), __shfl_xor(slots, off), __shfl_xor(tokens, off)});
   }
   // writes f and the count; this column's share of the loss
   __device__ __forceinline__ float write(const FoldArgs& a, int64_t at) const {
@@ -434,49 +440,50 @@ struct Column {
   }
 };
 
-// WHOLE: a workgroup to 16 columns of a sequence, of 64 rows of threads; else a wave, of four rows, and sixteen of them to a
-// workgroup.  Each row adds every so many places, then the rows' sums meet in order.  The only workgroup finishes the loss too.
-template <bool WHOLE>
-__global__ __launch_bounds__(1024) void balance_fold_kernel(FoldArgs a, int column_groups, FinishArgs fin) {
-  const int64_t unit = WHOLE ? int64_t(blockIdx.x) : int64_t(blockIdx.x) * 16 + (threadIdx.x >> 6);
-  const int64_t s = unit / column_groups;
-  const int part = int(unit - s * column_groups);
-  const int q = threadIdx.x & 15, e = part * 16 + q, col = e < a.b.E ? e : a.b.E - 1;
-  Column c{0.f, 0.f, 0, 0};
-  if (WHOLE || s < a.b.S) {
-    int64_t first, n;
-    places_of(a.b, s, first, n);
-    c.add(a.b, first, n, WHOLE ? threadIdx.x >> 4 : (threadIdx.x >> 4) & 3, WHOLE ? 64 : 4, col);
-  }
-  // the four rows of a wave
-#pragma unroll
-  for (int off = 16; off < 64; off <<= 1) {
-    c.p += __shfl_xor(c.p, off);
-    c.z += __shfl_xor(c.z, off);
-    c.slots += __shfl_xor(c.slots, off);
-    c.tokens += __shfl_xor(c.tokens, off);
-  }
-  bool mine = (threadIdx.x & 63) < 16 && s < a.b.S;
-  if constexpr (WHOLE) {   // and the sixteen waves
-    __shared__ Column waves[16][16];
-    if ((threadIdx.x & 63) < 16) waves[threadIdx.x >> 6][q] = c;
-    __syncthreads();
-    mine = threadIdx.x < 16;
-    if (mine) {
-      c = waves[0][q];
-      for (int i = 1; i < 16; ++i) {
-        c.p += waves[i][q].p;
-        c.z += waves[i][q].z;
-        c.slots += waves[i][q].slots;
-        c.tokens += waves[i][q].tokens;
-      }
+// C columns of each of 1024 / (C ROWS) sequences to a workgroup: a sequence's ROWS rows of threads (of one wave, or of all sixteen) add every
+// so many places, then the rows' sums meet in order.  Sequences of more than LONG places, which would hold their rows up, are the whole
+// workgroup's, one after the other.  The only workgroup finishes the loss too.
+template <int C, int ROWS, int LONG>
+__global__ __launch_bounds__(1024, ROWS == 1 ? 8 : 4) void balance_fold_kernel(FoldArgs a, int parts, FinishArgs fin) {
+  constexpr int kSeqs = 1024 / (C * ROWS), kAtOnce = ROWS == 1 ? 2 : 4;
+  __shared__ Column waves[16][C];
+  __shared__ bool many[kSeqs];
+  const int64_t block = blockIdx.x / uint32_t(parts);
+  const int q = threadIdx.x & (C - 1), row = (threadIdx.x / C) & (ROWS - 1), mine = threadIdx.x / (C * ROWS);
+  const int e = int(blockIdx.x - block * parts) * C + q, col = e < a.b.E ? e : a.b.E - 1;
+  const int64_t s = block * kSeqs + mine;
+  int64_t first = 0, n = 0;
+  if (s < a.b.S) places_of(a.b, s, first, n);
+  Share v{0.f, 0.f, 0, 0};
+  auto done = [&](const Column& c, int64_t seq) {
+    if (e < a.b.E) v.loss += c.write(a, seq * a.b.E + e);
+    if (e == 0) {
+      v.z += c.z;
+      v.tokens += c.tokens;
+      v.filled += c.tokens > 0;
     }
-  }
-  Share v{mine && e < a.b.E ? c.write(a, s * a.b.E + e) : 0.f, 0.f, 0, 0};
-  if (mine && e == 0) {
-    v.z = c.z;
-    v.tokens = c.tokens;
-    v.filled = c.tokens > 0;
+  };
+  if (q == 0 && row == 0) many[mine] = n > LONG;
+  Column c{0.f, 0.f, 0, 0};
+  if (n <= LONG) c.add<kAtOnce>(a.b, first, n, row, ROWS, col);
+  if constexpr (ROWS * C <= 64) c.join(C, C * ROWS);   // else there are none to add
+  if (row == 0 && s < a.b.S && n <= LONG) done(c, s);
+  if (__syncthreads_or(n > LONG)) {
+    for (int i = 0; i < kSeqs; ++i) {
+      if (!many[i]) continue;
+      places_of(a.b, block * kSeqs + i, first, n);
+      Column d{0.f, 0.f, 0, 0};
+      d.add<kAtOnce>(a.b, first, n, threadIdx.x / C, 1024 / C, col);
+      d.join(C, 64);
+      if ((threadIdx.x & 63) < C) waves[threadIdx.x >> 6][q] = d;
+      __syncthreads();
+      if (threadIdx.x < C) {
+        d = waves[0][q];
+        for (int w = 1; w < 16; ++w) d.add(waves[w][q]);
+        done(d, block * kSeqs + i);
+      }
+      __syncthreads();
+    }
   }
   if (gridDim.x == 1) {
     finish(fin, v);
@@ -500,7 +507,7 @@ __global__ __launch_bounds__(1024) void balance_one_kernel(FoldArgs a, FinishArg
     Column c{0.f, 0.f, 0, 0};
     int64_t first, n;
     places_of(a.b, s, first, n);
-    c.add(a.b, first, n, 0, 1, e);
+    c.add<4>(a.b, first, n, 0, 1, e);
     v.loss += c.write(a, i);
     if (e == 0) {
       v.z += c.z;
@@ -560,7 +567,7 @@ __global__ __launch_bounds__(256) void balance_backward_kernel(BalanceBwdArgs a)
   using R = Row<L, NV, QUADS>;
   const BalanceArgs& b = a.b;
   const int lane = threadIdx.x & 63, l = lane & (L - 1), sub = lane / L;
-  constexpr int kSide = 64 / L, kAhead = ahead<L>();
+  constexpr int kSide = 64 / L, kAhead = ahead<L, NV>();
   const int64_t p = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (p >= b.places) return;
   const Piece piece = piece_of(b, p, lane);
@@ -645,7 +652,7 @@ void for_experts(int E, F go) {
     else if (E <= 32) FM_ROW(8, 4, true);
     else if (E <= 64) FM_ROW(16, 4, true);
     else if (E <= 128) FM_ROW(32, 4, true);
-    else if (E <= 256) FM_ROW(64, 4, true);
+    else if (E <= 256) FM_ROW(32, 8, true);   // 65536 x 256: sums 19.3 us, backward 25.3; of (64, 4): 21 and 26.5
     else if (E <= 512) FM_ROW(64, 8, true);
     else FM_ROW(64, 16, true);
   } else {
@@ -749,7 +756,7 @@ int fm_balance_forward(const float* logits, int64_t ld, int64_t T, int E, const 
   if (w.places <= kOnePieces && T * E <= kOneLogits && E <= 256 && S * E <= kOneColumns) {
     const int64_t waves = w.places < 16 ? w.places : 16;
     for_experts(E, [&](auto l, auto n, auto q) {
-      if constexpr (decltype(n)::value <= 4)
+      if constexpr (decltype(n)::value <= 8)
         hipLaunchKernelGGL((balance_one_kernel<decltype(l)::value, decltype(n)::value, decltype(q)::value>), dim3(1), dim3(unsigned(64 * waves)),
                            unsigned(waves * E * sizeof(int32_t)), s, fold, fin);
     });
@@ -767,12 +774,19 @@ int fm_balance_forward(const float* logits, int64_t ld, int64_t T, int E, const 
         if (w.team == 4) hipLaunchKernelGGL((balance_sums_kernel<L, N, Q, 4>), dim3(unsigned(w.places)), dim3(256), unsigned(5 * E * 4), s, b);
         else hipLaunchKernelGGL((balance_sums_kernel<L, N, Q, 1>), dim3(unsigned((w.places + 3) / 4)), dim3(256), unsigned(4 * E * 4), s, b);
       });
-    // 16 columns of a sequence to a wave while sequences have 64 places or fewer on average, then to a workgroup
-    const int groups = (E + 15) / 16;
-    const bool whole = w.runs > 64 * S;
-    fin.parts = whole ? S * groups : (S * groups + 15) / 16;
-    if (whole && S > 0) hipLaunchKernelGGL(balance_fold_kernel<true>, dim3(unsigned(fin.parts)), dim3(1024), 0, s, fold, groups, fin);
-    else if (S > 0) hipLaunchKernelGGL(balance_fold_kernel<false>, dim3(unsigned(fin.parts)), dim3(1024), 0, s, fold, groups, fin);
+    // Sequences of more than 64 places on average take a workgroup for 16 columns; from four on, or while the rows do not fill the CUs,
+    // four rows of a wave; below that a row.  131072 tokens of 64, 30000 sequences: 58 us by four rows, 20 by one; 65536 of 128, 512
+    // sequences: 6.7 and 7.3.
+    auto fold_by = [&](auto c, auto rows, auto most) {
+      constexpr int C = decltype(c)::value, R = decltype(rows)::value, M = decltype(most)::value, G = 1024 / (C * R);
+      const int parts = (E + C - 1) / C;
+      fin.parts = (S + G - 1) / G * parts;
+      if (S > 0) hipLaunchKernelGGL((balance_fold_kernel<C, R, M>), dim3(unsigned(fin.parts)), dim3(1024), 0, s, fold, parts, fin);
+    };
+    if (w.runs > 64 * S) fold_by(std::integral_constant<int, 16>{}, std::integral_constant<int, 64>{}, std::integral_constant<int, 0>{});
+    else if (w.runs > 4 * S || S * E <= 1 << 17) fold_by(std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{}, std::integral_constant<int, 256>{});
+    else if (E > 32) fold_by(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
+    else fold_by(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
     if (fin.parts != 1) hipLaunchKernelGGL(balance_finish_kernel, dim3(1), dim3(1024), 0, s, fin);
   }
   if (acc && S > 0) hipLaunchKernelGGL(balance_track_kernel, dim3(unsigned(E)), dim3(256), 0, s, counts, S, E, acc);

@@ -303,3 +303,12 @@ def test_offsets_past_32_bits(dev):
     near, near_counts, near_state = fm.balance_forward(logits, idx)
     assert torch.equal(loss, near) and torch.equal(counts, near_counts)
     assert torch.equal(fm.balance_backward(state, one, add_to=d), fm.balance_backward(near_state, one))
+
+
+@pytest.mark.parametrize("S,E", [(3000, 64), (3000, 256), (9000, 20), (200, 24)])
+def test_one_long_sequence_among_short_ones(dev, S, E):
+    """Sequences of one token, an empty one, and two that hold nearly all."""
+    logits, idx = inputs(70000, E, 2, 40)
+    half = S // 2
+    borders = [*range(half), half - 1, 50000, *range(50001, 50000 + S - half), 70000]
+    check(logits, idx, borders, torch.rand(70000, generator=gen(41), device="cuda") < 0.9)
