@@ -28,14 +28,17 @@ __device__ __forceinline__ float exp_neg(float g) {
 // the reference's torch silu and its backward (x / (1 + exp(-x)), sigmoid =
 // 1 / (1 + exp(-x))).  Quotients from the hardware reciprocal with a
 // residual correction (within an ulp of the rounded quotient).  d infinite
-// (g < -88.7): sigmoid 0 and silu -0, as IEEE division gives.
-__device__ __forceinline__ float silu_only(float g) {
+// (g < -88.7): sigmoid 0 and silu -0, as IEEE division gives; g infinite: silu
+// infinite, where the residual is infinity less infinity (and a NaN is itself).
+__device__ __forceinline__ float silu_quotient(float g, float d, float r) {
 #pragma clang fp contract(off)
-  const float d = 1.f + exp_neg(g);
-  const float r = __builtin_amdgcn_rcpf(d);
   const float q0 = g * r;
   const float q = fmaf(fmaf(-d, q0, g), r, q0);
-  return d <= 3.40282347e38f ? q : g * 0.f;
+  return d <= 3.40282347e38f ? (g <= 3.40282347e38f ? q : g) : g * 0.f;
+}
+__device__ __forceinline__ float silu_only(float g) {
+  const float d = 1.f + exp_neg(g);
+  return silu_quotient(g, d, __builtin_amdgcn_rcpf(d));
 }
 
 struct SigSilu {
@@ -46,14 +49,12 @@ __device__ __forceinline__ SigSilu sig_silu(float g) {
   const float d = 1.f + exp_neg(g);
   float r = __builtin_amdgcn_rcpf(d);
   r = fmaf(fmaf(-d, r, 1.f), r, r);
-  const float q0 = g * r;
-  const float q = fmaf(fmaf(-d, q0, g), r, q0);
-  const bool fin = d <= 3.40282347e38f;
-  return SigSilu{fin ? r : 0.f, fin ? q : g * 0.f};
+  return SigSilu{d <= 3.40282347e38f ? r : 0.f, silu_quotient(g, d, r)};
 }
 
 // SwiGLU of eight values and its backward, every product and sum rounded (the same values in every kernel that inlines them):
-// h = silu(g) u; torch autograd of it: dg = (dh u) s (1 + g (1 - s)), du = dh silu(g), each operation rounded in this order.
+// h = silu(g) u; torch autograd of it: dg = (dh u) s (1 + g (1 - s)), du = dh silu(g), each operation rounded in this order (an
+// infinite g gives a NaN dg there and here).
 __device__ __forceinline__ void swiglu8(const float (&g)[8], const float (&u)[8], float (&h)[8]) {
 #pragma clang fp contract(off)
 #pragma unroll
