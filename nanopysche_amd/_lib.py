@@ -14,6 +14,7 @@ import threading
 from pathlib import Path
 
 import torch
+import torch.autograd.forward_ad as fwAD
 
 LIB_PATH = Path(__file__).resolve().parent / "libfm_hip.so"
 
@@ -264,6 +265,20 @@ def require_device(t: torch.Tensor, name: str = "tensor") -> None:
         raise RuntimeError(
             f"{name} must be on a ROCm device: the fp8_flow_moe kernels run only on the GPU "
             "(there is no CPU fallback)")
+
+
+def carried(*tensors):
+    """"gradient" where autograd would record a call of these tensors, "tangent" where forward mode would; else None."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return "gradient"
+    # tangents live inside a dual level, whether or not gradients are recorded
+    if fwAD._current_level >= 0 and torch._C._is_fwd_grad_enabled():
+        for t in tensors:
+            if t is not None and fwAD.unpack_dual(t).tangent is not None:
+                return "tangent"
+    return None
 
 
 def stream_of(t: torch.Tensor) -> int:

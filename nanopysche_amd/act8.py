@@ -19,6 +19,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
+import torch.autograd.forward_ad as fwAD
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -50,6 +51,15 @@ def _dtype(dtype: torch.dtype, what: str) -> int:
     if code is None:
         raise TypeError(f"{what} must be bfloat16 or float32, got {dtype}")
     return code
+
+
+def _no_gradients(name: str, instead: str, *tensors) -> None:
+    if not torch.is_grad_enabled() and fwAD._current_level < 0:   # as inside an autograd node: nothing is recorded
+        return
+    carried = _lib.carried(*tensors)
+    if carried:
+        raise RuntimeError(f"{name} records no {carried}: {instead} is differentiable (once, in reverse mode); call {name} under "
+                           "torch.no_grad() or on detached tensors")
 
 
 class Activation8:
@@ -123,7 +133,7 @@ class Activation8:
         return q, q + rows * pitch, pitch, pitch // ACT8_BLOCK
 
     def restore(self, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-        """The values that the 8 bits stand for, in ``out_dtype`` (default: the activation's type)."""
+        """The values that the 8 bits stand for, in ``out_dtype`` (default: the activation's type); they carry no gradient."""
         return _restore(self, None, self.rows, self._shape, out_dtype or self._dtype)
 
     def restore_rows(self, index: torch.Tensor, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
@@ -190,7 +200,8 @@ def _compress(x2: torch.Tensor, shape, tile_valid=None) -> Activation8:
 
 
 def compress_activation(x: torch.Tensor) -> Activation8:
-    """x [..., cols] (bf16 or fp32) in 8 bits.  Not differentiable: what a forward keeps of x for its backward."""
+    """x [..., cols] (bf16 or fp32) in 8 bits.  Not differentiable (x may require a gradient, which does not reach it through
+    what is kept): what a forward keeps of x for its backward."""
     x2 = _rows(x, "x")
     return _compress(x2, x.shape)
 
@@ -221,7 +232,9 @@ def _halves(gate: torch.Tensor, up: Optional[torch.Tensor]):
 
 def swiglu_compress(gate: torch.Tensor, up: Optional[torch.Tensor] = None) -> SwigluKept:
     """h = silu(gate) * up (fp32 arithmetic, rounded once) and gate and up in 8 bits, in one pass.
-    gate and up [..., H], bf16 or fp32, or one tensor [..., 2H] of the gate's columns and then up's."""
+    gate and up [..., H], bf16 or fp32, or one tensor [..., 2H] of the gate's columns and then up's.  Records no gradient, and
+    refuses tensors that want one recorded: ``swiglu_8bit``."""
+    _no_gradients("swiglu_compress", "swiglu_8bit", gate, up)
     g2, u2, at_u, shape = _halves(gate, up)
     H, rows, dtype, dev = shape[-1], g2.shape[0], g2.dtype, g2.device
     h = torch.empty(shape, dtype=dtype, device=dev)
@@ -236,7 +249,8 @@ def swiglu_compress(gate: torch.Tensor, up: Optional[torch.Tensor] = None) -> Sw
 
 def swiglu_backward_8bit(dh: torch.Tensor, gate: Activation8, up: Activation8, packed: bool = False):
     """(dgate, dup) of ``swiglu_compress`` from dh [..., H] and what it kept, in dh's type; with ``packed`` one
-    tensor [..., 2H]."""
+    tensor [..., 2H].  Records no gradient, as its forward."""
+    _no_gradients("swiglu_backward_8bit", "swiglu_8bit", dh)
     if dh.shape != gate.shape or up.shape != gate.shape:
         raise ValueError(f"dh, gate and up must be alike, got {tuple(dh.shape)}, {tuple(gate.shape)} and {tuple(up.shape)}")
     d2 = _rows(dh, "dh")
@@ -298,7 +312,9 @@ def _norm_weight(weight: torch.Tensor, D: int) -> torch.Tensor:
 
 def rmsnorm_compress(x: torch.Tensor, weight: torch.Tensor, eps: float = DEFAULT_EPS) -> RMSNormKept:
     """y = x * rsqrt(mean(x^2) + eps) * weight (fp32 arithmetic, rounded once to x's type) and x in 8 bits,
-    in one pass.  x [..., D] and weight [D] bf16 or fp32, D up to 16384."""
+    in one pass.  x [..., D] and weight [D] bf16 or fp32, D up to 16384.  Records no gradient, and refuses tensors that want one
+    recorded: ``rmsnorm_8bit``."""
+    _no_gradients("rmsnorm_compress", "rmsnorm_8bit", x, weight)
     x2 = _rows(x, "x", MAX_ACT8_NORM)
     T, D = x2.shape
     w = _norm_weight(weight, D)
@@ -315,7 +331,9 @@ def rmsnorm_compress(x: torch.Tensor, weight: torch.Tensor, eps: float = DEFAULT
 
 
 def rmsnorm_backward_8bit(dy: torch.Tensor, x: Activation8, weight: torch.Tensor, rstd: torch.Tensor, need_dw: bool = True):
-    """(dx in dy's type, dw in weight's or None) of ``rmsnorm_compress`` from dy [..., D] and what it kept."""
+    """(dx in dy's type, dw in weight's or None) of ``rmsnorm_compress`` from dy [..., D] and what it kept.  Records no gradient,
+    as its forward."""
+    _no_gradients("rmsnorm_backward_8bit", "rmsnorm_8bit", dy, weight)
     if dy.shape != x.shape:
         raise ValueError(f"dy must be {tuple(x.shape)}, got {tuple(dy.shape)}")
     d2 = _rows(dy, "dy", MAX_ACT8_NORM)

@@ -129,7 +129,7 @@ def balance_forward(logits: torch.Tensor, indices: torch.Tensor, *, cu_seqlens: 
 
 def balance_backward(state: BalanceState, dloss: torch.Tensor, add_to: Optional[torch.Tensor] = None) -> torch.Tensor:
     """dlogits (fp32, the logits' shape): dloss (0-d fp32) times the loss's gradient, zeros for tokens
-    that do not count.  ``add_to`` ([T, E] fp32): added to it in place instead."""
+    that do not count.  ``add_to`` ([T, E] fp32): added to it in place instead.  Records no gradient."""
     l2, cu = state.logits, state.cu_seqlens
     T, E = l2.shape
     S = 1 if cu is None else cu.numel() - 1
