@@ -681,10 +681,14 @@ int run_of(int64_t T, int E) {
 }
 // Waves to a piece: four where sequences have 64 tokens on average, sixteen from 1024 on; the fewer places to write and add.  One
 // sequence of 65536 tokens, 256 experts: fold 11.5 us of 1024 places, 7.0 of 256.
-// (Beyond 512 experts sixteen waves of a row's registers do not fit.)
+// (Sixteen waves' registers do not fit where a lane holds sixteen values of a row: beyond 512 experts, beyond 256 of no multiple of 4.
+// 65536 x 511 of one sequence: 57 us the forward in pieces of four, 249 in pieces cut for sixteen and taken by one.)
+constexpr int kTeamMaxValues = 8;   // of a lane, for sixteen waves
 int team_of(int64_t T, int E, int64_t S) {
   if (T <= 16 * run_of(T, E) || T < 64 * S) return 1;
-  return T < 1024 * S || E > 512 ? 4 : 16;
+  int values = 0;
+  for_experts(E, [&](auto, auto n, auto) { values = decltype(n)::value; });
+  return T < 1024 * S || values > kTeamMaxValues ? 4 : 16;
 }
 
 struct Space {
@@ -761,19 +765,23 @@ int fm_balance_forward(const float* logits, int64_t ld, int64_t T, int E, const 
                            unsigned(waves * E * sizeof(int32_t)), s, fold, fin);
     });
   } else {
+    // pieces are cut for w.team waves: another kernel's would leave waves idle
+    bool fits = true;
     if (w.runs > 0 && S > 0)
       for_experts(E, [&](auto l, auto n, auto q) {
         constexpr int L = decltype(l)::value, N = decltype(n)::value;
         constexpr bool Q = decltype(q)::value;
-        if constexpr (N <= 8) {
+        if constexpr (N <= kTeamMaxValues) {
           if (w.team == 16) {
             hipLaunchKernelGGL((balance_sums_kernel<L, N, Q, 16>), dim3(unsigned(w.places)), dim3(1024), unsigned(17 * E * 4), s, b);
             return;
           }
         }
         if (w.team == 4) hipLaunchKernelGGL((balance_sums_kernel<L, N, Q, 4>), dim3(unsigned(w.places)), dim3(256), unsigned(5 * E * 4), s, b);
-        else hipLaunchKernelGGL((balance_sums_kernel<L, N, Q, 1>), dim3(unsigned((w.places + 3) / 4)), dim3(256), unsigned(4 * E * 4), s, b);
+        else if (w.team == 1) hipLaunchKernelGGL((balance_sums_kernel<L, N, Q, 1>), dim3(unsigned((w.places + 3) / 4)), dim3(256), unsigned(4 * E * 4), s, b);
+        else fits = false;
       });
+    FM_REQUIRE(fits, "fm_balance_forward: no kernel for pieces of %d waves", w.team);
     // Sequences of more than 64 places on average take a workgroup for 16 columns; from four on, or while the rows do not fill the CUs,
     // four rows of a wave; below that a row.  131072 tokens of 64, 30000 sequences: 58 us by four rows, 20 by one; 65536 of 128, 512
     // sequences: 6.7 and 7.3.
