@@ -493,7 +493,10 @@ __global__ __launch_bounds__(1024, ROWS == 1 ? 8 : 4) void balance_fold_kernel(F
   if (threadIdx.x == 0) st_global(a.shares + blockIdx.x, make_uint4(f2u(v.loss), f2u(v.z), uint32_t(v.tokens), uint32_t(v.filled)));
 }
 
-// Few logits in few pieces: all of the forward in one workgroup, its waves taking the pieces in turn.
+// Few logits in few pieces: all of the forward in one workgroup, its sixteen waves taking the pieces in turn; the runs give each a piece at
+// most, of one run or of four.  Against three launches, whose host's 5.8 us more hide up to that much of the device's time, us on the
+// device: 512 tokens of 8 experts 6.9 and 7.1, 1024 7.0 and 8.4, 2048 9.2 and 8.5; 4096 of 4 9.2 and 8.8; 1000 of 7 13.3 and 7.6; beyond
+// sixteen pieces 1700 of 7 19.5 and 8.6.  (Pieces of four runs at 512 < T: 576 of 8 in pieces of one 7.5, of four 6.6.)
 constexpr int64_t kOnePieces = 32, kOneLogits = 16384, kOneColumns = 4096;
 template <int L, int NV, bool QUADS>
 __global__ __launch_bounds__(1024) void balance_one_kernel(FoldArgs a, FinishArgs fin) {
@@ -694,12 +697,17 @@ int team_of(int64_t T, int E, int64_t S) {
 struct Space {
   int64_t runs, places, sums, slots, tokens, z, shares, bytes;   // offsets in bytes
   int team, run;
+  bool one;   // all of it in one launch, a wave to a piece
 };
 Space space_of(int64_t T, int E, int64_t S) {
   Space w{};
   w.bytes = 256;   // never none: no tokens and no sequences are a call too
-  w.team = team_of(T, E, S);
-  w.run = w.team * run_of(T, E);
+  const int run = run_of(T, E);
+  const int longer = T > 16 * run ? 4 : 1;   // runs to a piece of the one launch
+  w.one = T <= 16 * longer * run && (T + longer * run - 1) / (longer * run) + S + 2 <= kOnePieces && T * E <= kOneLogits && E <= 256 &&
+          S * E <= kOneColumns;
+  w.team = w.one ? 1 : team_of(T, E, S);
+  w.run = (w.one ? longer : w.team) * run;
   w.runs = (T + w.run - 1) / w.run;
   w.places = w.runs + S + 2;
   auto take = [&](int64_t n) {
@@ -756,8 +764,7 @@ int fm_balance_forward(const float* logits, int64_t ld, int64_t T, int E, const 
   const FoldArgs fold{b, f, counts, reinterpret_cast<Share*>(ws + w.shares)};
   FinishArgs fin{fold.shares, 0, z_mult, loss, inverse, acc_total};
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  // a few pieces in one workgroup: 512 tokens of 8 experts 7.3 us in one launch, 3.0 + 2.9 + 3.0 in three, and the host's 2.9 for each
-  if (w.places <= kOnePieces && T * E <= kOneLogits && E <= 256 && S * E <= kOneColumns) {
+  if (w.one) {
     const int64_t waves = w.places < 16 ? w.places : 16;
     for_experts(E, [&](auto l, auto n, auto q) {
       if constexpr (decltype(n)::value <= 8)
