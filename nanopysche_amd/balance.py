@@ -24,6 +24,7 @@ from . import _lib
 MAX_BALANCE_EXPERTS = 1024
 MAX_BALANCE_TOP_K = 1024
 MAX_SEQUENCES = 2 ** 20 - 1
+_JOINT_BYTES = 1 << 18   # a workspace up to here lies behind f, an allocation (1.4 us) less a call; larger ones are freed with the forward
 
 
 class BalanceOutput(NamedTuple):
@@ -40,7 +41,7 @@ class BalanceState:
     logits: torch.Tensor               # [T, E]
     cu_seqlens: Optional[torch.Tensor]  # [S + 1] int32
     mask: Optional[torch.Tensor]       # [T] bool
-    f: torch.Tensor                    # fp32, S * E + 2 at least: E slots / n_s^2, then 1 / S' and 1 / tokens
+    f: torch.Tensor                    # fp32, S * E + 2 and 256 KiB at most behind: E slots / n_s^2, then 1 / S' and 1 / tokens
     sigmoid: bool
     z_mult: float
     shape: torch.Size                  # of the logits as given
@@ -115,15 +116,21 @@ def balance_forward(logits: torch.Tensor, indices: torch.Tensor, *, cu_seqlens: 
     dev = l2.device
     z = 0.0 if z_loss_multiplier is None else float(z_loss_multiplier)
     nbytes = _lib.size_of("fm_balance_workspace_bytes", T, E, S)
-    room = (S * E + 65) // 64 * 64   # f and its two factors, then the workspace, on 256 bytes: an allocation less a call
-    f = torch.empty(room + nbytes // 4, dtype=torch.float32, device=dev)
+    if nbytes <= _JOINT_BYTES:
+        room = (S * E + 65) // 64 * 64   # f and its two factors, then the workspace, on 256 bytes
+        f = torch.empty(room + nbytes // 4, dtype=torch.float32, device=dev)
+        workspace = f.data_ptr() + 4 * room
+    else:
+        f = torch.empty(S * E + 2, dtype=torch.float32, device=dev)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        workspace = scratch.data_ptr()
     loss = torch.empty((), dtype=torch.float32, device=dev)
     counts = torch.empty(E if cu is None else (S, E), dtype=torch.int32, device=dev)
     at = f.data_ptr()
     acc, total = (None, None) if load_tracker is None else (load_tracker.tokens_per_expert, load_tracker.total_tokens)
     _lib.call_on(l2, "fm_balance_forward", l2.data_ptr(), l2.stride(0) if T > 1 else E, T, E, idx.data_ptr(), int(idx.dtype == torch.int64),
                  idx.shape[1], _lib.addr(cu), S, _lib.addr(mask), int(sigmoid), z, at, counts.data_ptr(), at + 4 * S * E, loss.data_ptr(),
-                 _lib.addr(acc), _lib.addr(total), at + 4 * room, nbytes)
+                 _lib.addr(acc), _lib.addr(total), workspace, nbytes)
     return loss, counts, BalanceState(l2, cu, mask, f, sigmoid, z, logits.shape)
 
 
@@ -160,9 +167,9 @@ class _BalanceFunction(torch.autograd.Function):
     def forward(ctx, logits, indices, cu_seqlens, token_mask, scores, z_mult, load_tracker):
         loss, counts, state = balance_forward(logits, indices, cu_seqlens=cu_seqlens, token_mask=token_mask, scores=scores,
                                               z_loss_multiplier=z_mult, load_tracker=load_tracker)
-        ctx.save_for_backward(logits, state.cu_seqlens, state.mask)
+        ctx.save_for_backward(logits, state.cu_seqlens, state.mask, state.f)
         ctx.state = state
-        state.logits = state.cu_seqlens = state.mask = None   # kept by autograd, which sees changes in place
+        state.logits = state.cu_seqlens = state.mask = state.f = None   # kept by autograd, which sees changes in place
         ctx.mark_non_differentiable(counts)
         ctx.set_materialize_grads(False)
         return loss, counts
@@ -172,12 +179,12 @@ class _BalanceFunction(torch.autograd.Function):
     def backward(ctx, dloss, _dcounts):
         if dloss is None:
             return (None,) * 7
-        logits, cu, mask = ctx.saved_tensors
+        logits, cu, mask, f = ctx.saved_tensors
         l2 = logits.reshape(-1, logits.shape[-1])
         if l2.stride(1) != 1 or l2.stride(0) < l2.shape[1]:
             l2 = l2.contiguous()
         s = ctx.state
-        state = BalanceState(l2, cu, mask, s.f, s.sigmoid, s.z_mult, s.shape)
+        state = BalanceState(l2, cu, mask, f, s.sigmoid, s.z_mult, s.shape)
         return balance_backward(state, dloss.float()), None, None, None, None, None, None
 
 

@@ -96,6 +96,7 @@ class _MoELayerFunction(torch.autograd.Function):
         on_router_grad.fused_dot = True
         dx, _, dW1, dW2, dW3, _, _ = ctx.layer.block._backward(ctx.bctx, dout.reshape(T, D), on_router_grad)
         ctx.bctx = None
+        ctx.state.release()
         dx = None if not need_x else dx.to(ctx.x_dtype).reshape(*ctx.lead, D)
         dgw = grads.get("gw")
         if dgw is not None:

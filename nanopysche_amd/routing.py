@@ -361,17 +361,18 @@ class RouterState:
     balance: "BalanceState | None" = None   # the loss of sequences and masks, in place of the batch's
 
     def release(self):
-        """The caller's tensors that the loss's backward reads, for autograd to keep (it notices changes in place)."""
+        """What the loss's backward reads beside the logits, for autograd to keep: the caller's tensors (it notices changes in place)
+        and f (its hooks see it)."""
         if self.balance is None:
             return ()
         b = self.balance
-        kept = b.cu_seqlens, b.mask
-        b.cu_seqlens = b.mask = None
+        kept = b.cu_seqlens, b.mask, b.f
+        b.cu_seqlens = b.mask = b.f = None
         return kept
 
     def restore(self, kept) -> None:
         if self.balance is not None:
-            self.balance.cu_seqlens, self.balance.mask = kept
+            self.balance.cu_seqlens, self.balance.mask, self.balance.f = kept
 
 
 def router_forward(x2, gate_weight, gate_bias, score_bias, top_k, gating, replay=None, normalize=None,
@@ -512,6 +513,7 @@ class _RouterFunction(torch.autograd.Function):
         need_x, need_w, need_b = ctx.needs_input_grad[0], ctx.needs_input_grad[1], ctx.needs_input_grad[2]
         dx, dW, db, _ = router_backward(ctx.state, x2, gate_weight, dweights, daux, need_x, need_w,
                                         need_b and ctx.has_bias, bias_dtype=ctx.bias_dtype)
+        ctx.state.release()
         if dx is not None:
             dx = dx.reshape(*ctx.lead, x2.shape[1])
         if dW is not None:
