@@ -704,9 +704,10 @@ int fm_int8_combine(const float* y, int64_t D, const int32_t* row_of, const floa
  * fm_act8_compress: rows of x into the format; with tile_valid, rows of 128-row tiles with a negative entry are left alone.
  * fm_act8_restore: the values, row r from row index[r] (int32; zeros where it is outside [0, src_rows)) or, with a null
  *   index, from row r.
- * fm_act8_swiglu: h = silu(g) u in fp32, rounded once; g and u in the format.  fm_act8_swiglu_backward: dg = dh u s (1 + g (1 - s)),
+ * fm_act8_swiglu: h = silu(g) u in fp32, rounded once; g and u in the format (all four outputs of it null: h alone).  fm_act8_swiglu_backward: dg = dh u s (1 + g (1 - s)),
  *   du = dh silu(g) from them, s = sigmoid(g).
- * fm_act8_rmsnorm: y = x r w, r = 1 / sqrt(mean(x^2) + eps) (rstd [T] fp32); x in the format.  fm_act8_rmsnorm_backward: from it, with
+ * fm_act8_rmsnorm: y = x r w, r = 1 / sqrt(mean(x^2) + eps) (rstd [T] fp32); x in the format (q, codes and rstd null: y alone, the
+ *   same bits).  fm_act8_rmsnorm_backward: from it, with
  *   a = dy w, dx = r a - (r^3 / D) (sum a x) x and, through a workspace, dw = sum_t dy x r (w's dtype; null: not wanted).
  *   D up to 16384. */
 int fm_act8_compress(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t ld_x, void* q, int64_t ld_q, void* codes,

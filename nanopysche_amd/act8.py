@@ -9,9 +9,10 @@ bfloat16 value does), s being at most a 64th of its block's largest magnitude.  
 
 ``compress_activation`` keeps any activation; ``swiglu_8bit`` and ``rmsnorm_8bit`` are SwiGLU and
 RMSNorm (reference ``model/moe.py:1590``, ``model/norm.py:32-49``) whose backward reads their inputs
-from 8 bits.  Their forwards compute from the inputs themselves: the outputs are
-those of the layers that keep 16 or 32 bits, only the gradients see the rounding.  The reference keeps activations
-in the model's type or recomputes them (``distributed/fsdp.py:80-117``).
+from 8 bits.  Their forwards compute from the inputs themselves: only the gradients see the rounding.  SwiGLU's
+outputs are those of the layers that keep 16 bits, bit for bit; RMSNorm's differ from ``rmsnorm``'s in the last bits of some, its
+sum of squares being added in another order.  The reference keeps activations in the model's type or recomputes them
+(``distributed/fsdp.py:80-117``).
 """
 
 from __future__ import annotations
@@ -54,7 +55,7 @@ def _dtype(dtype: torch.dtype, what: str) -> int:
 
 
 def _no_gradients(name: str, instead: str, *tensors) -> None:
-    if not torch.is_grad_enabled() and fwAD._current_level < 0:   # as inside an autograd node: nothing is recorded
+    if not torch.is_grad_enabled() and fwAD._current_level < 0:   # as under no_grad and in a node: nothing is recorded
         return
     carried = _lib.carried(*tensors)
     if carried:
@@ -235,16 +236,24 @@ def swiglu_compress(gate: torch.Tensor, up: Optional[torch.Tensor] = None) -> Sw
     gate and up [..., H], bf16 or fp32, or one tensor [..., 2H] of the gate's columns and then up's.  Records no gradient, and
     refuses tensors that want one recorded: ``swiglu_8bit``."""
     _no_gradients("swiglu_compress", "swiglu_8bit", gate, up)
+    return _swiglu(gate, up, True)
+
+
+def _swiglu(gate, up, keep: bool):
+    """SwigluKept, or h alone where nothing is kept."""
     g2, u2, at_u, shape = _halves(gate, up)
     H, rows, dtype, dev = shape[-1], g2.shape[0], g2.dtype, g2.device
     h = torch.empty(shape, dtype=dtype, device=dev)
-    kept_g, kept_u = _empty(shape, rows, dtype, dev), _empty(shape, rows, dtype, dev)
-    if rows:
-        qg, cg, ld_q, ld_c = kept_g.at()
+    kept_g = kept_u = qg = cg = qu = cu = None
+    ld_q = _pitch(H)
+    if keep:
+        kept_g, kept_u = _empty(shape, rows, dtype, dev), _empty(shape, rows, dtype, dev)
+        qg, cg, _, _ = kept_g.at()
         qu, cu, _, _ = kept_u.at()
+    if rows:
         _lib.call_on(g2, "fm_act8_swiglu", g2.data_ptr(), g2.stride(0), at_u, u2.stride(0), _DTYPES[dtype], rows, H, h.data_ptr(), H,
-                     qg, cg, qu, cu, ld_q, ld_c)
-    return SwigluKept(h, kept_g, kept_u)
+                     qg, cg, qu, cu, ld_q, ld_q // ACT8_BLOCK)
+    return SwigluKept(h, kept_g, kept_u) if keep else h
 
 
 def swiglu_backward_8bit(dh: torch.Tensor, gate: Activation8, up: Activation8, packed: bool = False):
@@ -275,7 +284,7 @@ def swiglu_backward_8bit(dh: torch.Tensor, gate: Activation8, up: Activation8, p
 class _SwigluFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate, up):
-        h, kept_g, kept_u = swiglu_compress(gate, up)
+        h, kept_g, kept_u = _swiglu(gate, up, True)
         ctx.save_for_backward(kept_g.data, kept_u.data)
         ctx.packed, ctx.dtype = up is None, gate.dtype
         return h
@@ -290,8 +299,9 @@ class _SwigluFunction(torch.autograd.Function):
 
 
 def swiglu_8bit(gate: torch.Tensor, up: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Differentiable silu(gate) * up that keeps gate and up in 8 bits for its backward (``swiglu_compress``)."""
-    return _SwigluFunction.apply(gate, up)
+    """Differentiable silu(gate) * up that keeps gate and up in 8 bits for its backward (``swiglu_compress``); nothing is kept
+    where no gradient is recorded."""
+    return _SwigluFunction.apply(gate, up) if _lib.carried(gate, up) else _swiglu(gate, up, False)
 
 
 # ================================================================= RMSNorm ====
@@ -315,19 +325,27 @@ def rmsnorm_compress(x: torch.Tensor, weight: torch.Tensor, eps: float = DEFAULT
     in one pass.  x [..., D] and weight [D] bf16 or fp32, D up to 16384.  Records no gradient, and refuses tensors that want one
     recorded: ``rmsnorm_8bit``."""
     _no_gradients("rmsnorm_compress", "rmsnorm_8bit", x, weight)
+    return _rmsnorm(x, weight, eps, True)
+
+
+def _rmsnorm(x, weight, eps, keep: bool):
+    """RMSNormKept, or y alone where nothing is kept."""
     x2 = _rows(x, "x", MAX_ACT8_NORM)
     T, D = x2.shape
     w = _norm_weight(weight, D)
     _here(x2.get_device(), "weight", w)
     dev = x2.device
     y = _like(x)
-    rstd = torch.empty(T, dtype=torch.float32, device=dev)
-    kept = _empty(x.shape, T, x.dtype, dev)
+    rstd = kept = q = codes = None
+    ld_q = _pitch(D)
+    if keep:
+        rstd = torch.empty(T, dtype=torch.float32, device=dev)
+        kept = _empty(x.shape, T, x.dtype, dev)
+        q, codes, _, _ = kept.at()
     if T:
-        q, codes, ld_q, ld_c = kept.at()
         _lib.call_on(x2, "fm_act8_rmsnorm", x2.data_ptr(), _DTYPES[x2.dtype], x2.stride(0), T, D, w.data_ptr(), _DTYPES[w.dtype], eps,
-                     y.data_ptr(), D, q, ld_q, codes, ld_c, rstd.data_ptr())
-    return RMSNormKept(y, kept, rstd)
+                     y.data_ptr(), D, q, ld_q, codes, ld_q // ACT8_BLOCK, _lib.addr(rstd))
+    return RMSNormKept(y, kept, rstd) if keep else y
 
 
 def rmsnorm_backward_8bit(dy: torch.Tensor, x: Activation8, weight: torch.Tensor, rstd: torch.Tensor, need_dw: bool = True):
@@ -364,7 +382,7 @@ def rmsnorm_backward_8bit(dy: torch.Tensor, x: Activation8, weight: torch.Tensor
 class _RMSNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, eps):
-        y, kept, rstd = rmsnorm_compress(x, weight, eps)
+        y, kept, rstd = _rmsnorm(x, weight, eps, True)
         ctx.save_for_backward(kept.data, weight, rstd)
         ctx.dtype = x.dtype
         return y
@@ -378,5 +396,6 @@ class _RMSNormFunction(torch.autograd.Function):
 
 
 def rmsnorm_8bit(x: torch.Tensor, weight: torch.Tensor, eps: float = DEFAULT_EPS) -> torch.Tensor:
-    """Differentiable RMSNorm that keeps x in 8 bits for its backward (``rmsnorm_compress``)."""
-    return _RMSNormFunction.apply(x, weight, float(eps))
+    """Differentiable RMSNorm that keeps x in 8 bits for its backward (``rmsnorm_compress``); nothing is kept where no gradient is
+    recorded, and y is the same."""
+    return _RMSNormFunction.apply(x, weight, float(eps)) if _lib.carried(x, weight) else _rmsnorm(x, weight, float(eps), False)

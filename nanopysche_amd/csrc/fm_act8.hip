@@ -241,10 +241,11 @@ __global__ __launch_bounds__(256) void swiglu_kernel(Items t, SwigluArgs a) {
     g[u].widen(gv);
     up[u].widen(uv);
     swiglu8(gv, uv, h);
+    if (it[u].in) store8<T, true, (STREAM > 0)>(static_cast<T*>(a.h) + it[u].row * a.ld_h + it[u].col, h, it[u].n);
+    if (a.qg == nullptr) continue;   // no backward: h alone
     uint32_t gc, uc;
     const uint2 gb = act_encode8(gv, gc), ub = act_encode8(uv, uc);
     if (!it[u].in) continue;
-    store8<T, true, (STREAM > 0)>(static_cast<T*>(a.h) + it[u].row * a.ld_h + it[u].col, h, it[u].n);
     store_kept(a.qg, a.ld_q, a.cg, a.ld_c, it[u].row, it[u].col, gb, gc);
     store_kept(a.qu, a.ld_q, a.cu, a.ld_c, it[u].row, it[u].col, ub, uc);
   }
@@ -347,7 +348,7 @@ __global__ __launch_bounds__(L > 0 ? 256 : 1024) void norm_kernel(NormArgs a) {
   ss = row_sum<L>(ss, sums, 0, 0, int(blockDim.x >> 6));
   const float r = 1.0f / sqrtf(ss / float(a.D) + a.eps);
   if (!in) return;
-  if (lane == 0) st_global(a.rstd + row, r);
+  if (lane == 0 && a.q) st_global(a.rstd + row, r);
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     const int col = step * c + 8 * lane;
@@ -357,9 +358,10 @@ __global__ __launch_bounds__(L > 0 ? 256 : 1024) void norm_kernel(NormArgs a) {
     wr[c].widen(wv);
 #pragma unroll
     for (int j = 0; j < 8; ++j) yv[j] = (v[j] * r) * wv[j];
+    store8<T, TAIL, (STREAM > 0)>(static_cast<T*>(a.y) + row * a.ld_y + col, yv, a.D - col);
+    if (a.q == nullptr) continue;   // no backward: y alone
     uint32_t code;
     const uint2 b = act_encode8(v, code);
-    store8<T, TAIL, (STREAM > 0)>(static_cast<T*>(a.y) + row * a.ld_y + col, yv, a.D - col);
     store_kept(a.q, a.ld_q, a.codes, a.ld_c, row, col, b, code);
   }
 }
@@ -679,7 +681,8 @@ int fm_act8_swiglu(const void* g, int64_t ld_g, const void* u, int64_t ld_u, int
   FM_REQUIRE(dtype_ok(dtype), "fm_act8_swiglu: gate and up must be bf16 or fp32");
   if (rows == 0) return 0;
   FM_REQUIRE(g && u && h && ld_g >= 0 && ld_u >= 0 && ld_h >= H, "fm_act8_swiglu: null pointer or bad pitch");
-  FM_REQUIRE(kept_ok(qg, ld_q, cg, ld_c, H) && kept_ok(qu, ld_q, cu, ld_c, H), "fm_act8_swiglu: bad payload, codes or pitches");
+  const bool keep = qg || cg || qu || cu;
+  FM_REQUIRE(!keep || (kept_ok(qg, ld_q, cg, ld_c, H) && kept_ok(qu, ld_q, cu, ld_c, H)), "fm_act8_swiglu: bad payload, codes or pitches");
   const SwigluArgs a{g, u, ld_g, ld_u, h, ld_h, static_cast<uint8_t*>(qg), static_cast<uint8_t*>(qu), static_cast<uint8_t*>(cg),
                      static_cast<uint8_t*>(cu), ld_q, ld_c};
   const hipStream_t s = static_cast<hipStream_t>(stream);
@@ -719,8 +722,9 @@ int fm_act8_rmsnorm(const void* x, int dtype, int64_t ld_x, int64_t T, int64_t D
   FM_REQUIRE(T >= 0 && T < (int64_t(1) << 31) && D >= 1 && D <= kNormMaxD, "fm_act8_rmsnorm: D must be 1 to %d, T below 2^31", kNormMaxD);
   FM_REQUIRE(dtype_ok(dtype) && dtype_ok(w_dtype), "fm_act8_rmsnorm: x and the weight must be bf16 or fp32");
   if (T == 0) return 0;
-  FM_REQUIRE(x && w && y && rstd && ld_x >= 0 && ld_y >= D, "fm_act8_rmsnorm: null pointer or bad pitch");
-  FM_REQUIRE(kept_ok(q, ld_q, codes, ld_c, D) && ld_q == (D + 31) / 32 * 32, "fm_act8_rmsnorm: bad payload, codes or pitches");
+  const bool keep = q || codes || rstd;
+  FM_REQUIRE(x && w && y && (rstd || !keep) && ld_x >= 0 && ld_y >= D, "fm_act8_rmsnorm: null pointer or bad pitch");
+  FM_REQUIRE(ld_q == (D + 31) / 32 * 32 && (!keep || kept_ok(q, ld_q, codes, ld_c, D)), "fm_act8_rmsnorm: bad payload, codes or pitches");
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const int lanes = norm_lanes(D), threads = lanes ? 256 : 64 * norm_waves(D), rows = lanes ? 256 / lanes : 1;   // of a workgroup
   const int64_t run = (int64_t(1) << 31) / threads * rows;   // a launch has fewer than 2^32 threads
@@ -728,7 +732,8 @@ int fm_act8_rmsnorm(const void* x, int dtype, int64_t ld_x, int64_t T, int64_t D
     const int64_t n = T - r < run ? T - r : run;
     for_dtype(dtype, [&](auto t) {
       const NormArgs a{static_cast<const decltype(t)*>(x) + r * ld_x, ld_x, n, int(D), w, eps, static_cast<decltype(t)*>(y) + r * ld_y, ld_y,
-                       static_cast<uint8_t*>(q) + r * ld_q, ld_q, static_cast<uint8_t*>(codes) + r * ld_c, ld_c, rstd + r};
+                       keep ? static_cast<uint8_t*>(q) + r * ld_q : nullptr, ld_q, keep ? static_cast<uint8_t*>(codes) + r * ld_c : nullptr, ld_c,
+                       keep ? rstd + r : nullptr};
       for_dtype(w_dtype, [&](auto wt) {
         for_norm(D, [&](auto nc, auto l, auto tail) {
           for_stream<0, 1>(T * D * int64_t(sizeof(t)), [&](auto stream_) {
