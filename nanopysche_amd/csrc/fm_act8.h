@@ -78,4 +78,9 @@ struct Act8 {
   __device__ __forceinline__ uint32_t code(int64_t row, int64_t col) const { return codes[row * ld_c + (col >> 5)]; }
 };
 
+// Whether a caller's payload and codes are such a matrix of cols columns.
+inline bool kept_ok(const void* q, int64_t ld_q, const void* codes, int64_t ld_c, int64_t cols) {
+  return q && codes && ld_q >= cols && ld_q % kActBlock == 0 && ld_c * kActBlock >= ld_q && (reinterpret_cast<uintptr_t>(q) & 7) == 0;
+}
+
 }  // namespace fm

@@ -581,9 +581,6 @@ void for_dtype(int dtype, F go) {
 }
 
 bool dtype_ok(int d) { return d == FM_DTYPE_BF16 || d == FM_DTYPE_F32; }
-bool kept_ok(const void* q, int64_t ld_q, const void* codes, int64_t ld_c, int64_t cols) {
-  return q && codes && ld_q >= cols && ld_q % kActBlock == 0 && ld_c * kActBlock >= ld_q && (reinterpret_cast<uintptr_t>(q) & 7) == 0;
-}
 
 // ---- the norm's shapes
 int norm_waves(int64_t D) { return int((D + 1023) / 1024); }

@@ -161,9 +161,6 @@ __global__ __launch_bounds__(256) void kept_router_grad_kernel(const uint16_t* _
 Act8 kept_of(const void* q, int64_t ld_q, const void* codes, int64_t ld_c) {
   return Act8{static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(codes), ld_q, ld_c};
 }
-bool kept_ok(const void* q, int64_t ld_q, const void* codes, int64_t ld_c, int64_t cols) {
-  return q && codes && ld_q >= cols && ld_q % kActBlock == 0 && ld_c * kActBlock >= ld_q && (reinterpret_cast<uintptr_t>(q) & 7) == 0;
-}
 
 }  // namespace
 }  // namespace fm

@@ -1,4 +1,4 @@
-// Sums and maxima over groups of neighbouring lanes, without LDS: moves within rows of 16 lanes, then the
+// Sums and other folds over groups of neighbouring lanes, without LDS: moves within rows of 16 lanes, then the
 // swaps of rows and halves.
 #pragma once
 
@@ -8,7 +8,7 @@
 
 namespace fm {
 
-// lanes of a group of N (a power of two): sum and maximum, the same in every lane
+// lanes of a group of N (a power of two) folded by f, and their sum: the same in every lane
 template <int N, typename F>
 __device__ __forceinline__ float group_fold(float v, F f) {
   auto dpp = [](float x, auto ctrl) { return __builtin_bit_cast(float, dpp_move<decltype(ctrl)::value>(__builtin_bit_cast(int, x))); };
@@ -29,10 +29,6 @@ __device__ __forceinline__ float group_fold(float v, F f) {
 template <int N>
 __device__ __forceinline__ float group_sum(float v) {
   return group_fold<N>(v, [](float a, float b) { return a + b; });
-}
-template <int N>
-__device__ __forceinline__ float group_max(float v) {
-  return group_fold<N>(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
 }  // namespace fm
