@@ -1288,6 +1288,7 @@ class FP8FlowMoECompute:
                                       self._paired(kind), pcols.get(kind, False))
             _gemm_m(kind, rows, ew.w13, plan, GU, mask, want)
             saved[kind] = (cols, ew)
+        del rows
         h_cols = {}
         GU8 = _empty(GU.shape, R, torch.bfloat16, dev) if keep8 else None   # rows of tiles past the last group hold nothing
         for kind, want in ((fp8_kind, 1), (_lib.QUANT_BF16 if use_bf16 else None, 0)):
@@ -1305,14 +1306,17 @@ class FP8FlowMoECompute:
             else:
                 _lib.call("fm_swiglu_quantize", gu, 2 * H, gu + 2 * H, 2 * H, R, H, *args, valid, _lib.stream_of(GU))
             _gemm_m(kind, hrow, saved[kind][1].w2t, plan, Y, mask, want)
+        del hrow
+        if self.capture_intermediates is not None:
+            self.capture_intermediates["gate_up"] = GU.detach().clone()
+        if keep8:   # the 8 bits of the outputs and tokens take its room
+            GU = None
         if self._dense:
             # the output must not be a view made inside this Function (callers
             # combine it in place): the padded buffer itself when T fills it
             out = Y if R == T else Y[:T].clone()
         else:
             out = fused_unpermute_unpad(Y, plan, wts)
-        if self.capture_intermediates is not None:
-            self.capture_intermediates["gate_up"] = GU.detach().clone()
         ctx.compute = self
         ctx.plan = plan
         ctx.tiles = tiles
