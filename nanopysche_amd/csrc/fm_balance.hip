@@ -683,7 +683,7 @@ int run_of(int64_t T, int E) {
   return int(r <= least ? least : (r + least - 1) / least * least);
 }
 // Waves to a piece: four where sequences have 64 tokens on average, sixteen from 1024 on; the fewer places to write and add.  One
-// sequence of 65536 tokens, 256 experts: fold 11.5 us of 1024 places, 7.0 of 256.
+// sequence of 65536 tokens, 256 experts: sums and fold 18.6 + 23.0 us of 4096 places, 17.0 + 6.7 of 256.
 // (Sixteen waves' registers do not fit where a lane holds sixteen values of a row: beyond 512 experts, beyond 256 of no multiple of 4.
 // 65536 x 511 of one sequence: 57 us the forward in pieces of four, 249 in pieces cut for sixteen and taken by one.)
 constexpr int kTeamMaxValues = 8;   // of a lane, for sixteen waves
@@ -789,9 +789,10 @@ int fm_balance_forward(const float* logits, int64_t ld, int64_t T, int E, const 
         else fits = false;
       });
     FM_REQUIRE(fits, "fm_balance_forward: no kernel for pieces of %d waves", w.team);
-    // Sequences of more than 64 places on average take a workgroup for 16 columns; from four on, or while the rows do not fill the CUs,
-    // four rows of a wave; below that a row.  131072 tokens of 64, 30000 sequences: 58 us by four rows, 20 by one; 65536 of 128, 512
-    // sequences: 6.7 and 7.3.
+    // Sequences of more than 64 places on average take a workgroup for 16 columns (one of 65536 tokens, 256 experts: 6.7 us, by four rows 19.6).
+    // From four on, while the rows do not fill the CUs, and up to twice that from two on, four rows of a wave; below that a row.  By four
+    // rows and by one, us: 131072 tokens of 64, 30000 sequences 107 and 20; 65536 of 256, 512 sequences (two places each) 9.0 and 6.7, 1300
+    // sequences 23 and 15, 400 9.0 and 10.6; 65536 of 32, 2048 sequences 6.2 and 13.2, 4000 8.8 and 6.0; 65536 of 128, 700 8.7 and 6.1.
     auto fold_by = [&](auto c, auto rows, auto most) {
       constexpr int C = decltype(c)::value, R = decltype(rows)::value, M = decltype(most)::value, G = 1024 / (C * R);
       const int parts = (E + C - 1) / C;
@@ -799,7 +800,7 @@ int fm_balance_forward(const float* logits, int64_t ld, int64_t T, int E, const 
       if (S > 0) hipLaunchKernelGGL((balance_fold_kernel<C, R, M>), dim3(unsigned(fin.parts)), dim3(1024), 0, s, fold, parts, fin);
     };
     if (w.runs > 64 * S) fold_by(std::integral_constant<int, 16>{}, std::integral_constant<int, 64>{}, std::integral_constant<int, 0>{});
-    else if (w.runs > 4 * S || S * E <= 1 << 17) fold_by(std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{}, std::integral_constant<int, 256>{});
+    else if (w.runs > 4 * S || S * E <= 1 << 16 || (w.runs > 2 * S && S * E <= 1 << 17)) fold_by(std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{}, std::integral_constant<int, 256>{});
     else if (E > 32) fold_by(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
     else fold_by(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
     if (fin.parts != 1) hipLaunchKernelGGL(balance_finish_kernel, dim3(1), dim3(1024), 0, s, fin);
