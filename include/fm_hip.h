@@ -695,7 +695,7 @@ int fm_int8_combine(const float* y, int64_t D, const int32_t* row_of, const floa
 
 /* -------------------------------------- activations in 8 bits, for the backward ----
  * Blocks of 32 values along a row share a power of two s = 2^k, k = max(floor(log2 max|x|) - 6, -127)
- * (OCP MX int8); q = min(max(rint(x / s), -127), 127), the code is k + 127 (e8m0), 255 for a block with a NaN
+ * (the values of OCP MX int8, whose code of the same block is 6 above; its smallest scale is 2^-133); q = min(max(rint(x / s), -127), 127), the code is k + 127 (e8m0), 255 for a block with a NaN
  * or an infinity, which stands for NaNs.  q s is exact in bf16 and fp32.  No counterpart in the reference, which keeps activations in
  * the model's type or recomputes them (distributed/fsdp.py:80-117).
  * Payload int8 [rows, ld_q], ld_q = cols rounded up to 32, on 8 bytes, zeros behind cols; codes [rows, ld_c], ld_c = ld_q / 32.

@@ -3,7 +3,8 @@
     k = max(floor(log2 max|x|) - 6, -127) over a block of 32 values of a row,  s = 2^k
     q = min(max(rint(x / s), -127), 127),  the value that it stands for is q s
 
-(OCP MX int8: an e8m0 code per block; 33 bytes hold 32 values.)  q s is exact in bfloat16 and
+(an e8m0 code per block, k + 127; 33 bytes hold 32 values.  The values are those of OCP MX int8 down to its
+smallest scale, 2^-133; its code of the same block is 6 above this one, its element holding a 2^-6.)  q s is exact in bfloat16 and
 float32, so keeping rounds a value once, by at most s / 2 (s for what lies above 127.5 s, which no
 bfloat16 value does), s being at most a 64th of its block's largest magnitude.  A block that holds a NaN or an infinity stands for NaNs.
 

@@ -1,7 +1,9 @@
 // Activations in 8 bits: the format, and its conversions in registers.
 //
-// A row's blocks of 32 values share a power of two s = 2^k (OCP MX int8: an e8m0 code):
+// A row's blocks of 32 values share a power of two s = 2^k (an e8m0 code):
 //   k = max(floor(log2 max|x|) - 6, -127), q = min(max(rint(x / s), -127), 127), code = k + 127.
+// The values are those of OCP MX int8, the bytes are not: its element is q 2^-6, so its code of the same block is 6
+// above this one, and its smallest scale 2^-133.
 // x / s is exact, so q is the correctly rounded quotient (ties to even) in every order of work, and q s,
 // a 7-bit whole number times a power of two, is exact in bf16 as in fp32: what a kernel
 // rounds is the value once, in the forward.  |x - q s| <= s / 2 (s where |x| is above 127.5 s, which no

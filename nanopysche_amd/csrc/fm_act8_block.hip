@@ -1,10 +1,12 @@
 // The expert block's backward from activations in 8 bits (fm_act8.h): the operands of its grouped products, made from the
-// kept gate|up, tokens and expert outputs in the passes that the 16-bit ones take.
+// kept gate|up, tokens and expert outputs by the tile producers of the 16-bit ones.  The first and the fourth take the place of
+// passes there; the others are passes more, whose results the 16-bit block has from its forward, or (the last) forms with the gating's gradient.
 //   fm_act8_swiglu_keep_quantize      the forward's h, as fm_swiglu_quantize, keeping gate|up on the way
 //   fm_act8_permute                   the tokens in expert order, as fm_permute
 //   fm_act8_swiglu_quantize           h = silu(g) u of the kept g and u, as fm_swiglu_quantize
 //   fm_act8_swiglu_backward_quantize  [dg | du], as fm_swiglu_backward
 //   fm_act8_router_weight_grad        dw[t, k] = <dout[t], y[row(t, k)]>, as fm_router_weight_grad
+// 33664 rows, H 1408, D 2048, bf16 operands: 80, 80, 76, 172 and 25 us, of 62, 28, 31, 92 and 22 for the bytes: the transposed outputs.
 // The tile producer's 128 columns are four of the format's blocks, so a lane's eight values have one code.
 #include "fm_act8.h"
 #include "fm_lanes.h"
